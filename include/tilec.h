@@ -234,6 +234,43 @@ size_t tilec_sum_counter_bytes(int64_t R, int64_t C, int32_t layout,
  */
 int tilec_read_floor(const void* x, size_t bytes, float* sink, int32_t workgroups, void* stream);
 
+/*
+ * Training operators.  The reference has none; they are what a training step
+ * needs beside its products (tilec_matmul) and sums (tilec_sum), under the
+ * same conventions: asynchronous on `stream`, nothing allocated, a status
+ * code, caller-owned scratch.
+ */
+
+/*
+ * Layer norm over the rows of x [R, D], D >= 1:
+ *   y = (x - mean) rstd weight + bias,   rstd = 1 / sqrt(var + eps)
+ * with var the mean of the squared deviations.  x and y are float32 or
+ * bfloat16, each with its own dtype code and row stride (>= D elements, any
+ * alignment of the element); weight and bias [D], contiguous, share w_dtype
+ * and may each be NULL (1 and 0).  mean and rstd [R], float32, are written
+ * where not NULL.  Statistics are float32.  y may be x (same dtype and
+ * stride); otherwise outputs must not overlap inputs.
+ */
+int tilec_layer_norm(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd,
+                     int64_t R, int64_t D, int64_t ldx, int64_t ldy, int32_t x_dtype, int32_t y_dtype,
+                     int32_t w_dtype, float eps, void* stream);
+
+/*
+ * Its gradients, from the mean and rstd [R] of the forward pass:
+ *   dx = rstd (dy weight - c1 - xhat c2),  c1 = mean(dy weight),  c2 = mean(dy weight xhat)
+ *   dweight = sum over rows of dy xhat,    dbias = sum over rows of dy
+ * dy and dx have y_dtype; dweight and dbias [D] are float32 and may each be
+ * NULL.  Column sums are added in a fixed order: the same bits on every call
+ * on one device.  `workspace`: tilec_layer_norm_backward_workspace_bytes, any
+ * contents; 16-byte aligned.  dx may be dy.
+ */
+int tilec_layer_norm_backward(const void* dy, const void* x, const float* mean, const float* rstd,
+                              const void* weight, void* dx, float* dweight, float* dbias,
+                              int64_t R, int64_t D, int64_t lddy, int64_t ldx, int64_t lddx,
+                              int32_t x_dtype, int32_t y_dtype, int32_t w_dtype,
+                              void* workspace, size_t workspace_bytes, void* stream);
+size_t tilec_layer_norm_backward_workspace_bytes(int64_t R, int64_t D, int32_t x_dtype);
+
 /* Message describing the last failure on this thread ("" if none). */
 const char* tilec_last_error(void);
 

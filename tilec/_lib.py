@@ -41,6 +41,11 @@ SIGNATURES = {
     "tilec_auto_split_k": (_i32, [_i64, _i64, _i64, _i32, _i32]),
     "tilec_num_variants": (_i32, []),
     "tilec_variant_info": (ctypes.c_int, [_i32, ctypes.POINTER(_i32), ctypes.POINTER(ctypes.c_char_p)]),
+    "tilec_layer_norm": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _i32,
+                                        ctypes.c_float, _vp]),
+    "tilec_layer_norm_backward": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
+                                                 _i64, _i32, _i32, _i32, _vp, _sz, _vp]),
+    "tilec_layer_norm_backward_workspace_bytes": (_sz, [_i64, _i64, _i32]),
     "tilec_last_error": (ctypes.c_char_p, []),
     "tilec_version": (_i32, []),
 }

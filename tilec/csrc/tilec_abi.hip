@@ -13,6 +13,7 @@
 #include <mutex>
 #include <vector>
 
+#include "abi.h"
 #include "common.h"
 #include "../../include/tilec.h"
 
@@ -43,8 +44,10 @@ hipError_t launch_read_floor(const void* x, int64_t bytes, float* sink, int work
 using namespace tilec;
 
 namespace {
-
 thread_local char g_err[512] = "";
+}  // namespace
+
+namespace tilec {
 
 int fail(int code, const char* fmt, ...) {
   va_list ap;
@@ -53,6 +56,12 @@ int fail(int code, const char* fmt, ...) {
   va_end(ap);
   return code;
 }
+
+void clear_error() { g_err[0] = 0; }
+
+}  // namespace tilec
+
+namespace {
 
 const std::vector<const VariantDesc*>& table() {
   static std::vector<const VariantDesc*> t;
@@ -74,8 +83,6 @@ int find(const char* name) {
     if (strcmp(t[i]->name, name) == 0) return (int)i;
   return -1;
 }
-
-constexpr int64_t kMaxDim = (int64_t(1) << 31) - 1024;  // kernels index rows/cols in int32
 
 // The skinny kernel addresses its operands within one block with 32-bit byte
 // offsets: row-major x2 over 16 rows (16 * ldx2 * 4 bytes < 2^31), x1 over 16

@@ -533,3 +533,10 @@ def sum(x, axis=1):
     _lib.check(L.tilec_sum(t.data_ptr(), out.data_ptr(), R, C, ld, layout, dtype, axis,
                            ws_ptr, ws_bytes, cnt_ptr, cnt_bytes, stream))
     return out
+
+
+# The training operators (training.py) are part of this module's API; they use
+# the buffers above, so they come last.
+from .training import layer_norm, layer_norm_backward  # noqa: E402
+
+__all__ += ["layer_norm", "layer_norm_backward"]

@@ -1,0 +1,171 @@
+"""Training operators on PyTorch-ROCm tensors, reached as `tilec.ext.*`: layer
+norm and its gradients, the cross entropy of a linear layer's outputs and its
+gradients, and an AdamW step over many tensors.
+
+They are what a training step needs beside the products (`matrix_mul`) and the
+sums (`sum`) of its linear layers, and follow the same rules: arguments are
+checked before anything is enqueued (ValueError for shapes, TypeError for
+types and devices), work goes to the current stream of the tensors' device,
+scratch is the (device, stream) workspace of `ext`, and nothing synchronises.
+Like those two they are plain functions with no autograd of their own.
+"""
+
+import torch
+
+from . import _lib
+from .ext import workspace_for
+
+__all__ = ["layer_norm", "layer_norm_backward"]
+
+_CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+
+
+def _code(what, t):
+    code = _CODES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what}: unsupported tensor of dtype {t.dtype} (use float32 or bfloat16)")
+    return code
+
+
+def _on_gpu(what, first, *others):
+    """All tensors (None: absent) on the one GPU of `first`."""
+    if first.device.type != "cuda":
+        raise TypeError(f"{what} needs tensors on a ROCm GPU (got {first.device})")
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise TypeError(f"{what} needs all tensors on one GPU (got {first.device} and {t.device})")
+
+
+def _rows(what, name, x):
+    """x as a 2-D tensor whose rows are contiguous (copied if they are not),
+    and its row stride."""
+    if x.dim() == 1:
+        x = x.unsqueeze(0)
+    if x.dim() != 2:
+        raise ValueError(f"{what}: expected a 1-D or 2-D {name}, got shape {tuple(x.shape)}")
+    R, D = x.shape
+    if (D > 1 and x.stride(1) != 1) or (R > 1 and x.stride(0) < D):
+        x = x.contiguous()
+    return x, (x.stride(0) if R > 1 else D)
+
+
+def _vector(what, name, t, n, dtype=None):
+    if t is None:
+        return None
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected ({n},)")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{what}: {name} has dtype {t.dtype}, expected {dtype}")
+    return t.contiguous()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+class _on:
+    """The tensors' device as the current one, where it is not."""
+
+    def __new__(cls, device):
+        if device.index == torch.cuda.current_device():
+            return _HERE
+        return torch.cuda.device(device)
+
+
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *_):
+        return None
+
+
+_HERE = _Here()
+
+
+def _norm_params(what, D, weight, bias):
+    weight, bias = _vector(what, "weight", weight, D), _vector(what, "bias", bias, D)
+    codes = {_code(what, t) for t in (weight, bias) if t is not None}
+    if len(codes) > 1:
+        raise TypeError(f"{what}: weight and bias have different types ({weight.dtype} and {bias.dtype})")
+    return weight, bias, codes.pop() if codes else _lib.F32
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, dtype=None):
+    """(y, mean, rstd): every row of x normalised to mean 0 and variance 1,
+    times `weight` plus `bias`.
+
+        mean = sum(x) / D    rstd = 1 / sqrt(sum((x - mean)^2) / D + eps)
+        y = (x - mean) * rstd * weight + bias
+
+    x: [R, D] (or [D], one row) float32 or bfloat16, D >= 1; row-strided views
+    are read in place.  weight, bias: [D], of one type, or None.  y has x's
+    shape and its type, or `dtype` (the fp32 output of `matrix_mul` normalised
+    to the bf16 input of the next product).  mean and rstd are float32 [R]
+    whatever the types; `layer_norm_backward` takes them.
+    """
+    what = "layer_norm"
+    shape = x.shape
+    _on_gpu(what, x, weight, bias)
+    x_code = _code(what, x)
+    x, ldx = _rows(what, "x", x)
+    R, D = x.shape
+    if D == 0:
+        raise ValueError(f"{what}: rows without elements have no mean (shape {tuple(shape)})")
+    weight, bias, w_code = _norm_params(what, D, weight, bias)
+    y = torch.empty(shape, dtype=dtype or x.dtype, device=x.device)
+    y_code = _code(what, y)
+    stats = torch.empty((2, R), dtype=torch.float32, device=x.device)
+    mean, rstd = stats[0], stats[1]
+    if R:
+        with _on(x.device):
+            _lib.check(_lib.lib().tilec_layer_norm(
+                x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), R, D, ldx, D,
+                x_code, y_code, w_code, eps, _stream(x.device)))
+    return y, mean, rstd
+
+
+def layer_norm_backward(dy, x, mean, rstd, weight=None, param_grads=True):
+    """(dx, dweight, dbias) of `layer_norm` for the gradient dy of its y.
+
+        wdy = dy * weight;  xhat = (x - mean) * rstd
+        dx = rstd * (wdy - mean(wdy) - xhat * mean(wdy * xhat))
+        dweight = sum over rows of dy * xhat;  dbias = sum over rows of dy
+
+    x, mean, rstd: the forward pass's input and statistics.  dx has dy's shape
+    and type; dweight and dbias are float32 [D], added in a fixed order (the
+    same bits on every call).  param_grads=False leaves them out (None).
+    """
+    what = "layer_norm_backward"
+    shape = dy.shape
+    _on_gpu(what, dy, x, mean, rstd, weight)
+    y_code, x_code = _code(what, dy), _code(what, x)
+    if dy.shape != x.shape:
+        raise ValueError(f"{what}: dy has shape {tuple(shape)}, x {tuple(x.shape)}")
+    dy, lddy = _rows(what, "dy", dy)
+    x, ldx = _rows(what, "x", x)
+    R, D = x.shape
+    if D == 0:
+        raise ValueError(f"{what}: rows without elements have no mean (shape {tuple(shape)})")
+    mean = _vector(what, "mean", mean, R, torch.float32)
+    rstd = _vector(what, "rstd", rstd, R, torch.float32)
+    weight, _, w_code = _norm_params(what, D, weight, None)
+    dx = torch.empty(shape, dtype=dy.dtype, device=dy.device)
+    dw = db = None
+    if param_grads:
+        dw, db = torch.empty((2, D), dtype=torch.float32, device=dy.device)
+    elif R == 0:
+        return dx, None, None
+    L = _lib.lib()
+    with _on(dy.device):
+        stream = _stream(dy.device)
+        need = L.tilec_layer_norm_backward_workspace_bytes(R, D, x_code)
+        ws_ptr = workspace_for(dy.device, stream, need).data_ptr() if need else None
+        _lib.check(L.tilec_layer_norm_backward(
+            dy.data_ptr(), x.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _ptr(weight), dx.data_ptr(), _ptr(dw),
+            _ptr(db), R, D, lddy, ldx, D, x_code, y_code, w_code, ws_ptr, need, stream))
+    return dx, dw, db
