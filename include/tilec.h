@@ -271,6 +271,42 @@ int tilec_layer_norm_backward(const void* dy, const void* x, const float* mean, 
                               void* workspace, size_t workspace_bytes, void* stream);
 size_t tilec_layer_norm_backward_workspace_bytes(int64_t R, int64_t D, int32_t x_dtype);
 
+/*
+ * Cross entropy of logits = x weight^T, which are not kept: x [N, H], weight
+ * [V, H] (both float32 or both bfloat16, row-major with row strides ldx, ldw
+ * >= H), target [N] int64.
+ *   loss_r = log(sum_v exp(logits[r, v])) - logits[r, target_r]
+ * float32: `loss` [N] with TILEC_REDUCE_NONE, else one value, the sum or the
+ * mean over the rows that count.  Rows whose target is ignore_index do not:
+ * their loss and gradients are 0 whatever x holds there, and a mean over no
+ * rows is 0.  A target that is neither that nor a class in [0, V) makes its
+ * loss, and every gradient it reaches, NaN.
+ *
+ * grad != 0 also writes the gradients dx [N, H] and dweight [V, H],
+ * contiguous, of x's type, of
+ *   TILEC_REDUCE_NONE:       sum_r grad_loss[r] loss_r  (grad_loss [N] float32, NULL: ones)
+ *   TILEC_REDUCE_SUM, _MEAN: grad_loss[0] loss          (one float32 on the device, NULL: 1)
+ * Rows are worked through in chunks of chunk_rows (0: as many as keep the
+ * chunk's 16-bit (float32: 32-bit) values, one per row and class, within 2
+ * GiB); more than one chunk adds a float32 [V, H] to the workspace.
+ *
+ * tilec_linear_ce_scratch_bytes gives the workspace (any contents, 16-byte
+ * aligned) and counters (zeroed once, left zero) for exactly these arguments;
+ * of x and weight it reads the addresses' alignment only.  Every sum is
+ * float32 or wider, in a fixed order.
+ */
+#define TILEC_REDUCE_NONE 0
+#define TILEC_REDUCE_SUM 1
+#define TILEC_REDUCE_MEAN 2
+int tilec_linear_ce(const void* x, const void* weight, const int64_t* target, float* loss,
+                    const float* grad_loss, void* dx, void* dweight, int64_t N, int64_t H, int64_t V,
+                    int64_t ldx, int64_t ldw, int32_t dtype, int32_t reduction, int64_t ignore_index,
+                    int32_t grad, int64_t chunk_rows, void* workspace, size_t workspace_bytes,
+                    void* counters, size_t counter_bytes, void* stream);
+int tilec_linear_ce_scratch_bytes(const void* x, const void* weight, int64_t N, int64_t H, int64_t V,
+                                  int64_t ldx, int64_t ldw, int32_t dtype, int32_t reduction, int32_t grad,
+                                  int64_t chunk_rows, size_t* workspace_bytes, size_t* counter_bytes);
+
 /* Message describing the last failure on this thread ("" if none). */
 const char* tilec_last_error(void);
 

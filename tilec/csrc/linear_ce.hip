@@ -1,0 +1,786 @@
+// Cross entropy of a linear layer's outputs, without keeping them:
+//   l = x W^T  (x [N, H], W [V, H])        lse_r = log sum_v exp(l_rv)
+//   loss_r = lse_r - l[r, t_r]             (0 where t_r is ignored)
+//   d_rv = g_r (exp(l_rv - lse_r) - [v = t_r])   (0 in ignored rows)
+//   dx = d W       dW = d^T x
+// with g_r the gradient of row r's loss (1 / count times the scalar's for the
+// mean).
+//
+// Three products of 2 N H V operations bound it: the logits are formed once,
+// and what the gradients need of them is one 16-bit value each.  Rows are
+// taken in chunks, so that those values fit the workspace.
+//
+// bf16 inputs.  The logits' product ends in an epilogue that never stores
+// them.  It runs with W as its row operand, so a lane holds consecutive
+// vocabulary entries of one token: a wave takes the maximum m and the sum of
+// exp(l - m) over its 64 or 128 entries of a token in its own registers and
+// two shuffles, writes those two, and (for gradients) exp(l - m) 2^15 in fp16,
+// whose 11 bits leave the one rounding to bf16 that d itself gets as the only
+// one that counts; values below 2^-29 of the largest in their group lose bits,
+// below 2^-39 they are lost.  One pass over them (ce_rows_kernel) then joins the groups to lse
+// and turns each, in place, into d in bf16.  The target's own entry, where
+// exp(l - lse) - 1 cancels, is taken from the fp32 logit.  The scalar factor
+// of d (1 / count) is kept out of it and applied to the fp32 sums of dx and
+// dW, so that it costs no rounding of its own.
+//
+// fp32 inputs.  The library's own products (tilec_matmul) form the logits
+// chunk and the gradients; l becomes d in place, in fp32.
+#include <algorithm>
+#include <cfloat>
+
+#include "abi.h"
+#include "gemm_bf16_lds.h"
+#include "../../include/tilec.h"
+
+namespace tilec {
+
+namespace {
+
+typedef _Float16 f16;
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kScale16 = 32768.f;  // exp(l - m) <= 1 uses fp16's range up to 2^15
+
+__device__ __forceinline__ u16 bf16_bits(float f) { return __builtin_bit_cast(u16, (__bf16)f); }
+
+// ---------------------------------------------------------------------------
+// Epilogues of the bf16 products
+// ---------------------------------------------------------------------------
+
+// The logits: rows are vocabulary entries, columns tokens.
+struct CeLogits {
+  u16* e;      // exp(l - m) 2^15 in fp16, [token][lde]; NULL: losses only
+  int64_t lde;
+  f32x2* stat;  // (m, sum of exp(l - m)), [token][groups]
+  int groups;
+  const int64_t* target;
+  float* tlogit;  // the target's logit, [token]
+
+  template <class P, int MF>
+  __device__ __forceinline__ void run(const TileOut<P, MF>& t, typename P::Acc (&acc)[P::TM][P::TN], int V,
+                                      int N) const {
+    const int group = t.m0 / P::WTM + t.wm;
+#pragma unroll
+    for (int j = 0; j < P::TN; ++j) {
+      const int tok = t.col(j);
+      const bool ok = tok < N;
+      int64_t want = ok ? target[tok] : -1;
+      if (want < 0 || want >= V) want = -1;
+      float m = -FLT_MAX;
+#pragma unroll
+      for (int i = 0; i < P::TM; ++i)
+#pragma unroll
+        for (int r = 0; r < P::ACC; ++r)
+          if (t.interior || t.row(i, r) < V) m = fmaxf(m, acc[i][j][r]);
+      if constexpr (MF == 16) m = fmaxf(m, __shfl_xor(m, 16));
+      m = fmaxf(m, __shfl_xor(m, 32));
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < P::TM; ++i)
+#pragma unroll
+        for (int q = 0; q < P::ACC / 4; ++q) {
+          const int v0 = t.row(i, 4 * q);
+          f16x4 h;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float l = acc[i][j][4 * q + c];
+            const float x = t.interior || v0 + c < V ? __expf(l - m) : 0.f;
+            s += x;
+            h[c] = (f16)(x * kScale16);
+            if (v0 + c == (int)want) tlogit[tok] = l;
+          }
+          if (e != nullptr && ok && v0 < lde)
+            *reinterpret_cast<i32x2*>(e + (int64_t)tok * lde + v0) = __builtin_bit_cast(i32x2, h);
+        }
+      if constexpr (MF == 16) s += __shfl_xor(s, 16);
+      s += __shfl_xor(s, 32);
+      if (t.lane < MF && ok) stat[(int64_t)tok * groups + group] = f32x2{m, s};
+    }
+  }
+};
+
+// A gradient, stored transposed: rows are the hidden dimension, columns
+// tokens (dx) or vocabulary entries (dW).  Over several chunks of rows dW is
+// added up in fp32 and rounded once, by the last.
+struct CeGrad {
+  u16* out;  // bf16, [column][ldo]; NULL: not the last chunk
+  int64_t ldo;
+  float* acc32;  // fp32 sums, [column][ld32]
+  int64_t ld32;
+  bool add;            // to what acc32 holds
+  const float* scale;  // applied when out is written
+
+  template <class P, int MF>
+  __device__ __forceinline__ void run(const TileOut<P, MF>& t, typename P::Acc (&acc)[P::TM][P::TN], int H,
+                                      int N) const {
+    const float f = out != nullptr ? *scale : 1.f;
+    const bool vec = ldo % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0;
+#pragma unroll
+    for (int j = 0; j < P::TN; ++j) {
+      const int n = t.col(j);
+#pragma unroll
+      for (int i = 0; i < P::TM; ++i)
+#pragma unroll
+        for (int q = 0; q < P::ACC / 4; ++q) {
+          const int h0 = t.row(i, 4 * q);
+          if (n >= N || h0 >= H) continue;
+          f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+          if (acc32 != nullptr) {  // ld32 is a multiple of 4
+            f32x4* p = reinterpret_cast<f32x4*>(acc32 + (int64_t)n * ld32 + h0);
+            if (add) v += *p;
+            if (out == nullptr) {
+              *p = v;
+              continue;
+            }
+          }
+          u16* o = out + (int64_t)n * ldo + h0;
+          u16 b[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) b[c] = bf16_bits(v[c] * f);
+          if (vec && h0 + 4 <= H) {
+            *reinterpret_cast<i32x2*>(o) = i32x2{(int)(b[0] | (uint32_t)b[1] << 16), (int)(b[2] | (uint32_t)b[3] << 16)};
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (h0 + c < H) o[c] = b[c];
+          }
+        }
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Kernels around the products
+// ---------------------------------------------------------------------------
+
+enum Reduction { kNone, kSum, kMean };
+
+// xs = x with the ignored rows cleared (whatever they hold must not reach dW,
+// where 0 times a NaN would be one) and rows padded with zeros to Hp; and, by
+// one more workgroup where `scale` is set, the scalar factor of the gradients.
+template <typename T>
+__global__ __launch_bounds__(256) void ce_prepare_kernel(const T* __restrict__ x, int64_t ldx, T* __restrict__ xs,
+                                                         int64_t Hp, int64_t N, int64_t H,
+                                                         const int64_t* __restrict__ target, int64_t ignore,
+                                                         float* __restrict__ scale, int64_t all,
+                                                         const int64_t* __restrict__ all_targets, int reduction,
+                                                         const float* __restrict__ grad_loss) {
+  constexpr int E = 16 / (int)sizeof(T);
+  typedef i32x4 __attribute__((aligned(2))) i32x4_any;
+  __shared__ int count[256];
+  if (scale != nullptr && blockIdx.x == gridDim.x - 1) {
+    int n = 0;
+    for (int64_t i = threadIdx.x; i < all; i += 256) n += all_targets[i] != ignore;
+    count[threadIdx.x] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int64_t c = 0;
+      for (int i = 0; i < 256; ++i) c += count[i];
+      float f = 1.f;
+      if (reduction != kNone && grad_loss != nullptr) f = *grad_loss;
+      if (reduction == kMean) f /= (float)(c > 1 ? c : 1);
+      *scale = f;
+    }
+    return;
+  }
+  const int64_t blocks = gridDim.x - (scale != nullptr ? 1 : 0);
+  const int64_t per_row = Hp / E;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < N * per_row; i += blocks * 256) {
+    const int64_t r = i / per_row, c = (i - r * per_row) * E;
+    i32x4 v = {0, 0, 0, 0};
+    if (target[r] != ignore) {
+      const T* p = x + r * ldx + c;
+      if (c + E <= H) {
+        v = *reinterpret_cast<const i32x4_any*>(p);
+      } else {
+#pragma unroll
+        for (int k = 0; k < E; ++k)
+          if (c + k < H) {
+            if constexpr (sizeof(T) == 4) v[k] = reinterpret_cast<const int*>(p)[k];
+            else v[k / 2] |= (int)((uint32_t)p[k] << (16 * (k & 1)));
+          }
+      }
+    }
+    *reinterpret_cast<i32x4*>(xs + r * Hp + c) = v;
+  }
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// fp32 logits: (m, sum of exp(l - m)) of each group of kGroup32 columns (grid
+// y) of each row (grid x), and the target's logit.
+constexpr int kGroup32 = 4096;
+
+__global__ __launch_bounds__(256) void ce_stats_kernel(const float* __restrict__ l, int64_t ldl, int64_t V,
+                                                       const int64_t* __restrict__ target, f32x2* __restrict__ stat,
+                                                       float* __restrict__ tlogit) {
+  __shared__ float red[2][4];
+  const int64_t r = blockIdx.x;
+  const int64_t v0 = (int64_t)blockIdx.y * kGroup32;
+  const float* row = l + r * ldl;
+  const int64_t want = target[r];
+  f32x4 w[4];
+  float m = -FLT_MAX;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int64_t v = v0 + 4 * (threadIdx.x + 256 * q);
+    w[q] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (v < V) w[q] = *reinterpret_cast<const f32x4*>(row + v);  // ldl is a multiple of 4
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if (v + c >= V) w[q][c] = -INFINITY;  // adds exp(-inf) = 0
+      if (v + c < V && v + c == want) tlogit[r] = w[q][c];
+      m = fmaxf(m, w[q][c]);
+    }
+  }
+  m = wave_max(m);
+  if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  float s = 0.f;
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) s += __expf(w[q][c] - m);
+  s = wave_sum(s);
+  if ((threadIdx.x & 63) == 0) red[1][threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    stat[r * gridDim.y + blockIdx.y] = f32x2{m, (red[1][0] + red[1][1]) + (red[1][2] + red[1][3])};
+}
+
+// One row (grid x) of a chunk: lse from its groups, the loss, and, where p is
+// set, d in place of what the row holds (grid y workgroups share a row).
+//   T = u16: exp(l - m) 2^15 in fp16 -> d in bf16, without the scalar factor.
+//   T = float: l -> d, with it.
+struct CeRows {
+  void* p;
+  int64_t ldp, V;
+  const f32x2* stat;
+  int groups, group_shift;  // columns of a group: 2^group_shift
+  const int64_t* target;
+  int64_t ignore;
+  const float* tlogit;
+  float* loss;             // [row]
+  const float* row_grad;   // per-row gradients of the losses, or NULL
+  const float* scale;      // (T = float)
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
+  __shared__ float red[2][4];
+  const int64_t r = blockIdx.x;
+  const int tid = threadIdx.x;
+  const int64_t want = a.target[r];
+  const bool ignored = want == a.ignore, bad = !ignored && (want < 0 || want >= a.V);
+  constexpr int E = sizeof(T) == 2 ? 8 : 4;
+  T* row = static_cast<T*>(a.p) + r * a.ldp;
+  if (ignored) {
+    if (a.loss != nullptr && blockIdx.y == 0 && tid == 0) a.loss[r] = 0.f;
+    if (a.p == nullptr) return;
+    for (int64_t v = E * ((int64_t)blockIdx.y * 256 + tid); v < a.ldp; v += E * 256 * (int64_t)gridDim.y)
+      *reinterpret_cast<i32x4*>(row + v) = i32x4{0, 0, 0, 0};
+    return;
+  }
+  const f32x2* stat = a.stat + r * a.groups;
+  float m = -FLT_MAX;
+  for (int g = tid; g < a.groups; g += 256) m = fmaxf(m, stat[g].x);
+  m = wave_max(m);
+  if ((tid & 63) == 0) red[0][tid >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  float s = 0.f;
+  for (int g = tid; g < a.groups; g += 256) s += stat[g].y * __expf(stat[g].x - m);
+  s = wave_sum(s);
+  if ((tid & 63) == 0) red[1][tid >> 6] = s;
+  __syncthreads();
+  s = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  const float lse = m + logf(s);
+  const float tl = bad ? NAN : a.tlogit[r];  // a target that is no class: NaN, in loss and gradients
+  if (a.loss != nullptr && blockIdx.y == 0 && tid == 0) a.loss[r] = lse - tl;
+  if (a.p == nullptr) return;
+  float g = a.row_grad != nullptr ? a.row_grad[r] : 1.f;
+  if (sizeof(T) == 4) g *= *a.scale;
+  if (bad) g = NAN;
+  const float at_target = expm1f(tl - lse) * g;
+  for (int64_t v = E * ((int64_t)blockIdx.y * 256 + tid); v < a.ldp; v += E * 256 * (int64_t)gridDim.y) {
+    float d[E];
+    if constexpr (sizeof(T) == 2) {
+      const f16x8 e = *reinterpret_cast<const f16x8*>(row + v);
+      const float f = __expf(stat[min(v, a.V - 1) >> a.group_shift].x - lse) * (1.f / kScale16);
+#pragma unroll
+      for (int c = 0; c < E; ++c) d[c] = (float)e[c] * f * g;  // zeros from V on
+    } else {
+      const f32x4 l = *reinterpret_cast<const f32x4*>(row + v);
+#pragma unroll
+      for (int c = 0; c < E; ++c) d[c] = v + c < a.V ? __expf(l[c] - lse) * g : 0.f;
+    }
+    if ((uint64_t)(want - v) < (uint64_t)E) {
+#pragma unroll
+      for (int c = 0; c < E; ++c) d[c] = v + c == want ? at_target : d[c];
+    }
+    i32x4 o;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[c] = (int)(bf16_bits(d[2 * c]) | (uint32_t)bf16_bits(d[2 * c + 1]) << 16);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[c] = __float_as_int(d[c]);
+    }
+    *reinterpret_cast<i32x4*>(row + v) = o;
+  }
+}
+
+// The sum or mean of the rows' losses, in 64 bits and a fixed order.
+__global__ __launch_bounds__(1024) void ce_loss_kernel(const float* __restrict__ rows,
+                                                       const int64_t* __restrict__ target, int64_t N, int64_t ignore,
+                                                       int reduction, float* __restrict__ loss) {
+  __shared__ double sum[1024];
+  __shared__ int count[1024];
+  double s = 0;
+  int n = 0;
+  for (int64_t i = threadIdx.x; i < N; i += 1024) {
+    s += (double)rows[i];
+    n += target[i] != ignore;
+  }
+  sum[threadIdx.x] = s;
+  count[threadIdx.x] = n;
+  for (int o = 512; o > 0; o >>= 1) {
+    __syncthreads();
+    if ((int)threadIdx.x < o) {
+      sum[threadIdx.x] += sum[threadIdx.x + o];
+      count[threadIdx.x] += count[threadIdx.x + o];
+    }
+  }
+  if (threadIdx.x == 0) *loss = (float)(reduction == kMean ? sum[0] / (double)max(count[0], 1) : sum[0]);
+}
+
+// acc += part, or acc = part.
+__global__ __launch_bounds__(256) void ce_add_kernel(float* __restrict__ acc, const float* __restrict__ part,
+                                                     int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) acc[i] += part[i];
+}
+
+// A gradient of no rows.
+__global__ __launch_bounds__(256) void ce_zero_kernel(unsigned char* __restrict__ p, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
+}
+
+// ---------------------------------------------------------------------------
+// The bf16 products
+// ---------------------------------------------------------------------------
+
+// Output tiles: 256 x 256 (8 waves) where there are enough of them for the
+// chip, 128 x 128 (8 waves) below, 128 x 64 (4 waves, two workgroups a CU)
+// for up to 64 columns.
+enum CeTile { kT256, kT128, kT64 };
+
+struct CeProduct {
+  CeTile tile;
+  int splits;
+};
+
+int64_t tiles_of(CeTile t, int64_t M, int64_t N) {
+  return t == kT256 ? cdiv(M, 256) * cdiv(N, 256) : t == kT128 ? cdiv(M, 128) * cdiv(N, 128) : cdiv(M, 128) * cdiv(N, 64);
+}
+
+// rows M x columns N, N the one that may be small.
+CeProduct choose(int64_t M, int64_t N, int64_t K, bool can_split) {
+  const int64_t cus = device_cus();
+  CeProduct c{N <= 64 ? kT64 : kT128, 1};
+  if (N > 64 && tiles_of(kT256, M, N) >= cus) c.tile = kT256;
+  if (!can_split || c.tile == kT256) return c;
+  const int64_t tiles = tiles_of(c.tile, M, N), places = c.tile == kT64 ? 2 * cus : cus;
+  int64_t s = std::min<int64_t>({places / std::max<int64_t>(tiles, 1), cdiv(K, 64) / 4, 32});
+  c.splits = (int)std::max<int64_t>(s, 1);
+  return c;
+}
+
+size_t split_workspace(const CeProduct& c, int64_t M, int64_t N) {
+  const int64_t cells = c.tile == kT128 ? 128 * 128 : 128 * 64;
+  return c.splits > 1 ? (size_t)(c.splits * tiles_of(c.tile, M, N) * cells) * sizeof(float) : 0;
+}
+size_t split_counters(const CeProduct& c, int64_t M, int64_t N) {
+  return c.splits > 1 ? (size_t)tiles_of(c.tile, M, N) * kSplitCounterStride * sizeof(unsigned) : 0;
+}
+
+struct Operands {
+  const u16 *a, *b;
+  int64_t lda, ldb;
+  int64_t M, N, K;
+};
+
+template <int BM, int BN, int NBUF, int WM, int WN, KMask KM, bool CA, bool CB, int MF, class Epi>
+hipError_t run_tile(const Operands& o, const Epi& epi, int splits, float* ws, unsigned* counters, hipStream_t stream) {
+  using P = LdsGemm<BM, BN, 64, NBUF, WM, WN, CA, CB, MF>;
+  const int64_t tiles = cdiv(o.M, BM) * cdiv(o.N, BN);
+  const SplitGeom g = gemm_split_geom(o.K, 64, splits);
+  if (g.splits > 1 && P::TM * P::TN * P::ACC > kSplitMaxAccPerThread) return hipErrorInvalidConfiguration;
+  auto kern = gemm_bf16_lds_kernel<BM, BN, 64, NBUF, WM, WN, KM, CA, CB, MF, Epi>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)tiles, (unsigned)g.splits), dim3(P::NT), 0, stream, o.a, o.b, epi, (int)o.M,
+                     (int)o.N, (int)o.K, o.lda, o.ldb, 4, device_xcds(), (int)g.steps, ws, counters);
+  return hipGetLastError();
+}
+
+template <KMask KM, bool CA, bool CB, int MF, class Epi>
+hipError_t run_product(const Operands& o, const Epi& epi, const CeProduct& c, float* ws, unsigned* counters,
+                       hipStream_t stream) {
+  if (c.tile == kT256) return run_tile<256, 256, 2, 2, 4, KM, CA, CB, MF>(o, epi, c.splits, ws, counters, stream);
+  if (c.tile == kT128) return run_tile<128, 128, 4, 2, 4, KM, CA, CB, MF>(o, epi, c.splits, ws, counters, stream);
+  return run_tile<128, 64, 3, 2, 2, KM, CA, CB, MF>(o, epi, c.splits, ws, counters, stream);
+}
+
+// Vocabulary entries of a wave's group in the logits' product.
+int group_shift(CeTile t) { return t == kT256 ? 7 : 6; }
+
+// ---------------------------------------------------------------------------
+// Plan: chunking and where everything lies in the workspace
+// ---------------------------------------------------------------------------
+
+constexpr int64_t kChunkBytes = int64_t(2) << 30;  // of the values kept for the gradients
+constexpr int64_t kMaxChunkRows = int64_t(1) << 22;  // a workgroup a row: within the grid's 2^32 threads
+constexpr int64_t kMaxVocab = (int64_t(1) << 22) - 64;
+
+struct CeArgs {
+  const void *x, *w;
+  const int64_t* target;
+  float* loss;
+  const float* grad_loss;
+  void *dx, *dw;
+  int64_t N, H, V, ldx, ldw;
+  int dtype, reduction;
+  int64_t ignore;
+  bool grad;
+  int64_t chunk_rows;
+};
+
+struct CePlan {
+  int64_t R, chunks;     // rows of a chunk
+  int64_t Vp, Hp;        // padded row lengths of the kept values, of xs / wp
+  bool pad;              // bf16: operands copied with padded rows
+  bool copy_x;
+  int groups, shift;
+  CeProduct p1, p2, p3;  // bf16
+  size_t stat, tlogit, rows, scale, xs, wp, keep, acc, split;  // offsets
+  size_t split_bytes, bytes, counter_bytes;
+};
+
+size_t matmul_scratch(const CeArgs& a, int64_t M, int64_t N, int64_t K, int64_t ld1, int64_t ld2, int layout,
+                      size_t* counters) {
+  size_t ws = 0, cnt = 0;
+  if (tilec_matmul_scratch_bytes(M, N, K, ld1, ld2, layout, a.dtype, TILEC_VARIANT_AUTO, 0, &ws, &cnt) != TILEC_OK)
+    return 0;
+  *counters = std::max(*counters, cnt);
+  return ws;
+}
+
+CePlan make_plan(const CeArgs& a) {
+  CePlan p{};
+  const bool bf16 = a.dtype == TILEC_BF16;
+  const int64_t esz = bf16 ? 2 : 4;
+  p.Vp = bf16 ? cdiv(a.V, 64) * 64 : cdiv(a.V, 4) * 4;
+  // bf16 losses keep nothing but their groups' sums; fp32 losses go through
+  // the chunk's logits.
+  const int64_t row_bytes = p.Vp * (a.grad || !bf16 ? esz : 1);
+  p.R = std::max<int64_t>(256, kChunkBytes / row_bytes / 256 * 256);
+  if (a.chunk_rows > 0) p.R = a.chunk_rows;
+  p.R = std::min({a.N, p.R, kMaxChunkRows});
+  p.chunks = cdiv(a.N, p.R);
+  p.Hp = a.H;
+  if (bf16) {
+    auto fits = [&](const void* q, int64_t ld) {
+      return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % 8 == 0 && ld < (int64_t(1) << 22);
+    };
+    p.pad = a.H % 8 != 0 || !fits(a.w, a.ldw) || !fits(a.x, a.ldx);
+    if (p.pad) p.Hp = cdiv(a.H, 64) * 64;
+    p.p1 = choose(a.V, p.R, p.Hp, false);
+    p.p2 = choose(a.H, p.R, a.V, true);
+    p.p3 = choose(a.H, a.V, p.R, true);
+    p.shift = group_shift(p.p1.tile);
+    // A tile's groups are all written, those past the vocabulary's end too.
+    const int64_t bm = p.p1.tile == kT256 ? 256 : 128;
+    p.groups = (int)(cdiv(a.V, bm) * bm >> p.shift);
+  } else {
+    p.shift = 12;
+    p.groups = (int)cdiv(a.V, kGroup32);
+  }
+  p.copy_x = a.grad || p.pad;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  p.stat = take((size_t)(p.R * p.groups) * sizeof(f32x2));
+  p.tlogit = take((size_t)p.R * sizeof(float));
+  p.rows = take(a.reduction == kNone ? 0 : (size_t)a.N * sizeof(float));
+  p.scale = take(sizeof(float));
+  p.xs = take(p.copy_x ? (size_t)(p.R * (bf16 ? p.Hp : cdiv(a.H, 4) * 4) * esz) : 0);
+  p.wp = take(p.pad ? (size_t)(a.V * p.Hp * esz) : 0);
+  p.keep = take(a.grad || !bf16 ? (size_t)(p.R * p.Vp * esz) : 0);
+  p.acc = take(a.grad && p.chunks > 1 ? (size_t)(a.V * cdiv(a.H, 4) * 4) * sizeof(float) : 0);
+  if (bf16) {
+    if (a.grad) {
+      p.split_bytes = std::max(split_workspace(p.p2, a.H, p.R), split_workspace(p.p3, a.H, a.V));
+      p.counter_bytes = std::max(split_counters(p.p2, a.H, p.R), split_counters(p.p3, a.H, a.V));
+    }
+  } else {
+    const int64_t ldxs = p.copy_x ? cdiv(a.H, 4) * 4 : a.ldx;
+    for (const int64_t R : {p.R, a.N - (p.chunks - 1) * p.R}) {
+      p.split_bytes = std::max(
+          p.split_bytes, matmul_scratch(a, R, a.V, a.H, ldxs, a.ldw, TILEC_X2_COL_MAJOR, &p.counter_bytes));
+      if (!a.grad) continue;
+      p.split_bytes = std::max(p.split_bytes, matmul_scratch(a, R, a.H, a.V, p.Vp, a.ldw, 0, &p.counter_bytes));
+      p.split_bytes = std::max(p.split_bytes, matmul_scratch(a, a.V, a.H, R, p.Vp, ldxs, TILEC_X1_COL_MAJOR,
+                                                             &p.counter_bytes));
+    }
+  }
+  p.split = take(p.split_bytes);
+  p.bytes = at;
+  return p;
+}
+
+unsigned grid_for(int64_t n) { return (unsigned)std::min<int64_t>(std::max<int64_t>(cdiv(n, 256), 1), 1 << 16); }
+
+#define CE_TRY(call)                  \
+  do {                                \
+    const hipError_t e_ = (call);     \
+    if (e_ != hipSuccess) return e_;  \
+  } while (0)
+
+// The kernels around the products of one chunk.
+template <typename T>
+hipError_t run_prepare(const CeArgs& a, const CePlan& p, char* ws, int64_t r0, int64_t R, hipStream_t stream) {
+  if (!p.copy_x) return hipSuccess;
+  const int64_t ld = sizeof(T) == 2 ? p.Hp : cdiv(a.H, 4) * 4;
+  const bool count = a.grad && r0 == 0;
+  const unsigned blocks = grid_for(R * ld / (16 / (int64_t)sizeof(T)));
+  hipLaunchKernelGGL((ce_prepare_kernel<T>), dim3(blocks + (count ? 1 : 0)), dim3(256), 0, stream,
+                     static_cast<const T*>(a.x) + r0 * a.ldx, a.ldx, reinterpret_cast<T*>(ws + p.xs), ld, R, a.H,
+                     a.target + r0, a.ignore, count ? reinterpret_cast<float*>(ws + p.scale) : nullptr, a.N, a.target,
+                     a.reduction, a.grad_loss);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t run_rows(const CeArgs& a, const CePlan& p, char* ws, int64_t r0, int64_t R, hipStream_t stream) {
+  CeRows q{};
+  q.p = a.grad ? ws + p.keep : nullptr;
+  q.ldp = p.Vp, q.V = a.V;
+  q.stat = reinterpret_cast<const f32x2*>(ws + p.stat);
+  q.groups = p.groups, q.group_shift = p.shift;
+  q.target = a.target + r0, q.ignore = a.ignore;
+  q.tlogit = reinterpret_cast<const float*>(ws + p.tlogit);
+  q.loss = (a.reduction == kNone ? a.loss : reinterpret_cast<float*>(ws + p.rows)) + r0;
+  q.row_grad = a.reduction == kNone && a.grad_loss != nullptr ? a.grad_loss + r0 : nullptr;
+  q.scale = reinterpret_cast<const float*>(ws + p.scale);
+  // Workgroups that share a row each join its groups again: only as many as
+  // it takes to fill the chip.
+  const int64_t want = cdiv(4 * (int64_t)device_cus(), R), most = cdiv(p.Vp, 256 * 16 / (int64_t)sizeof(T));
+  const unsigned share = a.grad ? (unsigned)std::max<int64_t>(1, std::min(want, most)) : 1;
+  hipLaunchKernelGGL((ce_rows_kernel<T>), dim3((unsigned)R, share), dim3(256), 0, stream, q);
+  return hipGetLastError();
+}
+
+hipError_t run_bf16(const CeArgs& a, const CePlan& p, char* ws, unsigned* counters, hipStream_t stream) {
+  const u16 *x = static_cast<const u16*>(a.x), *w = static_cast<const u16*>(a.w);
+  u16* xs = reinterpret_cast<u16*>(ws + p.xs);
+  u16* keep = reinterpret_cast<u16*>(ws + p.keep);
+  float* split = reinterpret_cast<float*>(ws + p.split);
+  const float* scale = reinterpret_cast<const float*>(ws + p.scale);
+  int64_t ldw = a.ldw;
+  if (p.pad) {
+    u16* wp = reinterpret_cast<u16*>(ws + p.wp);
+    CE_TRY(pad_copy<2>(w, wp, a.V, a.H, a.ldw, a.V, p.Hp, w, wp, 0, 0, a.ldw, 0, 0, stream));
+    w = wp, ldw = p.Hp;
+  }
+  for (int64_t c = 0; c < p.chunks; ++c) {
+    const int64_t r0 = c * p.R, R = std::min(p.R, a.N - r0);
+    CE_TRY(run_prepare<u16>(a, p, ws, r0, R, stream));
+    const u16* xc = p.copy_x ? xs : x + r0 * a.ldx;
+    const int64_t ldx = p.copy_x ? p.Hp : a.ldx;
+    CeLogits le{a.grad ? keep : nullptr,
+                p.Vp,
+                reinterpret_cast<f32x2*>(ws + p.stat),
+                p.groups,
+                a.target + r0,
+                reinterpret_cast<float*>(ws + p.tlogit)};
+    const Operands o1{w, xc, ldw, ldx, a.V, R, p.Hp};
+    CE_TRY(p.Hp % 64 == 0
+               ? (run_product<kKFull, false, true, 16>(o1, le, p.p1, nullptr, nullptr, stream))
+               : (run_product<kKMasked, false, true, 32>(o1, le, p.p1, nullptr, nullptr, stream)));
+    CE_TRY(run_rows<u16>(a, p, ws, r0, R, stream));
+    if (!a.grad) continue;
+    // dx^T [H, R] = W^T d^T over the vocabulary; d is padded with zeros to
+    // whole K steps, W ends with its rows.
+    CeGrad gx{static_cast<u16*>(a.dx) + r0 * a.H, a.H, nullptr, 0, false, scale};
+    CE_TRY((run_product<kKRows, true, true, 16>(Operands{w, keep, ldw, p.Vp, a.H, R, a.V}, gx, p.p2, split, counters,
+                                                stream)));
+    // dW^T [H, V] = x^T d over the chunk's rows.
+    const bool last = c + 1 == p.chunks;
+    CeGrad gw{last ? static_cast<u16*>(a.dw) : nullptr, a.H, p.chunks > 1 ? reinterpret_cast<float*>(ws + p.acc) : nullptr,
+              cdiv(a.H, 4) * 4, c > 0, scale};
+    CE_TRY((run_product<kKRows, true, false, 16>(Operands{xs, keep, p.Hp, p.Vp, a.H, a.V, R}, gw, p.p3, split,
+                                                 counters, stream)));
+  }
+  return hipSuccess;
+}
+
+int run_f32(const CeArgs& a, const CePlan& p, char* ws, unsigned* counters, size_t counter_bytes, hipStream_t stream,
+            hipError_t* err) {
+  const float *x = static_cast<const float*>(a.x), *w = static_cast<const float*>(a.w);
+  float* xs = reinterpret_cast<float*>(ws + p.xs);
+  float* keep = reinterpret_cast<float*>(ws + p.keep);
+  float* part = reinterpret_cast<float*>(ws + p.acc);
+  const int64_t ldxs = cdiv(a.H, 4) * 4;
+  auto product = [&](const float* x1, const float* x2, float* out, int64_t M, int64_t N, int64_t K, int64_t ld1,
+                     int64_t ld2, int64_t ldo, int layout) {
+    return tilec_matmul(x1, x2, out, M, N, K, ld1, ld2, ldo, layout, TILEC_F32, TILEC_VARIANT_AUTO, 0, ws + p.split,
+                        p.split_bytes, counters, counter_bytes, stream);
+  };
+  for (int64_t c = 0; c < p.chunks; ++c) {
+    const int64_t r0 = c * p.R, R = std::min(p.R, a.N - r0);
+    if ((*err = run_prepare<float>(a, p, ws, r0, R, stream)) != hipSuccess) return TILEC_ERR_HIP;
+    const float* xc = p.copy_x ? xs : x + r0 * a.ldx;
+    const int64_t ldx = p.copy_x ? ldxs : a.ldx;
+    int rc = product(xc, w, keep, R, a.V, a.H, ldx, a.ldw, p.Vp, TILEC_X2_COL_MAJOR);
+    if (rc != TILEC_OK) return rc;
+    hipLaunchKernelGGL(ce_stats_kernel, dim3((unsigned)R, (unsigned)p.groups), dim3(256), 0, stream, keep, p.Vp, a.V,
+                       a.target + r0, reinterpret_cast<f32x2*>(ws + p.stat), reinterpret_cast<float*>(ws + p.tlogit));
+    if ((*err = hipGetLastError()) != hipSuccess) return TILEC_ERR_HIP;
+    if ((*err = run_rows<float>(a, p, ws, r0, R, stream)) != hipSuccess) return TILEC_ERR_HIP;
+    if (!a.grad) continue;
+    rc = product(keep, w, static_cast<float*>(a.dx) + r0 * a.H, R, a.H, a.V, p.Vp, a.ldw, a.H, 0);
+    if (rc != TILEC_OK) return rc;
+    float* dw = static_cast<float*>(a.dw);
+    rc = product(keep, xs, c == 0 ? dw : part, a.V, a.H, R, p.Vp, ldxs, a.H, TILEC_X1_COL_MAJOR);
+    if (rc != TILEC_OK) return rc;
+    if (c == 0) continue;
+    hipLaunchKernelGGL(ce_add_kernel, dim3(grid_for(a.V * a.H)), dim3(256), 0, stream, dw, part, a.V * a.H);
+    if ((*err = hipGetLastError()) != hipSuccess) return TILEC_ERR_HIP;
+  }
+  return TILEC_OK;
+}
+
+int check(const CeArgs& a) {
+  if (a.dtype != TILEC_F32 && a.dtype != TILEC_BF16)
+    return fail(TILEC_ERR_TYPE, "tilec: linear cross entropy: unsupported dtype code %d (use float32 or bfloat16)",
+                a.dtype);
+  if (a.N < 0 || a.H < 1 || a.V < 1 || a.N > kMaxDim || a.H > kMaxDim || a.V > kMaxDim)
+    return fail(TILEC_ERR_VALUE, "tilec: linear cross entropy: bad shape N=%lld H=%lld V=%lld", (long long)a.N,
+                (long long)a.H, (long long)a.V);
+  if (a.reduction < kNone || a.reduction > kMean)
+    return fail(TILEC_ERR_VALUE, "tilec: linear cross entropy: unknown reduction %d", a.reduction);
+  if (a.ldw < a.H || (a.N > 1 && a.ldx < a.H) || a.ldw > (int64_t(1) << 40) || a.ldx > (int64_t(1) << 40))
+    return fail(TILEC_ERR_VALUE, "tilec: linear cross entropy: bad row strides ldx=%lld ldw=%lld for H=%lld",
+                (long long)a.ldx, (long long)a.ldw, (long long)a.H);
+  if (a.chunk_rows < 0)
+    return fail(TILEC_ERR_VALUE, "tilec: linear cross entropy: chunk_rows=%lld < 0", (long long)a.chunk_rows);
+  if (a.dtype == TILEC_BF16 && (a.V > kMaxVocab || a.H > kMaxVocab))
+    return fail(TILEC_ERR_UNSUPPORTED, "tilec: linear cross entropy: bf16 takes V and H up to %lld (got %lld, %lld)",
+                (long long)kMaxVocab, (long long)a.V, (long long)a.H);
+  if (cdiv(a.V, kGroup32) > 65535)
+    return fail(TILEC_ERR_UNSUPPORTED, "tilec: linear cross entropy: V=%lld is too large", (long long)a.V);
+  return TILEC_OK;
+}
+
+}  // namespace
+
+}  // namespace tilec
+
+using namespace tilec;
+
+extern "C" {
+
+int tilec_linear_ce_scratch_bytes(const void* x, const void* weight, int64_t N, int64_t H, int64_t V, int64_t ldx,
+                                  int64_t ldw, int32_t dtype, int32_t reduction, int32_t grad, int64_t chunk_rows,
+                                  size_t* workspace_bytes, size_t* counter_bytes) {
+  clear_error();
+  if (workspace_bytes) *workspace_bytes = 0;
+  if (counter_bytes) *counter_bytes = 0;
+  CeArgs a{};
+  a.x = x, a.w = weight, a.N = N, a.H = H, a.V = V, a.ldx = ldx, a.ldw = ldw, a.dtype = dtype;
+  a.reduction = reduction, a.grad = grad != 0, a.chunk_rows = chunk_rows;
+  const int rc = check(a);
+  if (rc != TILEC_OK || N == 0) return rc;
+  const CePlan p = make_plan(a);
+  clear_error();
+  if (workspace_bytes) *workspace_bytes = p.bytes;
+  if (counter_bytes) *counter_bytes = p.counter_bytes;
+  return TILEC_OK;
+}
+
+int tilec_linear_ce(const void* x, const void* weight, const int64_t* target, float* loss, const float* grad_loss,
+                    void* dx, void* dweight, int64_t N, int64_t H, int64_t V, int64_t ldx, int64_t ldw, int32_t dtype,
+                    int32_t reduction, int64_t ignore_index, int32_t grad, int64_t chunk_rows, void* workspace,
+                    size_t workspace_bytes, void* counters, size_t counter_bytes, void* stream_ptr) {
+  clear_error();
+  CeArgs a{};
+  a.x = x, a.w = weight, a.target = target, a.loss = loss, a.grad_loss = grad_loss, a.dx = dx, a.dw = dweight;
+  a.N = N, a.H = H, a.V = V, a.ldx = ldx, a.ldw = ldw, a.dtype = dtype, a.reduction = reduction;
+  a.ignore = ignore_index, a.grad = grad != 0, a.chunk_rows = chunk_rows;
+  int rc = check(a);
+  if (rc != TILEC_OK) return rc;
+  if (a.grad && dweight == nullptr) return fail(TILEC_ERR_VALUE, "tilec: linear cross entropy: dweight is NULL");
+  if (loss == nullptr && (N > 0 || reduction != kNone))
+    return fail(TILEC_ERR_VALUE, "tilec: linear cross entropy: loss is NULL");
+  hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
+  hipError_t e = hipSuccess;
+  auto launched = [&](hipError_t err) {
+    return err == hipSuccess ? (int)TILEC_OK
+                             : fail(TILEC_ERR_HIP, "tilec: launching the linear cross entropy failed: %s",
+                                    hipGetErrorString(err));
+  };
+  if (N > 0) {
+    if (x == nullptr || weight == nullptr || target == nullptr || (a.grad && dx == nullptr))
+      return fail(TILEC_ERR_VALUE, "tilec: linear cross entropy: x/weight/target/dx is NULL");
+    const CePlan p = make_plan(a);
+    clear_error();
+    if (workspace == nullptr || workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+      return fail(TILEC_ERR_WORKSPACE, "tilec: linear cross entropy needs %zu workspace bytes, 16-byte aligned (got %zu)",
+                  p.bytes, workspace == nullptr ? (size_t)0 : workspace_bytes);
+    if (p.counter_bytes > 0 && (counters == nullptr || counter_bytes < p.counter_bytes))
+      return fail(TILEC_ERR_WORKSPACE, "tilec: linear cross entropy needs %zu bytes of counters (got %zu)",
+                  p.counter_bytes, counters == nullptr ? (size_t)0 : counter_bytes);
+    char* ws = static_cast<char*>(workspace);
+    if (dtype == TILEC_BF16) {
+      e = run_bf16(a, p, ws, static_cast<unsigned*>(counters), stream);
+      if (e != hipSuccess) return launched(e);
+    } else {
+      rc = run_f32(a, p, ws, static_cast<unsigned*>(counters), counter_bytes, stream, &e);
+      if (rc != TILEC_OK) return e != hipSuccess ? launched(e) : rc;
+    }
+    if (reduction != kNone) {
+      hipLaunchKernelGGL(ce_loss_kernel, dim3(1), dim3(1024), 0, stream, reinterpret_cast<const float*>(ws + p.rows),
+                         target, N, ignore_index, reduction, loss);
+      e = hipGetLastError();
+    }
+    return launched(e);
+  }
+  // No rows: a loss of 0 and a gradient of zeros.
+  if (reduction != kNone) {
+    hipLaunchKernelGGL(ce_zero_kernel, dim3(1), dim3(256), 0, stream, reinterpret_cast<unsigned char*>(loss),
+                       (int64_t)sizeof(float));
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess && a.grad) {
+    const int64_t n = V * H * (dtype == TILEC_BF16 ? 2 : 4);
+    hipLaunchKernelGGL(ce_zero_kernel, dim3(grid_for(n)), dim3(256), 0, stream, static_cast<unsigned char*>(dweight), n);
+    e = hipGetLastError();
+  }
+  return launched(e);
+}
+
+}  // extern "C"

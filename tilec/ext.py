@@ -537,6 +537,7 @@ def sum(x, axis=1):
 
 # The training operators (training.py) are part of this module's API; they use
 # the buffers above, so they come last.
-from .training import layer_norm, layer_norm_backward  # noqa: E402
+from . import training as _training  # noqa: E402
+from .training import *  # noqa: E402,F401,F403
 
-__all__ += ["layer_norm", "layer_norm_backward"]
+__all__ += _training.__all__

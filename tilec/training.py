@@ -10,12 +10,14 @@ scratch is the (device, stream) workspace of `ext`, and nothing synchronises.
 Like those two they are plain functions with no autograd of their own.
 """
 
+import ctypes
+
 import torch
 
 from . import _lib
-from .ext import workspace_for
+from .ext import counters_for, workspace_for
 
-__all__ = ["layer_norm", "layer_norm_backward"]
+__all__ = ["layer_norm", "layer_norm_backward", "linear_cross_entropy", "linear_cross_entropy_grad"]
 
 _CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
@@ -169,3 +171,91 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, param_grads=True):
             dy.data_ptr(), x.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _ptr(weight), dx.data_ptr(), _ptr(dw),
             _ptr(db), R, D, lddy, ldx, D, x_code, y_code, w_code, ws_ptr, need, stream))
     return dx, dw, db
+
+
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
+def _linear_ce(what, x, weight, target, reduction, ignore_index, grad, grad_loss, chunk_rows):
+    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
+        raise ValueError(f"{what}: expected x [N, H] and weight [V, H], got shapes {tuple(x.shape)} and "
+                         f"{tuple(weight.shape)}")
+    N, H = x.shape
+    V = weight.shape[0]
+    if H == 0 or V == 0:
+        raise ValueError(f"{what}: no features or no classes (x {tuple(x.shape)}, weight {tuple(weight.shape)})")
+    if tuple(target.shape) != (N,):
+        raise ValueError(f"{what}: target has shape {tuple(target.shape)}, expected ({N},)")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"{what}: reduction must be one of {sorted(_REDUCTIONS)} (got {reduction!r})")
+    if chunk_rows < 0:
+        raise ValueError(f"{what}: chunk_rows must be >= 0 (got {chunk_rows})")
+    dtype = _code(what, x)
+    if weight.dtype != x.dtype:
+        raise TypeError(f"{what}: x has dtype {x.dtype}, weight {weight.dtype}")
+    if target.dtype != torch.int64:
+        raise TypeError(f"{what}: target has dtype {target.dtype}, expected torch.int64")
+    _on_gpu(what, x, weight, target, grad_loss)
+    if grad_loss is not None:
+        want = (N,) if reduction == "none" else ()
+        if grad_loss.dtype != torch.float32:
+            raise TypeError(f"{what}: grad_loss has dtype {grad_loss.dtype}, expected torch.float32")
+        if tuple(grad_loss.shape) != want and not (want == () and tuple(grad_loss.shape) == (1,)):
+            raise ValueError(f"{what}: grad_loss has shape {tuple(grad_loss.shape)}, expected {want}")
+        grad_loss = grad_loss.contiguous()
+    x, ldx = _rows(what, "x", x)
+    weight, ldw = _rows(what, "weight", weight)
+    target = target.contiguous()
+    loss = torch.empty((N,) if reduction == "none" else (), dtype=torch.float32, device=x.device)
+    dx = torch.empty((N, H), dtype=x.dtype, device=x.device) if grad else None
+    dw = torch.empty((V, H), dtype=x.dtype, device=x.device) if grad else None
+    L = _lib.lib()
+    code = _REDUCTIONS[reduction]
+    with _on(x.device):
+        stream = _stream(x.device)
+        ws, cnt = ctypes.c_size_t(0), ctypes.c_size_t(0)
+        _lib.check(L.tilec_linear_ce_scratch_bytes(x.data_ptr(), weight.data_ptr(), N, H, V, ldx, ldw, dtype, code,
+                                                   grad, chunk_rows, ctypes.byref(ws), ctypes.byref(cnt)))
+        ws_ptr = workspace_for(x.device, stream, ws.value).data_ptr() if ws.value else None
+        cnt_ptr = counters_for(x.device, stream, cnt.value).data_ptr() if cnt.value else None
+        _lib.check(L.tilec_linear_ce(x.data_ptr(), weight.data_ptr(), target.data_ptr(), loss.data_ptr(),
+                                     _ptr(grad_loss), _ptr(dx), _ptr(dw), N, H, V, ldx, ldw, dtype, code,
+                                     int(ignore_index), grad, chunk_rows, ws_ptr, ws.value, cnt_ptr, cnt.value,
+                                     stream))
+    return loss, dx, dw
+
+
+def linear_cross_entropy(x, weight, target, reduction="mean", ignore_index=-100):
+    """Cross entropy of the logits x @ weight.T against `target`, without
+    keeping the logits.
+
+        loss_r = log(sum_v exp(logits[r, v])) - logits[r, target_r]
+
+    x [N, H], weight [V, H]: both float32 or both bfloat16 (row-strided views
+    are read in place).  target: int64 [N].  Returns float32: the N losses
+    (reduction "none"), or their "sum" or "mean" over the rows that count.
+    Rows whose target is `ignore_index` do not: their loss is 0, whatever x
+    holds there, and a mean over no rows is 0.  A target that is neither that
+    nor a class makes its loss NaN (nothing here reads the device back to
+    raise for it).
+    """
+    return _linear_ce("linear_cross_entropy", x, weight, target, reduction, ignore_index, 0, None, 0)[0]
+
+
+def linear_cross_entropy_grad(x, weight, target, reduction="mean", ignore_index=-100, grad_loss=None, chunk_rows=0):
+    """(loss, dx, dweight): `linear_cross_entropy` with its gradients, in x's
+    type, from one pass over the logits.
+
+        d[r, v] = g_r * (softmax(logits)[r, v] - [v = target_r]);  dx = d @ weight;  dweight = d.T @ x
+
+    grad_loss: the gradient of the loss on the GPU, float32: one value for
+    "mean" and "sum", [N] for "none"; None: ones.  Ignored rows add nothing,
+    whatever x holds there, and get a dx of zeros.
+
+    Of the logits, one 16-bit value each (float32 inputs: 32-bit) is kept for
+    a chunk of rows at a time, `chunk_rows` of them, or by default as many as
+    fit 2 GiB of workspace; with more than one chunk, dweight is added up in a
+    float32 workspace of its size.
+    """
+    return _linear_ce("linear_cross_entropy_grad", x, weight, target, reduction, ignore_index, 1, grad_loss,
+                      chunk_rows)
