@@ -305,9 +305,9 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void gemm_bf16_lds_kernel(
   const int64_t a_step = !CA ? BK : (int64_t)BK * lda;
   const int64_t b_step = CB ? BK : (int64_t)BK * ldb;
   auto op_recs = [&](bool kcontig, int64_t ld, int k0, bool live) -> uint32_t {
-    if (!live) return 0u;
-    if (!KFULL && !kcontig) return (uint32_t)min<int64_t>((int64_t)(K - k0) * ld * 2, 0x7FFFFFFF);
-    return 0x7FFFFFFFu;
+    // (32-bit and without a branch: one would split the step's schedule)
+    if (!KFULL && !kcontig) return (uint32_t)min(live ? K - k0 : 0, BK) * ((uint32_t)ld * 2u);
+    return live ? 0x7FFFFFFFu : 0u;
   };
   // The resources of step kt (the next step to copy); each advances its base.
   // Every input is wave-uniform; they go through readfirstlane so the
