@@ -307,6 +307,43 @@ int tilec_linear_ce_scratch_bytes(const void* x, const void* weight, int64_t N, 
                                   int64_t ldx, int64_t ldw, int32_t dtype, int32_t reduction, int32_t grad,
                                   int64_t chunk_rows, size_t* workspace_bytes, size_t* counter_bytes);
 
+/*
+ * One AdamW step over `count` tensors, in place:
+ *   g = grad * grad_scale;  p = p (1 - lr weight_decay)
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   p = p - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * with `step` counted from 1 and grad_scale one float32 on the device (NULL:
+ * 1).  The descriptions in `tensors` (host memory) are read before the call
+ * returns.  Every tensor is contiguous, of n elements, at any alignment of
+ * its element type; no two of them may overlap.
+ *
+ * state_bits 32: exp_avg and exp_avg_sq are float32 [n].  state_bits 8: they
+ * are codes, int8 and uint8 [n], with one float32 scale per 256 consecutive
+ * elements (ceil(n / 256) of them), the block's largest magnitude:
+ *   m = sign(c) (c / 127)^2 scale        v = (c / 255)^4 scale
+ * Zero codes and scales are zero states.
+ */
+typedef struct tilec_adamw_tensor {
+  void* param;              /* float32 or bfloat16 [n], read and written     */
+  const void* grad;         /* float32 or bfloat16 [n]                       */
+  void* exp_avg;            /* m                                             */
+  void* exp_avg_sq;         /* v                                             */
+  float* exp_avg_scale;     /* state_bits 8                                  */
+  float* exp_avg_sq_scale;  /* state_bits 8                                  */
+  void* copy;               /* bfloat16 [n] that gets the new param, or NULL */
+  int64_t n;
+  int32_t param_dtype, grad_dtype;
+} tilec_adamw_tensor;
+int tilec_adamw(const tilec_adamw_tensor* tensors, int32_t count, int32_t state_bits, int64_t step, double lr,
+                double beta1, double beta2, double eps, double weight_decay, const float* grad_scale, void* stream);
+
+/*
+ * The float32 values that 8-bit states stand for, into `param` [n] of each
+ * description: of exp_avg with its scales, or, where exp_avg is NULL, of
+ * exp_avg_sq.
+ */
+int tilec_adamw_values(const tilec_adamw_tensor* tensors, int32_t count, void* stream);
+
 /* Message describing the last failure on this thread ("" if none). */
 const char* tilec_last_error(void);
 

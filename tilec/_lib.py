@@ -23,6 +23,7 @@ VARIANT_AUTO = -1
 
 # Every function include/tilec.h declares: name -> (restype, argtypes).
 _i64, _i32, _vp, _sz = ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_size_t
+_f64 = ctypes.c_double
 SIGNATURES = {
     "tilec_matmul": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32,
                                     _i32, _i32, _i32, _vp, _sz, _vp, _sz, _vp]),
@@ -50,6 +51,8 @@ SIGNATURES = {
                                        _i64, _i32, _i64, _vp, _sz, _vp, _sz, _vp]),
     "tilec_linear_ce_scratch_bytes": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i64,
                                                      ctypes.POINTER(_sz), ctypes.POINTER(_sz)]),
+    "tilec_adamw": (ctypes.c_int, [_vp, _i32, _i32, _i64, _f64, _f64, _f64, _f64, _f64, _vp, _vp]),
+    "tilec_adamw_values": (ctypes.c_int, [_vp, _i32, _vp]),
     "tilec_last_error": (ctypes.c_char_p, []),
     "tilec_version": (_i32, []),
 }

@@ -10,6 +10,7 @@ scratch is the (device, stream) workspace of `ext`, and nothing synchronises.
 Like those two they are plain functions with no autograd of their own.
 """
 
+import array
 import ctypes
 
 import torch
@@ -17,7 +18,8 @@ import torch
 from . import _lib
 from .ext import counters_for, workspace_for
 
-__all__ = ["layer_norm", "layer_norm_backward", "linear_cross_entropy", "linear_cross_entropy_grad"]
+__all__ = ["layer_norm", "layer_norm_backward", "linear_cross_entropy", "linear_cross_entropy_grad",
+           "adamw_state", "adamw_step", "adamw_values", "ADAMW_BLOCK"]
 
 _CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
@@ -259,3 +261,156 @@ def linear_cross_entropy_grad(x, weight, target, reduction="mean", ignore_index=
     """
     return _linear_ce("linear_cross_entropy_grad", x, weight, target, reduction, ignore_index, 1, grad_loss,
                       chunk_rows)
+
+
+ADAMW_BLOCK = 256  # values per scale of an 8-bit state
+
+# A tensor's record for tilec_adamw (include/tilec.h, tilec_adamw_tensor): 8
+# pointers and sizes and two 32-bit type codes, the parameter's low.
+_BF16_PARAM, _BF16_GRAD = _lib.BF16, _lib.BF16 << 32
+
+
+def adamw_state(param, bits=32):
+    """(exp_avg, exp_avg_sq): the zero states of `adamw_step` for one
+    parameter, float32 tensors of its shape, or with bits=8 a (codes, scales)
+    pair each: int8 (exp_avg) and uint8 (exp_avg_sq) codes of the parameter's
+    shape and one float32 scale per 256 consecutive values."""
+    if bits not in (32, 8):
+        raise ValueError(f"adamw_state: states have 32 or 8 bits (got {bits})")
+    if bits == 32:
+        m, v = torch.zeros((2, *param.shape), dtype=torch.float32, device=param.device)
+        return m, v
+    scales = torch.zeros((2, -(-param.numel() // ADAMW_BLOCK)), dtype=torch.float32, device=param.device)
+    return ((torch.zeros(param.shape, dtype=torch.int8, device=param.device), scales[0]),
+            (torch.zeros(param.shape, dtype=torch.uint8, device=param.device), scales[1]))
+
+
+def _same(what, name, tensors, numels, dtypes, device):
+    """Contiguous tensors of the given sizes and types on one device."""
+    if [t.numel() for t in tensors] != numels:
+        raise ValueError(f"{what}: {name} and params differ in number or sizes")
+    wrong = {t.dtype for t in tensors}.difference(dtypes)
+    if wrong:
+        raise TypeError(f"{what}: {name} has a tensor of dtype {wrong.pop()}, expected "
+                        f"{' or '.join(str(d) for d in dtypes)}")
+    if {t.get_device() for t in tensors} - {device}:
+        raise TypeError(f"{what} needs all tensors on one ROCm GPU ({name} has others)")
+    if not all([t.is_contiguous() for t in tensors]):
+        raise ValueError(f"{what}: {name} has a tensor that is not contiguous")
+
+
+def _split_state(what, name, state):
+    """([codes], [scales]) of 8-bit states, or ([tensors], None) of 32-bit ones."""
+    if not isinstance(state[0], (tuple, list)):
+        return list(state), None
+    try:
+        codes, scales = zip(*state)
+    except (TypeError, ValueError):
+        raise ValueError(f"{what}: {name} mixes 32-bit and 8-bit states") from None
+    return list(codes), list(scales)
+
+
+def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+               grad_scale=None, copies=None):
+    """One AdamW step over lists of tensors, in place.
+
+        g = grad * grad_scale;  p = p * (1 - lr * weight_decay)
+        m = beta1 * m + (1 - beta1) * g;  v = beta2 * v + (1 - beta2) * g^2
+        p = p - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+
+    params: contiguous float32 or bfloat16 tensors; grads: float32 or bfloat16,
+    one of each parameter's size (None: that parameter and its states stay as
+    they are).  exp_avg, exp_avg_sq (m, v): a state of each parameter, all as
+    `adamw_state` makes them, 32-bit or 8-bit (codes, scales).  step counts
+    from 1.  grad_scale: a float32 value on the GPU that multiplies every
+    gradient (a clipping coefficient).  copies: bfloat16 tensors that get the
+    new parameters, rounded (None, or None for some: none).  All arithmetic is
+    float32; many tensors share a launch.
+    """
+    what = "adamw_step"
+    params = list(params)
+    if len(grads) != len(params) or (copies is not None and len(copies) != len(params)) \
+            or len(exp_avg) != len(params) or len(exp_avg_sq) != len(params):
+        raise ValueError(f"{what}: {len(params)} params, {len(grads)} grads, {len(exp_avg)} and {len(exp_avg_sq)} states")
+    if step < 1:
+        raise ValueError(f"{what}: steps count from 1 (got {step})")
+    if not params:
+        return
+    if None in [g if g is None else 0 for g in grads]:
+        have = [i for i, g in enumerate(grads) if g is not None]
+        if not have:
+            return
+        params, grads, exp_avg, exp_avg_sq = ([x[i] for i in have] for x in (params, grads, exp_avg, exp_avg_sq))
+        copies = None if copies is None else [copies[i] for i in have]
+    if params[0].device.type != "cuda":
+        raise TypeError(f"{what} needs tensors on a ROCm GPU (got {params[0].device})")
+    device = params[0].get_device()
+    numels = [p.numel() for p in params]
+    floats = (torch.float32, torch.bfloat16)
+    _same(what, "params", params, numels, floats, device)
+    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    _same(what, "grads", grads, numels, floats, device)
+    m, ms = _split_state(what, "exp_avg", exp_avg)
+    v, vs = _split_state(what, "exp_avg_sq", exp_avg_sq)
+    if (ms is None) != (vs is None):
+        raise ValueError(f"{what}: exp_avg and exp_avg_sq have states of different bits")
+    _same(what, "exp_avg", m, numels, (torch.float32,) if ms is None else (torch.int8,), device)
+    _same(what, "exp_avg_sq", v, numels, (torch.float32,) if vs is None else (torch.uint8,), device)
+    none = [0] * len(params)
+    ms_at = vs_at = copies_at = none
+    if ms is not None:
+        blocks = [-(-n // ADAMW_BLOCK) for n in numels]
+        _same(what, "exp_avg's scales", ms, blocks, (torch.float32,), device)
+        _same(what, "exp_avg_sq's scales", vs, blocks, (torch.float32,), device)
+        ms_at, vs_at = [t.data_ptr() for t in ms], [t.data_ptr() for t in vs]
+    if copies is not None:
+        given = [(c, n) for c, n in zip(copies, numels) if c is not None]
+        _same(what, "copies", [c for c, _ in given], [n for _, n in given], (torch.bfloat16,), device)
+        copies_at = [0 if c is None else c.data_ptr() for c in copies]
+    p_at = [p.data_ptr() for p in params]
+    # One memory for two parameters (a tied weight given twice) would be a race.
+    held = [a for a, n in zip(p_at, numels) if n]
+    if len(set(held)) < len(held):
+        raise ValueError(f"{what}: two params share their memory")
+    if grad_scale is not None:
+        if grad_scale.dtype != torch.float32 or grad_scale.get_device() != device:
+            raise TypeError(f"{what}: grad_scale must be float32 on the params' GPU (got {grad_scale.dtype}, "
+                            f"{grad_scale.device})")
+        if grad_scale.numel() != 1:
+            raise ValueError(f"{what}: grad_scale has shape {tuple(grad_scale.shape)}, expected one value")
+    types = [(_BF16_PARAM if p.dtype == torch.bfloat16 else 0) | (_BF16_GRAD if g.dtype == torch.bfloat16 else 0)
+             for p, g in zip(params, grads)]
+    table = array.array("q", [x for record in zip(p_at, [g.data_ptr() for g in grads], [t.data_ptr() for t in m],
+                                                  [t.data_ptr() for t in v], ms_at, vs_at, copies_at, numels, types)
+                              for x in record])
+    where = params[0].device
+    with _on(where):
+        _lib.check(_lib.lib().tilec_adamw(table.buffer_info()[0], len(params), 32 if ms is None else 8, step, lr,
+                                          betas[0], betas[1], eps, weight_decay, _ptr(grad_scale), _stream(where)))
+
+
+def adamw_values(states):
+    """The float32 values that a list of 8-bit states, (codes, scales) pairs of
+    `adamw_step`, stand for: a flat tensor each."""
+    what = "adamw_values"
+    states = list(states)
+    if not states:
+        return []
+    codes, scales = _split_state(what, "states", states)
+    if scales is None:
+        raise ValueError(f"{what}: expected (codes, scales) pairs")
+    if codes[0].device.type != "cuda":
+        raise TypeError(f"{what} needs tensors on a ROCm GPU (got {codes[0].device})")
+    device, where = codes[0].get_device(), codes[0].device
+    numels = [c.numel() for c in codes]
+    _same(what, "states", codes, numels, (torch.int8, torch.uint8), device)
+    _same(what, "scales", scales, [-(-n // ADAMW_BLOCK) for n in numels], (torch.float32,), device)
+    out = list(torch.empty(sum(numels), dtype=torch.float32, device=where).split(numels))
+    records = []
+    for o, c, s, n in zip(out, codes, scales, numels):
+        m = (c.data_ptr(), 0, s.data_ptr(), 0) if c.dtype == torch.int8 else (0, c.data_ptr(), 0, s.data_ptr())
+        records += (o.data_ptr(), 0, *m, 0, n, 0)
+    table = array.array("q", records)
+    with _on(where):
+        _lib.check(_lib.lib().tilec_adamw_values(table.buffer_info()[0], len(out), _stream(where)))
+    return out
