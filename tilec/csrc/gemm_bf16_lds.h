@@ -194,14 +194,47 @@ struct TileOut {
   int wm;                  // the wave's row of waves
   int lane;
   bool interior;           // no row or column past M or N
+  char* stage;             // the wave's own LDS, WTM x WTN 16-bit values (Epi::kStaged)
   __device__ __forceinline__ int row(int i, int r) const {
     return row_base + MF * i + (MF == 32 ? 8 * (r >> 2) + (r & 3) : r);
   }
   __device__ __forceinline__ int col(int j) const { return col_base + MF * j; }
+
+  // Outputs of 16 bits stored with the tile's rows contiguous.  A lane's own
+  // values would leave in pieces of 8 bytes, 16 columns x 32 bytes a store
+  // instruction; through LDS they leave in 16-byte pieces, 16 or 8 lanes to a
+  // column's run of WTM values.  put: the values of rows row(i, 4 q) .. + 3 of
+  // column col(j).  Then store_all: f(column, row, 8 values) of the tile, for
+  // all of the wave's columns and rows.  16-byte chunk c of a column's run
+  // lies at c ^ (column mod chunks): lanes of one instruction then spread
+  // over the banks.
+  static constexpr int kChunks = P::WTM / 8;
+  __device__ __forceinline__ char* chunk(int n, int c) const {
+    return stage + 16 * (n * kChunks + (c ^ (n & (kChunks - 1))));
+  }
+  __device__ __forceinline__ void put(int i, int q, int j, int lo, int hi) const {
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    const int m = row(i, 4 * q) - m0 - wm * P::WTM;
+    *reinterpret_cast<i32x2*>(chunk(MF * j + lane % MF, m >> 3) + 2 * (m & 4)) = i32x2{lo, hi};
+  }
+  template <class F>
+  __device__ __forceinline__ void store_all(F f) const {
+    // The wave's own writes, in order; other waves use other LDS.
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(15 << 14 | 15 | 7 << 4);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    const int n_base = col_base - lane % MF, m_base = m0 + wm * P::WTM;
+#pragma unroll
+    for (int k = 0; k < P::WTN * kChunks / 64; ++k) {
+      const int n = (64 * k + lane) / kChunks, c = lane % kChunks;
+      f(n_base + n, m_base + 8 * c, *reinterpret_cast<const i32x4*>(chunk(n, c)));
+    }
+  }
 };
 
 // The plain product: C[row][col], fp32.
 struct StoreC {
+  static constexpr bool kStaged = false;
   float* C;
   int64_t ldc;
   template <class P, int MF>
@@ -714,6 +747,13 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void gemm_bf16_lds_kernel(
   }
   TileOut<P, MF> t;
   t.m0 = m0, t.n0 = n0, t.row_base = row_base, t.col_base = col_base, t.wm = wm, t.lane = lane, t.interior = interior;
+  if constexpr (Epi::kStaged) {
+    // The ring is free once every wave's copies have landed.
+    constexpr int kWave = 2 * P::WTM * P::WTN, kHalf = P::NW * kWave > P::STAGE_BYTES ? P::NW / 2 : P::NW;
+    static_assert(kHalf * kWave <= P::STAGE_BYTES, "a wave's outputs fit the ring");
+    __syncthreads();
+    t.stage = (wave < kHalf ? lds0 : lds1) + wave % kHalf * kWave;
+  }
   epi.template run<P, MF>(t, acc, M, N);
 }
 

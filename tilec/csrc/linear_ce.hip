@@ -52,6 +52,7 @@ __device__ __forceinline__ u16 bf16_bits(float f) { return __builtin_bit_cast(u1
 
 // The logits: rows are vocabulary entries, columns tokens.
 struct CeLogits {
+  static constexpr bool kStaged = true;
   u16* e;      // exp(l - m) 2^15 in fp16, [token][lde]; NULL: losses only
   int64_t lde;
   f32x2* stat;  // (m, sum of exp(l - m)), [token][groups]
@@ -62,42 +63,68 @@ struct CeLogits {
   template <class P, int MF>
   __device__ __forceinline__ void run(const TileOut<P, MF>& t, typename P::Acc (&acc)[P::TM][P::TN], int V,
                                       int N) const {
-    const int group = t.m0 / P::WTM + t.wm;
+    if (t.interior) tile<P, MF, true>(t, acc, V, N);
+    else tile<P, MF, false>(t, acc, V, N);
+  }
+
+  template <class P, int MF, bool FULL>
+  __device__ __forceinline__ void tile(const TileOut<P, MF>& t, typename P::Acc (&acc)[P::TM][P::TN], int V,
+                                       int N) const {
+    constexpr float kLog2e = 1.44269504088896f;
+    const int first = t.m0 + t.wm * P::WTM, group = first / P::WTM;
+    int64_t want[P::TN];  // read ahead of their use
+#pragma unroll
+    for (int j = 0; j < P::TN; ++j) want[j] = FULL || t.col(j) < N ? target[t.col(j)] : -1;
 #pragma unroll
     for (int j = 0; j < P::TN; ++j) {
       const int tok = t.col(j);
-      const bool ok = tok < N;
-      int64_t want = ok ? target[tok] : -1;
-      if (want < 0 || want >= V) want = -1;
       float m = -FLT_MAX;
 #pragma unroll
       for (int i = 0; i < P::TM; ++i)
 #pragma unroll
         for (int r = 0; r < P::ACC; ++r)
-          if (t.interior || t.row(i, r) < V) m = fmaxf(m, acc[i][j][r]);
+          if (FULL || t.row(i, r) < V) m = fmaxf(m, acc[i][j][r]);
       if constexpr (MF == 16) m = fmaxf(m, __shfl_xor(m, 16));
       m = fmaxf(m, __shfl_xor(m, 32));
+      // exp(l - m) 2^15 = 2^((l - m) log2 e + 15): the difference first, so that
+      // it is exact where it matters.
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < P::TM; ++i)
 #pragma unroll
         for (int q = 0; q < P::ACC / 4; ++q) {
-          const int v0 = t.row(i, 4 * q);
-          f16x4 h;
+          f32x4 x;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const float l = acc[i][j][4 * q + c];
-            const float x = t.interior || v0 + c < V ? __expf(l - m) : 0.f;
-            s += x;
-            h[c] = (f16)(x * kScale16);
-            if (v0 + c == (int)want) tlogit[tok] = l;
+            x[c] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][4 * q + c] - m, kLog2e, 15.f));
+            if (!FULL && t.row(i, 4 * q) + c >= V) x[c] = 0.f;
           }
-          if (e != nullptr && ok && v0 < lde)
-            *reinterpret_cast<i32x2*>(e + (int64_t)tok * lde + v0) = __builtin_bit_cast(i32x2, h);
+          s += (x[0] + x[1]) + (x[2] + x[3]);
+          if (e != nullptr) {
+            const i32x2 h = __builtin_bit_cast(i32x2, __builtin_convertvector(x, f16x4));
+            t.put(i, q, j, h.x, h.y);
+          }
         }
       if constexpr (MF == 16) s += __shfl_xor(s, 16);
       s += __shfl_xor(s, 32);
-      if (t.lane < MF && ok) stat[(int64_t)tok * groups + group] = f32x2{m, s};
+      if (t.lane < MF && (FULL || tok < N))
+        stat[(int64_t)tok * groups + group] = f32x2{m, s * (1.f / kScale16)};
+    }
+    if (e != nullptr)
+      t.store_all([&](int n, int v, i32x4 x) {
+        if (FULL || (n < N && v < lde)) *reinterpret_cast<i32x4*>(e + (int64_t)n * lde + v) = x;
+      });
+#pragma unroll
+    for (int j = 0; j < P::TN; ++j) {
+      // The target's logit: one wave in V / WTM holds it.
+      const int64_t at = want[j] - first;
+      if (want[j] >= 0 && at >= 0 && at < P::WTM && want[j] < V) {
+#pragma unroll
+        for (int i = 0; i < P::TM; ++i)
+#pragma unroll
+          for (int r = 0; r < P::ACC; ++r)
+            if (t.row(i, r) - first == (int)at) tlogit[t.col(j)] = acc[i][j][r];
+      }
     }
   }
 };
@@ -106,6 +133,7 @@ struct CeLogits {
 // tokens (dx) or vocabulary entries (dW).  Over several chunks of rows dW is
 // added up in fp32 and rounded once, by the last.
 struct CeGrad {
+  static constexpr bool kStaged = true;
   u16* out;  // bf16, [column][ldo]; NULL: not the last chunk
   int64_t ldo;
   float* acc32;  // fp32 sums, [column][ld32]
@@ -117,38 +145,34 @@ struct CeGrad {
   __device__ __forceinline__ void run(const TileOut<P, MF>& t, typename P::Acc (&acc)[P::TM][P::TN], int H,
                                       int N) const {
     const float f = out != nullptr ? *scale : 1.f;
-    const bool vec = ldo % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0;
 #pragma unroll
-    for (int j = 0; j < P::TN; ++j) {
-      const int n = t.col(j);
+    for (int j = 0; j < P::TN; ++j)
 #pragma unroll
       for (int i = 0; i < P::TM; ++i)
 #pragma unroll
         for (int q = 0; q < P::ACC / 4; ++q) {
-          const int h0 = t.row(i, 4 * q);
-          if (n >= N || h0 >= H) continue;
           f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-          if (acc32 != nullptr) {  // ld32 is a multiple of 4
-            f32x4* p = reinterpret_cast<f32x4*>(acc32 + (int64_t)n * ld32 + h0);
+          if (acc32 != nullptr && t.col(j) < N && t.row(i, 4 * q) < H) {  // ld32 is a multiple of 4
+            f32x4* p = reinterpret_cast<f32x4*>(acc32 + (int64_t)t.col(j) * ld32 + t.row(i, 4 * q));
             if (add) v += *p;
-            if (out == nullptr) {
-              *p = v;
-              continue;
-            }
+            if (out == nullptr) *p = v;
           }
-          u16* o = out + (int64_t)n * ldo + h0;
-          u16 b[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) b[c] = bf16_bits(v[c] * f);
-          if (vec && h0 + 4 <= H) {
-            *reinterpret_cast<i32x2*>(o) = i32x2{(int)(b[0] | (uint32_t)b[1] << 16), (int)(b[2] | (uint32_t)b[3] << 16)};
-          } else {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              if (h0 + c < H) o[c] = b[c];
-          }
+          if (out != nullptr)
+            t.put(i, q, j, (int)(bf16_bits(v[0] * f) | (uint32_t)bf16_bits(v[1] * f) << 16),
+                  (int)(bf16_bits(v[2] * f) | (uint32_t)bf16_bits(v[3] * f) << 16));
         }
-    }
+    if (out == nullptr) return;
+    t.store_all([&](int n, int h, i32x4 x) {
+      typedef i32x4 __attribute__((aligned(2))) i32x4_any;
+      u16* o = out + (int64_t)n * ldo + h;
+      if (t.interior || (n < N && h + 8 <= H)) {
+        *reinterpret_cast<i32x4_any*>(o) = x;
+      } else if (n < N) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          if (h + c < H) o[c] = (u16)((uint32_t)x[c / 2] >> (16 * (c & 1)));
+      }
+    });
   }
 };
 
