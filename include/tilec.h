@@ -292,8 +292,14 @@ size_t tilec_layer_norm_backward_workspace_bytes(int64_t R, int64_t D, int32_t x
  *
  * tilec_linear_ce_scratch_bytes gives the workspace (any contents, 16-byte
  * aligned) and counters (zeroed once, left zero) for exactly these arguments;
- * of x and weight it reads the addresses' alignment only.  Every sum is
- * float32 or wider, in a fixed order.
+ * of x and weight it reads the addresses' alignment only.  rows_per_chunk
+ * (may be NULL) receives the rows of a chunk.  Every sum is float32 or wider,
+ * in a fixed order.
+ *
+ * configs (float32 only; NULL: the built-in rule): the variant and split_k, as
+ * tilec_matmul takes them, of a whole chunk's three products: the logits
+ * (chunk rows x V, K = H, x2 column-major), dx (chunk rows x H, K = V) and
+ * dweight (V x H, K = chunk rows, x1 column-major).
  */
 #define TILEC_REDUCE_NONE 0
 #define TILEC_REDUCE_SUM 1
@@ -301,11 +307,12 @@ size_t tilec_layer_norm_backward_workspace_bytes(int64_t R, int64_t D, int32_t x
 int tilec_linear_ce(const void* x, const void* weight, const int64_t* target, float* loss,
                     const float* grad_loss, void* dx, void* dweight, int64_t N, int64_t H, int64_t V,
                     int64_t ldx, int64_t ldw, int32_t dtype, int32_t reduction, int64_t ignore_index,
-                    int32_t grad, int64_t chunk_rows, void* workspace, size_t workspace_bytes,
-                    void* counters, size_t counter_bytes, void* stream);
+                    int32_t grad, int64_t chunk_rows, const int32_t* configs,
+                    void* workspace, size_t workspace_bytes, void* counters, size_t counter_bytes, void* stream);
 int tilec_linear_ce_scratch_bytes(const void* x, const void* weight, int64_t N, int64_t H, int64_t V,
                                   int64_t ldx, int64_t ldw, int32_t dtype, int32_t reduction, int32_t grad,
-                                  int64_t chunk_rows, size_t* workspace_bytes, size_t* counter_bytes);
+                                  int64_t chunk_rows, const int32_t* configs, size_t* workspace_bytes,
+                                  size_t* counter_bytes, int64_t* rows_per_chunk);
 
 /*
  * One AdamW step over `count` tensors, in place:

@@ -48,9 +48,10 @@ SIGNATURES = {
                                                  _i64, _i32, _i32, _i32, _vp, _sz, _vp]),
     "tilec_layer_norm_backward_workspace_bytes": (_sz, [_i64, _i64, _i32]),
     "tilec_linear_ce": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _i32,
-                                       _i64, _i32, _i64, _vp, _sz, _vp, _sz, _vp]),
+                                       _i64, _i32, _i64, _vp, _vp, _sz, _vp, _sz, _vp]),
     "tilec_linear_ce_scratch_bytes": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i64,
-                                                     ctypes.POINTER(_sz), ctypes.POINTER(_sz)]),
+                                                     _vp, ctypes.POINTER(_sz), ctypes.POINTER(_sz),
+                                                     ctypes.POINTER(_i64)]),
     "tilec_adamw": (ctypes.c_int, [_vp, _i32, _i32, _i64, _f64, _f64, _f64, _f64, _f64, _vp, _vp]),
     "tilec_adamw_values": (ctypes.c_int, [_vp, _i32, _vp]),
     "tilec_last_error": (ctypes.c_char_p, []),

@@ -182,8 +182,9 @@ __device__ __forceinline__ void sched_rows() {
 
 // How K is masked: kKMasked for any K; kKFull where K is a multiple of BK;
 // kKRows where every k-contiguous operand is padded to whole K steps (with
-// zeros), so that only the rows of an r-contiguous operand end at K.
-enum KMask { kKMasked, kKFull, kKRows };
+// zeros), so that only the rows of an r-contiguous operand end at K; kKColsA
+// where that holds for all but a k-contiguous A, masked per lane.
+enum KMask { kKMasked, kKFull, kKRows, kKColsA };
 
 // What becomes of a tile.  A lane holds, of each block (i, j), the accumulators
 // of rows row(i, r), r < ACC, of one column col(j).
@@ -194,6 +195,7 @@ struct TileOut {
   int wm;                  // the wave's row of waves
   int lane;
   bool interior;           // no row or column past M or N
+  int split;               // the K split (kOwnSplits: whose sums these are)
   char* stage;             // the wave's own LDS, WTM x WTN 16-bit values (Epi::kStaged)
   __device__ __forceinline__ int row(int i, int r) const {
     return row_base + MF * i + (MF == 32 ? 8 * (r >> 2) + (r & 3) : r);
@@ -233,8 +235,11 @@ struct TileOut {
 };
 
 // The plain product: C[row][col], fp32.
+//   kStaged: the epilogue needs TileOut::stage.
+//   kOwnSplits: it takes the sums of one K split as they are; otherwise the
+//   splits are combined here and only the last gets to it.
 struct StoreC {
-  static constexpr bool kStaged = false;
+  static constexpr bool kStaged = false, kOwnSplits = false;
   float* C;
   int64_t ldc;
   template <class P, int MF>
@@ -258,7 +263,7 @@ template <int BM, int BN, int BK, int NBUF, int WM, int WN, KMask KM, bool CA, b
 __global__ __launch_bounds__(WM * WN * 64, 1) void gemm_bf16_lds_kernel(
     const u16* __restrict__ A, const u16* __restrict__ B, Epi epi, int M, int N, int K, int64_t lda, int64_t ldb,
     int group_m, int xcds, int split_steps, float* __restrict__ ws, unsigned* __restrict__ counters) {
-  constexpr bool KFULL = KM == kKFull, KCOLS = KM == kKMasked;
+  constexpr bool KFULL = KM == kKFull, KCOLS_B = KM == kKMasked, KCOLS_A = KCOLS_B || KM == kKColsA;
   using P = LdsGemm<BM, BN, BK, NBUF, WM, WN, CA, CB, MF>;
   using SA = typename P::SA;
   using SB = typename P::SB;
@@ -363,13 +368,13 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void gemm_bf16_lds_kernel(
     const int k0 = (kt0 + kt) * BK;
     if (q < P::A_INSTR) {
       uint32_t off = off_a[q];
-      if constexpr (KCOLS && !CA) off = k0 + kcol(SA{}, q) < K ? off : kOob;
+      if constexpr (KCOLS_A && !CA) off = k0 + kcol(SA{}, q) < K ? off : kOob;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr_t)(st + 16 * 64 * (wave * P::A_INSTR + q)), 16, off, 0,
                                                0, 0);
     } else {
       const int i = q - P::A_INSTR;
       uint32_t off = off_b[i];
-      if constexpr (KCOLS && CB) off = k0 + kcol(SB{}, i) < K ? off : kOob;
+      if constexpr (KCOLS_B && CB) off = k0 + kcol(SB{}, i) < K ? off : kOob;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr_t)(st + P::A_BYTES + 16 * 64 * (wave * P::B_INSTR + i)),
                                                16, off, 0, 0, 0);
     }
@@ -736,7 +741,8 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void gemm_bf16_lds_kernel(
   const bool interior = (m0 + BM <= M) && (n0 + BN <= N);
   const int row_base = m0 + wm * P::WTM + 4 * (MF == 32 ? kg : g);
   const int col_base = n0 + wn * P::WTN + (lane % MF);
-  if constexpr (MF == 32) {
+  if constexpr (Epi::kOwnSplits) {
+  } else if constexpr (MF == 32) {
     if (S > 1 && !splitk_tile<P::TM, P::TN, P::NT>(acc, split, S, blockIdx.x, gridDim.x, ws, counters, &last_flag,
                                                     row_base, col_base, M, N))
       return;
@@ -747,6 +753,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void gemm_bf16_lds_kernel(
   }
   TileOut<P, MF> t;
   t.m0 = m0, t.n0 = n0, t.row_base = row_base, t.col_base = col_base, t.wm = wm, t.lane = lane, t.interior = interior;
+  t.split = split;
   if constexpr (Epi::kStaged) {
     // The ring is free once every wave's copies have landed.
     constexpr int kWave = 2 * P::WTM * P::WTN, kHalf = P::NW * kWave > P::STAGE_BYTES ? P::NW / 2 : P::NW;

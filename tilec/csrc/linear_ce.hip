@@ -52,7 +52,7 @@ __device__ __forceinline__ u16 bf16_bits(float f) { return __builtin_bit_cast(u1
 
 // The logits: rows are vocabulary entries, columns tokens.
 struct CeLogits {
-  static constexpr bool kStaged = true;
+  static constexpr bool kStaged = true, kOwnSplits = false;
   u16* e;      // exp(l - m) 2^15 in fp16, [token][lde]; NULL: losses only
   int64_t lde;
   f32x2* stat;  // (m, sum of exp(l - m)), [token][groups]
@@ -131,15 +131,18 @@ struct CeLogits {
 
 // A gradient, stored transposed: rows are the hidden dimension, columns
 // tokens (dx) or vocabulary entries (dW).  Over several chunks of rows dW is
-// added up in fp32 and rounded once, by the last.
+// added up in fp32 and rounded once, by the last; each K split of a product
+// stores its own fp32 sums, which ce_join_kernel adds in order (the tile
+// kernel's own combine, in which a tile's last workgroup reads every split,
+// took 16 of the 31 us of a 7 x 32768 x 1024 dx in 32 splits).
 struct CeGrad {
-  static constexpr bool kStaged = true;
-  u16* out;  // bf16, [column][ldo]; NULL: not the last chunk
+  static constexpr bool kStaged = true, kOwnSplits = true;
+  u16* out;  // bf16, [column][ldo]; NULL: fp32 sums only
   int64_t ldo;
-  float* acc32;  // fp32 sums, [column][ld32]
-  int64_t ld32;
-  bool add;            // to what acc32 holds
-  const float* scale;  // applied when out is written
+  float* acc32;         // fp32 sums, [split][column][ld32]
+  int64_t ld32, split;  // split: elements of one
+  bool add;             // to what acc32 holds
+  const float* scale;   // applied when out is written
 
   template <class P, int MF>
   __device__ __forceinline__ void run(const TileOut<P, MF>& t, typename P::Acc (&acc)[P::TM][P::TN], int H,
@@ -152,8 +155,8 @@ struct CeGrad {
 #pragma unroll
         for (int q = 0; q < P::ACC / 4; ++q) {
           f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-          if (acc32 != nullptr && t.col(j) < N && t.row(i, 4 * q) < H) {  // ld32 is a multiple of 4
-            f32x4* p = reinterpret_cast<f32x4*>(acc32 + (int64_t)t.col(j) * ld32 + t.row(i, 4 * q));
+          if (acc32 != nullptr && t.col(j) < N && t.row(i, 4 * q) < H) {  // ld32 is a multiple of 16
+            f32x4* p = reinterpret_cast<f32x4*>(acc32 + t.split * split + (int64_t)t.col(j) * ld32 + t.row(i, 4 * q));
             if (add) v += *p;
             if (out == nullptr) *p = v;
           }
@@ -182,16 +185,19 @@ struct CeGrad {
 
 enum Reduction { kNone, kSum, kMean };
 
+constexpr int kFewRows = 32;  // of ce_few_rows_kernel
+
 // xs = x with the ignored rows cleared (whatever they hold must not reach dW,
-// where 0 times a NaN would be one) and rows padded with zeros to Hp; and, by
-// one more workgroup where `scale` is set, the scalar factor of the gradients.
+// where 0 times a NaN would be one) and rows padded with zeros to Hp; where xt
+// is set, also its transpose [H][kFewRows], padded with zeros; and, by one more
+// workgroup where `scale` is set, the scalar factor of the gradients.
 template <typename T>
 __global__ __launch_bounds__(256) void ce_prepare_kernel(const T* __restrict__ x, int64_t ldx, T* __restrict__ xs,
                                                          int64_t Hp, int64_t N, int64_t H,
                                                          const int64_t* __restrict__ target, int64_t ignore,
                                                          float* __restrict__ scale, int64_t all,
                                                          const int64_t* __restrict__ all_targets, int reduction,
-                                                         const float* __restrict__ grad_loss) {
+                                                         const float* __restrict__ grad_loss, T* __restrict__ xt) {
   constexpr int E = 16 / (int)sizeof(T);
   typedef i32x4 __attribute__((aligned(2))) i32x4_any;
   __shared__ int count[256];
@@ -199,13 +205,14 @@ __global__ __launch_bounds__(256) void ce_prepare_kernel(const T* __restrict__ x
     int n = 0;
     for (int64_t i = threadIdx.x; i < all; i += 256) n += all_targets[i] != ignore;
     count[threadIdx.x] = n;
-    __syncthreads();
+    for (int o = 128; o > 0; o >>= 1) {
+      __syncthreads();
+      if ((int)threadIdx.x < o) count[threadIdx.x] += count[threadIdx.x + o];
+    }
     if (threadIdx.x == 0) {
-      int64_t c = 0;
-      for (int i = 0; i < 256; ++i) c += count[i];
       float f = 1.f;
       if (reduction != kNone && grad_loss != nullptr) f = *grad_loss;
-      if (reduction == kMean) f /= (float)(c > 1 ? c : 1);
+      if (reduction == kMean) f /= (float)max(count[0], 1);
       *scale = f;
     }
     return;
@@ -229,6 +236,11 @@ __global__ __launch_bounds__(256) void ce_prepare_kernel(const T* __restrict__ x
       }
     }
     *reinterpret_cast<i32x4*>(xs + r * Hp + c) = v;
+  }
+  if (xt == nullptr) return;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < kFewRows * H; i += blocks * 256) {
+    const int64_t r = i / H, h = i - r * H;
+    xt[h * kFewRows + r] = r < N && target[r] != ignore ? x[r * ldx + h] : T{0};
   }
 }
 
@@ -367,28 +379,142 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
   }
 }
 
-// The sum or mean of the rows' losses, in 64 bits and a fixed order.
-__global__ __launch_bounds__(1024) void ce_loss_kernel(const float* __restrict__ rows,
-                                                       const int64_t* __restrict__ target, int64_t N, int64_t ignore,
-                                                       int reduction, float* __restrict__ loss) {
-  __shared__ double sum[1024];
-  __shared__ int count[1024];
-  double s = 0;
-  int n = 0;
-  for (int64_t i = threadIdx.x; i < N; i += 1024) {
-    s += (double)rows[i];
-    n += target[i] != ignore;
+// The K splits of a gradient, added in order: out = bf16(scale sum), or acc =
+// sum, in both cases onto acc where `add` is set; and, by one more workgroup
+// where `loss` is set, the sum or mean of the rows' losses, in 64 bits and a
+// fixed order.
+struct CeJoin {
+  const float* part;  // [splits][rows][ld]
+  int splits, lanes;  // lanes: threads that share the splits of a result
+  int64_t rows, cols, ld;
+  u16* out;  // [rows][cols]
+  float* acc;
+  bool add;
+  const float* scale;
+  float* loss;
+  const float* row_loss;
+  const int64_t* target;
+  int64_t N, ignore;
+  int reduction;
+};
+
+__global__ __launch_bounds__(256) void ce_join_kernel(CeJoin a) {
+  __shared__ double sum[256];
+  __shared__ int count[256];
+  if (a.loss != nullptr && blockIdx.x == gridDim.x - 1) {
+    double s = 0;
+    int n = 0;
+    for (int64_t i = threadIdx.x; i < a.N; i += 256) {
+      s += (double)a.row_loss[i];
+      n += a.target[i] != a.ignore;
+    }
+    sum[threadIdx.x] = s;
+    count[threadIdx.x] = n;
+    for (int o = 128; o > 0; o >>= 1) {
+      __syncthreads();
+      if ((int)threadIdx.x < o) {
+        sum[threadIdx.x] += sum[threadIdx.x + o];
+        count[threadIdx.x] += count[threadIdx.x + o];
+      }
+    }
+    if (threadIdx.x == 0) *a.loss = (float)(a.reduction == kMean ? sum[0] / (double)max(count[0], 1) : sum[0]);
+    return;
   }
-  sum[threadIdx.x] = s;
-  count[threadIdx.x] = n;
-  for (int o = 512; o > 0; o >>= 1) {
-    __syncthreads();
-    if ((int)threadIdx.x < o) {
-      sum[threadIdx.x] += sum[threadIdx.x + o];
-      count[threadIdx.x] += count[threadIdx.x + o];
+  // Each thread every lanes-th split, then those sums in order.
+  __shared__ f32x4 share[256];
+  const int64_t blocks = gridDim.x - (a.loss != nullptr ? 1 : 0), per_row = a.ld / 4, stride = a.rows * a.ld;
+  const int per = 256 / a.lanes, mine = (int)threadIdx.x % per, lane = (int)threadIdx.x / per;
+  const float f = a.out != nullptr ? *a.scale : 1.f;
+  for (int64_t i0 = (int64_t)blockIdx.x * per; i0 < a.rows * per_row; i0 += blocks * per) {
+    const int64_t i = i0 + mine;
+    const bool live = i < a.rows * per_row;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (live) {
+      const float* p = a.part + 4 * i;
+#pragma unroll 4
+      for (int k = lane; k < a.splits; k += a.lanes) v += *reinterpret_cast<const f32x4*>(p + k * stride);
+    }
+    if (a.lanes > 1) {
+      __syncthreads();
+      share[threadIdx.x] = v;
+      __syncthreads();
+      for (int k = 1; k < a.lanes && lane == 0; ++k) v += share[k * per + mine];
+    }
+    if (!live || lane != 0) continue;
+    const int64_t r = i / per_row, c = 4 * (i - r * per_row);
+    f32x4* acc = reinterpret_cast<f32x4*>(a.acc + 4 * i);
+    if (a.add) v += *acc;
+    if (a.out == nullptr) {
+      *acc = v;
+      continue;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c + k < a.cols) a.out[r * a.cols + c + k] = bf16_bits(v[k] * f);
+  }
+}
+
+// dW [V, H] of up to 32 rows: one k-slice of a 16x16x32 MFMA, so no tile is
+// worth staging; the kernel is bound by writing dW.  A wave keeps the x
+// operand of its 128 columns of h (grid x) in registers, 16 bytes a lane from
+// the transposed x, and walks over tiles of 16 vocabulary entries.  Row i of the MFMA's output is column 8 (i / 4) +
+// 4 t + i % 4 of a block of 32, for the two MFMAs t = 0, 1 of the block: a
+// lane's 4 + 4 results are then 8 consecutive h, one 16-byte store, and the
+// four lanes of an entry write 64 bytes.
+__global__ __launch_bounds__(256) void ce_few_rows_kernel(const u16* __restrict__ d, int64_t ldd,
+                                                          const u16* __restrict__ xt, u16* __restrict__ dw, int R,
+                                                          int H, int V, const float* __restrict__ scale) {
+  typedef u16 u16x8 __attribute__((ext_vector_type(8)));
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int i = lane & 15, g = lane >> 4;  // MFMA row or column; k group, and group of output rows
+  const int h0 = blockIdx.x * 128;
+  const float f = *scale;
+  bf16x8 a[4][2];
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int h = min(h0 + 32 * b + 8 * (i >> 2) + 4 * t + (i & 3), H - 1);  // past H: not stored
+      a[b][t] = *reinterpret_cast<const bf16x8*>(xt + (int64_t)h * kFewRows + 8 * g);
+    }
+  auto load = [&](int v0) {  // rows of d are padded past V
+    u16x8 v;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const u16 t = d[(int64_t)min(8 * g + k, R - 1) * ldd + v0 + i];
+      v[k] = 8 * g + k < R ? t : (u16)0;
+    }
+    return __builtin_bit_cast(bf16x8, v);
+  };
+  const int step = 64 * gridDim.y;
+  int v0 = 16 * (4 * (int)blockIdx.y + wave);
+  if (v0 >= V) return;
+  bf16x8 next = load(v0);
+  for (; v0 < V; v0 += step) {
+    const bf16x8 b8 = next;
+    if (v0 + step < V) next = load(v0 + step);
+    const int v = v0 + i;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const f32x4 lo = mfma16x16x32bf16(a[b][0], b8, f32x4{0.f, 0.f, 0.f, 0.f});
+      const f32x4 hi = mfma16x16x32bf16(a[b][1], b8, f32x4{0.f, 0.f, 0.f, 0.f});
+      const int h = h0 + 32 * b + 8 * g;
+      u16* o = dw + (int64_t)v * H + h;
+      u16 w[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = bf16_bits(lo[k] * f), w[4 + k] = bf16_bits(hi[k] * f);
+      if (v < V && h + 8 <= H) {
+        typedef i32x4 __attribute__((aligned(2))) i32x4_any;
+        *reinterpret_cast<i32x4_any*>(o) =
+            i32x4{(int)(w[0] | (uint32_t)w[1] << 16), (int)(w[2] | (uint32_t)w[3] << 16),
+                  (int)(w[4] | (uint32_t)w[5] << 16), (int)(w[6] | (uint32_t)w[7] << 16)};
+      } else if (v < V) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (h + k < H) o[k] = w[k];
+      }
     }
   }
-  if (threadIdx.x == 0) *loss = (float)(reduction == kMean ? sum[0] / (double)max(count[0], 1) : sum[0]);
 }
 
 // acc += part, or acc = part.
@@ -424,20 +550,20 @@ int64_t tiles_of(CeTile t, int64_t M, int64_t N) {
 CeProduct choose(int64_t M, int64_t N, int64_t K, bool can_split) {
   const int64_t cus = device_cus();
   CeProduct c{N <= 64 ? kT64 : kT128, 1};
-  if (N > 64 && tiles_of(kT256, M, N) >= cus) c.tile = kT256;
+  if (c.tile == kT128 && tiles_of(kT256, M, N) >= cus) c.tile = kT256;
   if (!can_split || c.tile == kT256) return c;
   const int64_t tiles = tiles_of(c.tile, M, N), places = c.tile == kT64 ? 2 * cus : cus;
-  int64_t s = std::min<int64_t>({places / std::max<int64_t>(tiles, 1), cdiv(K, 64) / 4, 32});
+  int64_t s = std::min<int64_t>({places / std::max<int64_t>(tiles, 1), cdiv(K, 64) / 4, 64});
   c.splits = (int)std::max<int64_t>(s, 1);
   return c;
 }
 
+// Row length of fp32 sums of M: the lanes' 64-byte pieces are whole sectors.
+int64_t sum_ld(int64_t M) { return cdiv(M, 16) * 16; }
+
+// The splits' fp32 sums of an N x M gradient.
 size_t split_workspace(const CeProduct& c, int64_t M, int64_t N) {
-  const int64_t cells = c.tile == kT128 ? 128 * 128 : 128 * 64;
-  return c.splits > 1 ? (size_t)(c.splits * tiles_of(c.tile, M, N) * cells) * sizeof(float) : 0;
-}
-size_t split_counters(const CeProduct& c, int64_t M, int64_t N) {
-  return c.splits > 1 ? (size_t)tiles_of(c.tile, M, N) * kSplitCounterStride * sizeof(unsigned) : 0;
+  return c.splits > 1 ? (size_t)(c.splits * N * sum_ld(M)) * sizeof(float) : 0;
 }
 
 struct Operands {
@@ -447,23 +573,21 @@ struct Operands {
 };
 
 template <int BM, int BN, int NBUF, int WM, int WN, KMask KM, bool CA, bool CB, int MF, class Epi>
-hipError_t run_tile(const Operands& o, const Epi& epi, int splits, float* ws, unsigned* counters, hipStream_t stream) {
+hipError_t run_tile(const Operands& o, const Epi& epi, int splits, hipStream_t stream) {
   using P = LdsGemm<BM, BN, 64, NBUF, WM, WN, CA, CB, MF>;
   const int64_t tiles = cdiv(o.M, BM) * cdiv(o.N, BN);
   const SplitGeom g = gemm_split_geom(o.K, 64, splits);
-  if (g.splits > 1 && P::TM * P::TN * P::ACC > kSplitMaxAccPerThread) return hipErrorInvalidConfiguration;
   auto kern = gemm_bf16_lds_kernel<BM, BN, 64, NBUF, WM, WN, KM, CA, CB, MF, Epi>;
   hipLaunchKernelGGL(kern, dim3((unsigned)tiles, (unsigned)g.splits), dim3(P::NT), 0, stream, o.a, o.b, epi, (int)o.M,
-                     (int)o.N, (int)o.K, o.lda, o.ldb, 4, device_xcds(), (int)g.steps, ws, counters);
+                     (int)o.N, (int)o.K, o.lda, o.ldb, 4, device_xcds(), (int)g.steps, nullptr, nullptr);
   return hipGetLastError();
 }
 
-template <KMask KM, bool CA, bool CB, int MF, class Epi>
-hipError_t run_product(const Operands& o, const Epi& epi, const CeProduct& c, float* ws, unsigned* counters,
-                       hipStream_t stream) {
-  if (c.tile == kT256) return run_tile<256, 256, 2, 2, 4, KM, CA, CB, MF>(o, epi, c.splits, ws, counters, stream);
-  if (c.tile == kT128) return run_tile<128, 128, 4, 2, 4, KM, CA, CB, MF>(o, epi, c.splits, ws, counters, stream);
-  return run_tile<128, 64, 3, 2, 2, KM, CA, CB, MF>(o, epi, c.splits, ws, counters, stream);
+template <KMask KM, bool CA, bool CB, class Epi>
+hipError_t run_product(const Operands& o, const Epi& epi, const CeProduct& c, hipStream_t stream) {
+  if (c.tile == kT256) return run_tile<256, 256, 2, 2, 4, KM, CA, CB, 16>(o, epi, c.splits, stream);
+  if (c.tile == kT128) return run_tile<128, 128, 4, 2, 4, KM, CA, CB, 16>(o, epi, c.splits, stream);
+  return run_tile<128, 64, 3, 2, 2, KM, CA, CB, 16>(o, epi, c.splits, stream);
 }
 
 // Vocabulary entries of a wave's group in the logits' product.
@@ -488,23 +612,36 @@ struct CeArgs {
   int64_t ignore;
   bool grad;
   int64_t chunk_rows;
+  const int32_t* configs;  // fp32: variant and split of each product, or NULL
 };
 
 struct CePlan {
   int64_t R, chunks;     // rows of a chunk
-  int64_t Vp, Hp;        // padded row lengths of the kept values, of xs / wp
+  int64_t Vp, Hp;        // padded row lengths of the kept values, of xs and wp
   bool pad;              // bf16: operands copied with padded rows
   bool copy_x;
+  bool few;              // bf16: dW by ce_few_rows_kernel
   int groups, shift;
   CeProduct p1, p2, p3;  // bf16
-  size_t stat, tlogit, rows, scale, xs, wp, keep, acc, split;  // offsets
+  size_t stat, tlogit, rows, scale, xs, xt, wp, keep, acc, split;  // offsets
   size_t split_bytes, bytes, counter_bytes;
 };
 
-size_t matmul_scratch(const CeArgs& a, int64_t M, int64_t N, int64_t K, int64_t ld1, int64_t ld2, int layout,
+// The variant and K split of a product (0: logits, 1: dx, 2: dW) of a chunk of
+// R rows: the caller's for whole chunks, the library's rule for a shorter last.
+struct Config {
+  int32_t variant, split;
+};
+Config config_of(const CeArgs& a, const CePlan& p, int which, int64_t R) {
+  if (a.configs == nullptr || R != p.R) return {TILEC_VARIANT_AUTO, 0};
+  return {a.configs[2 * which], a.configs[2 * which + 1]};
+}
+
+// Where a configuration is refused, the product's own call says so.
+size_t matmul_scratch(const CeArgs& a, Config c, int64_t M, int64_t N, int64_t K, int64_t ld1, int64_t ld2, int layout,
                       size_t* counters) {
   size_t ws = 0, cnt = 0;
-  if (tilec_matmul_scratch_bytes(M, N, K, ld1, ld2, layout, a.dtype, TILEC_VARIANT_AUTO, 0, &ws, &cnt) != TILEC_OK)
+  if (tilec_matmul_scratch_bytes(M, N, K, ld1, ld2, layout, a.dtype, c.variant, c.split, &ws, &cnt) != TILEC_OK)
     return 0;
   *counters = std::max(*counters, cnt);
   return ws;
@@ -522,14 +659,13 @@ CePlan make_plan(const CeArgs& a) {
   if (a.chunk_rows > 0) p.R = a.chunk_rows;
   p.R = std::min({a.N, p.R, kMaxChunkRows});
   p.chunks = cdiv(a.N, p.R);
-  p.Hp = a.H;
+  p.Hp = cdiv(a.H, bf16 ? 64 : 4) * (bf16 ? 64 : 4);
   if (bf16) {
     auto fits = [&](const void* q, int64_t ld) {
       return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % 8 == 0 && ld < (int64_t(1) << 22);
     };
     p.pad = a.H % 8 != 0 || !fits(a.w, a.ldw) || !fits(a.x, a.ldx);
-    if (p.pad) p.Hp = cdiv(a.H, 64) * 64;
-    p.p1 = choose(a.V, p.R, p.Hp, false);
+    p.p1 = choose(a.V, p.R, a.H, false);
     p.p2 = choose(a.H, p.R, a.V, true);
     p.p3 = choose(a.H, a.V, p.R, true);
     p.shift = group_shift(p.p1.tile);
@@ -540,7 +676,7 @@ CePlan make_plan(const CeArgs& a) {
     p.shift = 12;
     p.groups = (int)cdiv(a.V, kGroup32);
   }
-  p.copy_x = a.grad || p.pad;
+  p.copy_x = a.grad || p.pad || (bf16 && p.Hp != a.H);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -551,24 +687,27 @@ CePlan make_plan(const CeArgs& a) {
   p.tlogit = take((size_t)p.R * sizeof(float));
   p.rows = take(a.reduction == kNone ? 0 : (size_t)a.N * sizeof(float));
   p.scale = take(sizeof(float));
-  p.xs = take(p.copy_x ? (size_t)(p.R * (bf16 ? p.Hp : cdiv(a.H, 4) * 4) * esz) : 0);
+  p.xs = take(p.copy_x ? (size_t)(p.R * p.Hp * esz) : 0);
+  p.few = bf16 && a.grad && p.chunks == 1 && p.R <= kFewRows;
+  p.xt = take(p.few ? (size_t)(a.H * kFewRows * 2) : 0);
   p.wp = take(p.pad ? (size_t)(a.V * p.Hp * esz) : 0);
   p.keep = take(a.grad || !bf16 ? (size_t)(p.R * p.Vp * esz) : 0);
-  p.acc = take(a.grad && p.chunks > 1 ? (size_t)(a.V * cdiv(a.H, 4) * 4) * sizeof(float) : 0);
+  p.acc = take(a.grad && p.chunks > 1 ? (size_t)(a.V * sum_ld(a.H)) * sizeof(float) : 0);
   if (bf16) {
     if (a.grad) {
-      p.split_bytes = std::max(split_workspace(p.p2, a.H, p.R), split_workspace(p.p3, a.H, a.V));
-      p.counter_bytes = std::max(split_counters(p.p2, a.H, p.R), split_counters(p.p3, a.H, a.V));
+      p.split_bytes = std::max(split_workspace(p.p2, a.H, p.R), p.few ? 0 : split_workspace(p.p3, a.H, a.V));
     }
   } else {
-    const int64_t ldxs = p.copy_x ? cdiv(a.H, 4) * 4 : a.ldx;
+    const int64_t ldxs = p.copy_x ? p.Hp : a.ldx;
     for (const int64_t R : {p.R, a.N - (p.chunks - 1) * p.R}) {
-      p.split_bytes = std::max(
-          p.split_bytes, matmul_scratch(a, R, a.V, a.H, ldxs, a.ldw, TILEC_X2_COL_MAJOR, &p.counter_bytes));
+      auto more = [&](int which, int64_t M, int64_t N, int64_t K, int64_t ld1, int64_t ld2, int layout) {
+        p.split_bytes = std::max(p.split_bytes, matmul_scratch(a, config_of(a, p, which, R), M, N, K, ld1, ld2, layout,
+                                                               &p.counter_bytes));
+      };
+      more(0, R, a.V, a.H, ldxs, a.ldw, TILEC_X2_COL_MAJOR);
       if (!a.grad) continue;
-      p.split_bytes = std::max(p.split_bytes, matmul_scratch(a, R, a.H, a.V, p.Vp, a.ldw, 0, &p.counter_bytes));
-      p.split_bytes = std::max(p.split_bytes, matmul_scratch(a, a.V, a.H, R, p.Vp, ldxs, TILEC_X1_COL_MAJOR,
-                                                             &p.counter_bytes));
+      more(1, R, a.H, a.V, p.Vp, a.ldw, 0);
+      more(2, a.V, a.H, R, p.Vp, ldxs, TILEC_X1_COL_MAJOR);
     }
   }
   p.split = take(p.split_bytes);
@@ -588,13 +727,12 @@ unsigned grid_for(int64_t n) { return (unsigned)std::min<int64_t>(std::max<int64
 template <typename T>
 hipError_t run_prepare(const CeArgs& a, const CePlan& p, char* ws, int64_t r0, int64_t R, hipStream_t stream) {
   if (!p.copy_x) return hipSuccess;
-  const int64_t ld = sizeof(T) == 2 ? p.Hp : cdiv(a.H, 4) * 4;
   const bool count = a.grad && r0 == 0;
-  const unsigned blocks = grid_for(R * ld / (16 / (int64_t)sizeof(T)));
+  const unsigned blocks = grid_for(std::max(R * p.Hp / (16 / (int64_t)sizeof(T)), p.few ? kFewRows * a.H : 0));
   hipLaunchKernelGGL((ce_prepare_kernel<T>), dim3(blocks + (count ? 1 : 0)), dim3(256), 0, stream,
-                     static_cast<const T*>(a.x) + r0 * a.ldx, a.ldx, reinterpret_cast<T*>(ws + p.xs), ld, R, a.H,
+                     static_cast<const T*>(a.x) + r0 * a.ldx, a.ldx, reinterpret_cast<T*>(ws + p.xs), p.Hp, R, a.H,
                      a.target + r0, a.ignore, count ? reinterpret_cast<float*>(ws + p.scale) : nullptr, a.N, a.target,
-                     a.reduction, a.grad_loss);
+                     a.reduction, a.grad_loss, p.few ? reinterpret_cast<T*>(ws + p.xt) : nullptr);
   return hipGetLastError();
 }
 
@@ -618,12 +756,46 @@ hipError_t run_rows(const CeArgs& a, const CePlan& p, char* ws, int64_t r0, int6
   return hipGetLastError();
 }
 
-hipError_t run_bf16(const CeArgs& a, const CePlan& p, char* ws, unsigned* counters, hipStream_t stream) {
+// The sum or mean of the losses, beside the joining of a gradient's splits
+// where one is left to do.
+hipError_t run_join(const CeArgs& a, const CePlan& p, char* ws, CeJoin q, bool loss, hipStream_t stream) {
+  if (loss && a.reduction != kNone) {
+    q.loss = a.loss;
+    q.row_loss = reinterpret_cast<const float*>(ws + p.rows);
+    q.target = a.target, q.N = a.N, q.ignore = a.ignore, q.reduction = a.reduction;
+  }
+  q.lanes = q.splits >= 32 ? 8 : q.splits >= 8 ? 2 : 1;
+  const int64_t groups = q.rows * q.ld / 4 * q.lanes;
+  const unsigned grid = (groups > 0 ? grid_for(groups) : 0) + (q.loss != nullptr ? 1 : 0);
+  if (grid == 0) return hipSuccess;
+  hipLaunchKernelGGL(ce_join_kernel, dim3(grid), dim3(256), 0, stream, q);
+  return hipGetLastError();
+}
+
+// One gradient: its product, in splits or not, and what joins them.  `acc`:
+// fp32 sums over the chunks (NULL: one chunk), written to `out` by the last.
+template <bool CB>
+hipError_t run_grad(const CeArgs& a, const CePlan& p, char* ws, const Operands& o, const CeProduct& c, u16* out,
+                    float* acc, bool add, bool loss, hipStream_t stream) {
+  const float* scale = reinterpret_cast<const float*>(ws + p.scale);
+  float* part = reinterpret_cast<float*>(ws + p.split);
+  const int64_t ld = sum_ld(a.H);
+  const int64_t splits = gemm_split_geom(o.K, 64, c.splits).splits;
+  CeGrad g{out, a.H, acc, ld, 0, add, scale};
+  if (splits > 1) g = CeGrad{nullptr, 0, part, ld, o.N * ld, false, nullptr};
+  CE_TRY((run_product<kKRows, true, CB>(o, g, c, stream)));
+  CeJoin q{};
+  if (splits > 1) {
+    q.part = part, q.splits = (int)splits, q.rows = o.N, q.cols = a.H, q.ld = ld;
+    q.out = out, q.acc = acc, q.add = add, q.scale = scale;
+  }
+  return run_join(a, p, ws, q, loss, stream);
+}
+
+hipError_t run_bf16(const CeArgs& a, const CePlan& p, char* ws, hipStream_t stream) {
   const u16 *x = static_cast<const u16*>(a.x), *w = static_cast<const u16*>(a.w);
   u16* xs = reinterpret_cast<u16*>(ws + p.xs);
   u16* keep = reinterpret_cast<u16*>(ws + p.keep);
-  float* split = reinterpret_cast<float*>(ws + p.split);
-  const float* scale = reinterpret_cast<const float*>(ws + p.scale);
   int64_t ldw = a.ldw;
   if (p.pad) {
     u16* wp = reinterpret_cast<u16*>(ws + p.wp);
@@ -632,6 +804,7 @@ hipError_t run_bf16(const CeArgs& a, const CePlan& p, char* ws, unsigned* counte
   }
   for (int64_t c = 0; c < p.chunks; ++c) {
     const int64_t r0 = c * p.R, R = std::min(p.R, a.N - r0);
+    const bool last = c + 1 == p.chunks;
     CE_TRY(run_prepare<u16>(a, p, ws, r0, R, stream));
     const u16* xc = p.copy_x ? xs : x + r0 * a.ldx;
     const int64_t ldx = p.copy_x ? p.Hp : a.ldx;
@@ -641,23 +814,34 @@ hipError_t run_bf16(const CeArgs& a, const CePlan& p, char* ws, unsigned* counte
                 p.groups,
                 a.target + r0,
                 reinterpret_cast<float*>(ws + p.tlogit)};
-    const Operands o1{w, xc, ldw, ldx, a.V, R, p.Hp};
-    CE_TRY(p.Hp % 64 == 0
-               ? (run_product<kKFull, false, true, 16>(o1, le, p.p1, nullptr, nullptr, stream))
-               : (run_product<kKMasked, false, true, 32>(o1, le, p.p1, nullptr, nullptr, stream)));
+    // Rows of x end in zeros to a whole K step, rows of W only where it was
+    // copied.
+    if (p.pad || a.H % 64 == 0)
+      CE_TRY((run_product<kKFull, false, true>(Operands{w, xc, ldw, ldx, a.V, R, p.Hp}, le, p.p1, stream)));
+    else
+      CE_TRY((run_product<kKColsA, false, true>(Operands{w, xc, ldw, ldx, a.V, R, a.H}, le, p.p1, stream)));
     CE_TRY(run_rows<u16>(a, p, ws, r0, R, stream));
-    if (!a.grad) continue;
-    // dx^T [H, R] = W^T d^T over the vocabulary; d is padded with zeros to
+    if (!a.grad) {
+      if (last) CE_TRY(run_join(a, p, ws, CeJoin{}, true, stream));
+      continue;
+    }
+    // dx^T [H, R] = W^T d^T over the vocabulary, first, while d is in the caches
+    // (1000 rows x 50021: 110 us, 130 after dW); d is padded with zeros to
     // whole K steps, W ends with its rows.
-    CeGrad gx{static_cast<u16*>(a.dx) + r0 * a.H, a.H, nullptr, 0, false, scale};
-    CE_TRY((run_product<kKRows, true, true, 16>(Operands{w, keep, ldw, p.Vp, a.H, R, a.V}, gx, p.p2, split, counters,
-                                                stream)));
+    CE_TRY(run_grad<true>(a, p, ws, Operands{w, keep, ldw, p.Vp, a.H, R, a.V}, p.p2,
+                          static_cast<u16*>(a.dx) + r0 * a.H, nullptr, false, last, stream));
     // dW^T [H, V] = x^T d over the chunk's rows.
-    const bool last = c + 1 == p.chunks;
-    CeGrad gw{last ? static_cast<u16*>(a.dw) : nullptr, a.H, p.chunks > 1 ? reinterpret_cast<float*>(ws + p.acc) : nullptr,
-              cdiv(a.H, 4) * 4, c > 0, scale};
-    CE_TRY((run_product<kKRows, true, false, 16>(Operands{xs, keep, p.Hp, p.Vp, a.H, a.V, R}, gw, p.p3, split,
-                                                 counters, stream)));
+    u16* dw = static_cast<u16*>(a.dw);
+    if (p.few) {
+      const unsigned gx = (unsigned)cdiv(a.H, 128);
+      const unsigned gy = (unsigned)std::min<int64_t>(cdiv(a.V, 64), std::max<int64_t>(1, 4 * device_cus() / gx));
+      hipLaunchKernelGGL(ce_few_rows_kernel, dim3(gx, gy), dim3(256), 0, stream, keep, p.Vp,
+                         reinterpret_cast<const u16*>(ws + p.xt), dw, (int)R, (int)a.H, (int)a.V, reinterpret_cast<const float*>(ws + p.scale));
+      CE_TRY(hipGetLastError());
+    } else {
+      CE_TRY(run_grad<false>(a, p, ws, Operands{xs, keep, p.Hp, p.Vp, a.H, a.V, R}, p.p3, last ? dw : nullptr,
+                             p.chunks > 1 ? reinterpret_cast<float*>(ws + p.acc) : nullptr, c > 0, false, stream));
+    }
   }
   return hipSuccess;
 }
@@ -668,10 +852,11 @@ int run_f32(const CeArgs& a, const CePlan& p, char* ws, unsigned* counters, size
   float* xs = reinterpret_cast<float*>(ws + p.xs);
   float* keep = reinterpret_cast<float*>(ws + p.keep);
   float* part = reinterpret_cast<float*>(ws + p.acc);
-  const int64_t ldxs = cdiv(a.H, 4) * 4;
-  auto product = [&](const float* x1, const float* x2, float* out, int64_t M, int64_t N, int64_t K, int64_t ld1,
-                     int64_t ld2, int64_t ldo, int layout) {
-    return tilec_matmul(x1, x2, out, M, N, K, ld1, ld2, ldo, layout, TILEC_F32, TILEC_VARIANT_AUTO, 0, ws + p.split,
+  const int64_t ldxs = p.Hp;
+  auto product = [&](int which, int64_t R, const float* x1, const float* x2, float* out, int64_t M, int64_t N,
+                     int64_t K, int64_t ld1, int64_t ld2, int64_t ldo, int layout) {
+    const Config c = config_of(a, p, which, R);
+    return tilec_matmul(x1, x2, out, M, N, K, ld1, ld2, ldo, layout, TILEC_F32, c.variant, c.split, ws + p.split,
                         p.split_bytes, counters, counter_bytes, stream);
   };
   for (int64_t c = 0; c < p.chunks; ++c) {
@@ -679,22 +864,23 @@ int run_f32(const CeArgs& a, const CePlan& p, char* ws, unsigned* counters, size
     if ((*err = run_prepare<float>(a, p, ws, r0, R, stream)) != hipSuccess) return TILEC_ERR_HIP;
     const float* xc = p.copy_x ? xs : x + r0 * a.ldx;
     const int64_t ldx = p.copy_x ? ldxs : a.ldx;
-    int rc = product(xc, w, keep, R, a.V, a.H, ldx, a.ldw, p.Vp, TILEC_X2_COL_MAJOR);
+    int rc = product(0, R, xc, w, keep, R, a.V, a.H, ldx, a.ldw, p.Vp, TILEC_X2_COL_MAJOR);
     if (rc != TILEC_OK) return rc;
     hipLaunchKernelGGL(ce_stats_kernel, dim3((unsigned)R, (unsigned)p.groups), dim3(256), 0, stream, keep, p.Vp, a.V,
                        a.target + r0, reinterpret_cast<f32x2*>(ws + p.stat), reinterpret_cast<float*>(ws + p.tlogit));
     if ((*err = hipGetLastError()) != hipSuccess) return TILEC_ERR_HIP;
     if ((*err = run_rows<float>(a, p, ws, r0, R, stream)) != hipSuccess) return TILEC_ERR_HIP;
     if (!a.grad) continue;
-    rc = product(keep, w, static_cast<float*>(a.dx) + r0 * a.H, R, a.H, a.V, p.Vp, a.ldw, a.H, 0);
+    rc = product(1, R, keep, w, static_cast<float*>(a.dx) + r0 * a.H, R, a.H, a.V, p.Vp, a.ldw, a.H, 0);
     if (rc != TILEC_OK) return rc;
     float* dw = static_cast<float*>(a.dw);
-    rc = product(keep, xs, c == 0 ? dw : part, a.V, a.H, R, p.Vp, ldxs, a.H, TILEC_X1_COL_MAJOR);
+    rc = product(2, R, keep, xs, c == 0 ? dw : part, a.V, a.H, R, p.Vp, ldxs, a.H, TILEC_X1_COL_MAJOR);
     if (rc != TILEC_OK) return rc;
     if (c == 0) continue;
     hipLaunchKernelGGL(ce_add_kernel, dim3(grid_for(a.V * a.H)), dim3(256), 0, stream, dw, part, a.V * a.H);
     if ((*err = hipGetLastError()) != hipSuccess) return TILEC_ERR_HIP;
   }
+  if ((*err = run_join(a, p, ws, CeJoin{}, true, stream)) != hipSuccess) return TILEC_ERR_HIP;
   return TILEC_OK;
 }
 
@@ -730,31 +916,34 @@ extern "C" {
 
 int tilec_linear_ce_scratch_bytes(const void* x, const void* weight, int64_t N, int64_t H, int64_t V, int64_t ldx,
                                   int64_t ldw, int32_t dtype, int32_t reduction, int32_t grad, int64_t chunk_rows,
-                                  size_t* workspace_bytes, size_t* counter_bytes) {
+                                  const int32_t* configs, size_t* workspace_bytes, size_t* counter_bytes,
+                                  int64_t* rows_per_chunk) {
   clear_error();
   if (workspace_bytes) *workspace_bytes = 0;
   if (counter_bytes) *counter_bytes = 0;
+  if (rows_per_chunk) *rows_per_chunk = 0;
   CeArgs a{};
   a.x = x, a.w = weight, a.N = N, a.H = H, a.V = V, a.ldx = ldx, a.ldw = ldw, a.dtype = dtype;
-  a.reduction = reduction, a.grad = grad != 0, a.chunk_rows = chunk_rows;
+  a.reduction = reduction, a.grad = grad != 0, a.chunk_rows = chunk_rows, a.configs = configs;
   const int rc = check(a);
   if (rc != TILEC_OK || N == 0) return rc;
   const CePlan p = make_plan(a);
   clear_error();
   if (workspace_bytes) *workspace_bytes = p.bytes;
   if (counter_bytes) *counter_bytes = p.counter_bytes;
+  if (rows_per_chunk) *rows_per_chunk = p.R;
   return TILEC_OK;
 }
 
 int tilec_linear_ce(const void* x, const void* weight, const int64_t* target, float* loss, const float* grad_loss,
                     void* dx, void* dweight, int64_t N, int64_t H, int64_t V, int64_t ldx, int64_t ldw, int32_t dtype,
-                    int32_t reduction, int64_t ignore_index, int32_t grad, int64_t chunk_rows, void* workspace,
-                    size_t workspace_bytes, void* counters, size_t counter_bytes, void* stream_ptr) {
+                    int32_t reduction, int64_t ignore_index, int32_t grad, int64_t chunk_rows, const int32_t* configs,
+                    void* workspace, size_t workspace_bytes, void* counters, size_t counter_bytes, void* stream_ptr) {
   clear_error();
   CeArgs a{};
   a.x = x, a.w = weight, a.target = target, a.loss = loss, a.grad_loss = grad_loss, a.dx = dx, a.dw = dweight;
   a.N = N, a.H = H, a.V = V, a.ldx = ldx, a.ldw = ldw, a.dtype = dtype, a.reduction = reduction;
-  a.ignore = ignore_index, a.grad = grad != 0, a.chunk_rows = chunk_rows;
+  a.ignore = ignore_index, a.grad = grad != 0, a.chunk_rows = chunk_rows, a.configs = configs;
   int rc = check(a);
   if (rc != TILEC_OK) return rc;
   if (a.grad && dweight == nullptr) return fail(TILEC_ERR_VALUE, "tilec: linear cross entropy: dweight is NULL");
@@ -780,16 +969,10 @@ int tilec_linear_ce(const void* x, const void* weight, const int64_t* target, fl
                   p.counter_bytes, counters == nullptr ? (size_t)0 : counter_bytes);
     char* ws = static_cast<char*>(workspace);
     if (dtype == TILEC_BF16) {
-      e = run_bf16(a, p, ws, static_cast<unsigned*>(counters), stream);
-      if (e != hipSuccess) return launched(e);
+      e = run_bf16(a, p, ws, stream);
     } else {
       rc = run_f32(a, p, ws, static_cast<unsigned*>(counters), counter_bytes, stream, &e);
-      if (rc != TILEC_OK) return e != hipSuccess ? launched(e) : rc;
-    }
-    if (reduction != kNone) {
-      hipLaunchKernelGGL(ce_loss_kernel, dim3(1), dim3(1024), 0, stream, reinterpret_cast<const float*>(ws + p.rows),
-                         target, N, ignore_index, reduction, loss);
-      e = hipGetLastError();
+      if (rc != TILEC_OK && e == hipSuccess) return rc;
     }
     return launched(e);
   }

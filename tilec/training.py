@@ -12,11 +12,12 @@ Like those two they are plain functions with no autograd of their own.
 
 import array
 import ctypes
+from functools import lru_cache
 
 import torch
 
 from . import _lib
-from .ext import counters_for, workspace_for
+from .ext import _tuned, counters_for, workspace_for
 
 __all__ = ["layer_norm", "layer_norm_backward", "linear_cross_entropy", "linear_cross_entropy_grad",
            "adamw_state", "adamw_step", "adamw_values", "ADAMW_BLOCK"]
@@ -178,6 +179,28 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, param_grads=True):
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
+@lru_cache(4096)
+def _ce_plan(N, H, V, ldx, ldw, dtype, code, grad, chunk_rows, x_off, w_off):
+    """(workspace bytes, counter bytes, configs) of a call; float32 products run
+    the tuned pick of their shapes, as `matrix_mul` does.  x_off, w_off: the
+    addresses modulo 16, all of them that the C side looks at."""
+    ws, cnt, rows = ctypes.c_size_t(0), ctypes.c_size_t(0), ctypes.c_int64(0)
+
+    def ask(configs):
+        _lib.check(_lib.lib().tilec_linear_ce_scratch_bytes(
+            x_off or 16, w_off or 16, N, H, V, ldx, ldw, dtype, code, grad, chunk_rows, configs, ctypes.byref(ws),
+            ctypes.byref(cnt), ctypes.byref(rows)))
+        return ws.value, cnt.value, configs
+
+    plan = ask(None)
+    R = rows.value
+    if dtype != _lib.F32 or R == 0:
+        return plan
+    picks = [_tuned(R, H, V, "f32", _lib.X2_COL_MAJOR)]
+    picks += [_tuned(R, V, H, "f32", 0), _tuned(V, R, H, "f32", _lib.X1_COL_MAJOR)] if grad else [(-1, 0)] * 2
+    return ask((ctypes.c_int32 * 6)(*[v for pick in picks for v in pick]))
+
+
 def _linear_ce(what, x, weight, target, reduction, ignore_index, grad, grad_loss, chunk_rows):
     if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
         raise ValueError(f"{what}: expected x [N, H] and weight [V, H], got shapes {tuple(x.shape)} and "
@@ -211,19 +234,17 @@ def _linear_ce(what, x, weight, target, reduction, ignore_index, grad, grad_loss
     loss = torch.empty((N,) if reduction == "none" else (), dtype=torch.float32, device=x.device)
     dx = torch.empty((N, H), dtype=x.dtype, device=x.device) if grad else None
     dw = torch.empty((V, H), dtype=x.dtype, device=x.device) if grad else None
-    L = _lib.lib()
     code = _REDUCTIONS[reduction]
     with _on(x.device):
         stream = _stream(x.device)
-        ws, cnt = ctypes.c_size_t(0), ctypes.c_size_t(0)
-        _lib.check(L.tilec_linear_ce_scratch_bytes(x.data_ptr(), weight.data_ptr(), N, H, V, ldx, ldw, dtype, code,
-                                                   grad, chunk_rows, ctypes.byref(ws), ctypes.byref(cnt)))
-        ws_ptr = workspace_for(x.device, stream, ws.value).data_ptr() if ws.value else None
-        cnt_ptr = counters_for(x.device, stream, cnt.value).data_ptr() if cnt.value else None
-        _lib.check(L.tilec_linear_ce(x.data_ptr(), weight.data_ptr(), target.data_ptr(), loss.data_ptr(),
-                                     _ptr(grad_loss), _ptr(dx), _ptr(dw), N, H, V, ldx, ldw, dtype, code,
-                                     int(ignore_index), grad, chunk_rows, ws_ptr, ws.value, cnt_ptr, cnt.value,
-                                     stream))
+        ws, cnt, configs = _ce_plan(N, H, V, ldx, ldw, dtype, code, grad, chunk_rows, x.data_ptr() % 16,
+                                    weight.data_ptr() % 16)
+        ws_ptr = workspace_for(x.device, stream, ws).data_ptr() if ws else None
+        cnt_ptr = counters_for(x.device, stream, cnt).data_ptr() if cnt else None
+        _lib.check(_lib.lib().tilec_linear_ce(x.data_ptr(), weight.data_ptr(), target.data_ptr(), loss.data_ptr(),
+                                              _ptr(grad_loss), _ptr(dx), _ptr(dw), N, H, V, ldx, ldw, dtype, code,
+                                              int(ignore_index), grad, chunk_rows, configs, ws_ptr, ws, cnt_ptr, cnt,
+                                              stream))
     return loss, dx, dw
 
 
