@@ -159,23 +159,57 @@ __device__ __forceinline__ f32x4 v_values(uint32_t codes, float scale) {
   return r;
 }
 
-// The codes of 4 values; scale > 0, or 1 for a block of zeros.
+// The codes of 4 values; scale > 0, or 1 for a block of zeros.  The code is by
+// definition that of correctly rounded quotients and roots, which are long
+// sequences; an approximation (a product with 1 / scale and the hardware's
+// root, together under 2^-21 of the result, so 2e-5 and 5e-5 of a code) settles
+// all values but those within 1e-4 of a code from halfway between two, two in
+// ten thousand.  Scales outside 2^-60 .. 2^100, where the approximation could
+// leave the range of normal numbers, go the long way.  (151 M values: 627 us
+// the long way for all, 3.9 TB/s.)
+__device__ __forceinline__ bool plain_scale(float s) { return s >= 0x1p-60f && s <= 0x1p100f; }
+__device__ __forceinline__ bool near_half(float t) { return fabsf(fabsf(t - rintf(t)) - 0.5f) < 1e-4f; }
+
 __device__ __forceinline__ uint32_t m_codes(f32x4 m, float scale) {
 #pragma clang fp contract(off)
+  float t[4];
+  const float inv = 1.f / scale;
+  bool exact = !plain_scale(scale);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    t[i] = __builtin_amdgcn_sqrtf(fabsf(m[i]) * inv) * 127.f;
+    exact |= near_half(t[i]);
+  }
+  if (exact) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = sqrtf(fabsf(m[i]) / scale) * 127.f;
+  }
   uint32_t w = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int c = (int)rintf(sqrtf(fabsf(m[i]) / scale) * 127.f);
+    const int c = (int)rintf(t[i]);
     w |= ((uint32_t)(m[i] < 0.f ? -c : c) & 255u) << (8 * i);
   }
   return w;
 }
 __device__ __forceinline__ uint32_t v_codes(f32x4 v, float scale) {
 #pragma clang fp contract(off)
+  float t[4];
+  const float inv = 1.f / scale;
+  bool exact = !plain_scale(scale);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    t[i] = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(v[i] * inv)) * 255.f;
+    exact |= near_half(t[i]);
+  }
+  if (exact) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = sqrtf(sqrtf(v[i] / scale)) * 255.f;
+  }
   uint32_t w = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    int c = (int)rintf(sqrtf(sqrtf(v[i] / scale)) * 255.f);
+    int c = (int)rintf(t[i]);
     c = v[i] > 0.f && c < 1 ? 1 : c;
     w |= ((uint32_t)c & 255u) << (8 * i);
   }

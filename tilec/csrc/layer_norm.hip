@@ -352,9 +352,21 @@ __global__ __launch_bounds__(NT) void norm_grad_kernel(NormArgs a) {
     }
   }
   if (!a.dw && !a.db) return;
-  // The rows that ran side by side in this workgroup, in order.
+  // The rows that ran side by side: within a wave by shuffles, then the waves
+  // in order through LDS.  (Through LDS alone, by a row's 8 threads, it took 25
+  // of the 28 us of a 20000 x 79 pass.)
   if constexpr (NT == 256) {
     if (rpb > 1) {
+      for (int o = tpr; o < 64; o <<= 1) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            dw[i][e] += __shfl_xor(dw[i][e], o);
+            db[i][e] += __shfl_xor(db[i][e], o);
+          }
+      }
+      const int stride = max(tpr, 64);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -367,7 +379,7 @@ __global__ __launch_bounds__(NT) void norm_grad_kernel(NormArgs a) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
               float t = sums[e * 256 + threadIdx.x];
-              for (int g = 1; g < rpb; ++g) t += sums[e * 256 + g * tpr + threadIdx.x];
+              for (int at = stride; at < 256; at += stride) t += sums[e * 256 + at + threadIdx.x];
               (k ? db[i][e] : dw[i][e]) = t;
             }
           }
@@ -448,24 +460,37 @@ __global__ __launch_bounds__(256) void norm_grad_cols_kernel(NormArgs a, const f
   if (a.dw || a.db) store_sums<E>(a, blockIdx.y, gridDim.y, c, dw, db);
 }
 
-// dw[c] and db[c]: the sums of `parts` partial rows, 32 columns a workgroup,
-// 32 threads a column (every 32nd row each, then those in order).  No parts: zeros.
+// dw[c] and db[c]: the sums of `parts` partial rows, 16 columns a workgroup,
+// 64 threads a column (every 64th row each, then those in order).  No parts: zeros.
 __global__ __launch_bounds__(1024) void norm_grad_sum_kernel(NormArgs a, int parts) {
-  __shared__ float red[32][33];
-  const int col = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int blocks = (a.D + 31) / 32;
+  __shared__ float red[64][17];
+  const int col = threadIdx.x & 15, g = threadIdx.x >> 4;
+  const int blocks = (a.D + 15) / 16;
   const int which = (int)blockIdx.x >= blocks;  // 0: dw, 1: db
   float* out = which ? a.db : a.dw;
   if (out == nullptr) return;
-  const int c = 32 * ((int)blockIdx.x - which * blocks) + col;
+  const int c = 16 * ((int)blockIdx.x - which * blocks) + col;
   float s = 0.f;
   if (c < a.D) {
-    for (int p = g; p < parts; p += 32) s += a.partial[(int64_t)(2 * p + which) * a.Dp + c];
+    const float* p = a.partial + (int64_t)which * a.Dp + c;
+#pragma unroll 8
+    for (int k = g; k < parts; k += 64) s += p[(int64_t)(2 * k) * a.Dp];
   }
   red[g][col] = s;
   __syncthreads();
+  // Each wave's first 16 threads take 4 rows of `red`, then one wave those 16.
+  if (g < 16) {
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s += red[4 * g + k][col];
+  }
+  __syncthreads();
+  if (g < 16) red[g][col] = s;
+  __syncthreads();
   if (g == 0 && c < a.D) {
-    for (int k = 1; k < 32; ++k) s += red[k][col];
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += red[k][col];
     out[c] = s;
   }
 }
@@ -476,8 +501,9 @@ struct NormGeom {
 };
 
 // The fewest idle lanes; then, with enough rows to fill the chip anyway, the
-// fewest threads a row (fewer steps of the sums, more loads in flight each),
-// and with few rows the most.
+// fewest threads a row (fewer steps of the sums, more loads in flight each) up
+// to 4 groups a thread (4099 x 3001 fp32, 1, 2, 4 and 8 groups: 42, 28, 23 and
+// 28 us), and with few rows the most.
 NormGeom norm_geom(int64_t R, int64_t D, int e, int max_nv) {
   const int64_t groups = cdiv(D, e);
   NormGeom best{0, 0, 0};
@@ -486,11 +512,11 @@ NormGeom norm_geom(int64_t R, int64_t D, int e, int max_nv) {
   for (int nv = 1; nv <= max_nv; nv *= 2) {
     int64_t tpr = 1;
     while (tpr * nv < groups) tpr *= 2;
-    if (tpr > (nv == 8 ? 256 : 1024)) continue;  // 16 waves have 128 registers each
+    if (tpr > 1024) continue;
     const int64_t w = tpr * nv;
     if (w < waste || (w == waste && many)) {
       waste = w;
-      best = {(int)tpr, nv, tpr <= 256 ? 256 : 1024};
+      best = {(int)tpr, nv, tpr <= 256 ? 256 : (int)tpr};
     }
   }
   return best;
@@ -501,14 +527,14 @@ constexpr int kMaxGrid = 1 << 20;  // workgroups; the row loops stride over the 
 template <typename TX, typename TY>
 hipError_t launch_norm(NormArgs a, hipStream_t stream) {
   constexpr int E = 16 / (int)sizeof(TX);
-  const NormGeom g = norm_geom(a.R, a.D, E, 8);
+  const NormGeom g = norm_geom(a.R, a.D, E, 4);
   if (g.nv == 0) {
     const unsigned grid = (unsigned)std::min<int64_t>(a.R, kMaxGrid);
     hipLaunchKernelGGL((norm_long_kernel<TX, TY>), dim3(grid), dim3(1024), 0, stream, a);
     return hipGetLastError();
   }
   a.tpr = g.tpr;
-  const int threads = g.nt == 256 ? 256 : g.tpr;
+  const int threads = g.nt;
   const dim3 grid((unsigned)std::min<int64_t>(cdiv(a.R, threads / g.tpr), kMaxGrid)), block(threads);
   auto go = [&](auto nv, auto nt) {
     hipLaunchKernelGGL((norm_kernel<TX, TY, decltype(nv)::value, decltype(nt)::value>), grid, block, 0, stream, a);
@@ -516,14 +542,13 @@ hipError_t launch_norm(NormArgs a, hipStream_t stream) {
   };
   using std::integral_constant;
   auto by_nv = [&](auto nt) {
-    if constexpr (decltype(nt)::value == 256) {
-      if (g.nv == 8) return go(integral_constant<int, 8>{}, nt);
-    }
     return g.nv == 1   ? go(integral_constant<int, 1>{}, nt)
            : g.nv == 2 ? go(integral_constant<int, 2>{}, nt)
                        : go(integral_constant<int, 4>{}, nt);
   };
-  return g.nt == 256 ? by_nv(integral_constant<int, 256>{}) : by_nv(integral_constant<int, 1024>{});
+  return g.nt == 256   ? by_nv(integral_constant<int, 256>{})
+         : g.nt == 512 ? by_nv(integral_constant<int, 512>{})
+                       : by_nv(integral_constant<int, 1024>{});
 }
 
 // The backward pass holds 16 columns a thread: their two sums, w, x and dy.
@@ -540,8 +565,12 @@ GradGeom grad_geom(int64_t R, int64_t D, int xsz) {
   q.g = norm_geom(R, D, e, 16 / e);
   q.Dp = cdiv(D, 8) * 8;
   if (q.g.nv > 0) {
-    const int rpb = q.g.nt == 256 ? 256 / q.g.tpr : 1;
-    q.parts = std::min<int64_t>(cdiv(R, rpb), 2 * (int64_t)device_cus());
+    const int rpb = q.g.nt / q.g.tpr;
+    // 8 waves a CU, and 12 for bf16, which has twice the arithmetic a byte:
+    // fewer leave the memory idle, more write more partials (8192 x 4096, 1, 2,
+    // 3 and 4 workgroups of 4 waves a CU: fp32 98, 83, 89, 92 us, bf16 74, 52,
+    // 49, 53; 4096 x 8192, 1 and 2 of 8 waves: fp32 88 and 95, bf16 60 and 53).
+    q.parts = std::min<int64_t>(cdiv(R, rpb), cdiv(xsz == 4 ? 8 : 12, q.g.nt / 64) * device_cus());
   } else {
     q.parts = std::min<int64_t>(R, std::max<int64_t>(1, cdiv(4 * (int64_t)device_cus(), cdiv(D, 256 * e))));
     q.c12_bytes = (size_t)(R * 2 * sizeof(float) + 15) / 16 * 16;
@@ -564,7 +593,7 @@ hipError_t launch_norm_grad(NormArgs a, const GradGeom& q, float* c12, hipStream
     e = hipGetLastError();
   } else if (a.R > 0) {
     a.tpr = q.g.tpr;
-    const dim3 grid((unsigned)q.parts), block(q.g.nt == 256 ? 256 : q.g.tpr);
+    const dim3 grid((unsigned)q.parts), block(q.g.nt);
     auto go = [&](auto nv, auto nt) {
       hipLaunchKernelGGL((norm_grad_kernel<TX, TY, decltype(nv)::value, decltype(nt)::value>), grid, block, 0, stream,
                          a);
@@ -577,10 +606,12 @@ hipError_t launch_norm_grad(NormArgs a, const GradGeom& q, float* c12, hipStream
       }
       return q.g.nv == 1 ? go(integral_constant<int, 1>{}, nt) : go(integral_constant<int, 2>{}, nt);
     };
-    e = q.g.nt == 256 ? by_nv(integral_constant<int, 256>{}) : by_nv(integral_constant<int, 1024>{});
+    e = q.g.nt == 256   ? by_nv(integral_constant<int, 256>{})
+        : q.g.nt == 512 ? by_nv(integral_constant<int, 512>{})
+                        : by_nv(integral_constant<int, 1024>{});
   }
   if (e != hipSuccess || (!a.dw && !a.db) || q.parts == 1) return e;
-  hipLaunchKernelGGL(norm_grad_sum_kernel, dim3((unsigned)(2 * cdiv(a.D, 32))), dim3(1024), 0, stream, a,
+  hipLaunchKernelGGL(norm_grad_sum_kernel, dim3((unsigned)(2 * cdiv(a.D, 16))), dim3(1024), 0, stream, a,
                      (int)q.parts);
   return hipGetLastError();
 }

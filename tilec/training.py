@@ -13,6 +13,8 @@ Like those two they are plain functions with no autograd of their own.
 import array
 import ctypes
 from functools import lru_cache
+from itertools import chain
+from operator import attrgetter
 
 import torch
 
@@ -33,12 +35,14 @@ def _code(what, t):
 
 
 def _on_gpu(what, first, *others):
-    """All tensors (None: absent) on the one GPU of `first`."""
-    if first.device.type != "cuda":
+    """The index of the one GPU that all tensors (None: absent) are on."""
+    if not first.is_cuda:
         raise TypeError(f"{what} needs tensors on a ROCm GPU (got {first.device})")
+    at = first.get_device()
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != at:
             raise TypeError(f"{what} needs all tensors on one GPU (got {first.device} and {t.device})")
+    return at
 
 
 def _rows(what, name, x):
@@ -68,17 +72,9 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-class _on:
-    """The tensors' device as the current one, where it is not."""
-
-    def __new__(cls, device):
-        if device.index == torch.cuda.current_device():
-            return _HERE
-        return torch.cuda.device(device)
+# Per call these cost less than torch.cuda.current_stream and current_device,
+# which build objects and check for initialisation (a GPU tensor is at hand).
+_raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 class _Here:
@@ -92,12 +88,18 @@ class _Here:
 _HERE = _Here()
 
 
+def _on(index):
+    """The GPU of that index as the current one, where it is not."""
+    return _HERE if index == _current() else torch.cuda.device(index)
+
+
 def _norm_params(what, D, weight, bias):
     weight, bias = _vector(what, "weight", weight, D), _vector(what, "bias", bias, D)
-    codes = {_code(what, t) for t in (weight, bias) if t is not None}
-    if len(codes) > 1:
+    if weight is None:
+        return weight, bias, _lib.F32 if bias is None else _code(what, bias)
+    if bias is not None and bias.dtype != weight.dtype:
         raise TypeError(f"{what}: weight and bias have different types ({weight.dtype} and {bias.dtype})")
-    return weight, bias, codes.pop() if codes else _lib.F32
+    return weight, bias, _code(what, weight)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, dtype=None):
@@ -115,7 +117,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, dtype=None):
     """
     what = "layer_norm"
     shape = x.shape
-    _on_gpu(what, x, weight, bias)
+    at = _on_gpu(what, x, weight, bias)
     x_code = _code(what, x)
     x, ldx = _rows(what, "x", x)
     R, D = x.shape
@@ -124,13 +126,13 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, dtype=None):
     weight, bias, w_code = _norm_params(what, D, weight, bias)
     y = torch.empty(shape, dtype=dtype or x.dtype, device=x.device)
     y_code = _code(what, y)
-    stats = torch.empty((2, R), dtype=torch.float32, device=x.device)
-    mean, rstd = stats[0], stats[1]
+    mean = torch.empty(R, dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
     if R:
-        with _on(x.device):
+        with _on(at):
             _lib.check(_lib.lib().tilec_layer_norm(
                 x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), R, D, ldx, D,
-                x_code, y_code, w_code, eps, _stream(x.device)))
+                x_code, y_code, w_code, eps, _raw_stream(at)))
     return y, mean, rstd
 
 
@@ -147,7 +149,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, param_grads=True):
     """
     what = "layer_norm_backward"
     shape = dy.shape
-    _on_gpu(what, dy, x, mean, rstd, weight)
+    at = _on_gpu(what, dy, x, mean, rstd, weight)
     y_code, x_code = _code(what, dy), _code(what, x)
     if dy.shape != x.shape:
         raise ValueError(f"{what}: dy has shape {tuple(shape)}, x {tuple(x.shape)}")
@@ -162,12 +164,13 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, param_grads=True):
     dx = torch.empty(shape, dtype=dy.dtype, device=dy.device)
     dw = db = None
     if param_grads:
-        dw, db = torch.empty((2, D), dtype=torch.float32, device=dy.device)
+        dw = torch.empty(D, dtype=torch.float32, device=dy.device)
+        db = torch.empty_like(dw)
     elif R == 0:
         return dx, None, None
     L = _lib.lib()
-    with _on(dy.device):
-        stream = _stream(dy.device)
+    with _on(at):
+        stream = _raw_stream(at)
         need = L.tilec_layer_norm_backward_workspace_bytes(R, D, x_code)
         ws_ptr = workspace_for(dy.device, stream, need).data_ptr() if need else None
         _lib.check(L.tilec_layer_norm_backward(
@@ -220,7 +223,7 @@ def _linear_ce(what, x, weight, target, reduction, ignore_index, grad, grad_loss
         raise TypeError(f"{what}: x has dtype {x.dtype}, weight {weight.dtype}")
     if target.dtype != torch.int64:
         raise TypeError(f"{what}: target has dtype {target.dtype}, expected torch.int64")
-    _on_gpu(what, x, weight, target, grad_loss)
+    at = _on_gpu(what, x, weight, target, grad_loss)
     if grad_loss is not None:
         want = (N,) if reduction == "none" else ()
         if grad_loss.dtype != torch.float32:
@@ -235,8 +238,8 @@ def _linear_ce(what, x, weight, target, reduction, ignore_index, grad, grad_loss
     dx = torch.empty((N, H), dtype=x.dtype, device=x.device) if grad else None
     dw = torch.empty((V, H), dtype=x.dtype, device=x.device) if grad else None
     code = _REDUCTIONS[reduction]
-    with _on(x.device):
-        stream = _stream(x.device)
+    with _on(at):
+        stream = _raw_stream(at)
         ws, cnt, configs = _ce_plan(N, H, V, ldx, ldw, dtype, code, grad, chunk_rows, x.data_ptr() % 16,
                                     weight.data_ptr() % 16)
         ws_ptr = workspace_for(x.device, stream, ws).data_ptr() if ws else None
@@ -288,7 +291,7 @@ ADAMW_BLOCK = 256  # values per scale of an 8-bit state
 
 # A tensor's record for tilec_adamw (include/tilec.h, tilec_adamw_tensor): 8
 # pointers and sizes and two 32-bit type codes, the parameter's low.
-_BF16_PARAM, _BF16_GRAD = _lib.BF16, _lib.BF16 << 32
+_TYPES = {(p, g): _CODES[p] | _CODES[g] << 32 for p in _CODES for g in _CODES}
 
 
 def adamw_state(param, bits=32):
@@ -306,17 +309,21 @@ def adamw_state(param, bits=32):
             (torch.zeros(param.shape, dtype=torch.uint8, device=param.device), scales[1]))
 
 
+_numel, _data_ptr = torch.Tensor.numel, torch.Tensor.data_ptr
+_get_device, _is_contiguous, _dtype = torch.Tensor.get_device, torch.Tensor.is_contiguous, attrgetter("dtype")
+
+
 def _same(what, name, tensors, numels, dtypes, device):
     """Contiguous tensors of the given sizes and types on one device."""
-    if [t.numel() for t in tensors] != numels:
+    if list(map(_numel, tensors)) != numels:
         raise ValueError(f"{what}: {name} and params differ in number or sizes")
-    wrong = {t.dtype for t in tensors}.difference(dtypes)
+    wrong = set(map(_dtype, tensors)).difference(dtypes)
     if wrong:
         raise TypeError(f"{what}: {name} has a tensor of dtype {wrong.pop()}, expected "
                         f"{' or '.join(str(d) for d in dtypes)}")
-    if {t.get_device() for t in tensors} - {device}:
+    if set(map(_get_device, tensors)) - {device}:
         raise TypeError(f"{what} needs all tensors on one ROCm GPU ({name} has others)")
-    if not all([t.is_contiguous() for t in tensors]):
+    if not all(map(_is_contiguous, tensors)):
         raise ValueError(f"{what}: {name} has a tensor that is not contiguous")
 
 
@@ -357,7 +364,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
         raise ValueError(f"{what}: steps count from 1 (got {step})")
     if not params:
         return
-    if None in [g if g is None else 0 for g in grads]:
+    if any(g is None for g in grads):
         have = [i for i, g in enumerate(grads) if g is not None]
         if not have:
             return
@@ -366,10 +373,11 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     if params[0].device.type != "cuda":
         raise TypeError(f"{what} needs tensors on a ROCm GPU (got {params[0].device})")
     device = params[0].get_device()
-    numels = [p.numel() for p in params]
+    numels = list(map(_numel, params))
     floats = (torch.float32, torch.bfloat16)
     _same(what, "params", params, numels, floats, device)
-    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    if not all(map(_is_contiguous, grads)):
+        grads = [g.contiguous() for g in grads]
     _same(what, "grads", grads, numels, floats, device)
     m, ms = _split_state(what, "exp_avg", exp_avg)
     v, vs = _split_state(what, "exp_avg_sq", exp_avg_sq)
@@ -383,15 +391,14 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
         blocks = [-(-n // ADAMW_BLOCK) for n in numels]
         _same(what, "exp_avg's scales", ms, blocks, (torch.float32,), device)
         _same(what, "exp_avg_sq's scales", vs, blocks, (torch.float32,), device)
-        ms_at, vs_at = [t.data_ptr() for t in ms], [t.data_ptr() for t in vs]
+        ms_at, vs_at = map(_data_ptr, ms), map(_data_ptr, vs)
     if copies is not None:
         given = [(c, n) for c, n in zip(copies, numels) if c is not None]
         _same(what, "copies", [c for c, _ in given], [n for _, n in given], (torch.bfloat16,), device)
         copies_at = [0 if c is None else c.data_ptr() for c in copies]
-    p_at = [p.data_ptr() for p in params]
+    p_at = list(map(_data_ptr, params))
     # One memory for two parameters (a tied weight given twice) would be a race.
-    held = [a for a, n in zip(p_at, numels) if n]
-    if len(set(held)) < len(held):
+    if len(set(p_at)) < len(p_at) and len({a for a, n in zip(p_at, numels) if n}) < len(numels) - numels.count(0):
         raise ValueError(f"{what}: two params share their memory")
     if grad_scale is not None:
         if grad_scale.dtype != torch.float32 or grad_scale.get_device() != device:
@@ -399,15 +406,12 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
                             f"{grad_scale.device})")
         if grad_scale.numel() != 1:
             raise ValueError(f"{what}: grad_scale has shape {tuple(grad_scale.shape)}, expected one value")
-    types = [(_BF16_PARAM if p.dtype == torch.bfloat16 else 0) | (_BF16_GRAD if g.dtype == torch.bfloat16 else 0)
-             for p, g in zip(params, grads)]
-    table = array.array("q", [x for record in zip(p_at, [g.data_ptr() for g in grads], [t.data_ptr() for t in m],
-                                                  [t.data_ptr() for t in v], ms_at, vs_at, copies_at, numels, types)
-                              for x in record])
-    where = params[0].device
-    with _on(where):
+    types = map(_TYPES.__getitem__, zip(map(_dtype, params), map(_dtype, grads)))
+    table = array.array("q", chain.from_iterable(zip(p_at, map(_data_ptr, grads), map(_data_ptr, m), map(_data_ptr, v),
+                                                     ms_at, vs_at, copies_at, numels, types)))
+    with _on(device):
         _lib.check(_lib.lib().tilec_adamw(table.buffer_info()[0], len(params), 32 if ms is None else 8, step, lr,
-                                          betas[0], betas[1], eps, weight_decay, _ptr(grad_scale), _stream(where)))
+                                          betas[0], betas[1], eps, weight_decay, _ptr(grad_scale), _raw_stream(device)))
 
 
 def adamw_values(states):
@@ -432,6 +436,6 @@ def adamw_values(states):
         m = (c.data_ptr(), 0, s.data_ptr(), 0) if c.dtype == torch.int8 else (0, c.data_ptr(), 0, s.data_ptr())
         records += (o.data_ptr(), 0, *m, 0, n, 0)
     table = array.array("q", records)
-    with _on(where):
-        _lib.check(_lib.lib().tilec_adamw_values(table.buffer_info()[0], len(out), _stream(where)))
+    with _on(device):
+        _lib.check(_lib.lib().tilec_adamw_values(table.buffer_info()[0], len(out), _raw_stream(device)))
     return out
