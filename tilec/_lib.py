@@ -78,6 +78,17 @@ def lib():
     return L
 
 
+@lru_cache(None)
+def host():
+    """The module tilec._host (csrc/host.cpp); raise if it has not been built."""
+    try:
+        from . import _host
+    except ImportError as e:
+        raise LibraryMissing(f"tilec/_host.so is not built or does not load ({e}); run `python -m tilec.build` "
+                             "(or __graft_entry__.build()) first") from e
+    return _host
+
+
 def last_error():
     return lib().tilec_last_error().decode(errors="replace")
 

@@ -5,6 +5,8 @@
 Each .hip file under csrc/ is compiled to an object in csrc/_build/ in
 parallel, then linked into tilec/libtilec_hip.so, which ext.py loads with
 ctypes.  The library is written for MI355X only (--offload-arch=gfx950).
+csrc/host.cpp, host code that reads torch tensors, becomes the Python module
+tilec/_host.so beside it.
 """
 
 import concurrent.futures as cf
@@ -13,11 +15,13 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJDIR = os.path.join(CSRC, "_build")
 LIB = os.path.join(HERE, "libtilec_hip.so")
+HOST = os.path.join(HERE, "_host.so")
 ARCH = "gfx950"
 
 # -packed-fp32-ops: keep v_pk_{add,mul,fma}_f32 out of the generated code.
@@ -44,11 +48,30 @@ def _compile(src):
     return obj
 
 
+def _host():
+    """tilec/_host.so: a CPython module against torch's headers and libraries."""
+    import torch
+    from torch.utils import cpp_extension
+    torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    tmp = HOST + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I" + sysconfig.get_paths()["include"], *("-isystem" + p for p in cpp_extension.include_paths()),
+           os.path.join(CSRC, "host.cpp"), "-o", tmp, "-L" + torch_lib, "-Wl,-rpath," + torch_lib,
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"building {HOST} failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, HOST)
+
+
 def build(verbose=False):
     os.makedirs(OBJDIR, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
-    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
+        host = ex.submit(_host)
         objs = list(ex.map(_compile, srcs))
+        host.result()
     tmp = LIB + ".tmp"
     # --no-undefined: a kernel whose host stub the compiler dropped fails here,
     # not when the library is first loaded.
@@ -58,7 +81,7 @@ def build(verbose=False):
         raise RuntimeError(f"link failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
     if verbose:
-        print(f"built {LIB}")
+        print(f"built {LIB} and {HOST}")
     return LIB
 
 

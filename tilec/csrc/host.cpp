@@ -1,0 +1,163 @@
+// tilec._host: what a step over many tensors needs of them, read in C++.
+//
+//   adamw_table(params, grads, exp_avg, exp_avg_sq, copies)
+//       -> None (nothing to do) or (table, count, bits, device, kept)
+//
+// checks the lists and packs a tilec_adamw_tensor (include/tilec.h) for each
+// parameter with a gradient into the bytes `table`.  The same checks attribute
+// by attribute in Python take 1.1 us a tensor (80 us for 72 tensors, whose
+// kernels take 12); these take 0.05.  `kept`: contiguous copies of gradients
+// that were not, to be held until the launch.
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <algorithm>
+#include <string>
+#include <vector>
+
+#include "../../include/tilec.h"
+
+namespace {
+
+constexpr int64_t kBlock = 256;  // values per scale of an 8-bit state
+
+struct Refused {
+  PyObject* type;
+  std::string what;
+};
+
+[[noreturn]] void bad_value(const std::string& what) { throw Refused{PyExc_ValueError, "adamw_step: " + what}; }
+[[noreturn]] void bad_type(const std::string& what) { throw Refused{PyExc_TypeError, "adamw_step: " + what}; }
+
+// A list or tuple, or whatever else is a sequence.
+struct List {
+  PyObject* seq;
+  explicit List(PyObject* o) : seq(PySequence_Fast(o, "adamw_step: expected lists of tensors")) {
+    if (seq == nullptr) throw python_error();
+  }
+  ~List() { Py_DECREF(seq); }
+  List(const List&) = delete;
+  Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(seq); }
+  PyObject* operator[](Py_ssize_t i) const { return PySequence_Fast_GET_ITEM(seq, i); }
+};
+
+const at::Tensor& tensor(const char* name, PyObject* o) {
+  if (!THPVariable_Check(o)) bad_type(std::string(name) + " holds a " + Py_TYPE(o)->tp_name + ", expected tensors");
+  return THPVariable_Unpack(o);
+}
+
+struct Reader {
+  int64_t device = -1;
+
+  // A dense tensor of n values on the parameters' GPU, of one of two types.
+  const at::Tensor& read(const char* name, PyObject* o, int64_t n, at::ScalarType a, at::ScalarType b,
+                         bool contiguous = true) {
+    const at::Tensor& t = tensor(name, o);
+    if (!t.is_cuda()) bad_type("needs tensors on a ROCm GPU (" + std::string(name) + " has one on " + t.device().str() + ")");
+    if (t.layout() != at::kStrided) bad_type(std::string(name) + " has a tensor that is not dense");
+    if (device < 0) device = t.get_device();
+    if (t.get_device() != device) bad_type("needs all tensors on one ROCm GPU (" + std::string(name) + " has others)");
+    if (t.scalar_type() != a && t.scalar_type() != b)
+      bad_type(std::string(name) + " has a tensor of dtype " + toString(t.scalar_type()) + ", expected " + toString(a) +
+               (a == b ? "" : std::string(" or ") + toString(b)));
+    if (n >= 0 && t.numel() != n) bad_value(std::string(name) + " and params differ in sizes");
+    if (contiguous && !t.is_contiguous()) bad_value(std::string(name) + " has a tensor that is not contiguous");
+    return t;
+  }
+};
+
+int32_t code(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? TILEC_BF16 : TILEC_F32; }
+
+// A state: its values or codes, and the scales of codes (bits 8).
+void read_state(Reader& r, const char* name, PyObject* o, int64_t n, at::ScalarType codes, int& bits, void*& values,
+                float*& scales) {
+  const bool pair = PyTuple_Check(o) || PyList_Check(o);
+  if (bits == 0) bits = pair ? 8 : 32;
+  if ((bits == 8) != pair) bad_value("states of 32 and of 8 bits are mixed");
+  if (!pair) {
+    values = r.read(name, o, n, at::kFloat, at::kFloat).data_ptr();
+    return;
+  }
+  const List both(o);
+  if (both.size() != 2) bad_value(std::string(name) + ": an 8-bit state is a pair (codes, scales)");
+  values = r.read(name, both[0], n, codes, codes).data_ptr();
+  scales = static_cast<float*>(r.read("scales", both[1], (n + kBlock - 1) / kBlock, at::kFloat, at::kFloat).data_ptr());
+}
+
+PyObject* build(PyObject* const* args) {
+  const List params(args[0]), grads(args[1]), m(args[2]), v(args[3]);
+  const bool copied = args[4] != Py_None;
+  const List copies(copied ? args[4] : args[0]);
+  const Py_ssize_t count = params.size();
+  if (grads.size() != count || m.size() != count || v.size() != count || copies.size() != count)
+    bad_value(std::to_string(count) + " params, " + std::to_string(grads.size()) + " grads, " +
+              std::to_string(m.size()) + " and " + std::to_string(v.size()) + " states, " +
+              std::to_string(copied ? copies.size() : count) + " copies");
+  Reader r;
+  int bits = 0;
+  std::vector<tilec_adamw_tensor> table;
+  std::vector<at::Tensor> kept;
+  table.reserve(count);
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    if (grads[i] == Py_None) continue;
+    tilec_adamw_tensor d{};
+    const at::Tensor& p = r.read("params", params[i], -1, at::kFloat, at::kBFloat16);
+    const int64_t n = p.numel();
+    const at::Tensor* g = &r.read("grads", grads[i], n, at::kFloat, at::kBFloat16, false);
+    if (!g->is_contiguous()) {
+      kept.push_back(g->contiguous());
+      g = &kept.back();
+    }
+    d.param = p.data_ptr();
+    d.grad = g->const_data_ptr();
+    d.param_dtype = code(p);
+    d.grad_dtype = code(*g);
+    d.n = n;
+    read_state(r, "exp_avg", m[i], n, at::kChar, bits, d.exp_avg, d.exp_avg_scale);
+    read_state(r, "exp_avg_sq", v[i], n, at::kByte, bits, d.exp_avg_sq, d.exp_avg_sq_scale);
+    if (copied && copies[i] != Py_None) d.copy = r.read("copies", copies[i], n, at::kBFloat16, at::kBFloat16).data_ptr();
+    table.push_back(d);
+  }
+  if (table.empty()) Py_RETURN_NONE;
+  // One memory for two parameters (a tied weight given twice) would be a race.
+  std::vector<void*> starts;
+  starts.reserve(table.size());
+  for (const auto& d : table)
+    if (d.n > 0) starts.push_back(d.param);
+  std::sort(starts.begin(), starts.end());
+  if (std::adjacent_find(starts.begin(), starts.end()) != starts.end()) bad_value("two params share their memory");
+  PyObject* held = PyList_New((Py_ssize_t)kept.size());
+  if (held == nullptr) throw python_error();
+  for (size_t i = 0; i < kept.size(); ++i) PyList_SET_ITEM(held, (Py_ssize_t)i, THPVariable_Wrap(kept[i]));
+  return Py_BuildValue("(y#iiLN)", reinterpret_cast<const char*>(table.data()),
+                       (Py_ssize_t)(table.size() * sizeof(tilec_adamw_tensor)), (int)table.size(), bits,
+                       (long long)r.device, held);
+}
+
+PyObject* adamw_table(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  if (count != 5) {
+    PyErr_SetString(PyExc_TypeError, "adamw_table takes 5 arguments");
+    return nullptr;
+  }
+  try {
+    return build(args);
+  } catch (const Refused& e) {
+    PyErr_SetString(e.type, e.what.c_str());
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef kMethods[] = {
+    {"adamw_table", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw_table)), METH_FASTCALL,
+     "adamw_table(params, grads, exp_avg, exp_avg_sq, copies) -> None or (table, count, bits, device, kept)"},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__host() { return PyModule_Create(&kModule); }

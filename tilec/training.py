@@ -13,8 +13,6 @@ Like those two they are plain functions with no autograd of their own.
 import array
 import ctypes
 from functools import lru_cache
-from itertools import chain
-from operator import attrgetter
 
 import torch
 
@@ -289,11 +287,6 @@ def linear_cross_entropy_grad(x, weight, target, reduction="mean", ignore_index=
 
 ADAMW_BLOCK = 256  # values per scale of an 8-bit state
 
-# A tensor's record for tilec_adamw (include/tilec.h, tilec_adamw_tensor): 8
-# pointers and sizes and two 32-bit type codes, the parameter's low.
-_TYPES = {(p, g): _CODES[p] | _CODES[g] << 32 for p in _CODES for g in _CODES}
-
-
 def adamw_state(param, bits=32):
     """(exp_avg, exp_avg_sq): the zero states of `adamw_step` for one
     parameter, float32 tensors of its shape, or with bits=8 a (codes, scales)
@@ -307,35 +300,6 @@ def adamw_state(param, bits=32):
     scales = torch.zeros((2, -(-param.numel() // ADAMW_BLOCK)), dtype=torch.float32, device=param.device)
     return ((torch.zeros(param.shape, dtype=torch.int8, device=param.device), scales[0]),
             (torch.zeros(param.shape, dtype=torch.uint8, device=param.device), scales[1]))
-
-
-_numel, _data_ptr = torch.Tensor.numel, torch.Tensor.data_ptr
-_get_device, _is_contiguous, _dtype = torch.Tensor.get_device, torch.Tensor.is_contiguous, attrgetter("dtype")
-
-
-def _same(what, name, tensors, numels, dtypes, device):
-    """Contiguous tensors of the given sizes and types on one device."""
-    if list(map(_numel, tensors)) != numels:
-        raise ValueError(f"{what}: {name} and params differ in number or sizes")
-    wrong = set(map(_dtype, tensors)).difference(dtypes)
-    if wrong:
-        raise TypeError(f"{what}: {name} has a tensor of dtype {wrong.pop()}, expected "
-                        f"{' or '.join(str(d) for d in dtypes)}")
-    if set(map(_get_device, tensors)) - {device}:
-        raise TypeError(f"{what} needs all tensors on one ROCm GPU ({name} has others)")
-    if not all(map(_is_contiguous, tensors)):
-        raise ValueError(f"{what}: {name} has a tensor that is not contiguous")
-
-
-def _split_state(what, name, state):
-    """([codes], [scales]) of 8-bit states, or ([tensors], None) of 32-bit ones."""
-    if not isinstance(state[0], (tuple, list)):
-        return list(state), None
-    try:
-        codes, scales = zip(*state)
-    except (TypeError, ValueError):
-        raise ValueError(f"{what}: {name} mixes 32-bit and 8-bit states") from None
-    return list(codes), list(scales)
 
 
 def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
@@ -356,62 +320,21 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     float32; many tensors share a launch.
     """
     what = "adamw_step"
-    params = list(params)
-    if len(grads) != len(params) or (copies is not None and len(copies) != len(params)) \
-            or len(exp_avg) != len(params) or len(exp_avg_sq) != len(params):
-        raise ValueError(f"{what}: {len(params)} params, {len(grads)} grads, {len(exp_avg)} and {len(exp_avg_sq)} states")
     if step < 1:
         raise ValueError(f"{what}: steps count from 1 (got {step})")
-    if not params:
+    packed = _lib.host().adamw_table(params, grads, exp_avg, exp_avg_sq, copies)
+    if packed is None:
         return
-    if any(g is None for g in grads):
-        have = [i for i, g in enumerate(grads) if g is not None]
-        if not have:
-            return
-        params, grads, exp_avg, exp_avg_sq = ([x[i] for i in have] for x in (params, grads, exp_avg, exp_avg_sq))
-        copies = None if copies is None else [copies[i] for i in have]
-    if params[0].device.type != "cuda":
-        raise TypeError(f"{what} needs tensors on a ROCm GPU (got {params[0].device})")
-    device = params[0].get_device()
-    numels = list(map(_numel, params))
-    floats = (torch.float32, torch.bfloat16)
-    _same(what, "params", params, numels, floats, device)
-    if not all(map(_is_contiguous, grads)):
-        grads = [g.contiguous() for g in grads]
-    _same(what, "grads", grads, numels, floats, device)
-    m, ms = _split_state(what, "exp_avg", exp_avg)
-    v, vs = _split_state(what, "exp_avg_sq", exp_avg_sq)
-    if (ms is None) != (vs is None):
-        raise ValueError(f"{what}: exp_avg and exp_avg_sq have states of different bits")
-    _same(what, "exp_avg", m, numels, (torch.float32,) if ms is None else (torch.int8,), device)
-    _same(what, "exp_avg_sq", v, numels, (torch.float32,) if vs is None else (torch.uint8,), device)
-    none = [0] * len(params)
-    ms_at = vs_at = copies_at = none
-    if ms is not None:
-        blocks = [-(-n // ADAMW_BLOCK) for n in numels]
-        _same(what, "exp_avg's scales", ms, blocks, (torch.float32,), device)
-        _same(what, "exp_avg_sq's scales", vs, blocks, (torch.float32,), device)
-        ms_at, vs_at = map(_data_ptr, ms), map(_data_ptr, vs)
-    if copies is not None:
-        given = [(c, n) for c, n in zip(copies, numels) if c is not None]
-        _same(what, "copies", [c for c, _ in given], [n for _, n in given], (torch.bfloat16,), device)
-        copies_at = [0 if c is None else c.data_ptr() for c in copies]
-    p_at = list(map(_data_ptr, params))
-    # One memory for two parameters (a tied weight given twice) would be a race.
-    if len(set(p_at)) < len(p_at) and len({a for a, n in zip(p_at, numels) if n}) < len(numels) - numels.count(0):
-        raise ValueError(f"{what}: two params share their memory")
+    table, count, bits, device, kept = packed
     if grad_scale is not None:
         if grad_scale.dtype != torch.float32 or grad_scale.get_device() != device:
             raise TypeError(f"{what}: grad_scale must be float32 on the params' GPU (got {grad_scale.dtype}, "
                             f"{grad_scale.device})")
         if grad_scale.numel() != 1:
             raise ValueError(f"{what}: grad_scale has shape {tuple(grad_scale.shape)}, expected one value")
-    types = map(_TYPES.__getitem__, zip(map(_dtype, params), map(_dtype, grads)))
-    table = array.array("q", chain.from_iterable(zip(p_at, map(_data_ptr, grads), map(_data_ptr, m), map(_data_ptr, v),
-                                                     ms_at, vs_at, copies_at, numels, types)))
     with _on(device):
-        _lib.check(_lib.lib().tilec_adamw(table.buffer_info()[0], len(params), 32 if ms is None else 8, step, lr,
-                                          betas[0], betas[1], eps, weight_decay, _ptr(grad_scale), _raw_stream(device)))
+        _lib.check(_lib.lib().tilec_adamw(table, count, bits, step, lr, betas[0], betas[1], eps, weight_decay,
+                                          _ptr(grad_scale), _raw_stream(device)))
 
 
 def adamw_values(states):
@@ -419,23 +342,27 @@ def adamw_values(states):
     `adamw_step`, stand for: a flat tensor each."""
     what = "adamw_values"
     states = list(states)
+    if not all(isinstance(s, (tuple, list)) and len(s) == 2 for s in states):
+        raise ValueError(f"{what}: expected (codes, scales) pairs")
     if not states:
         return []
-    codes, scales = _split_state(what, "states", states)
-    if scales is None:
-        raise ValueError(f"{what}: expected (codes, scales) pairs")
-    if codes[0].device.type != "cuda":
-        raise TypeError(f"{what} needs tensors on a ROCm GPU (got {codes[0].device})")
-    device, where = codes[0].get_device(), codes[0].device
-    numels = [c.numel() for c in codes]
-    _same(what, "states", codes, numels, (torch.int8, torch.uint8), device)
-    _same(what, "scales", scales, [-(-n // ADAMW_BLOCK) for n in numels], (torch.float32,), device)
-    out = list(torch.empty(sum(numels), dtype=torch.float32, device=where).split(numels))
-    records = []
-    for o, c, s, n in zip(out, codes, scales, numels):
+    at = _on_gpu(what, states[0][0], *(t for s in states for t in s))
+    for codes, scales in states:
+        if codes.dtype not in (torch.int8, torch.uint8) or scales.dtype != torch.float32:
+            raise TypeError(f"{what}: codes and scales have dtypes {codes.dtype} and {scales.dtype}, expected int8 or "
+                            "uint8 and float32")
+        if scales.numel() != -(-codes.numel() // ADAMW_BLOCK):
+            raise ValueError(f"{what}: {codes.numel()} codes have {scales.numel()} scales, one per {ADAMW_BLOCK} expected")
+        if not (codes.is_contiguous() and scales.is_contiguous()):
+            raise ValueError(f"{what}: codes or scales that are not contiguous")
+    sizes = [c.numel() for c, _ in states]
+    out = list(torch.empty(sum(sizes), dtype=torch.float32, device=states[0][0].device).split(sizes))
+    # A tilec_adamw_tensor each: 7 pointers, the size, and two type codes that
+    # play no part here.
+    records = array.array("q")
+    for o, (c, s), n in zip(out, states, sizes):
         m = (c.data_ptr(), 0, s.data_ptr(), 0) if c.dtype == torch.int8 else (0, c.data_ptr(), 0, s.data_ptr())
-        records += (o.data_ptr(), 0, *m, 0, n, 0)
-    table = array.array("q", records)
-    with _on(device):
-        _lib.check(_lib.lib().tilec_adamw_values(table.buffer_info()[0], len(out), _raw_stream(device)))
+        records.extend((o.data_ptr(), 0, *m, 0, n, 0))
+    with _on(at):
+        _lib.check(_lib.lib().tilec_adamw_values(records.buffer_info()[0], len(out), _raw_stream(at)))
     return out
