@@ -2,15 +2,19 @@
 //
 //   adamw_table(params, grads, exp_avg, exp_avg_sq, copies)
 //       -> None (nothing to do) or (table, count, bits, device, kept)
+//   adamw_values_table(states)
+//       -> (table, count, device, outputs)
 //
-// checks the lists and packs a tilec_adamw_tensor (include/tilec.h) for each
+// The first checks the lists and packs a tilec_adamw_tensor (include/tilec.h) for each
 // parameter with a gradient into the bytes `table`.  The same checks attribute
 // by attribute in Python take 1.1 us a tensor (80 us for 72 tensors, whose
 // kernels take 12); these take 0.05.  `kept`: contiguous copies of gradients
-// that were not, to be held until the launch.
+// that were not, to be held until the launch.  The second does the same for
+// tilec_adamw_values, whose float32 outputs it allocates, views of one storage.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/ops/empty.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -29,13 +33,13 @@ struct Refused {
   std::string what;
 };
 
-[[noreturn]] void bad_value(const std::string& what) { throw Refused{PyExc_ValueError, "adamw_step: " + what}; }
-[[noreturn]] void bad_type(const std::string& what) { throw Refused{PyExc_TypeError, "adamw_step: " + what}; }
+[[noreturn]] void bad_value(const std::string& what) { throw Refused{PyExc_ValueError, "adamw: " + what}; }
+[[noreturn]] void bad_type(const std::string& what) { throw Refused{PyExc_TypeError, "adamw: " + what}; }
 
 // A list or tuple, or whatever else is a sequence.
 struct List {
   PyObject* seq;
-  explicit List(PyObject* o) : seq(PySequence_Fast(o, "adamw_step: expected lists of tensors")) {
+  explicit List(PyObject* o) : seq(PySequence_Fast(o, "adamw: expected lists of tensors")) {
     if (seq == nullptr) throw python_error();
   }
   ~List() { Py_DECREF(seq); }
@@ -63,7 +67,8 @@ struct Reader {
     if (t.scalar_type() != a && t.scalar_type() != b)
       bad_type(std::string(name) + " has a tensor of dtype " + toString(t.scalar_type()) + ", expected " + toString(a) +
                (a == b ? "" : std::string(" or ") + toString(b)));
-    if (n >= 0 && t.numel() != n) bad_value(std::string(name) + " and params differ in sizes");
+    if (n >= 0 && t.numel() != n)
+      bad_value(std::string(name) + " has a tensor of " + std::to_string(t.numel()) + " values, expected " + std::to_string(n));
     if (contiguous && !t.is_contiguous()) bad_value(std::string(name) + " has a tensor that is not contiguous");
     return t;
   }
@@ -137,14 +142,50 @@ PyObject* build(PyObject* const* args) {
                        (long long)r.device, held);
 }
 
-PyObject* adamw_table(PyObject*, PyObject* const* args, Py_ssize_t count) {
+PyObject* build_values(PyObject* const* args) {
+  const List states(args[0]);
+  const Py_ssize_t count = states.size();
+  if (count == 0) Py_RETURN_NONE;
+  Reader r;
+  std::vector<tilec_adamw_tensor> table(count);
+  int64_t total = 0;
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    if (!PyTuple_Check(states[i]) && !PyList_Check(states[i])) bad_value("expected (codes, scales) pairs");
+    const List both(states[i]);
+    if (both.size() != 2) bad_value("expected (codes, scales) pairs");
+    tilec_adamw_tensor& d = table[i];
+    const at::Tensor& c = r.read("codes", both[0], -1, at::kChar, at::kByte);
+    d.n = c.numel();
+    const at::Tensor& s = r.read("scales", both[1], (d.n + kBlock - 1) / kBlock, at::kFloat, at::kFloat);
+    const bool m = c.scalar_type() == at::kChar;
+    (m ? d.exp_avg : d.exp_avg_sq) = c.data_ptr();
+    (m ? d.exp_avg_scale : d.exp_avg_sq_scale) = static_cast<float*>(s.data_ptr());
+    total += d.n;
+  }
+  const at::Tensor all =
+      at::empty({total}, at::TensorOptions().dtype(at::kFloat).device(at::kCUDA, (c10::DeviceIndex)r.device));
+  PyObject* outs = PyList_New(count);
+  if (outs == nullptr) throw python_error();
+  int64_t at = 0;
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    const at::Tensor o = all.narrow(0, at, table[i].n);
+    table[i].param = o.data_ptr();
+    at += table[i].n;
+    PyList_SET_ITEM(outs, i, THPVariable_Wrap(o));
+  }
+  return Py_BuildValue("(y#iLN)", reinterpret_cast<const char*>(table.data()),
+                       (Py_ssize_t)(table.size() * sizeof(tilec_adamw_tensor)), (int)count, (long long)r.device, outs);
+}
+
+template <PyObject* (*BUILD)(PyObject* const*), int ARGS>
+PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t count) {
   HANDLE_TH_ERRORS
-  if (count != 5) {
-    PyErr_SetString(PyExc_TypeError, "adamw_table takes 5 arguments");
+  if (count != ARGS) {
+    PyErr_Format(PyExc_TypeError, "expected %d arguments, got %zd", ARGS, count);
     return nullptr;
   }
   try {
-    return build(args);
+    return BUILD(args);
   } catch (const Refused& e) {
     PyErr_SetString(e.type, e.what.c_str());
     return nullptr;
@@ -152,9 +193,16 @@ PyObject* adamw_table(PyObject*, PyObject* const* args, Py_ssize_t count) {
   END_HANDLE_TH_ERRORS
 }
 
+template <PyObject* (*BUILD)(PyObject* const*), int ARGS>
+PyCFunction function() {
+  return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&call<BUILD, ARGS>));
+}
+
 PyMethodDef kMethods[] = {
-    {"adamw_table", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw_table)), METH_FASTCALL,
+    {"adamw_table", function<build, 5>(), METH_FASTCALL,
      "adamw_table(params, grads, exp_avg, exp_avg_sq, copies) -> None or (table, count, bits, device, kept)"},
+    {"adamw_values_table", function<build_values, 1>(), METH_FASTCALL,
+     "adamw_values_table(states) -> None or (table, count, device, outputs)"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -10,7 +10,6 @@ scratch is the (device, stream) workspace of `ext`, and nothing synchronises.
 Like those two they are plain functions with no autograd of their own.
 """
 
-import array
 import ctypes
 from functools import lru_cache
 
@@ -287,6 +286,7 @@ def linear_cross_entropy_grad(x, weight, target, reduction="mean", ignore_index=
 
 ADAMW_BLOCK = 256  # values per scale of an 8-bit state
 
+
 def adamw_state(param, bits=32):
     """(exp_avg, exp_avg_sq): the zero states of `adamw_step` for one
     parameter, float32 tensors of its shape, or with bits=8 a (codes, scales)
@@ -340,29 +340,10 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
 def adamw_values(states):
     """The float32 values that a list of 8-bit states, (codes, scales) pairs of
     `adamw_step`, stand for: a flat tensor each."""
-    what = "adamw_values"
-    states = list(states)
-    if not all(isinstance(s, (tuple, list)) and len(s) == 2 for s in states):
-        raise ValueError(f"{what}: expected (codes, scales) pairs")
-    if not states:
+    packed = _lib.host().adamw_values_table(states)
+    if packed is None:
         return []
-    at = _on_gpu(what, states[0][0], *(t for s in states for t in s))
-    for codes, scales in states:
-        if codes.dtype not in (torch.int8, torch.uint8) or scales.dtype != torch.float32:
-            raise TypeError(f"{what}: codes and scales have dtypes {codes.dtype} and {scales.dtype}, expected int8 or "
-                            "uint8 and float32")
-        if scales.numel() != -(-codes.numel() // ADAMW_BLOCK):
-            raise ValueError(f"{what}: {codes.numel()} codes have {scales.numel()} scales, one per {ADAMW_BLOCK} expected")
-        if not (codes.is_contiguous() and scales.is_contiguous()):
-            raise ValueError(f"{what}: codes or scales that are not contiguous")
-    sizes = [c.numel() for c, _ in states]
-    out = list(torch.empty(sum(sizes), dtype=torch.float32, device=states[0][0].device).split(sizes))
-    # A tilec_adamw_tensor each: 7 pointers, the size, and two type codes that
-    # play no part here.
-    records = array.array("q")
-    for o, (c, s), n in zip(out, states, sizes):
-        m = (c.data_ptr(), 0, s.data_ptr(), 0) if c.dtype == torch.int8 else (0, c.data_ptr(), 0, s.data_ptr())
-        records.extend((o.data_ptr(), 0, *m, 0, n, 0))
-    with _on(at):
-        _lib.check(_lib.lib().tilec_adamw_values(records.buffer_info()[0], len(out), _raw_stream(at)))
+    table, count, device, out = packed
+    with _on(device):
+        _lib.check(_lib.lib().tilec_adamw_values(table, count, _raw_stream(device)))
     return out
