@@ -122,10 +122,13 @@ def test_chunks(N, H, V, rows, dt):
 
 
 @pytest.mark.gpu
-def test_many_tiles():
-    # Enough output tiles for the largest ones, in all three products.
-    x, w, t = make(2304, 2304, 16500, "bf16", seed=4, ignored=0.1)
-    check(x, w, t)
+@pytest.mark.parametrize("N,H,V,rows", [(2304, 2304, 16500, 0), (600, 520, 25000, 0), (600, 520, 25000, 512),
+                                        (1300, 130, 40000, 0)])
+def test_many_tiles(N, H, V, rows):
+    # Enough output tiles for the largest ones, in whole turns over the chip and
+    # with a rest in smaller ones.
+    x, w, t = make(N, H, V, "bf16", seed=4, ignored=0.1)
+    check(x, w, t, chunk_rows=rows)
 
 
 @pytest.mark.gpu

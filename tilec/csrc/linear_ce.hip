@@ -13,8 +13,7 @@
 // bf16 inputs.  The logits' product ends in an epilogue that never stores
 // them.  It runs with W as its row operand, so a lane holds consecutive
 // vocabulary entries of one token: a wave takes the maximum m and the sum of
-// exp(l - m) over its 64 or 128 entries of a token in its own registers and
-// two shuffles, writes those two, and (for gradients) exp(l - m) 2^15 in fp16,
+// exp(l - m) over 64 entries of a token in its own registers and two shuffles, writes those two, and (for gradients) exp(l - m) 2^15 in fp16,
 // whose 11 bits leave the one rounding to bf16 that d itself gets as the only
 // one that counts; values below 2^-29 of the largest in their group lose bits,
 // below 2^-39 they are lost.  One pass over them (ce_rows_kernel) then joins the groups to lse
@@ -50,13 +49,16 @@ __device__ __forceinline__ u16 bf16_bits(float f) { return __builtin_bit_cast(u1
 // Epilogues of the bf16 products
 // ---------------------------------------------------------------------------
 
-// The logits: rows are vocabulary entries, columns tokens.
+constexpr int kGroup = 64;  // vocabulary entries of one (m, sum) pair
+
+// The logits: rows are vocabulary entries (from v0 on), columns tokens.
 struct CeLogits {
   static constexpr bool kStaged = true, kOwnSplits = false;
   u16* e;      // exp(l - m) 2^15 in fp16, [token][lde]; NULL: losses only
   int64_t lde;
   f32x2* stat;  // (m, sum of exp(l - m)), [token][groups]
-  int groups;
+  int groups;   // even
+  int v0;
   const int64_t* target;
   float* tlogit;  // the target's logit, [token]
 
@@ -70,59 +72,73 @@ struct CeLogits {
   template <class P, int MF, bool FULL>
   __device__ __forceinline__ void tile(const TileOut<P, MF>& t, typename P::Acc (&acc)[P::TM][P::TN], int V,
                                        int N) const {
+    static_assert(MF == 16 && P::WTM % kGroup == 0, "a wave's rows are whole groups");
     constexpr float kLog2e = 1.44269504088896f;
-    const int first = t.m0 + t.wm * P::WTM, group = first / P::WTM;
+    constexpr int G = P::WTM / kGroup, BPG = P::TM / G;  // groups of a wave, row blocks of a group
+    const int first = t.m0 + t.wm * P::WTM;
     int64_t want[P::TN];  // read ahead of their use
 #pragma unroll
     for (int j = 0; j < P::TN; ++j) want[j] = FULL || t.col(j) < N ? target[t.col(j)] : -1;
 #pragma unroll
     for (int j = 0; j < P::TN; ++j) {
       const int tok = t.col(j);
-      float m = -FLT_MAX;
+      float m[G], s[G];
 #pragma unroll
-      for (int i = 0; i < P::TM; ++i)
+      for (int g = 0; g < G; ++g) {
+        m[g] = -FLT_MAX;
 #pragma unroll
-        for (int r = 0; r < P::ACC; ++r)
-          if (FULL || t.row(i, r) < V) m = fmaxf(m, acc[i][j][r]);
-      if constexpr (MF == 16) m = fmaxf(m, __shfl_xor(m, 16));
-      m = fmaxf(m, __shfl_xor(m, 32));
+        for (int i = g * BPG; i < (g + 1) * BPG; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (FULL || t.row(i, r) < V) m[g] = fmaxf(m[g], acc[i][j][r]);
+        m[g] = fmaxf(m[g], __shfl_xor(m[g], 16));
+        m[g] = fmaxf(m[g], __shfl_xor(m[g], 32));
+      }
       // exp(l - m) 2^15 = 2^((l - m) log2 e + 15): the difference first, so that
       // it is exact where it matters.
-      float s = 0.f;
 #pragma unroll
-      for (int i = 0; i < P::TM; ++i)
+      for (int g = 0; g < G; ++g) {
+        s[g] = 0.f;
 #pragma unroll
-        for (int q = 0; q < P::ACC / 4; ++q) {
+        for (int i = g * BPG; i < (g + 1) * BPG; ++i) {
           f32x4 x;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            x[c] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][4 * q + c] - m, kLog2e, 15.f));
-            if (!FULL && t.row(i, 4 * q) + c >= V) x[c] = 0.f;
+            x[c] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][c] - m[g], kLog2e, 15.f));
+            if (!FULL && t.row(i, c) >= V) x[c] = 0.f;
           }
-          s += (x[0] + x[1]) + (x[2] + x[3]);
+          s[g] += (x[0] + x[1]) + (x[2] + x[3]);
           if (e != nullptr) {
             const i32x2 h = __builtin_bit_cast(i32x2, __builtin_convertvector(x, f16x4));
-            t.put(i, q, j, h.x, h.y);
+            t.put(i, 0, j, h.x, h.y);
           }
         }
-      if constexpr (MF == 16) s += __shfl_xor(s, 16);
-      s += __shfl_xor(s, 32);
-      if (t.lane < MF && (FULL || tok < N))
-        stat[(int64_t)tok * groups + group] = f32x2{m, s * (1.f / kScale16)};
+        s[g] += __shfl_xor(s[g], 16);
+        s[g] += __shfl_xor(s[g], 32);
+      }
+      if (t.lane < 16 && (FULL || tok < N)) {
+        f32x2* to = stat + (int64_t)tok * groups + (v0 + first) / kGroup;
+        if constexpr (G == 2) {
+          *reinterpret_cast<f32x4*>(to) = f32x4{m[0], s[0] * (1.f / kScale16), m[1], s[1] * (1.f / kScale16)};
+        } else {
+#pragma unroll
+          for (int g = 0; g < G; ++g) to[g] = f32x2{m[g], s[g] * (1.f / kScale16)};
+        }
+      }
     }
     if (e != nullptr)
       t.store_all([&](int n, int v, i32x4 x) {
-        if (FULL || (n < N && v < lde)) *reinterpret_cast<i32x4*>(e + (int64_t)n * lde + v) = x;
+        if (FULL || (n < N && v0 + v < lde)) *reinterpret_cast<i32x4*>(e + (int64_t)n * lde + v0 + v) = x;
       });
 #pragma unroll
     for (int j = 0; j < P::TN; ++j) {
       // The target's logit: one wave in V / WTM holds it.
-      const int64_t at = want[j] - first;
-      if (want[j] >= 0 && at >= 0 && at < P::WTM && want[j] < V) {
+      const int64_t at = want[j] - v0 - first;
+      if (want[j] >= 0 && at >= 0 && at < P::WTM && first + at < V) {
 #pragma unroll
         for (int i = 0; i < P::TM; ++i)
 #pragma unroll
-          for (int r = 0; r < P::ACC; ++r)
+          for (int r = 0; r < 4; ++r)
             if (t.row(i, r) - first == (int)at) tlogit[t.col(j)] = acc[i][j][r];
       }
     }
@@ -203,6 +219,7 @@ __global__ __launch_bounds__(256) void ce_prepare_kernel(const T* __restrict__ x
   __shared__ int count[256];
   if (scale != nullptr && blockIdx.x == gridDim.x - 1) {
     int n = 0;
+#pragma unroll 8
     for (int64_t i = threadIdx.x; i < all; i += 256) n += all_targets[i] != ignore;
     count[threadIdx.x] = n;
     for (int o = 128; o > 0; o >>= 1) {
@@ -305,7 +322,7 @@ struct CeRows {
   void* p;
   int64_t ldp, V;
   const f32x2* stat;
-  int groups, group_shift;  // columns of a group: 2^group_shift
+  int groups, stride, group_shift;  // groups of a row, from one row's to the next, columns of one: 2^group_shift
   const int64_t* target;
   int64_t ignore;
   const float* tlogit;
@@ -330,7 +347,7 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
       *reinterpret_cast<i32x4*>(row + v) = i32x4{0, 0, 0, 0};
     return;
   }
-  const f32x2* stat = a.stat + r * a.groups;
+  const f32x2* stat = a.stat + r * a.stride;
   float m = -FLT_MAX;
   for (int g = tid; g < a.groups; g += 256) m = fmaxf(m, stat[g].x);
   m = wave_max(m);
@@ -404,6 +421,7 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeJoin a) {
   if (a.loss != nullptr && blockIdx.x == gridDim.x - 1) {
     double s = 0;
     int n = 0;
+#pragma unroll 8
     for (int64_t i = threadIdx.x; i < a.N; i += 256) {
       s += (double)a.row_loss[i];
       n += a.target[i] != a.ignore;
@@ -532,30 +550,69 @@ __global__ __launch_bounds__(256) void ce_zero_kernel(unsigned char* __restrict_
 // The bf16 products
 // ---------------------------------------------------------------------------
 
-// Output tiles: 256 x 256 (8 waves) where there are enough of them for the
-// chip, 128 x 128 (8 waves) below, 128 x 64 (4 waves, two workgroups a CU)
-// for up to 64 columns.
+// Output tiles: 256 x 256 and 128 x 128 (8 waves, one workgroup a CU), 128 x
+// 64 (4 waves, two a CU).
 enum CeTile { kT256, kT128, kT64 };
 
+// How a product runs: K in `splits`, its long extent (the vocabulary) up to
+// `main` in tiles of one kind and the rest, unsplit, in smaller ones: at 3.06
+// turns of tiles over the chip the last 16 of 784 took a turn of their own.
 struct CeProduct {
   CeTile tile;
   int splits;
+  int64_t main;
+  CeTile tail;
 };
 
-int64_t tiles_of(CeTile t, int64_t M, int64_t N) {
-  return t == kT256 ? cdiv(M, 256) * cdiv(N, 256) : t == kT128 ? cdiv(M, 128) * cdiv(N, 128) : cdiv(M, 128) * cdiv(N, 64);
+struct TileCost {
+  int bm, bn, per_cu;
+  double step, fixed;  // us of a 64-deep K step, and of a tile beside them
+};
+constexpr TileCost kTiles[] = {{256, 256, 1, 1.5, 9.0}, {128, 128, 1, 0.5, 6.0}, {128, 64, 2, 0.75, 5.0}};
+
+int64_t tiles_of(CeTile t, int64_t M, int64_t N) { return cdiv(M, kTiles[t].bm) * cdiv(N, kTiles[t].bn); }
+
+// Estimated us, from what the tiles measured: turns over the chip, and for a
+// split K the fp32 sums written by the tiles (20 KB/us a CU) and joined.
+double product_cost(CeTile t, int64_t splits, int64_t M, int64_t N, int64_t K) {
+  const TileCost& c = kTiles[t];
+  const int64_t cus = device_cus();
+  const double steps = (double)cdiv(cdiv(K, 64), splits);
+  double one = steps * c.step + c.fixed, join = 0;
+  if (splits > 1) {
+    one += c.bm * c.bn * 4 * c.per_cu / 20e3;
+    join = 5 + (double)splits * M * N * 4 / 4e6;
+  }
+  return (double)cdiv(tiles_of(t, M, N) * splits, c.per_cu * cus) * one + join;
 }
 
-// rows M x columns N, N the one that may be small.
-CeProduct choose(int64_t M, int64_t N, int64_t K, bool can_split) {
-  const int64_t cus = device_cus();
-  CeProduct c{N <= 64 ? kT64 : kT128, 1};
-  if (c.tile == kT128 && tiles_of(kT256, M, N) >= cus) c.tile = kT256;
-  if (!can_split || c.tile == kT256) return c;
-  const int64_t tiles = tiles_of(c.tile, M, N), places = c.tile == kT64 ? 2 * cus : cus;
-  int64_t s = std::min<int64_t>({places / std::max<int64_t>(tiles, 1), cdiv(K, 64) / 4, 64});
-  c.splits = (int)std::max<int64_t>(s, 1);
-  return c;
+// The cheapest way for an M x N output; `long_m`, `long_n`: which extent may be
+// cut in two (then K is not split).
+CeProduct choose(int64_t M, int64_t N, int64_t K, bool can_split, bool long_m, bool long_n) {
+  const int64_t cus = device_cus(), extent = long_m ? M : N;
+  CeProduct best{kT256, 1, extent, kT128};
+  double least = 1e30;
+  auto offer = [&](const CeProduct& p, double cost) {
+    if (cost < least) least = cost, best = p;
+  };
+  for (const CeTile t : {kT256, kT128, kT64}) {
+    const int64_t most = can_split ? std::min<int64_t>(64, std::max<int64_t>(1, cdiv(K, 64) / 4)) : 1;
+    for (int64_t s = 1; s <= most; ++s) {
+      if (s > 1 && tiles_of(t, M, N) * s > 2 * kTiles[t].per_cu * cus) break;
+      offer(CeProduct{t, (int)s, extent, t}, product_cost(t, s, M, N, K));
+    }
+    if (t == kT64 || !(long_m || long_n)) continue;
+    // Whole turns of these tiles, the rest in the next smaller ones.
+    const int64_t across = long_m ? cdiv(N, kTiles[t].bn) : cdiv(M, kTiles[t].bm);
+    const int64_t turns = tiles_of(t, M, N) / cus, b = long_m ? kTiles[t].bm : kTiles[t].bn;
+    const int64_t main = turns * cus / across * b;
+    if (main <= 0 || main >= extent) continue;
+    const CeTile small = t == kT256 ? kT128 : kT64;
+    const double cost = long_m ? product_cost(t, 1, main, N, K) + product_cost(small, 1, M - main, N, K)
+                               : product_cost(t, 1, M, main, K) + product_cost(small, 1, M, N - main, K);
+    offer(CeProduct{t, 1, main, small}, cost + 2);
+  }
+  return best;
 }
 
 // Row length of fp32 sums of M: the lanes' 64-byte pieces are whole sectors.
@@ -584,14 +641,11 @@ hipError_t run_tile(const Operands& o, const Epi& epi, int splits, hipStream_t s
 }
 
 template <KMask KM, bool CA, bool CB, class Epi>
-hipError_t run_product(const Operands& o, const Epi& epi, const CeProduct& c, hipStream_t stream) {
-  if (c.tile == kT256) return run_tile<256, 256, 2, 2, 4, KM, CA, CB, 16>(o, epi, c.splits, stream);
-  if (c.tile == kT128) return run_tile<128, 128, 4, 2, 4, KM, CA, CB, 16>(o, epi, c.splits, stream);
-  return run_tile<128, 64, 3, 2, 2, KM, CA, CB, 16>(o, epi, c.splits, stream);
+hipError_t run_product(const Operands& o, const Epi& epi, CeTile tile, int splits, hipStream_t stream) {
+  if (tile == kT256) return run_tile<256, 256, 2, 2, 4, KM, CA, CB, 16>(o, epi, splits, stream);
+  if (tile == kT128) return run_tile<128, 128, 4, 2, 4, KM, CA, CB, 16>(o, epi, splits, stream);
+  return run_tile<128, 64, 3, 2, 2, KM, CA, CB, 16>(o, epi, splits, stream);
 }
-
-// Vocabulary entries of a wave's group in the logits' product.
-int group_shift(CeTile t) { return t == kT256 ? 7 : 6; }
 
 // ---------------------------------------------------------------------------
 // Plan: chunking and where everything lies in the workspace
@@ -665,13 +719,12 @@ CePlan make_plan(const CeArgs& a) {
       return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % 8 == 0 && ld < (int64_t(1) << 22);
     };
     p.pad = a.H % 8 != 0 || !fits(a.w, a.ldw) || !fits(a.x, a.ldx);
-    p.p1 = choose(a.V, p.R, a.H, false);
-    p.p2 = choose(a.H, p.R, a.V, true);
-    p.p3 = choose(a.H, a.V, p.R, true);
-    p.shift = group_shift(p.p1.tile);
-    // A tile's groups are all written, those past the vocabulary's end too.
-    const int64_t bm = p.p1.tile == kT256 ? 256 : 128;
-    p.groups = (int)(cdiv(a.V, bm) * bm >> p.shift);
+    p.p1 = choose(a.V, p.R, a.H, false, true, false);
+    p.p2 = choose(a.H, p.R, a.V, true, false, false);
+    p.p3 = choose(a.H, a.V, p.R, true, false, true);
+    p.shift = 6;
+    // The largest tiles write groups past the vocabulary's end too.
+    p.groups = (int)(cdiv(a.V, 256) * 4);
   } else {
     p.shift = 12;
     p.groups = (int)cdiv(a.V, kGroup32);
@@ -742,7 +795,7 @@ hipError_t run_rows(const CeArgs& a, const CePlan& p, char* ws, int64_t r0, int6
   q.p = a.grad ? ws + p.keep : nullptr;
   q.ldp = p.Vp, q.V = a.V;
   q.stat = reinterpret_cast<const f32x2*>(ws + p.stat);
-  q.groups = p.groups, q.group_shift = p.shift;
+  q.groups = (int)cdiv(a.V, int64_t(1) << p.shift), q.stride = p.groups, q.group_shift = p.shift;
   q.target = a.target + r0, q.ignore = a.ignore;
   q.tlogit = reinterpret_cast<const float*>(ws + p.tlogit);
   q.loss = (a.reduction == kNone ? a.loss : reinterpret_cast<float*>(ws + p.rows)) + r0;
@@ -783,7 +836,18 @@ hipError_t run_grad(const CeArgs& a, const CePlan& p, char* ws, const Operands& 
   const int64_t splits = gemm_split_geom(o.K, 64, c.splits).splits;
   CeGrad g{out, a.H, acc, ld, 0, add, scale};
   if (splits > 1) g = CeGrad{nullptr, 0, part, ld, o.N * ld, false, nullptr};
-  CE_TRY((run_product<kKRows, true, CB>(o, g, c, stream)));
+  Operands main = o;
+  if (c.main < o.N) {  // CB false: d's rows, N the vocabulary
+    Operands rest = o;
+    rest.N = o.N - c.main;
+    rest.b += c.main;
+    CeGrad gr = g;
+    if (gr.out != nullptr) gr.out += c.main * a.H;
+    if (gr.acc32 != nullptr) gr.acc32 += c.main * ld;
+    CE_TRY((run_product<kKRows, true, CB>(rest, gr, c.tail, 1, stream)));
+    main.N = c.main;
+  }
+  CE_TRY((run_product<kKRows, true, CB>(main, g, c.tile, c.splits, stream)));
   CeJoin q{};
   if (splits > 1) {
     q.part = part, q.splits = (int)splits, q.rows = o.N, q.cols = a.H, q.ld = ld;
@@ -812,14 +876,21 @@ hipError_t run_bf16(const CeArgs& a, const CePlan& p, char* ws, hipStream_t stre
                 p.Vp,
                 reinterpret_cast<f32x2*>(ws + p.stat),
                 p.groups,
+                0,
                 a.target + r0,
                 reinterpret_cast<float*>(ws + p.tlogit)};
     // Rows of x end in zeros to a whole K step, rows of W only where it was
     // copied.
-    if (p.pad || a.H % 64 == 0)
-      CE_TRY((run_product<kKFull, false, true>(Operands{w, xc, ldw, ldx, a.V, R, p.Hp}, le, p.p1, stream)));
-    else
-      CE_TRY((run_product<kKColsA, false, true>(Operands{w, xc, ldw, ldx, a.V, R, a.H}, le, p.p1, stream)));
+    for (int64_t v0 = 0; v0 < a.V; v0 += p.p1.main) {
+      const bool rest = v0 > 0;
+      const int64_t V = rest ? a.V - v0 : p.p1.main;
+      const CeTile tile = rest ? p.p1.tail : p.p1.tile;
+      const Operands o{w + v0 * ldw, xc, ldw, ldx, V, R, p.pad || a.H % 64 == 0 ? p.Hp : a.H};
+      le.v0 = (int)v0;
+      if (o.K % 64 == 0) CE_TRY((run_product<kKFull, false, true>(o, le, tile, 1, stream)));
+      else CE_TRY((run_product<kKColsA, false, true>(o, le, tile, 1, stream)));
+      if (rest) break;
+    }
     CE_TRY(run_rows<u16>(a, p, ws, r0, R, stream));
     if (!a.grad) {
       if (last) CE_TRY(run_join(a, p, ws, CeJoin{}, true, stream));
