@@ -177,13 +177,15 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, param_grads=True):
 
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+_KEPT_SCRATCH = 64 << 20  # a larger workspace is not kept between calls
 
 
 @lru_cache(4096)
-def _ce_plan(N, H, V, ldx, ldw, dtype, code, grad, chunk_rows, x_off, w_off):
-    """(workspace bytes, counter bytes, configs) of a call; float32 products run
-    the tuned pick of their shapes, as `matrix_mul` does.  x_off, w_off: the
-    addresses modulo 16, all of them that the C side looks at."""
+def _ce_plan(device, N, H, V, ldx, ldw, dtype, code, grad, chunk_rows, x_off, w_off):
+    """(workspace bytes, counter bytes, configs) of a call on the current GPU,
+    `device`; float32 products run the tuned pick of their shapes, as
+    `matrix_mul` does.  x_off, w_off: the addresses modulo 16, all of them that
+    the C side looks at."""
     ws, cnt, rows = ctypes.c_size_t(0), ctypes.c_size_t(0), ctypes.c_int64(0)
 
     def ask(configs):
@@ -237,13 +239,18 @@ def _linear_ce(what, x, weight, target, reduction, ignore_index, grad, grad_loss
     code = _REDUCTIONS[reduction]
     with _on(at):
         stream = _raw_stream(at)
-        ws, cnt, configs = _ce_plan(N, H, V, ldx, ldw, dtype, code, grad, chunk_rows, x.data_ptr() % 16,
+        ws, cnt, configs = _ce_plan(at, N, H, V, ldx, ldw, dtype, code, grad, chunk_rows, x.data_ptr() % 16,
                                     weight.data_ptr() % 16)
-        ws_ptr = workspace_for(x.device, stream, ws).data_ptr() if ws else None
+        # Up to 2 GiB and more: what is large goes back to torch's allocator.
+        scratch = None
+        if ws > _KEPT_SCRATCH:
+            scratch = torch.empty(ws, dtype=torch.uint8, device=x.device)
+        elif ws:
+            scratch = workspace_for(x.device, stream, ws)
         cnt_ptr = counters_for(x.device, stream, cnt).data_ptr() if cnt else None
         _lib.check(_lib.lib().tilec_linear_ce(x.data_ptr(), weight.data_ptr(), target.data_ptr(), loss.data_ptr(),
                                               _ptr(grad_loss), _ptr(dx), _ptr(dw), N, H, V, ldx, ldw, dtype, code,
-                                              int(ignore_index), grad, chunk_rows, configs, ws_ptr, ws, cnt_ptr, cnt,
+                                              int(ignore_index), grad, chunk_rows, configs, _ptr(scratch), ws, cnt_ptr, cnt,
                                               stream))
     return loss, dx, dw
 
