@@ -9,7 +9,7 @@
 // Both passes are bound by HBM: forward reads x and writes y, backward reads
 // x and dy and writes dx.  So each value is read once: a row is held in
 // registers by the TPR threads that serve it (16-byte loads; a power of two
-// of threads, from 1 to a 1024-thread workgroup) and both statistics are
+// of threads up to a wave, whole waves up to a 1024-thread workgroup) and both statistics are
 // taken from there, the variance from the deviations themselves, not from a
 // difference of sums; the deviations' own sum, what the rounded mean left
 // out, corrects both (a row of equal values comes out as zeros).  Rows of any length, stride and element alignment take
@@ -136,28 +136,32 @@ __device__ __forceinline__ void row_sums(float (&s)[NS], int tpr, float (*red)[1
     for (int i = 0; i < NS; ++i) s[i] += __shfl_xor(s[i], o);
   }
   if (tpr <= 64) return;
-  const int wave = threadIdx.x >> 6, per = tpr >> 6, first = wave / per * per;
+  const int wave = threadIdx.x >> 6, waves = tpr >> 6;  // past a wave a row has the workgroup to itself
   if ((threadIdx.x & 63) == 0) {
 #pragma unroll
     for (int i = 0; i < NS; ++i) red[slot][wave][i] = s[i];
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < NS; ++i) s[i] = red[slot][first][i];
-  for (int w = 1; w < per; ++w) {
+  for (int i = 0; i < NS; ++i) s[i] = red[slot][0][i];
+  for (int w = 1; w < waves; ++w) {
 #pragma unroll
-    for (int i = 0; i < NS; ++i) s[i] += red[slot][first + w][i];
+    for (int i = 0; i < NS; ++i) s[i] += red[slot][w][i];
   }
   slot ^= 1;
 }
 
 // The row's statistics from its rounded mean and the sums of the deviations
-// from that and of their squares.
-__device__ __forceinline__ void finish_stats(float& mean, float& rstd, const float (&q)[2], float d, float eps) {
-  const float off = q[0] / d;
+// from that and of their squares; inv_d = 1 / D, whose rounding the deviations'
+// sum makes up for in the mean.  (Divisions and a correctly rounded root instead, by
+// every lane of every row: 35.5 us for 8192 x 4096 bf16, 34.9 so.)
+__device__ __forceinline__ void finish_stats(float& mean, float& rstd, const float (&q)[2], float inv_d, float eps) {
+  const float off = q[0] * inv_d;
   mean += off;
-  const float var = fmaf(-off, off, q[1] / d);
-  rstd = 1.f / sqrtf((var < 0.f ? 0.f : var) + eps);  // a NaN stays one
+  const float var = fmaf(-off, off, q[1] * inv_d), v = (var < 0.f ? 0.f : var) + eps;  // a NaN stays one
+  // One Newton step on the hardware's root, which is 1 ulp off.
+  const float y = rsqrtf(v), r = fmaf(-v * y, y, 1.f);
+  rstd = v > 0.f && v < INFINITY ? fmaf(0.5f * y, r, y) : y;
 }
 
 struct NormArgs {
@@ -170,7 +174,7 @@ struct NormArgs {
   int64_t R;
   int D, Dp;  // Dp: columns of a partial row
   int w_bf16, tpr;
-  float eps;
+  float eps, inv_d;
 };
 
 // NV groups of E values a thread: rows of up to tpr * NV * E values.
@@ -180,10 +184,16 @@ __global__ __launch_bounds__(NT) void norm_kernel(NormArgs a) {
   __shared__ float red1[2][16][1], red2[2][16][2];
   int slot1 = 0, slot2 = 0;
   const int tpr = a.tpr, D = a.D;
-  const int sub = threadIdx.x & (tpr - 1);
   const int rpb = blockDim.x / tpr;
+  const int sub = rpb == 1 ? threadIdx.x : threadIdx.x & (tpr - 1);
+  float w[NV][E], b[NV][E];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    load_params<E>(a.w, a.w_bf16, E * (sub + i * tpr), D, 1.f, w[i]);
+    load_params<E>(a.b, a.w_bf16, E * (sub + i * tpr), D, 0.f, b[i]);
+  }
   for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < a.R; r0 += (int64_t)gridDim.x * rpb) {
-    const int64_t r = r0 + threadIdx.x / tpr;
+    const int64_t r = r0 + (rpb == 1 ? 0 : threadIdx.x / tpr);
     const bool live = r < a.R;  // rows past the end: read as the last one, not stored
     const TX* row = static_cast<const TX*>(a.x) + (live ? r : a.R - 1) * a.ldx;
     Group<TX, E> g[NV];
@@ -195,7 +205,7 @@ __global__ __launch_bounds__(NT) void norm_kernel(NormArgs a) {
 #pragma unroll
       for (int e = 0; e < E; ++e) s[0] += g[i].get(e);
     row_sums(s, tpr, red1, slot1);
-    float mean = s[0] / (float)D, rstd;
+    float mean = s[0] * a.inv_d, rstd;
     float q[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -206,7 +216,7 @@ __global__ __launch_bounds__(NT) void norm_kernel(NormArgs a) {
         q[1] = fmaf(d, d, q[1]);
       }
     row_sums(q, tpr, red2, slot2);
-    finish_stats(mean, rstd, q, (float)D, a.eps);
+    finish_stats(mean, rstd, q, a.inv_d, a.eps);
     if (!live) continue;
     if (sub == 0) {
       if (a.mean) a.mean[r] = mean;
@@ -217,11 +227,9 @@ __global__ __launch_bounds__(NT) void norm_kernel(NormArgs a) {
     for (int i = 0; i < NV; ++i) {
       const int c = E * (sub + i * tpr);
       if (c >= D) continue;
-      float w[E], b[E], y[E];
-      load_params<E>(a.w, a.w_bf16, c, D, 1.f, w);
-      load_params<E>(a.b, a.w_bf16, c, D, 0.f, b);
+      float y[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) y[e] = fmaf((g[i].get(e) - mean) * rstd, w[e], b[e]);
+      for (int e = 0; e < E; ++e) y[e] = fmaf((g[i].get(e) - mean) * rstd, w[i][e], b[i][e]);
       store_group<TY, E>(out, c, D, y);
     }
   }
@@ -245,7 +253,7 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a) {
       for (int e = 0; e < E; ++e) s[0] += g.get(e);
     }
     row_sums(s, 1024, red1, slot1);
-    float mean = s[0] / (float)D, rstd;
+    float mean = s[0] * a.inv_d, rstd;
     float q[2] = {0.f, 0.f};
     for (int64_t c = E * threadIdx.x; c < D; c += E * 1024) {
       Group<TX, E> g;
@@ -258,7 +266,7 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a) {
       }
     }
     row_sums(q, 1024, red2, slot2);
-    finish_stats(mean, rstd, q, (float)D, a.eps);
+    finish_stats(mean, rstd, q, a.inv_d, a.eps);
     if (threadIdx.x == 0) {
       if (a.mean) a.mean[r] = mean;
       if (a.rstd) a.rstd[r] = rstd;
@@ -298,8 +306,8 @@ __global__ __launch_bounds__(NT) void norm_grad_kernel(NormArgs a) {
   __shared__ float sums[NT == 256 ? 256 * E : 1];
   int slot = 0;
   const int tpr = a.tpr, D = a.D;
-  const int sub = threadIdx.x & (tpr - 1);
   const int rpb = blockDim.x / tpr;
+  const int sub = rpb == 1 ? threadIdx.x : threadIdx.x & (tpr - 1);
   float w[NV][E], dw[NV][E], db[NV][E];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -308,7 +316,7 @@ __global__ __launch_bounds__(NT) void norm_grad_kernel(NormArgs a) {
     for (int e = 0; e < E; ++e) dw[i][e] = db[i][e] = 0.f;
   }
   for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < a.R; r0 += (int64_t)gridDim.x * rpb) {
-    const int64_t r = r0 + threadIdx.x / tpr;
+    const int64_t r = r0 + (rpb == 1 ? 0 : threadIdx.x / tpr);
     const bool live = r < a.R;
     const int64_t rr = live ? r : a.R - 1;
     const TX* row = static_cast<const TX*>(a.x) + rr * a.ldx;
@@ -336,7 +344,7 @@ __global__ __launch_bounds__(NT) void norm_grad_kernel(NormArgs a) {
       }
     row_sums(s, tpr, red, slot);
     if (!live) continue;
-    const float c1 = s[0] / (float)D, c2 = s[1] / (float)D;
+    const float c1 = s[0] * a.inv_d, c2 = s[1] * a.inv_d;
     TY* out = static_cast<TY*>(a.dx) + r * a.lddx;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -366,7 +374,6 @@ __global__ __launch_bounds__(NT) void norm_grad_kernel(NormArgs a) {
             db[i][e] += __shfl_xor(db[i][e], o);
           }
       }
-      const int stride = max(tpr, 64);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -379,7 +386,7 @@ __global__ __launch_bounds__(NT) void norm_grad_kernel(NormArgs a) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
               float t = sums[e * 256 + threadIdx.x];
-              for (int at = stride; at < 256; at += stride) t += sums[e * 256 + at + threadIdx.x];
+              for (int at = 64; at < 256; at += 64) t += sums[e * 256 + at + threadIdx.x];
               (k ? db[i][e] : dw[i][e]) = t;
             }
           }
@@ -422,8 +429,8 @@ __global__ __launch_bounds__(1024) void norm_grad_rows_kernel(NormArgs a, float*
     }
     row_sums(s, 1024, red, slot);
     if (threadIdx.x == 0) {
-      c12[2 * r] = s[0] / (float)D;
-      c12[2 * r + 1] = s[1] / (float)D;
+      c12[2 * r] = s[0] * a.inv_d;
+      c12[2 * r + 1] = s[1] * a.inv_d;
     }
   }
 }
@@ -497,32 +504,43 @@ __global__ __launch_bounds__(1024) void norm_grad_sum_kernel(NormArgs a, int par
 
 // How a row is spread: tpr threads of nv groups each (nv 0: too long).
 struct NormGeom {
-  int tpr, nv, nt;
+  int tpr, nv, nt;  // nt: threads of a workgroup
 };
 
-// The fewest idle lanes; then, with enough rows to fill the chip anyway, the
-// fewest threads a row (fewer steps of the sums, more loads in flight each) up
-// to 4 groups a thread (4099 x 3001 fp32, 1, 2, 4 and 8 groups: 42, 28, 23 and
-// 28 us), and with few rows the most.
+// Among the spreads that leave few lanes idle (within a third of the fewest):
+// with enough rows to fill the chip anyway, the fewest threads a row (fewer
+// steps of the sums, more loads in flight each) up to 4 groups a thread (4099 x
+// 3001 fp32, 1, 2, 4 and 8 groups: 42, 28, 23 and 28 us; 8192 x 1600, 1 group
+// in 448 threads 40 us, 4 in 128 24), and with few rows the most.
 NormGeom norm_geom(int64_t R, int64_t D, int e, int max_nv) {
   const int64_t groups = cdiv(D, e);
   NormGeom best{0, 0, 0};
-  int64_t waste = INT64_MAX;
+  auto threads = [&](int nv) {  // of a row: a power of two up to a wave, then whole waves
+    const int64_t n = cdiv(groups, nv);
+    if (n > 64) return cdiv(n, 64) * 64;
+    int64_t t = 1;
+    while (t < n) t *= 2;
+    return t;
+  };
+  int64_t least = INT64_MAX;
+  for (int nv = 1; nv <= max_nv; nv *= 2)
+    if (threads(nv) <= 1024) least = std::min(least, threads(nv) * nv);
   const bool many = R >= 8 * (int64_t)device_cus();
   for (int nv = 1; nv <= max_nv; nv *= 2) {
-    int64_t tpr = 1;
-    while (tpr * nv < groups) tpr *= 2;
-    if (tpr > 1024) continue;
-    const int64_t w = tpr * nv;
-    if (w < waste || (w == waste && many)) {
-      waste = w;
-      best = {(int)tpr, nv, tpr <= 256 ? 256 : (int)tpr};
-    }
+    const int64_t tpr = threads(nv);
+    if (tpr > 1024 || 3 * tpr * nv > 4 * least || (best.nv != 0 && !many)) continue;
+    best = {(int)tpr, nv, tpr <= 64 ? 256 : (int)tpr};
   }
   return best;
 }
 
-constexpr int kMaxGrid = 1 << 20;  // workgroups; the row loops stride over the rest
+constexpr int kMaxGrid = 1 << 20;  // workgroups of the passes over long rows; their loops stride over the rest
+
+// Waves a CU of the forward pass, whose workgroups walk over rows with their
+// parameters in registers: read again for every row, from the caches, they made
+// 8192 x 4096 bf16 35 us instead of 28, 4099 x 3001 fp32 22 instead of 20 (16,
+// 24 and 32 waves: 28, 30 and 31 us).
+constexpr int kWaves = 16;
 
 template <typename TX, typename TY>
 hipError_t launch_norm(NormArgs a, hipStream_t stream) {
@@ -535,7 +553,7 @@ hipError_t launch_norm(NormArgs a, hipStream_t stream) {
   }
   a.tpr = g.tpr;
   const int threads = g.nt;
-  const dim3 grid((unsigned)std::min<int64_t>(cdiv(a.R, threads / g.tpr), kMaxGrid)), block(threads);
+  const dim3 grid((unsigned)std::min<int64_t>(cdiv(a.R, threads / g.tpr), kWaves * 64 / threads * (int64_t)device_cus())), block(threads);
   auto go = [&](auto nv, auto nt) {
     hipLaunchKernelGGL((norm_kernel<TX, TY, decltype(nv)::value, decltype(nt)::value>), grid, block, 0, stream, a);
     return hipGetLastError();
@@ -546,8 +564,8 @@ hipError_t launch_norm(NormArgs a, hipStream_t stream) {
            : g.nv == 2 ? go(integral_constant<int, 2>{}, nt)
                        : go(integral_constant<int, 4>{}, nt);
   };
-  return g.nt == 256   ? by_nv(integral_constant<int, 256>{})
-         : g.nt == 512 ? by_nv(integral_constant<int, 512>{})
+  return g.nt <= 256   ? by_nv(integral_constant<int, 256>{})
+         : g.nt <= 512 ? by_nv(integral_constant<int, 512>{})
                        : by_nv(integral_constant<int, 1024>{});
 }
 
@@ -606,8 +624,8 @@ hipError_t launch_norm_grad(NormArgs a, const GradGeom& q, float* c12, hipStream
       }
       return q.g.nv == 1 ? go(integral_constant<int, 1>{}, nt) : go(integral_constant<int, 2>{}, nt);
     };
-    e = q.g.nt == 256   ? by_nv(integral_constant<int, 256>{})
-        : q.g.nt == 512 ? by_nv(integral_constant<int, 512>{})
+    e = q.g.nt <= 256   ? by_nv(integral_constant<int, 256>{})
+        : q.g.nt <= 512 ? by_nv(integral_constant<int, 512>{})
                         : by_nv(integral_constant<int, 1024>{});
   }
   if (e != hipSuccess || (!a.dw && !a.db) || q.parts == 1) return e;
@@ -661,7 +679,7 @@ int tilec_layer_norm(const void* x, const void* weight, const void* bias, void* 
   if (rc != TILEC_OK || R == 0) return rc;
   NormArgs a{};
   a.x = x, a.w = weight, a.b = bias, a.y = y, a.mean = mean, a.rstd = rstd;
-  a.ldx = ldx, a.ldy = ldy, a.R = R, a.D = (int)D, a.w_bf16 = w_dtype == TILEC_BF16, a.eps = eps;
+  a.ldx = ldx, a.ldy = ldy, a.R = R, a.D = (int)D, a.w_bf16 = w_dtype == TILEC_BF16, a.eps = eps, a.inv_d = 1.f / (float)D;
   const hipError_t e = by_types(x_dtype, y_dtype, [&](auto tx, auto ty) {
     return launch_norm<decltype(tx), decltype(ty)>(a, static_cast<hipStream_t>(stream));
   });
@@ -695,7 +713,7 @@ int tilec_layer_norm_backward(const void* dy, const void* x, const float* mean, 
   NormArgs a{};
   a.x = x, a.dy = dy, a.w = weight, a.dx = dx, a.mean_in = mean, a.rstd_in = rstd, a.dw = dweight, a.db = dbias;
   a.ldx = ldx, a.ldy = lddy, a.lddx = lddx, a.R = R, a.D = (int)D, a.Dp = (int)q.Dp;
-  a.w_bf16 = w_dtype == TILEC_BF16;
+  a.w_bf16 = w_dtype == TILEC_BF16, a.inv_d = 1.f / (float)D;
   a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + q.c12_bytes);
   float* c12 = static_cast<float*>(workspace);
   const hipError_t e = by_types(x_dtype, y_dtype, [&](auto tx, auto ty) {

@@ -99,6 +99,12 @@ def _norm_params(what, D, weight, bias):
     return weight, bias, _code(what, weight)
 
 
+@lru_cache(4096)
+def _norm_workspace(device, R, D, x_code):
+    """Bytes the backward pass needs on the current GPU, `device`."""
+    return _lib.lib().tilec_layer_norm_backward_workspace_bytes(R, D, x_code)
+
+
 def layer_norm(x, weight=None, bias=None, eps=1e-5, dtype=None):
     """(y, mean, rstd): every row of x normalised to mean 0 and variance 1,
     times `weight` plus `bias`.
@@ -168,7 +174,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, param_grads=True):
     L = _lib.lib()
     with _on(at):
         stream = _raw_stream(at)
-        need = L.tilec_layer_norm_backward_workspace_bytes(R, D, x_code)
+        need = _norm_workspace(at, R, D, x_code)
         ws_ptr = workspace_for(dy.device, stream, need).data_ptr() if need else None
         _lib.check(L.tilec_layer_norm_backward(
             dy.data_ptr(), x.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _ptr(weight), dx.data_ptr(), _ptr(dw),
