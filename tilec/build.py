@@ -49,7 +49,8 @@ def _compile(src):
 
 
 def _host():
-    """tilec/_host.so: a CPython module against torch's headers and libraries."""
+    """tilec/_host.so: a CPython module against torch's headers and libraries and
+    libtilec_hip.so beside it."""
     import torch
     from torch.utils import cpp_extension
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
@@ -58,7 +59,7 @@ def _host():
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-I" + sysconfig.get_paths()["include"], *("-isystem" + p for p in cpp_extension.include_paths()),
            os.path.join(CSRC, "host.cpp"), "-o", tmp, "-L" + torch_lib, "-Wl,-rpath," + torch_lib,
-           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-L" + HERE, "-Wl,-rpath,$ORIGIN", "-ltilec_hip"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"building {HOST} failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
@@ -68,10 +69,8 @@ def _host():
 def build(verbose=False):
     os.makedirs(OBJDIR, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
-    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
-        host = ex.submit(_host)
+    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
         objs = list(ex.map(_compile, srcs))
-        host.result()
     tmp = LIB + ".tmp"
     # --no-undefined: a kernel whose host stub the compiler dropped fails here,
     # not when the library is first loaded.
@@ -80,6 +79,7 @@ def build(verbose=False):
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
+    _host()
     if verbose:
         print(f"built {LIB} and {HOST}")
     return LIB

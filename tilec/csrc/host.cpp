@@ -1,20 +1,32 @@
-// tilec._host: what a step over many tensors needs of them, read in C++.
+// tilec._host: host code that reads torch tensors, where reading them from Python
+// costs more than the kernels they are for.
 //
 //   adamw_table(params, grads, exp_avg, exp_avg_sq, copies)
 //       -> None (nothing to do) or (table, count, bits, device, kept)
 //   adamw_values_table(states)
-//       -> (table, count, device, outputs)
+//       -> None or (table, count, device, outputs)
 //
-// The first checks the lists and packs a tilec_adamw_tensor (include/tilec.h) for each
-// parameter with a gradient into the bytes `table`.  The same checks attribute
-// by attribute in Python take 1.1 us a tensor (80 us for 72 tensors, whose
-// kernels take 12); these take 0.05.  `kept`: contiguous copies of gradients
+// The first checks the lists and packs a tilec_adamw_tensor (include/tilec.h)
+// for each parameter with a gradient into the bytes `table`.  The same checks
+// attribute by attribute in Python take 1.1 us a tensor (80 us for 72 tensors,
+// whose kernels take 12); these take 0.05.  `kept`: contiguous copies of gradients
 // that were not, to be held until the launch.  The second does the same for
 // tilec_adamw_values, whose float32 outputs it allocates, views of one storage.
+//
+//   layer_norm(x, weight, bias, eps, dtype, stream) -> (y, mean, rstd)
+//   layer_norm_backward(dy, x, mean, rstd, weight, param_grads, stream)
+//       -> (dx, dweight, dbias)
+//
+// check their arguments, allocate the outputs and enqueue the kernels on `stream`
+// (the handle of the tensors' device's current stream): one row of 4096 then
+// costs 6 us a call instead of 10.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include <ATen/ops/empty.h>
+#include <ATen/ops/empty_like.h>
+#include <c10/core/DeviceGuard.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -33,13 +45,13 @@ struct Refused {
   std::string what;
 };
 
-[[noreturn]] void bad_value(const std::string& what) { throw Refused{PyExc_ValueError, "adamw: " + what}; }
-[[noreturn]] void bad_type(const std::string& what) { throw Refused{PyExc_TypeError, "adamw: " + what}; }
+[[noreturn]] void bad_value(const std::string& what) { throw Refused{PyExc_ValueError, what}; }
+[[noreturn]] void bad_type(const std::string& what) { throw Refused{PyExc_TypeError, what}; }
 
 // A list or tuple, or whatever else is a sequence.
 struct List {
   PyObject* seq;
-  explicit List(PyObject* o) : seq(PySequence_Fast(o, "adamw: expected lists of tensors")) {
+  explicit List(PyObject* o) : seq(PySequence_Fast(o, "expected lists of tensors")) {
     if (seq == nullptr) throw python_error();
   }
   ~List() { Py_DECREF(seq); }
@@ -177,7 +189,158 @@ PyObject* build_values(PyObject* const* args) {
                        (Py_ssize_t)(table.size() * sizeof(tilec_adamw_tensor)), (int)count, (long long)r.device, outs);
 }
 
-template <PyObject* (*BUILD)(PyObject* const*), int ARGS>
+// A status of the library as the exception the ctypes binding raises for it.
+void check(int rc) {
+  if (rc == TILEC_OK) return;
+  throw Refused{rc == TILEC_ERR_VALUE ? PyExc_ValueError : rc == TILEC_ERR_TYPE ? PyExc_TypeError : PyExc_RuntimeError,
+                tilec_last_error()};
+}
+
+std::string shape(const at::Tensor& t) {
+  std::string s = "(";
+  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+  return s + (t.dim() == 1 ? ",)" : ")");
+}
+
+// A tensor of one GPU, float32 or bfloat16.
+struct OneGpu {
+  int64_t device = -1;
+  int32_t code(const char* name, const at::Tensor& t) {
+    if (!t.is_cuda()) bad_type("needs tensors on a ROCm GPU (" + std::string(name) + " is on " + t.device().str() + ")");
+    if (device < 0) device = t.get_device();
+    if (t.get_device() != device) bad_type("needs all tensors on one GPU (" + std::string(name) + " is on another)");
+    if (t.layout() != at::kStrided) bad_type(std::string(name) + " is not a dense tensor");
+    if (t.scalar_type() != at::kFloat && t.scalar_type() != at::kBFloat16)
+      bad_type("unsupported tensor " + std::string(name) + " of dtype " + toString(t.scalar_type()) +
+               " (use float32 or bfloat16)");
+    return ::code(t);
+  }
+};
+
+// A matrix whose rows are contiguous (copied if they are not); one dimension is
+// one row.
+struct Rows {
+  at::Tensor t;
+  int64_t R, D, ld;
+  Rows(const char* name, const at::Tensor& x) : t(x) {
+    if (x.dim() != 1 && x.dim() != 2)
+      bad_value("expected a 1-D or 2-D " + std::string(name) + ", got shape " + shape(x));
+    R = x.dim() == 1 ? 1 : x.size(0);
+    D = x.size(-1);
+    if (D == 0) bad_value("rows without elements have no mean (shape " + shape(x) + ")");
+    if ((D > 1 && x.stride(-1) != 1) || (R > 1 && x.stride(0) < D)) t = x.contiguous();
+    ld = R > 1 ? t.stride(0) : D;
+  }
+};
+
+at::Tensor vector(const char* name, const at::Tensor& t, int64_t n) {
+  if (t.dim() != 1 || t.size(0) != n)
+    bad_value(std::string(name) + " has shape " + shape(t) + ", expected (" + std::to_string(n) + ",)");
+  return t.contiguous();
+}
+
+// weight or bias: absent, or [D] of one type for both.
+struct Params {
+  at::Tensor weight, bias;
+  int32_t code = TILEC_F32;
+  Params(OneGpu& gpu, PyObject* w, PyObject* b, int64_t D) {
+    if (w != Py_None) {
+      const at::Tensor& t = tensor("weight", w);
+      code = gpu.code("weight", t);
+      weight = vector("weight", t, D);
+    }
+    if (b != Py_None) {
+      const at::Tensor& t = tensor("bias", b);
+      const int32_t c = gpu.code("bias", t);
+      if (w != Py_None && c != code) bad_type("weight and bias have different types");
+      code = c;
+      bias = vector("bias", t, D);
+    }
+  }
+};
+
+const void* data(const at::Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+
+void* stream_of(PyObject* o) {
+  void* s = PyLong_AsVoidPtr(o);
+  if (s == nullptr && PyErr_Occurred()) throw python_error();
+  return s;
+}
+
+PyObject* three(const at::Tensor& a, const at::Tensor& b, const at::Tensor& c) {
+  PyObject* t = PyTuple_New(3);
+  if (t == nullptr) throw python_error();
+  const at::Tensor* all[3] = {&a, &b, &c};
+  for (int i = 0; i < 3; ++i) {
+    PyObject* o = all[i]->defined() ? THPVariable_Wrap(*all[i]) : nullptr;
+    if (o == nullptr) Py_INCREF(o = Py_None);
+    PyTuple_SET_ITEM(t, i, o);
+  }
+  return t;
+}
+
+PyObject* build_norm(PyObject* const* args) {
+  const at::Tensor& x = tensor("x", args[0]);
+  OneGpu gpu;
+  const int32_t x_code = gpu.code("x", x);
+  const Rows r("x", x);
+  const Params p(gpu, args[1], args[2], r.D);
+  const double eps = PyFloat_AsDouble(args[3]);
+  if (eps == -1.0 && PyErr_Occurred()) throw python_error();
+  at::ScalarType type = x.scalar_type();
+  if (args[4] != Py_None) {
+    if (!THPDtype_Check(args[4])) bad_type("dtype is no torch.dtype");
+    type = reinterpret_cast<THPDtype*>(args[4])->scalar_type;
+    if (type != at::kFloat && type != at::kBFloat16)
+      bad_type(std::string("unsupported dtype ") + toString(type) + " (use float32 or bfloat16)");
+  }
+  const c10::DeviceGuard guard(x.device());
+  const at::Tensor y = at::empty(x.sizes(), x.options().dtype(type));
+  const at::Tensor mean = at::empty({r.R}, x.options().dtype(at::kFloat)), rstd = at::empty_like(mean);
+  check(tilec_layer_norm(r.t.const_data_ptr(), data(p.weight), data(p.bias), y.data_ptr(),
+                         static_cast<float*>(mean.data_ptr()), static_cast<float*>(rstd.data_ptr()), r.R, r.D, r.ld,
+                         r.D, x_code, code(y), p.code, (float)eps, stream_of(args[5])));
+  return three(y, mean, rstd);
+}
+
+PyObject* build_norm_backward(PyObject* const* args) {
+  const at::Tensor &dy = tensor("dy", args[0]), &x = tensor("x", args[1]);
+  const at::Tensor &mean_in = tensor("mean", args[2]), &rstd_in = tensor("rstd", args[3]);
+  OneGpu gpu;
+  const int32_t y_code = gpu.code("dy", dy), x_code = gpu.code("x", x);
+  if (dy.sizes() != x.sizes()) bad_value("dy has shape " + shape(dy) + ", x " + shape(x));
+  const Rows d("dy", dy), r("x", x);
+  for (const at::Tensor* t : {&mean_in, &rstd_in}) {
+    gpu.code("mean and rstd", *t);
+    if (t->scalar_type() != at::kFloat) bad_type("mean and rstd are float32");
+  }
+  const at::Tensor mean = vector("mean", mean_in, r.R), rstd = vector("rstd", rstd_in, r.R);
+  const Params p(gpu, args[4], Py_None, r.D);
+  const int sums = PyObject_IsTrue(args[5]);
+  if (sums < 0) throw python_error();
+  const c10::DeviceGuard guard(dy.device());
+  const at::Tensor dx = at::empty(dy.sizes(), dy.options());
+  at::Tensor dw, db, scratch;
+  if (sums) {
+    dw = at::empty({r.D}, dy.options().dtype(at::kFloat));
+    db = at::empty_like(dw);
+  }
+  if (sums || r.R > 0) {
+    const size_t need = tilec_layer_norm_backward_workspace_bytes(r.R, r.D, x_code);
+    if (need > 0) scratch = at::empty({(int64_t)need}, dy.options().dtype(at::kByte));
+    check(tilec_layer_norm_backward(
+        d.t.const_data_ptr(), r.t.const_data_ptr(), static_cast<const float*>(mean.const_data_ptr()),
+        static_cast<const float*>(rstd.const_data_ptr()), data(p.weight), dx.data_ptr(),
+        sums ? static_cast<float*>(dw.data_ptr()) : nullptr, sums ? static_cast<float*>(db.data_ptr()) : nullptr, r.R,
+        r.D, d.ld, r.ld, r.D, x_code, y_code, p.code, need > 0 ? scratch.data_ptr() : nullptr, need,
+        stream_of(args[6])));
+  }
+  return three(dx, dw, db);
+}
+
+constexpr char kAdamw[] = "adamw", kNorm[] = "layer_norm", kNormBackward[] = "layer_norm_backward";
+
+template <PyObject* (*BUILD)(PyObject* const*), int ARGS, const char* NAME>
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t count) {
   HANDLE_TH_ERRORS
   if (count != ARGS) {
@@ -187,22 +350,26 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t count) {
   try {
     return BUILD(args);
   } catch (const Refused& e) {
-    PyErr_SetString(e.type, e.what.c_str());
+    PyErr_SetString(e.type, (std::string(NAME) + ": " + e.what).c_str());
     return nullptr;
   }
   END_HANDLE_TH_ERRORS
 }
 
-template <PyObject* (*BUILD)(PyObject* const*), int ARGS>
+template <PyObject* (*BUILD)(PyObject* const*), int ARGS, const char* NAME>
 PyCFunction function() {
-  return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&call<BUILD, ARGS>));
+  return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&call<BUILD, ARGS, NAME>));
 }
 
 PyMethodDef kMethods[] = {
-    {"adamw_table", function<build, 5>(), METH_FASTCALL,
+    {"adamw_table", function<build, 5, kAdamw>(), METH_FASTCALL,
      "adamw_table(params, grads, exp_avg, exp_avg_sq, copies) -> None or (table, count, bits, device, kept)"},
-    {"adamw_values_table", function<build_values, 1>(), METH_FASTCALL,
+    {"adamw_values_table", function<build_values, 1, kAdamw>(), METH_FASTCALL,
      "adamw_values_table(states) -> None or (table, count, device, outputs)"},
+    {"layer_norm", function<build_norm, 6, kNorm>(), METH_FASTCALL,
+     "layer_norm(x, weight, bias, eps, dtype, stream) -> (y, mean, rstd)"},
+    {"layer_norm_backward", function<build_norm_backward, 7, kNormBackward>(), METH_FASTCALL,
+     "layer_norm_backward(dy, x, mean, rstd, weight, param_grads, stream) -> (dx, dweight, dbias)"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -55,16 +55,6 @@ def _rows(what, name, x):
     return x, (x.stride(0) if R > 1 else D)
 
 
-def _vector(what, name, t, n, dtype=None):
-    if t is None:
-        return None
-    if t.dim() != 1 or t.shape[0] != n:
-        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected ({n},)")
-    if dtype is not None and t.dtype != dtype:
-        raise TypeError(f"{what}: {name} has dtype {t.dtype}, expected {dtype}")
-    return t.contiguous()
-
-
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -72,6 +62,11 @@ def _ptr(t):
 # Per call these cost less than torch.cuda.current_stream and current_device,
 # which build objects and check for initialisation (a GPU tensor is at hand).
 _raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
+def _stream_of(x):
+    """The current stream of the GPU that x is on (0 elsewhere: x is refused)."""
+    return _raw_stream(x.get_device()) if x.is_cuda else 0
 
 
 class _Here:
@@ -90,21 +85,6 @@ def _on(index):
     return _HERE if index == _current() else torch.cuda.device(index)
 
 
-def _norm_params(what, D, weight, bias):
-    weight, bias = _vector(what, "weight", weight, D), _vector(what, "bias", bias, D)
-    if weight is None:
-        return weight, bias, _lib.F32 if bias is None else _code(what, bias)
-    if bias is not None and bias.dtype != weight.dtype:
-        raise TypeError(f"{what}: weight and bias have different types ({weight.dtype} and {bias.dtype})")
-    return weight, bias, _code(what, weight)
-
-
-@lru_cache(4096)
-def _norm_workspace(device, R, D, x_code):
-    """Bytes the backward pass needs on the current GPU, `device`."""
-    return _lib.lib().tilec_layer_norm_backward_workspace_bytes(R, D, x_code)
-
-
 def layer_norm(x, weight=None, bias=None, eps=1e-5, dtype=None):
     """(y, mean, rstd): every row of x normalised to mean 0 and variance 1,
     times `weight` plus `bias`.
@@ -118,25 +98,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, dtype=None):
     to the bf16 input of the next product).  mean and rstd are float32 [R]
     whatever the types; `layer_norm_backward` takes them.
     """
-    what = "layer_norm"
-    shape = x.shape
-    at = _on_gpu(what, x, weight, bias)
-    x_code = _code(what, x)
-    x, ldx = _rows(what, "x", x)
-    R, D = x.shape
-    if D == 0:
-        raise ValueError(f"{what}: rows without elements have no mean (shape {tuple(shape)})")
-    weight, bias, w_code = _norm_params(what, D, weight, bias)
-    y = torch.empty(shape, dtype=dtype or x.dtype, device=x.device)
-    y_code = _code(what, y)
-    mean = torch.empty(R, dtype=torch.float32, device=x.device)
-    rstd = torch.empty_like(mean)
-    if R:
-        with _on(at):
-            _lib.check(_lib.lib().tilec_layer_norm(
-                x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), R, D, ldx, D,
-                x_code, y_code, w_code, eps, _raw_stream(at)))
-    return y, mean, rstd
+    return _lib.host().layer_norm(x, weight, bias, eps, dtype, _stream_of(x))
 
 
 def layer_norm_backward(dy, x, mean, rstd, weight=None, param_grads=True):
@@ -150,36 +112,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, param_grads=True):
     and type; dweight and dbias are float32 [D], added in a fixed order (the
     same bits on every call).  param_grads=False leaves them out (None).
     """
-    what = "layer_norm_backward"
-    shape = dy.shape
-    at = _on_gpu(what, dy, x, mean, rstd, weight)
-    y_code, x_code = _code(what, dy), _code(what, x)
-    if dy.shape != x.shape:
-        raise ValueError(f"{what}: dy has shape {tuple(shape)}, x {tuple(x.shape)}")
-    dy, lddy = _rows(what, "dy", dy)
-    x, ldx = _rows(what, "x", x)
-    R, D = x.shape
-    if D == 0:
-        raise ValueError(f"{what}: rows without elements have no mean (shape {tuple(shape)})")
-    mean = _vector(what, "mean", mean, R, torch.float32)
-    rstd = _vector(what, "rstd", rstd, R, torch.float32)
-    weight, _, w_code = _norm_params(what, D, weight, None)
-    dx = torch.empty(shape, dtype=dy.dtype, device=dy.device)
-    dw = db = None
-    if param_grads:
-        dw = torch.empty(D, dtype=torch.float32, device=dy.device)
-        db = torch.empty_like(dw)
-    elif R == 0:
-        return dx, None, None
-    L = _lib.lib()
-    with _on(at):
-        stream = _raw_stream(at)
-        need = _norm_workspace(at, R, D, x_code)
-        ws_ptr = workspace_for(dy.device, stream, need).data_ptr() if need else None
-        _lib.check(L.tilec_layer_norm_backward(
-            dy.data_ptr(), x.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _ptr(weight), dx.data_ptr(), _ptr(dw),
-            _ptr(db), R, D, lddy, ldx, D, x_code, y_code, w_code, ws_ptr, need, stream))
-    return dx, dw, db
+    return _lib.host().layer_norm_backward(dy, x, mean, rstd, weight, param_grads, _stream_of(dy))
 
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
