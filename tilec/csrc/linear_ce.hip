@@ -205,60 +205,74 @@ constexpr int kFewRows = 32;  // of ce_few_rows_kernel
 
 // xs = x with the ignored rows cleared (whatever they hold must not reach dW,
 // where 0 times a NaN would be one) and rows padded with zeros to Hp; where xt
-// is set, also its transpose [H][kFewRows], padded with zeros; and, by one more
+// is set, also its transpose [H][kFewRows], padded with zeros; and, by the last
 // workgroup where `scale` is set, the scalar factor of the gradients.
 template <typename T>
-__global__ __launch_bounds__(256) void ce_prepare_kernel(const T* __restrict__ x, int64_t ldx, T* __restrict__ xs,
-                                                         int64_t Hp, int64_t N, int64_t H,
-                                                         const int64_t* __restrict__ target, int64_t ignore,
-                                                         float* __restrict__ scale, int64_t all,
-                                                         const int64_t* __restrict__ all_targets, int reduction,
-                                                         const float* __restrict__ grad_loss, T* __restrict__ xt) {
-  constexpr int E = 16 / (int)sizeof(T);
-  typedef i32x4 __attribute__((aligned(2))) i32x4_any;
-  __shared__ int count[256];
-  if (scale != nullptr && blockIdx.x == gridDim.x - 1) {
-    int n = 0;
+struct CePrepare {
+  const T* x;
+  int64_t ldx;
+  T *xs, *xt;
+  int64_t Hp, N, H;
+  const int64_t* target;
+  int64_t ignore;
+  float* scale;
+  int64_t all;  // rows of all chunks, and their targets
+  const int64_t* all_targets;
+  int reduction;
+  const float* grad_loss;
+
+  // Workgroup `block` of `blocks` (two at least where scale is set), 256 threads.
+  __device__ void run(int64_t block, int64_t blocks, int* count) const {
+    constexpr int E = 16 / (int)sizeof(T);
+    typedef i32x4 __attribute__((aligned(2))) i32x4_any;
+    if (scale != nullptr && block == --blocks) {
+      int n = 0;
 #pragma unroll 8
-    for (int64_t i = threadIdx.x; i < all; i += 256) n += all_targets[i] != ignore;
-    count[threadIdx.x] = n;
-    for (int o = 128; o > 0; o >>= 1) {
-      __syncthreads();
-      if ((int)threadIdx.x < o) count[threadIdx.x] += count[threadIdx.x + o];
-    }
-    if (threadIdx.x == 0) {
-      float f = 1.f;
-      if (reduction != kNone && grad_loss != nullptr) f = *grad_loss;
-      if (reduction == kMean) f /= (float)max(count[0], 1);
-      *scale = f;
-    }
-    return;
-  }
-  const int64_t blocks = gridDim.x - (scale != nullptr ? 1 : 0);
-  const int64_t per_row = Hp / E;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < N * per_row; i += blocks * 256) {
-    const int64_t r = i / per_row, c = (i - r * per_row) * E;
-    i32x4 v = {0, 0, 0, 0};
-    if (target[r] != ignore) {
-      const T* p = x + r * ldx + c;
-      if (c + E <= H) {
-        v = *reinterpret_cast<const i32x4_any*>(p);
-      } else {
-#pragma unroll
-        for (int k = 0; k < E; ++k)
-          if (c + k < H) {
-            if constexpr (sizeof(T) == 4) v[k] = reinterpret_cast<const int*>(p)[k];
-            else v[k / 2] |= (int)((uint32_t)p[k] << (16 * (k & 1)));
-          }
+      for (int64_t i = threadIdx.x; i < all; i += 256) n += all_targets[i] != ignore;
+      count[threadIdx.x] = n;
+      for (int o = 128; o > 0; o >>= 1) {
+        __syncthreads();
+        if ((int)threadIdx.x < o) count[threadIdx.x] += count[threadIdx.x + o];
       }
+      if (threadIdx.x == 0) {
+        float f = 1.f;
+        if (reduction != kNone && grad_loss != nullptr) f = *grad_loss;
+        if (reduction == kMean) f /= (float)max(count[0], 1);
+        *scale = f;
+      }
+      return;
     }
-    *reinterpret_cast<i32x4*>(xs + r * Hp + c) = v;
+    const int64_t per_row = Hp / E;
+    for (int64_t i = block * 256 + threadIdx.x; i < N * per_row; i += blocks * 256) {
+      const int64_t r = i / per_row, c = (i - r * per_row) * E;
+      i32x4 v = {0, 0, 0, 0};
+      if (target[r] != ignore) {
+        const T* p = x + r * ldx + c;
+        if (c + E <= H) {
+          v = *reinterpret_cast<const i32x4_any*>(p);
+        } else {
+#pragma unroll
+          for (int k = 0; k < E; ++k)
+            if (c + k < H) {
+              if constexpr (sizeof(T) == 4) v[k] = reinterpret_cast<const int*>(p)[k];
+              else v[k / 2] |= (int)((uint32_t)p[k] << (16 * (k & 1)));
+            }
+        }
+      }
+      *reinterpret_cast<i32x4*>(xs + r * Hp + c) = v;
+    }
+    if (xt == nullptr) return;
+    for (int64_t i = block * 256 + threadIdx.x; i < kFewRows * H; i += blocks * 256) {
+      const int64_t r = i / H, h = i - r * H;
+      xt[h * kFewRows + r] = r < N && target[r] != ignore ? x[r * ldx + h] : T{0};
+    }
   }
-  if (xt == nullptr) return;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < kFewRows * H; i += blocks * 256) {
-    const int64_t r = i / H, h = i - r * H;
-    xt[h * kFewRows + r] = r < N && target[r] != ignore ? x[r * ldx + h] : T{0};
-  }
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void ce_prepare_kernel(CePrepare<T> a) {
+  __shared__ int count[256];
+  a.run(blockIdx.x, gridDim.x, count);
 }
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -331,9 +345,18 @@ struct CeRows {
   const float* scale;      // (T = float)
 };
 
+// The workgroups from grid y = `share` on prepare the operands of the
+// gradients instead, where the logits' product did not need them (one launch
+// less, 3 us).
 template <typename T>
-__global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
+__global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a, int share, CePrepare<T> prepare) {
   __shared__ float red[2][4];
+  if ((int)blockIdx.y >= share) {
+    __shared__ int count[256];
+    prepare.run((int64_t)((int)blockIdx.y - share) * gridDim.x + blockIdx.x, (int64_t)((int)gridDim.y - share) * gridDim.x,
+                count);
+    return;
+  }
   const int64_t r = blockIdx.x;
   const int tid = threadIdx.x;
   const int64_t want = a.target[r];
@@ -343,7 +366,7 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
   if (ignored) {
     if (a.loss != nullptr && blockIdx.y == 0 && tid == 0) a.loss[r] = 0.f;
     if (a.p == nullptr) return;
-    for (int64_t v = E * ((int64_t)blockIdx.y * 256 + tid); v < a.ldp; v += E * 256 * (int64_t)gridDim.y)
+    for (int64_t v = E * ((int64_t)blockIdx.y * 256 + tid); v < a.ldp; v += E * 256 * (int64_t)share)
       *reinterpret_cast<i32x4*>(row + v) = i32x4{0, 0, 0, 0};
     return;
   }
@@ -368,7 +391,7 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
   if (sizeof(T) == 4) g *= *a.scale;
   if (bad) g = NAN;
   const float at_target = expm1f(tl - lse) * g;
-  for (int64_t v = E * ((int64_t)blockIdx.y * 256 + tid); v < a.ldp; v += E * 256 * (int64_t)gridDim.y) {
+  for (int64_t v = E * ((int64_t)blockIdx.y * 256 + tid); v < a.ldp; v += E * 256 * (int64_t)share) {
     float d[E];
     if constexpr (sizeof(T) == 2) {
       const f16x8 e = *reinterpret_cast<const f16x8*>(row + v);
@@ -673,7 +696,8 @@ struct CePlan {
   int64_t R, chunks;     // rows of a chunk
   int64_t Vp, Hp;        // padded row lengths of the kept values, of xs and wp
   bool pad;              // bf16: operands copied with padded rows
-  bool copy_x;
+  bool copy_x;           // xs is needed
+  bool copy_first;       // by the logits' product too
   bool few;              // bf16: dW by ce_few_rows_kernel
   int groups, shift;
   CeProduct p1, p2, p3;  // bf16
@@ -729,7 +753,8 @@ CePlan make_plan(const CeArgs& a) {
     p.shift = 12;
     p.groups = (int)cdiv(a.V, kGroup32);
   }
-  p.copy_x = a.grad || p.pad || (bf16 && p.Hp != a.H);
+  p.copy_first = bf16 ? p.pad || p.Hp != a.H : a.grad;  // (fp32: the factor goes into d)
+  p.copy_x = a.grad || p.copy_first;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -778,14 +803,25 @@ unsigned grid_for(int64_t n) { return (unsigned)std::min<int64_t>(std::max<int64
 
 // The kernels around the products of one chunk.
 template <typename T>
+CePrepare<T> prepare_of(const CeArgs& a, const CePlan& p, char* ws, int64_t r0, int64_t R) {
+  CePrepare<T> q{};
+  q.x = static_cast<const T*>(a.x) + r0 * a.ldx, q.ldx = a.ldx;
+  q.xs = reinterpret_cast<T*>(ws + p.xs), q.xt = p.few ? reinterpret_cast<T*>(ws + p.xt) : nullptr;
+  q.Hp = p.Hp, q.N = R, q.H = a.H, q.target = a.target + r0, q.ignore = a.ignore;
+  q.scale = a.grad && r0 == 0 ? reinterpret_cast<float*>(ws + p.scale) : nullptr;
+  q.all = a.N, q.all_targets = a.target, q.reduction = a.reduction, q.grad_loss = a.grad_loss;
+  return q;
+}
+template <typename T>
+unsigned prepare_blocks(const CeArgs& a, const CePlan& p, int64_t R) {
+  return grid_for(std::max(R * p.Hp / (16 / (int64_t)sizeof(T)), p.few ? kFewRows * a.H : 0)) + 1;
+}
+
+template <typename T>
 hipError_t run_prepare(const CeArgs& a, const CePlan& p, char* ws, int64_t r0, int64_t R, hipStream_t stream) {
-  if (!p.copy_x) return hipSuccess;
-  const bool count = a.grad && r0 == 0;
-  const unsigned blocks = grid_for(std::max(R * p.Hp / (16 / (int64_t)sizeof(T)), p.few ? kFewRows * a.H : 0));
-  hipLaunchKernelGGL((ce_prepare_kernel<T>), dim3(blocks + (count ? 1 : 0)), dim3(256), 0, stream,
-                     static_cast<const T*>(a.x) + r0 * a.ldx, a.ldx, reinterpret_cast<T*>(ws + p.xs), p.Hp, R, a.H,
-                     a.target + r0, a.ignore, count ? reinterpret_cast<float*>(ws + p.scale) : nullptr, a.N, a.target,
-                     a.reduction, a.grad_loss, p.few ? reinterpret_cast<T*>(ws + p.xt) : nullptr);
+  if (!p.copy_first) return hipSuccess;
+  hipLaunchKernelGGL((ce_prepare_kernel<T>), dim3(prepare_blocks<T>(a, p, R)), dim3(256), 0, stream,
+                     prepare_of<T>(a, p, ws, r0, R));
   return hipGetLastError();
 }
 
@@ -805,7 +841,10 @@ hipError_t run_rows(const CeArgs& a, const CePlan& p, char* ws, int64_t r0, int6
   // it takes to fill the chip.
   const int64_t want = cdiv(4 * (int64_t)device_cus(), R), most = cdiv(p.Vp, 256 * 16 / (int64_t)sizeof(T));
   const unsigned share = a.grad ? (unsigned)std::max<int64_t>(1, std::min(want, most)) : 1;
-  hipLaunchKernelGGL((ce_rows_kernel<T>), dim3((unsigned)R, share), dim3(256), 0, stream, q);
+  const bool late = a.grad && !p.copy_first;
+  const unsigned more = late ? (unsigned)std::max<int64_t>(cdiv(prepare_blocks<T>(a, p, R), R), R == 1 ? 2 : 1) : 0;
+  hipLaunchKernelGGL((ce_rows_kernel<T>), dim3((unsigned)R, share + more), dim3(256), 0, stream, q, (int)share,
+                     late ? prepare_of<T>(a, p, ws, r0, R) : CePrepare<T>{});
   return hipGetLastError();
 }
 
@@ -870,8 +909,8 @@ hipError_t run_bf16(const CeArgs& a, const CePlan& p, char* ws, hipStream_t stre
     const int64_t r0 = c * p.R, R = std::min(p.R, a.N - r0);
     const bool last = c + 1 == p.chunks;
     CE_TRY(run_prepare<u16>(a, p, ws, r0, R, stream));
-    const u16* xc = p.copy_x ? xs : x + r0 * a.ldx;
-    const int64_t ldx = p.copy_x ? p.Hp : a.ldx;
+    const u16* xc = p.copy_first ? xs : x + r0 * a.ldx;
+    const int64_t ldx = p.copy_first ? p.Hp : a.ldx;
     CeLogits le{a.grad ? keep : nullptr,
                 p.Vp,
                 reinterpret_cast<f32x2*>(ws + p.stat),
