@@ -11,6 +11,9 @@ libtilec_hip.so instead of a JIT-compiled Metal tile kernel.
     out = tilec.ext.matrix_mul(x1, x2)
     rows = tilec.ext.sum(x1, axis=1)       # [512] fp32 row sums
 
+The training operators of training.py (layer norm, linear cross entropy, AdamW)
+are part of this module too.
+
 Kernel choice per shape comes from `tune.pick` (the shape→config model trained
 on MI355X), falling back to the library's built-in rule when no model is
 present.  The legacy config-space helpers of the reference (`plan`,
