@@ -287,13 +287,21 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 
 // fp32 logits: (m, sum of exp(l - m)) of each group of kGroup32 columns (grid
-// y) of each row (grid x), and the target's logit.
+// y < groups) of each row (grid x), and the target's logit; the workgroups from
+// grid y = groups on prepare the gradients' operands.
 constexpr int kGroup32 = 4096;
 
 __global__ __launch_bounds__(256) void ce_stats_kernel(const float* __restrict__ l, int64_t ldl, int64_t V,
                                                        const int64_t* __restrict__ target, f32x2* __restrict__ stat,
-                                                       float* __restrict__ tlogit) {
+                                                       int groups, float* __restrict__ tlogit,
+                                                       CePrepare<float> prepare) {
   __shared__ float red[2][4];
+  if ((int)blockIdx.y >= groups) {
+    __shared__ int count[256];
+    prepare.run((int64_t)((int)blockIdx.y - groups) * gridDim.x + blockIdx.x,
+                (int64_t)((int)gridDim.y - groups) * gridDim.x, count);
+    return;
+  }
   const int64_t r = blockIdx.x;
   const int64_t v0 = (int64_t)blockIdx.y * kGroup32;
   const float* row = l + r * ldl;
@@ -325,7 +333,7 @@ __global__ __launch_bounds__(256) void ce_stats_kernel(const float* __restrict__
   if ((threadIdx.x & 63) == 0) red[1][threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0)
-    stat[r * gridDim.y + blockIdx.y] = f32x2{m, (red[1][0] + red[1][1]) + (red[1][2] + red[1][3])};
+    stat[r * groups + blockIdx.y] = f32x2{m, (red[1][0] + red[1][1]) + (red[1][2] + red[1][3])};
 }
 
 // One row (grid x) of a chunk: lse from its groups, the loss, and, where p is
@@ -346,8 +354,8 @@ struct CeRows {
 };
 
 // The workgroups from grid y = `share` on prepare the operands of the
-// gradients instead, where the logits' product did not need them (one launch
-// less, 3 us).
+// gradients instead (bf16), where the logits' product did not need them (one
+// launch less, 3 us).
 template <typename T>
 __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a, int share, CePrepare<T> prepare) {
   __shared__ float red[2][4];
@@ -696,8 +704,7 @@ struct CePlan {
   int64_t R, chunks;     // rows of a chunk
   int64_t Vp, Hp;        // padded row lengths of the kept values, of xs and wp
   bool pad;              // bf16: operands copied with padded rows
-  bool copy_x;           // xs is needed
-  bool copy_first;       // by the logits' product too
+  bool copy_first;       // the logits' product needs xs too
   bool few;              // bf16: dW by ce_few_rows_kernel
   int groups, shift;
   CeProduct p1, p2, p3;  // bf16
@@ -753,8 +760,7 @@ CePlan make_plan(const CeArgs& a) {
     p.shift = 12;
     p.groups = (int)cdiv(a.V, kGroup32);
   }
-  p.copy_first = bf16 ? p.pad || p.Hp != a.H : a.grad;  // (fp32: the factor goes into d)
-  p.copy_x = a.grad || p.copy_first;
+  p.copy_first = bf16 && (p.pad || p.Hp != a.H);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -765,7 +771,7 @@ CePlan make_plan(const CeArgs& a) {
   p.tlogit = take((size_t)p.R * sizeof(float));
   p.rows = take(a.reduction == kNone ? 0 : (size_t)a.N * sizeof(float));
   p.scale = take(sizeof(float));
-  p.xs = take(p.copy_x ? (size_t)(p.R * p.Hp * esz) : 0);
+  p.xs = take(a.grad || p.copy_first ? (size_t)(p.R * p.Hp * esz) : 0);
   p.few = bf16 && a.grad && p.chunks == 1 && p.R <= kFewRows;
   p.xt = take(p.few ? (size_t)(a.H * kFewRows * 2) : 0);
   p.wp = take(p.pad ? (size_t)(a.V * p.Hp * esz) : 0);
@@ -776,16 +782,15 @@ CePlan make_plan(const CeArgs& a) {
       p.split_bytes = std::max(split_workspace(p.p2, a.H, p.R), p.few ? 0 : split_workspace(p.p3, a.H, a.V));
     }
   } else {
-    const int64_t ldxs = p.copy_x ? p.Hp : a.ldx;
     for (const int64_t R : {p.R, a.N - (p.chunks - 1) * p.R}) {
       auto more = [&](int which, int64_t M, int64_t N, int64_t K, int64_t ld1, int64_t ld2, int layout) {
         p.split_bytes = std::max(p.split_bytes, matmul_scratch(a, config_of(a, p, which, R), M, N, K, ld1, ld2, layout,
                                                                &p.counter_bytes));
       };
-      more(0, R, a.V, a.H, ldxs, a.ldw, TILEC_X2_COL_MAJOR);
+      more(0, R, a.V, a.H, a.ldx, a.ldw, TILEC_X2_COL_MAJOR);
       if (!a.grad) continue;
       more(1, R, a.H, a.V, p.Vp, a.ldw, 0);
-      more(2, a.V, a.H, R, p.Vp, ldxs, TILEC_X1_COL_MAJOR);
+      more(2, a.V, a.H, R, p.Vp, p.Hp, TILEC_X1_COL_MAJOR);
     }
   }
   p.split = take(p.split_bytes);
@@ -817,6 +822,17 @@ unsigned prepare_blocks(const CeArgs& a, const CePlan& p, int64_t R) {
   return grid_for(std::max(R * p.Hp / (16 / (int64_t)sizeof(T)), p.few ? kFewRows * a.H : 0)) + 1;
 }
 
+// The same as rows of a grid R wide, where they run beside another kernel's: not
+// more than fit into grid y with that kernel's own (each takes what is left over
+// in steps).
+constexpr unsigned kMoreBlocks = 1024;
+constexpr int64_t kMaxGroups = 65535 - kMoreBlocks;
+template <typename T>
+unsigned more_blocks(const CeArgs& a, const CePlan& p, int64_t R) {
+  if (!a.grad || p.copy_first) return 0;
+  return (unsigned)std::min<int64_t>(std::max<int64_t>(cdiv(prepare_blocks<T>(a, p, R), R), R == 1 ? 2 : 1), kMoreBlocks);
+}
+
 template <typename T>
 hipError_t run_prepare(const CeArgs& a, const CePlan& p, char* ws, int64_t r0, int64_t R, hipStream_t stream) {
   if (!p.copy_first) return hipSuccess;
@@ -841,10 +857,9 @@ hipError_t run_rows(const CeArgs& a, const CePlan& p, char* ws, int64_t r0, int6
   // it takes to fill the chip.
   const int64_t want = cdiv(4 * (int64_t)device_cus(), R), most = cdiv(p.Vp, 256 * 16 / (int64_t)sizeof(T));
   const unsigned share = a.grad ? (unsigned)std::max<int64_t>(1, std::min(want, most)) : 1;
-  const bool late = a.grad && !p.copy_first;
-  const unsigned more = late ? (unsigned)std::max<int64_t>(cdiv(prepare_blocks<T>(a, p, R), R), R == 1 ? 2 : 1) : 0;
+  const unsigned more = sizeof(T) == 2 ? more_blocks<T>(a, p, R) : 0;  // (fp32: beside the statistics)
   hipLaunchKernelGGL((ce_rows_kernel<T>), dim3((unsigned)R, share + more), dim3(256), 0, stream, q, (int)share,
-                     late ? prepare_of<T>(a, p, ws, r0, R) : CePrepare<T>{});
+                     prepare_of<T>(a, p, ws, r0, R));
   return hipGetLastError();
 }
 
@@ -962,7 +977,6 @@ int run_f32(const CeArgs& a, const CePlan& p, char* ws, unsigned* counters, size
   float* xs = reinterpret_cast<float*>(ws + p.xs);
   float* keep = reinterpret_cast<float*>(ws + p.keep);
   float* part = reinterpret_cast<float*>(ws + p.acc);
-  const int64_t ldxs = p.Hp;
   auto product = [&](int which, int64_t R, const float* x1, const float* x2, float* out, int64_t M, int64_t N,
                      int64_t K, int64_t ld1, int64_t ld2, int64_t ldo, int layout) {
     const Config c = config_of(a, p, which, R);
@@ -971,20 +985,18 @@ int run_f32(const CeArgs& a, const CePlan& p, char* ws, unsigned* counters, size
   };
   for (int64_t c = 0; c < p.chunks; ++c) {
     const int64_t r0 = c * p.R, R = std::min(p.R, a.N - r0);
-    if ((*err = run_prepare<float>(a, p, ws, r0, R, stream)) != hipSuccess) return TILEC_ERR_HIP;
-    const float* xc = p.copy_x ? xs : x + r0 * a.ldx;
-    const int64_t ldx = p.copy_x ? ldxs : a.ldx;
-    int rc = product(0, R, xc, w, keep, R, a.V, a.H, ldx, a.ldw, p.Vp, TILEC_X2_COL_MAJOR);
+    int rc = product(0, R, x + r0 * a.ldx, w, keep, R, a.V, a.H, a.ldx, a.ldw, p.Vp, TILEC_X2_COL_MAJOR);
     if (rc != TILEC_OK) return rc;
-    hipLaunchKernelGGL(ce_stats_kernel, dim3((unsigned)R, (unsigned)p.groups), dim3(256), 0, stream, keep, p.Vp, a.V,
-                       a.target + r0, reinterpret_cast<f32x2*>(ws + p.stat), reinterpret_cast<float*>(ws + p.tlogit));
+    hipLaunchKernelGGL(ce_stats_kernel, dim3((unsigned)R, (unsigned)p.groups + more_blocks<float>(a, p, R)), dim3(256), 0,
+                       stream, keep, p.Vp, a.V, a.target + r0, reinterpret_cast<f32x2*>(ws + p.stat), p.groups,
+                       reinterpret_cast<float*>(ws + p.tlogit), prepare_of<float>(a, p, ws, r0, R));
     if ((*err = hipGetLastError()) != hipSuccess) return TILEC_ERR_HIP;
     if ((*err = run_rows<float>(a, p, ws, r0, R, stream)) != hipSuccess) return TILEC_ERR_HIP;
     if (!a.grad) continue;
     rc = product(1, R, keep, w, static_cast<float*>(a.dx) + r0 * a.H, R, a.H, a.V, p.Vp, a.ldw, a.H, 0);
     if (rc != TILEC_OK) return rc;
     float* dw = static_cast<float*>(a.dw);
-    rc = product(2, R, keep, xs, c == 0 ? dw : part, a.V, a.H, R, p.Vp, ldxs, a.H, TILEC_X1_COL_MAJOR);
+    rc = product(2, R, keep, xs, c == 0 ? dw : part, a.V, a.H, R, p.Vp, p.Hp, a.H, TILEC_X1_COL_MAJOR);
     if (rc != TILEC_OK) return rc;
     if (c == 0) continue;
     hipLaunchKernelGGL(ce_add_kernel, dim3(grid_for(a.V * a.H)), dim3(256), 0, stream, dw, part, a.V * a.H);
@@ -1011,7 +1023,7 @@ int check(const CeArgs& a) {
   if (a.dtype == TILEC_BF16 && (a.V > kMaxVocab || a.H > kMaxVocab))
     return fail(TILEC_ERR_UNSUPPORTED, "tilec: linear cross entropy: bf16 takes V and H up to %lld (got %lld, %lld)",
                 (long long)kMaxVocab, (long long)a.V, (long long)a.H);
-  if (cdiv(a.V, kGroup32) > 65535)
+  if (cdiv(a.V, kGroup32) > kMaxGroups)
     return fail(TILEC_ERR_UNSUPPORTED, "tilec: linear cross entropy: V=%lld is too large", (long long)a.V);
   return TILEC_OK;
 }
