@@ -168,6 +168,31 @@ def test_non_finite_gradients_show(value):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_offsets_past_32_bits(bits):
+    # One tensor of more than 2^31 values, checked at both ends and around 2^31.
+    n = (1 << 31) + 1003
+    p, g = torch.zeros(n, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    m, v = tilec.ext.adamw_state(p, bits)
+    near_ends = [slice(0, 512), slice((1 << 31) - 256, (1 << 31) + 256), slice(n - 1003 % 256, n)]
+    gen = torch.Generator().manual_seed(7)
+    for s in near_ends:
+        size = p[s].numel()
+        p[s] = torch.randn(size, generator=gen).cuda()
+        g[s] = (torch.randn(size, generator=gen) * 1e-3).cuda()
+    want = [plain(p[s], g[s], torch.zeros_like(p[s]), torch.zeros_like(p[s]), 1, **HYPER) for s in near_ends]
+    tilec.ext.adamw_step([p], [g], [m], [v], step=1, **HYPER)
+    for s, ((rp, rm, rv), (ep, em, ev)) in zip(near_ends, want):
+        near(p[s], rp, ep, 2.0 ** -8)
+        if bits == 32:
+            near(m[s], rm, em)
+            near(v[s], rv, ev)
+        else:
+            assert (m[0][s].sign() == rm.sign()).logical_or(m[0][s] == 0).all() and (v[0][s] > 0).all()
+    assert not p[1 << 20:1 << 21].any()
+
+
+@pytest.mark.gpu
 def test_8_bits_train_like_32():
     # A least-squares problem of 64 x 512 unknowns with noisy gradients.
     g = torch.Generator().manual_seed(3)

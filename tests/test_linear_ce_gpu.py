@@ -132,6 +132,40 @@ def test_many_tiles(N, H, V, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("N", [3, 40])
+def test_offsets_past_32_bits(N):
+    # A weight and a gradient of more than 2^31 values, checked for the last
+    # classes and the targets'.  x is zero but in 64 columns, the last one among
+    # them: what the logits and dw round is the sums of those alone, so that the
+    # bounds stay as narrow as those of a small problem.
+    H, V, L = 32776, 65600, 64
+    g = torch.Generator(device="cuda").manual_seed(12)
+    w = torch.randn(V, H, generator=g, device="cuda", dtype=torch.bfloat16).mul_(0.25)
+    cols = torch.cat([torch.randperm(H - 1, generator=g, device="cuda")[:L - 1], torch.tensor([H - 1], device="cuda")])
+    x = torch.zeros(N, H, device="cuda", dtype=torch.bfloat16)
+    x[:, cols] = torch.randn(N, L, generator=g, device="cuda").to(torch.bfloat16)
+    t = torch.randint(V, (N,), generator=g, device="cuda")
+    t[0] = V - 1
+    loss, dx, dw = tilec.ext.linear_cross_entropy_grad(x, w, t, "sum")
+    xl, wl = x[:, cols], w[:, cols]
+    rl, _, rdw, d, gr = plain(xl, wl, t, "sum")
+    erow, _, edw = bounds(xl, wl, t, d, gr)
+    assert (loss.double() - rl).abs() <= erow.sum() + 4 * E32 * rl.abs()
+    assert ((dw[:, cols].double() - rdw).abs() <= edw + 2.0 ** -8 * (rdw.abs() + edw)).all()
+    rest = torch.ones(H, dtype=torch.bool, device="cuda")
+    rest[cols] = False
+    assert not dw[-300:, rest].any() and not dw[t][:, rest].any()
+    # dx for a few columns of w, the last one among them.
+    some = torch.cat([torch.arange(8, device="cuda"), torch.arange(H - 56, H, device="cuda")])
+    ws = w[:, some].double()
+    ed = d.abs() * (2 * erow + 2.0 ** -8 + 2.0 ** -11)[:, None] + 2.0 ** -38
+    ed[torch.arange(N, device="cuda"), t] += 2 * erow
+    edx = ed @ ws.abs() + (V + 2) * E32 * (d.abs() @ ws.abs())
+    rdx = d @ ws
+    assert ((dx[:, some].double() - rdx).abs() <= edx + 2.0 ** -8 * (rdx.abs() + edx)).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 def test_views(dt):
     # Rows of wider matrices, aligned and from an odd element on.
