@@ -13,11 +13,12 @@
 // bf16 inputs.  The logits' product ends in an epilogue that never stores
 // them.  It runs with W as its row operand, so a lane holds consecutive
 // vocabulary entries of one token: a wave takes the maximum m and the sum of
-// exp(l - m) over 64 entries of a token in its own registers and two shuffles, writes those two, and (for gradients) exp(l - m) 2^15 in fp16,
-// whose 11 bits leave the one rounding to bf16 that d itself gets as the only
-// one that counts; values below 2^-29 of the largest in their group lose bits,
-// below 2^-39 they are lost.  One pass over them (ce_rows_kernel) then joins the groups to lse
-// and turns each, in place, into d in bf16.  The target's own entry, where
+// exp(l - m) over 64 entries of a token in its own registers and two shuffles,
+// writes those two, and (for gradients) exp(l - m) 2^15 in fp16, whose 11 bits
+// leave the one rounding to bf16 that d itself gets as the only one that
+// counts; values below 2^-29 of the largest in their group lose bits, below
+// 2^-39 they are lost.  One pass over them (ce_rows_kernel) then joins the
+// groups to lse and turns each, in place, into d in bf16.  The target's own entry, where
 // exp(l - lse) - 1 cancels, is taken from the fp32 logit.  The scalar factor
 // of d (1 / count) is kept out of it and applied to the fp32 sums of dx and
 // dW, so that it costs no rounding of its own.
@@ -148,7 +149,7 @@ struct CeLogits {
 // A gradient, stored transposed: rows are the hidden dimension, columns
 // tokens (dx) or vocabulary entries (dW).  Over several chunks of rows dW is
 // added up in fp32 and rounded once, by the last; each K split of a product
-// stores its own fp32 sums, which ce_join_kernel adds in order (the tile
+// stores its own fp32 sums, which ce_finish_kernel adds in order (the tile
 // kernel's own combine, in which a tile's last workgroup reads every split,
 // took 16 of the 31 us of a 7 x 32768 x 1024 dx in 32 splits).
 struct CeGrad {
@@ -428,34 +429,68 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a, int share, CePre
 }
 
 // The K splits of a gradient, added in order: out = bf16(scale sum), or acc =
-// sum, in both cases onto acc where `add` is set; and, by one more workgroup
-// where `loss` is set, the sum or mean of the rows' losses, in 64 bits and a
-// fixed order.
+// sum, in both cases onto acc where `add` is set.
 struct CeJoin {
   const float* part;  // [splits][rows][ld]
-  int splits, lanes;  // lanes: threads that share the splits of a result
+  int splits, lanes;  // lanes: threads that share the splits of a result; splits 0: nothing to join
   int64_t rows, cols, ld;
   u16* out;  // [rows][cols]
   float* acc;
   bool add;
   const float* scale;
-  float* loss;
+
+  // Workgroup `block` of `blocks`: each thread every lanes-th split, then those
+  // sums in order.
+  __device__ void run(int64_t block, int64_t blocks, f32x4* share) const {
+    const int64_t per_row = ld / 4, stride = rows * ld;
+    const int per = 256 / lanes, mine = (int)threadIdx.x % per, lane = (int)threadIdx.x / per;
+    const float f = out != nullptr ? *scale : 1.f;
+    for (int64_t i0 = block * per; i0 < rows * per_row; i0 += blocks * per) {
+      const int64_t i = i0 + mine;
+      const bool live = i < rows * per_row;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      if (live) {
+        const float* p = part + 4 * i;
+#pragma unroll 4
+        for (int k = lane; k < splits; k += lanes) v += *reinterpret_cast<const f32x4*>(p + k * stride);
+      }
+      if (lanes > 1) {
+        __syncthreads();
+        share[threadIdx.x] = v;
+        __syncthreads();
+        for (int k = 1; k < lanes && lane == 0; ++k) v += share[k * per + mine];
+      }
+      if (!live || lane != 0) continue;
+      const int64_t r = i / per_row, c = 4 * (i - r * per_row);
+      f32x4* to = reinterpret_cast<f32x4*>(acc + 4 * i);
+      if (add) v += *to;
+      if (out == nullptr) {
+        *to = v;
+        continue;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (c + k < cols) out[r * cols + c + k] = bf16_bits(v[k] * f);
+    }
+  }
+};
+
+// The sum or mean of the rows' losses by one workgroup, in 64 bits and a fixed
+// order.
+struct CeLoss {
+  float* loss;  // NULL: not wanted, or not yet
   const float* row_loss;
   const int64_t* target;
   int64_t N, ignore;
   int reduction;
-};
 
-__global__ __launch_bounds__(256) void ce_join_kernel(CeJoin a) {
-  __shared__ double sum[256];
-  __shared__ int count[256];
-  if (a.loss != nullptr && blockIdx.x == gridDim.x - 1) {
+  __device__ void run(double* sum, int* count) const {
     double s = 0;
     int n = 0;
 #pragma unroll 8
-    for (int64_t i = threadIdx.x; i < a.N; i += 256) {
-      s += (double)a.row_loss[i];
-      n += a.target[i] != a.ignore;
+    for (int64_t i = threadIdx.x; i < N; i += 256) {
+      s += (double)row_loss[i];
+      n += target[i] != ignore;
     }
     sum[threadIdx.x] = s;
     count[threadIdx.x] = n;
@@ -466,53 +501,44 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeJoin a) {
         count[threadIdx.x] += count[threadIdx.x + o];
       }
     }
-    if (threadIdx.x == 0) *a.loss = (float)(a.reduction == kMean ? sum[0] / (double)max(count[0], 1) : sum[0]);
-    return;
+    if (threadIdx.x == 0) *loss = (float)(reduction == kMean ? sum[0] / (double)max(count[0], 1) : sum[0]);
   }
-  // Each thread every lanes-th split, then those sums in order.
-  __shared__ f32x4 share[256];
-  const int64_t blocks = gridDim.x - (a.loss != nullptr ? 1 : 0), per_row = a.ld / 4, stride = a.rows * a.ld;
-  const int per = 256 / a.lanes, mine = (int)threadIdx.x % per, lane = (int)threadIdx.x / per;
-  const float f = a.out != nullptr ? *a.scale : 1.f;
-  for (int64_t i0 = (int64_t)blockIdx.x * per; i0 < a.rows * per_row; i0 += blocks * per) {
-    const int64_t i = i0 + mine;
-    const bool live = i < a.rows * per_row;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (live) {
-      const float* p = a.part + 4 * i;
-#pragma unroll 4
-      for (int k = lane; k < a.splits; k += a.lanes) v += *reinterpret_cast<const f32x4*>(p + k * stride);
-    }
-    if (a.lanes > 1) {
-      __syncthreads();
-      share[threadIdx.x] = v;
-      __syncthreads();
-      for (int k = 1; k < a.lanes && lane == 0; ++k) v += share[k * per + mine];
-    }
-    if (!live || lane != 0) continue;
-    const int64_t r = i / per_row, c = 4 * (i - r * per_row);
-    f32x4* acc = reinterpret_cast<f32x4*>(a.acc + 4 * i);
-    if (a.add) v += *acc;
-    if (a.out == nullptr) {
-      *acc = v;
-      continue;
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (c + k < a.cols) a.out[r * a.cols + c + k] = bf16_bits(v[k] * f);
+};
+
+// What is left after a gradient's product: its join by the first `join_blocks`
+// workgroups, and the loss by one more.
+struct CeFinish {
+  CeJoin join;
+  CeLoss loss;
+  int join_blocks;
+
+  int blocks() const { return join_blocks + (loss.loss != nullptr ? 1 : 0); }
+  __device__ void run(int64_t block) const {
+    __shared__ f32x4 share[256];  // (also the losses' sums, 12 bytes a thread)
+    if (block < join_blocks) join.run(block, join_blocks, share);
+    else if (block == join_blocks && loss.loss != nullptr)
+      loss.run(reinterpret_cast<double*>(share), reinterpret_cast<int*>(share) + 512);
   }
-}
+};
+
+__global__ __launch_bounds__(256) void ce_finish_kernel(CeFinish a) { a.run(blockIdx.x); }
 
 // dW [V, H] of up to 32 rows: one k-slice of a 16x16x32 MFMA, so no tile is
 // worth staging; the kernel is bound by writing dW.  A wave keeps the x
 // operand of its 128 columns of h (grid x) in registers, 16 bytes a lane from
-// the transposed x, and walks over tiles of 16 vocabulary entries.  Row i of the MFMA's output is column 8 (i / 4) +
-// 4 t + i % 4 of a block of 32, for the two MFMAs t = 0, 1 of the block: a
-// lane's 4 + 4 results are then 8 consecutive h, one 16-byte store, and the
-// four lanes of an entry write 64 bytes.
+// the transposed x, and walks over tiles of 16 vocabulary entries.  Row i of
+// the MFMA's output is column 8 (i / 4) + 4 t + i % 4 of a block of 32, for the
+// two MFMAs t = 0, 1 of the block: a lane's 4 + 4 results are then 8
+// consecutive h, one 16-byte store, and the four lanes of an entry write 64
+// bytes.  The workgroups from grid y = `ys` on join dx and the loss.
 __global__ __launch_bounds__(256) void ce_few_rows_kernel(const u16* __restrict__ d, int64_t ldd,
                                                           const u16* __restrict__ xt, u16* __restrict__ dw, int R,
-                                                          int H, int V, const float* __restrict__ scale) {
+                                                          int H, int V, const float* __restrict__ scale, int ys,
+                                                          CeFinish finish) {
+  if ((int)blockIdx.y >= ys) {
+    finish.run((int64_t)((int)blockIdx.y - ys) * gridDim.x + blockIdx.x);
+    return;
+  }
   typedef u16 u16x8 __attribute__((ext_vector_type(8)));
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i = lane & 15, g = lane >> 4;  // MFMA row or column; k group, and group of output rows
@@ -535,7 +561,7 @@ __global__ __launch_bounds__(256) void ce_few_rows_kernel(const u16* __restrict_
     }
     return __builtin_bit_cast(bf16x8, v);
   };
-  const int step = 64 * gridDim.y;
+  const int step = 64 * ys;
   int v0 = 16 * (4 * (int)blockIdx.y + wave);
   if (v0 >= V) return;
   bf16x8 next = load(v0);
@@ -863,27 +889,30 @@ hipError_t run_rows(const CeArgs& a, const CePlan& p, char* ws, int64_t r0, int6
   return hipGetLastError();
 }
 
-// The sum or mean of the losses, beside the joining of a gradient's splits
-// where one is left to do.
-hipError_t run_join(const CeArgs& a, const CePlan& p, char* ws, CeJoin q, bool loss, hipStream_t stream) {
-  if (loss && a.reduction != kNone) {
-    q.loss = a.loss;
-    q.row_loss = reinterpret_cast<const float*>(ws + p.rows);
-    q.target = a.target, q.N = a.N, q.ignore = a.ignore, q.reduction = a.reduction;
+// `last`: all rows are through.
+CeFinish finish_of(const CeArgs& a, const CePlan& p, char* ws, const CeJoin& join, bool last) {
+  CeFinish f{join, {}, 0};
+  if (join.splits > 0) {
+    f.join.lanes = join.splits >= 32 ? 8 : join.splits >= 8 ? 2 : 1;
+    f.join_blocks = (int)grid_for(join.rows * join.ld / 4 * f.join.lanes);
   }
-  q.lanes = q.splits >= 32 ? 8 : q.splits >= 8 ? 2 : 1;
-  const int64_t groups = q.rows * q.ld / 4 * q.lanes;
-  const unsigned grid = (groups > 0 ? grid_for(groups) : 0) + (q.loss != nullptr ? 1 : 0);
-  if (grid == 0) return hipSuccess;
-  hipLaunchKernelGGL(ce_join_kernel, dim3(grid), dim3(256), 0, stream, q);
+  if (last && a.reduction != kNone)
+    f.loss = {a.loss, reinterpret_cast<const float*>(ws + p.rows), a.target, a.N, a.ignore, a.reduction};
+  return f;
+}
+
+hipError_t run_finish(const CeFinish& f, hipStream_t stream) {
+  if (f.blocks() == 0) return hipSuccess;
+  hipLaunchKernelGGL(ce_finish_kernel, dim3((unsigned)f.blocks()), dim3(256), 0, stream, f);
   return hipGetLastError();
 }
 
-// One gradient: its product, in splits or not, and what joins them.  `acc`:
-// fp32 sums over the chunks (NULL: one chunk), written to `out` by the last.
+// One gradient: its product, in splits or not, and in `join` what joins them.
+// `acc`: fp32 sums over the chunks (NULL: one chunk), written to
+// `out` by the last.
 template <bool CB>
 hipError_t run_grad(const CeArgs& a, const CePlan& p, char* ws, const Operands& o, const CeProduct& c, u16* out,
-                    float* acc, bool add, bool loss, hipStream_t stream) {
+                    float* acc, bool add, CeJoin* join, hipStream_t stream) {
   const float* scale = reinterpret_cast<const float*>(ws + p.scale);
   float* part = reinterpret_cast<float*>(ws + p.split);
   const int64_t ld = sum_ld(a.H);
@@ -902,12 +931,8 @@ hipError_t run_grad(const CeArgs& a, const CePlan& p, char* ws, const Operands& 
     main.N = c.main;
   }
   CE_TRY((run_product<kKRows, true, CB>(main, g, c.tile, c.splits, stream)));
-  CeJoin q{};
-  if (splits > 1) {
-    q.part = part, q.splits = (int)splits, q.rows = o.N, q.cols = a.H, q.ld = ld;
-    q.out = out, q.acc = acc, q.add = add, q.scale = scale;
-  }
-  return run_join(a, p, ws, q, loss, stream);
+  if (splits > 1) *join = CeJoin{part, (int)splits, 1, o.N, a.H, ld, out, acc, add, scale};
+  return hipSuccess;
 }
 
 hipError_t run_bf16(const CeArgs& a, const CePlan& p, char* ws, hipStream_t stream) {
@@ -947,26 +972,34 @@ hipError_t run_bf16(const CeArgs& a, const CePlan& p, char* ws, hipStream_t stre
     }
     CE_TRY(run_rows<u16>(a, p, ws, r0, R, stream));
     if (!a.grad) {
-      if (last) CE_TRY(run_join(a, p, ws, CeJoin{}, true, stream));
+      if (last) CE_TRY(run_finish(finish_of(a, p, ws, {}, true), stream));
       continue;
     }
     // dx^T [H, R] = W^T d^T over the vocabulary, first, while d is in the caches
     // (1000 rows x 50021: 110 us, 130 after dW); d is padded with zeros to
     // whole K steps, W ends with its rows.
+    CeJoin jx{}, jw{};
     CE_TRY(run_grad<true>(a, p, ws, Operands{w, keep, ldw, p.Vp, a.H, R, a.V}, p.p2,
-                          static_cast<u16*>(a.dx) + r0 * a.H, nullptr, false, last, stream));
-    // dW^T [H, V] = x^T d over the chunk's rows.
+                          static_cast<u16*>(a.dx) + r0 * a.H, nullptr, false, &jx, stream));
+    const CeFinish f = finish_of(a, p, ws, jx, last);
+    // dW^T [H, V] = x^T d over the chunk's rows.  Its kernel of few rows joins
+    // dx and the losses beside it (7 x 1024 x 32768: 52.5 -> 48.9 us for all);
+    // a tile kernel's dW would evict the split sums (1000 x 1000 x 50021: 407
+    // and 408 us).
     u16* dw = static_cast<u16*>(a.dw);
     if (p.few) {
       const unsigned gx = (unsigned)cdiv(a.H, 128);
       const unsigned gy = (unsigned)std::min<int64_t>(cdiv(a.V, 64), std::max<int64_t>(1, 4 * device_cus() / gx));
-      hipLaunchKernelGGL(ce_few_rows_kernel, dim3(gx, gy), dim3(256), 0, stream, keep, p.Vp,
-                         reinterpret_cast<const u16*>(ws + p.xt), dw, (int)R, (int)a.H, (int)a.V, reinterpret_cast<const float*>(ws + p.scale));
+      hipLaunchKernelGGL(ce_few_rows_kernel, dim3(gx, gy + (unsigned)cdiv(f.blocks(), gx)), dim3(256), 0, stream, keep,
+                         p.Vp, reinterpret_cast<const u16*>(ws + p.xt), dw, (int)R, (int)a.H, (int)a.V,
+                         reinterpret_cast<const float*>(ws + p.scale), (int)gy, f);
       CE_TRY(hipGetLastError());
-    } else {
-      CE_TRY(run_grad<false>(a, p, ws, Operands{xs, keep, p.Hp, p.Vp, a.H, a.V, R}, p.p3, last ? dw : nullptr,
-                             p.chunks > 1 ? reinterpret_cast<float*>(ws + p.acc) : nullptr, c > 0, false, stream));
+      continue;
     }
+    CE_TRY(run_finish(f, stream));
+    CE_TRY(run_grad<false>(a, p, ws, Operands{xs, keep, p.Hp, p.Vp, a.H, a.V, R}, p.p3, last ? dw : nullptr,
+                           p.chunks > 1 ? reinterpret_cast<float*>(ws + p.acc) : nullptr, c > 0, &jw, stream));
+    CE_TRY(run_finish(finish_of(a, p, ws, jw, false), stream));
   }
   return hipSuccess;
 }
@@ -1002,7 +1035,7 @@ int run_f32(const CeArgs& a, const CePlan& p, char* ws, unsigned* counters, size
     hipLaunchKernelGGL(ce_add_kernel, dim3(grid_for(a.V * a.H)), dim3(256), 0, stream, dw, part, a.V * a.H);
     if ((*err = hipGetLastError()) != hipSuccess) return TILEC_ERR_HIP;
   }
-  if ((*err = run_join(a, p, ws, CeJoin{}, true, stream)) != hipSuccess) return TILEC_ERR_HIP;
+  if ((*err = run_finish(finish_of(a, p, ws, {}, true), stream)) != hipSuccess) return TILEC_ERR_HIP;
   return TILEC_OK;
 }
 
