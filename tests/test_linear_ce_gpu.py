@@ -132,6 +132,19 @@ def test_many_tiles(N, H, V, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("N,H,V", [(640, 928, 978), (100, 520, 3000), (40, 200, 1000), (9, 72, 257), (2048, 1000, 16000)])
+def test_widths_of_no_whole_steps(N, H, V, dt):
+    # Whatever lies past a row's end must not get in.
+    x, w, t = make(N, H, V, dt, seed=H, ignored=0.1)
+    wide_x = torch.full((N + 1, H + 8), math.nan, dtype=x.dtype, device="cuda")
+    wide_w = torch.full((V + 1, H + 16), math.nan, dtype=x.dtype, device="cuda")
+    wide_x[:N, :H], wide_w[:V, :H] = x, w
+    got = check(wide_x[:N, :H], wide_w[:V, :H], t)
+    assert all(torch.equal(a, b) for a, b in zip(got, tilec.ext.linear_cross_entropy_grad(x, w, t)))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("N", [3, 40])
 def test_offsets_past_32_bits(N):
     # A weight and a gradient of more than 2^31 values, checked for the last

@@ -786,7 +786,10 @@ CePlan make_plan(const CeArgs& a) {
     p.shift = 12;
     p.groups = (int)cdiv(a.V, kGroup32);
   }
-  p.copy_first = bf16 && (p.pad || p.Hp != a.H);
+  // Widths of no whole K steps: the largest tiles have no registers left to mask
+  // both operands by (1000 x 1000 x 50021: 398 us with x copied, 404 in place);
+  // the smaller ones save the copy's launch (640 x 928 x 978: 42.7, 40.3).
+  p.copy_first = bf16 && (p.pad || (p.Hp != a.H && p.p1.tile == kT256));
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -908,8 +911,8 @@ hipError_t run_finish(const CeFinish& f, hipStream_t stream) {
 }
 
 // One gradient: its product, in splits or not, and in `join` what joins them.
-// `acc`: fp32 sums over the chunks (NULL: one chunk), written to
-// `out` by the last.
+// `acc`: fp32 sums over the chunks (NULL: one chunk), written to `out` by the
+// last.
 template <bool CB>
 hipError_t run_grad(const CeArgs& a, const CePlan& p, char* ws, const Operands& o, const CeProduct& c, u16* out,
                     float* acc, bool add, CeJoin* join, hipStream_t stream) {
@@ -958,16 +961,16 @@ hipError_t run_bf16(const CeArgs& a, const CePlan& p, char* ws, hipStream_t stre
                 0,
                 a.target + r0,
                 reinterpret_cast<float*>(ws + p.tlogit)};
-    // Rows of x end in zeros to a whole K step, rows of W only where it was
-    // copied.
     for (int64_t v0 = 0; v0 < a.V; v0 += p.p1.main) {
       const bool rest = v0 > 0;
       const int64_t V = rest ? a.V - v0 : p.p1.main;
       const CeTile tile = rest ? p.p1.tail : p.p1.tile;
-      const Operands o{w + v0 * ldw, xc, ldw, ldx, V, R, p.pad || a.H % 64 == 0 ? p.Hp : a.H};
+      const Operands o{w + v0 * ldw, xc, ldw, ldx, V, R, p.pad ? p.Hp : a.H};
       le.v0 = (int)v0;
       if (o.K % 64 == 0) CE_TRY((run_product<kKFull, false, true>(o, le, tile, 1, stream)));
-      else CE_TRY((run_product<kKColsA, false, true>(o, le, tile, 1, stream)));
+      else if (tile == kT256) CE_TRY((run_tile<256, 256, 2, 2, 4, kKColsA, false, true, 16>(o, le, 1, stream)));
+      else if (tile == kT128) CE_TRY((run_tile<128, 128, 4, 2, 4, kKMasked, false, true, 16>(o, le, 1, stream)));
+      else CE_TRY((run_tile<128, 64, 3, 2, 2, kKMasked, false, true, 16>(o, le, 1, stream)));
       if (rest) break;
     }
     CE_TRY(run_rows<u16>(a, p, ws, r0, R, stream));
