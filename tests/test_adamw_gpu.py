@@ -6,8 +6,9 @@ of the magnitudes added.  p adds to its own 3 roundings the error of the step
 taken, rate |m / denom| times at most 12 roundings plus the relative error of m
 where its terms cancel.  The value of a v code: 1 / 255 and its product with
 the code are rounded (2 roundings), their square doubles that and adds one (5),
-the fourth power again (11), the scale adds one: 12; of an m code: 6.  An 8-bit code is at most half a code (and the
-roundings of its root and quotient, 1e-4 of a code) from the exact one.
+the fourth power again (11), the scale adds one: 12; of an m code: 6.  An 8-bit
+code is at most half a code (and the roundings of its root and quotient, 1e-4 of
+a code) from the exact one.
 """
 
 import math

@@ -165,8 +165,8 @@ __device__ __forceinline__ f32x4 v_values(uint32_t codes, float scale) {
 // root, together under 2^-21 of the result, so 2e-5 and 5e-5 of a code) settles
 // all values but those within 1e-4 of a code from halfway between two, two in
 // ten thousand.  Scales outside 2^-60 .. 2^100, where the approximation could
-// leave the range of normal numbers, go the long way.  (151 M values: 627 us
-// the long way for all, 3.9 TB/s.)
+// leave the range of normal numbers, go the long way.  (151 M values: 496 us,
+// 627 with the long way for all.)
 __device__ __forceinline__ bool plain_scale(float s) { return s >= 0x1p-60f && s <= 0x1p100f; }
 __device__ __forceinline__ bool near_half(float t) { return fabsf(fabsf(t - rintf(t)) - 0.5f) < 1e-4f; }
 

@@ -6,7 +6,8 @@ They are what a training step needs beside the products (`matrix_mul`) and the
 sums (`sum`) of its linear layers, and follow the same rules: arguments are
 checked before anything is enqueued (ValueError for shapes, TypeError for
 types and devices), work goes to the current stream of the tensors' device,
-scratch is the (device, stream) workspace of `ext`, and nothing synchronises.
+scratch is the (device, stream) workspace of `ext` or, where it is large or the
+call is made in C++, torch's allocator's, and nothing synchronises.
 Like those two they are plain functions with no autograd of their own.
 """
 
