@@ -145,6 +145,19 @@ def test_widths_of_no_whole_steps(N, H, V, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("N,H,V", [(2047, 64, 130), (2050, 40, 1), (4099, 72, 1001), (6001, 16, 4097), (2049, 64, 16500)])
+def test_many_rows(N, H, V, dt):
+    # About where rows are given a wave or a workgroup each, by their number and
+    # length.
+    x, w, t = make(N, H, V, dt, seed=N + V, ignored=0.2)
+    t[N - 1] = V - 1
+    check(x, w, t)
+    g = torch.Generator().manual_seed(2)
+    check(x, w, t, "none", torch.randn(N, generator=g).cuda())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("N", [3, 40])
 def test_offsets_past_32_bits(N):
     # A weight and a gradient of more than 2^31 values, checked for the last

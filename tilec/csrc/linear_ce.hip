@@ -343,7 +343,7 @@ __global__ __launch_bounds__(256) void ce_stats_kernel(const float* __restrict__
 //   T = float: l -> d, with it.
 struct CeRows {
   void* p;
-  int64_t ldp, V;
+  int64_t ldp, V, R;
   const f32x2* stat;
   int groups, stride, group_shift;  // groups of a row, from one row's to the next, columns of one: 2^group_shift
   const int64_t* target;
@@ -354,11 +354,13 @@ struct CeRows {
   const float* scale;      // (T = float)
 };
 
-// The workgroups from grid y = `share` on prepare the operands of the
-// gradients instead (bf16), where the logits' product did not need them (one
-// launch less, 3 us).
-template <typename T>
+// ROWS = 4: a wave a row, no barriers, for short rows.  The workgroups from grid
+// y = `share` on prepare the operands of the gradients instead (bf16), where the
+// logits' product did not need them (one launch less, 3 us).
+template <typename T, int ROWS>
 __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a, int share, CePrepare<T> prepare) {
+  constexpr int NT = 256 / ROWS;  // threads of a row
+  static_assert(ROWS == 1 || NT == 64, "a row is a workgroup's or a wave's");
   __shared__ float red[2][4];
   if ((int)blockIdx.y >= share) {
     __shared__ int count[256];
@@ -366,8 +368,9 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a, int share, CePre
                 count);
     return;
   }
-  const int64_t r = blockIdx.x;
-  const int tid = threadIdx.x;
+  const int64_t r = ROWS == 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * ROWS + (threadIdx.x >> 6);
+  if (ROWS > 1 && r >= a.R) return;
+  const int tid = threadIdx.x % NT;
   const int64_t want = a.target[r];
   const bool ignored = want == a.ignore, bad = !ignored && (want < 0 || want >= a.V);
   constexpr int E = sizeof(T) == 2 ? 8 : 4;
@@ -375,23 +378,27 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a, int share, CePre
   if (ignored) {
     if (a.loss != nullptr && blockIdx.y == 0 && tid == 0) a.loss[r] = 0.f;
     if (a.p == nullptr) return;
-    for (int64_t v = E * ((int64_t)blockIdx.y * 256 + tid); v < a.ldp; v += E * 256 * (int64_t)share)
+    for (int64_t v = E * ((int64_t)blockIdx.y * NT + tid); v < a.ldp; v += E * NT * (int64_t)share)
       *reinterpret_cast<i32x4*>(row + v) = i32x4{0, 0, 0, 0};
     return;
   }
   const f32x2* stat = a.stat + r * a.stride;
   float m = -FLT_MAX;
-  for (int g = tid; g < a.groups; g += 256) m = fmaxf(m, stat[g].x);
+  for (int g = tid; g < a.groups; g += NT) m = fmaxf(m, stat[g].x);
   m = wave_max(m);
-  if ((tid & 63) == 0) red[0][tid >> 6] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  if constexpr (ROWS == 1) {
+    if ((tid & 63) == 0) red[0][tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  }
   float s = 0.f;
-  for (int g = tid; g < a.groups; g += 256) s += stat[g].y * __expf(stat[g].x - m);
+  for (int g = tid; g < a.groups; g += NT) s += stat[g].y * __expf(stat[g].x - m);
   s = wave_sum(s);
-  if ((tid & 63) == 0) red[1][tid >> 6] = s;
-  __syncthreads();
-  s = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  if constexpr (ROWS == 1) {
+    if ((tid & 63) == 0) red[1][tid >> 6] = s;
+    __syncthreads();
+    s = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  }
   const float lse = m + logf(s);
   const float tl = bad ? NAN : a.tlogit[r];  // a target that is no class: NaN, in loss and gradients
   if (a.loss != nullptr && blockIdx.y == 0 && tid == 0) a.loss[r] = lse - tl;
@@ -400,7 +407,7 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a, int share, CePre
   if (sizeof(T) == 4) g *= *a.scale;
   if (bad) g = NAN;
   const float at_target = expm1f(tl - lse) * g;
-  for (int64_t v = E * ((int64_t)blockIdx.y * 256 + tid); v < a.ldp; v += E * 256 * (int64_t)share) {
+  for (int64_t v = E * ((int64_t)blockIdx.y * NT + tid); v < a.ldp; v += E * NT * (int64_t)share) {
     float d[E];
     if constexpr (sizeof(T) == 2) {
       const f16x8 e = *reinterpret_cast<const f16x8*>(row + v);
@@ -851,15 +858,15 @@ unsigned prepare_blocks(const CeArgs& a, const CePlan& p, int64_t R) {
   return grid_for(std::max(R * p.Hp / (16 / (int64_t)sizeof(T)), p.few ? kFewRows * a.H : 0)) + 1;
 }
 
-// The same as rows of a grid R wide, where they run beside another kernel's: not
+// The same as rows of a grid `width` wide, where they run beside another kernel's: not
 // more than fit into grid y with that kernel's own (each takes what is left over
 // in steps).
 constexpr unsigned kMoreBlocks = 1024;
 constexpr int64_t kMaxGroups = 65535 - kMoreBlocks;
 template <typename T>
-unsigned more_blocks(const CeArgs& a, const CePlan& p, int64_t R) {
+unsigned more_blocks(const CeArgs& a, const CePlan& p, int64_t R, int64_t width) {
   if (!a.grad || p.copy_first) return 0;
-  return (unsigned)std::min<int64_t>(std::max<int64_t>(cdiv(prepare_blocks<T>(a, p, R), R), R == 1 ? 2 : 1), kMoreBlocks);
+  return (unsigned)std::min<int64_t>(std::max<int64_t>(cdiv(prepare_blocks<T>(a, p, R), width), width == 1 ? 2 : 1), kMoreBlocks);
 }
 
 template <typename T>
@@ -874,7 +881,7 @@ template <typename T>
 hipError_t run_rows(const CeArgs& a, const CePlan& p, char* ws, int64_t r0, int64_t R, hipStream_t stream) {
   CeRows q{};
   q.p = a.grad ? ws + p.keep : nullptr;
-  q.ldp = p.Vp, q.V = a.V;
+  q.ldp = p.Vp, q.V = a.V, q.R = R;
   q.stat = reinterpret_cast<const f32x2*>(ws + p.stat);
   q.groups = (int)cdiv(a.V, int64_t(1) << p.shift), q.stride = p.groups, q.group_shift = p.shift;
   q.target = a.target + r0, q.ignore = a.ignore;
@@ -886,8 +893,15 @@ hipError_t run_rows(const CeArgs& a, const CePlan& p, char* ws, int64_t r0, int6
   // it takes to fill the chip.
   const int64_t want = cdiv(4 * (int64_t)device_cus(), R), most = cdiv(p.Vp, 256 * 16 / (int64_t)sizeof(T));
   const unsigned share = a.grad ? (unsigned)std::max<int64_t>(1, std::min(want, most)) : 1;
-  const unsigned more = sizeof(T) == 2 ? more_blocks<T>(a, p, R) : 0;  // (fp32: beside the statistics)
-  hipLaunchKernelGGL((ce_rows_kernel<T>), dim3((unsigned)R, share + more), dim3(256), 0, stream, q, (int)share,
+  // A wave a row where rows are short and many: 20000 rows x 128 x 1000 in 98 us
+  // for all, 114 with a workgroup each; 1024 x 128 x 3000 would go from 40.1 to
+  // 41.5.  (16-byte pieces of a row; groups are read twice.)
+  const int64_t pieces = a.grad ? p.Vp * (int64_t)sizeof(T) / 16 : 2 * q.groups;
+  const bool waves = pieces <= 512 && R >= 8 * (int64_t)device_cus();
+  const int64_t width = waves ? cdiv(R, 4) : R;
+  const unsigned more = sizeof(T) == 2 ? more_blocks<T>(a, p, R, width) : 0;  // (fp32: beside the statistics)
+  const auto kern = waves ? ce_rows_kernel<T, 4> : ce_rows_kernel<T, 1>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)width, share + more), dim3(256), 0, stream, q, (int)share,
                      prepare_of<T>(a, p, ws, r0, R));
   return hipGetLastError();
 }
@@ -1023,7 +1037,7 @@ int run_f32(const CeArgs& a, const CePlan& p, char* ws, unsigned* counters, size
     const int64_t r0 = c * p.R, R = std::min(p.R, a.N - r0);
     int rc = product(0, R, x + r0 * a.ldx, w, keep, R, a.V, a.H, a.ldx, a.ldw, p.Vp, TILEC_X2_COL_MAJOR);
     if (rc != TILEC_OK) return rc;
-    hipLaunchKernelGGL(ce_stats_kernel, dim3((unsigned)R, (unsigned)p.groups + more_blocks<float>(a, p, R)), dim3(256), 0,
+    hipLaunchKernelGGL(ce_stats_kernel, dim3((unsigned)R, (unsigned)p.groups + more_blocks<float>(a, p, R, R)), dim3(256), 0,
                        stream, keep, p.Vp, a.V, a.target + r0, reinterpret_cast<f32x2*>(ws + p.stat), p.groups,
                        reinterpret_cast<float*>(ws + p.tlogit), prepare_of<float>(a, p, ws, r0, R));
     if ((*err = hipGetLastError()) != hipSuccess) return TILEC_ERR_HIP;
