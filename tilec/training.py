@@ -6,8 +6,9 @@ They are what a training step needs beside the products (`matrix_mul`) and the
 sums (`sum`) of its linear layers, and follow the same rules: arguments are
 checked before anything is enqueued (ValueError for shapes, TypeError for
 types and devices), work goes to the current stream of the tensors' device,
-scratch is the (device, stream) workspace of `ext` or, where it is large or the
-call is made in C++, torch's allocator's, and nothing synchronises.
+and nothing synchronises.  Scratch that carries values from one kernel of a call
+to the next is torch's allocator's, each call's own: calls of other host threads
+on the same stream may put their kernels in between.
 Like those two they are plain functions with no autograd of their own.
 """
 
@@ -17,7 +18,7 @@ from functools import lru_cache
 import torch
 
 from . import _lib
-from .ext import _tuned, counters_for, workspace_for
+from .ext import _tuned, counters_for
 
 __all__ = ["layer_norm", "layer_norm_backward", "linear_cross_entropy", "linear_cross_entropy_grad",
            "adamw_state", "adamw_step", "adamw_values", "ADAMW_BLOCK"]
@@ -117,7 +118,6 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, param_grads=True):
 
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
-_KEPT_SCRATCH = 64 << 20  # a larger workspace is not kept between calls
 
 
 @lru_cache(4096)
@@ -181,12 +181,7 @@ def _linear_ce(what, x, weight, target, reduction, ignore_index, grad, grad_loss
         stream = _raw_stream(at)
         ws, cnt, configs = _ce_plan(at, N, H, V, ldx, ldw, dtype, code, grad, chunk_rows, x.data_ptr() % 16,
                                     weight.data_ptr() % 16)
-        # Up to 2 GiB and more: what is large goes back to torch's allocator.
-        scratch = None
-        if ws > _KEPT_SCRATCH:
-            scratch = torch.empty(ws, dtype=torch.uint8, device=x.device)
-        elif ws:
-            scratch = workspace_for(x.device, stream, ws)
+        scratch = torch.empty(ws, dtype=torch.uint8, device=x.device) if ws else None
         cnt_ptr = counters_for(x.device, stream, cnt).data_ptr() if cnt else None
         _lib.check(_lib.lib().tilec_linear_ce(x.data_ptr(), weight.data_ptr(), target.data_ptr(), loss.data_ptr(),
                                               _ptr(grad_loss), _ptr(dx), _ptr(dw), N, H, V, ldx, ldw, dtype, code,
