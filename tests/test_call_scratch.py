@@ -1,16 +1,20 @@
 """Scratch of the linear cross entropy, whose kernels hand values to each other
 through it: each call's own, also where two host threads enqueue on one stream
 (the C call gives up the interpreter's lock) and where a graph has recorded it.
+And the split-K buffers that calls on a stream share, where a graph has recorded
+them.
 """
 
 import contextlib
+import gc
 import threading
+import weakref
 
 import pytest
 import torch
 
 import tilec
-from tilec import training
+from tilec import ext, training
 
 
 def test_calls_at_the_same_time_share_no_scratch(monkeypatch):
@@ -41,6 +45,35 @@ def test_calls_at_the_same_time_share_no_scratch(monkeypatch):
         th.join()
     _, (a, n), (b, m) = seen
     assert n == m == 4096 and (a + n <= b or b + m <= a)
+
+
+@pytest.mark.parametrize("get", [ext.workspace_for, ext.counters_for])
+def test_buffers_and_captures(monkeypatch, get):
+    # The host code alone, on CPU memory: what a capture used outlives a larger
+    # call, and what a capture allocated (zeroed only when the graph runs) does
+    # not reach the calls after it.
+    now = [False]
+    monkeypatch.setattr(ext, "_capturing", lambda device: now[0], raising=False)
+    cpu, stream = torch.device("cpu"), 987654321
+    now[0] = True
+    inside = get(cpu, stream, 100)
+    now[0] = False
+    eager = get(cpu, stream, 100)
+    assert eager.data_ptr() != inside.data_ptr() and get(cpu, stream, 50) is eager
+    now[0] = True
+    assert get(cpu, stream, 100) is eager
+    larger = get(cpu, stream, 5 << 20)
+    assert larger.numel() >= 5 << 20 and get(cpu, stream, 100) is eager
+    now[0] = False
+    recorded = weakref.ref(eager.untyped_storage())
+    eager = None
+    assert get(cpu, stream, 6 << 20).numel() >= 6 << 20
+    gc.collect()
+    assert recorded() is not None
+    unrecorded = weakref.ref(get(cpu, stream, 100).untyped_storage())
+    get(cpu, stream, 7 << 20)
+    gc.collect()
+    assert unrecorded() is None
 
 
 def make(N, H, V, dt, seed):
@@ -74,9 +107,10 @@ def test_two_threads_on_one_stream(dt):
             assert all(torch.equal(a, b) for a, b in zip(want[k], out))
 
 
-def replay_after_a_larger_call(call, small, large):
+def replay_after_a_larger_call(call, small, large, replaced=()):
     """A graph of call(small), replayed after call(large) on the stream it was
-    recorded on and with all memory that was free then filled."""
+    recorded on and with all memory that was free then filled.  `replaced`:
+    tables of ext whose buffer of that stream call(large) replaces."""
     want = call(*small)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -86,9 +120,12 @@ def replay_after_a_larger_call(call, small, large):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph, stream=side):
         out = call(*small)
+    key = (torch.cuda.current_device(), side.cuda_stream)
+    before = [table[key].data_ptr() for table in replaced]
     with torch.cuda.stream(side):
         call(*large)
     torch.cuda.synchronize()
+    assert all(table[key].data_ptr() != p for table, p in zip(replaced, before))
     for _ in range(3):
         with torch.cuda.stream(side):
             filled = [torch.full((1 << k,), 0x55, dtype=torch.uint8, device="cuda") for k in range(9, 27) for _ in range(4)]
@@ -105,3 +142,43 @@ def test_graph_after_a_larger_call():
     bf16 = torch.bfloat16
     replay_after_a_larger_call(tilec.ext.linear_cross_entropy_grad, make(40, 128, 1000, bf16, 3),
                                make(2000, 256, 6000, bf16, 4))
+
+
+@pytest.mark.gpu
+def test_graph_of_split_products_after_a_larger_call():
+    # Products and sums that split K, and the float32 loss, whose products may:
+    # their counters have to be there, and zero, at every replay.
+    variant = next(v["name"] for v in tilec._lib.variants()
+                   if v["dtype"] == tilec._lib.F32 and v["family"] == tilec._lib.FAMILY_SKINNY and not ext.rows_variant(v))
+
+    def call(x, w, t):
+        return (ext.matrix_mul(x, w.t().contiguous(), (variant, 8)), ext.sum(x), *ext.linear_cross_entropy_grad(x, w, t))
+
+    f32 = torch.float32
+    small, large = make(4, 4096, 64, f32, 5), make(16, 4096, 30000, f32, 6)
+    replay_after_a_larger_call(call, small, large, (ext._SCRATCH, ext._COUNTERS))
+
+
+@pytest.mark.gpu
+def test_graph_without_calls_before_it():
+    x, w, t = make(4, 4096, 64, torch.float32, 7)
+    variant = next(v["name"] for v in tilec._lib.variants()
+                   if v["dtype"] == tilec._lib.F32 and v["family"] == tilec._lib.FAMILY_SKINNY and not ext.rows_variant(v))
+    b = w.t().contiguous()
+
+    def call():
+        return ext.matrix_mul(x, b, (variant, 8)), ext.matrix_mul(x, b, (variant, 4))
+
+    want = call()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = call()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            eager = call()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, out)) and all(torch.equal(a, b) for a, b in zip(want, eager))
