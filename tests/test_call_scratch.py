@@ -1,13 +1,14 @@
 """Scratch of the linear cross entropy, whose kernels hand values to each other
 through it: each call's own, also where two host threads enqueue on one stream
 (the C call gives up the interpreter's lock) and where a graph has recorded it.
-And the split-K buffers that calls on a stream share, where a graph has recorded
-them.
+And the buffers that products and sums on a stream share, where a graph has
+recorded them and where two host threads use them.
 """
 
 import contextlib
 import gc
 import threading
+import time
 import weakref
 
 import pytest
@@ -76,6 +77,32 @@ def test_buffers_and_captures(monkeypatch, get):
     assert unrecorded() is None
 
 
+def test_products_that_share_scratch_are_enqueued_one_by_one(monkeypatch):
+    # The host code alone, on CPU tensors: while one call is inside the library
+    # another does not get there.
+    inside, most = [], []
+
+    class Library:
+        @staticmethod
+        def tilec_matmul(*args):
+            inside.append(args[13])
+            most.append(len(inside))
+            time.sleep(0.05)
+            inside.pop()
+            return 0
+
+    monkeypatch.setattr(ext._lib, "lib", lambda: Library)
+    monkeypatch.setattr(ext, "_raw_stream", lambda device: 987654320)
+    monkeypatch.setattr(ext, "_scratch_sizes", lambda *a: (4096, 64))
+    x = torch.zeros(8, 8)
+    threads = [threading.Thread(target=ext._launch, args=(x, x, 8, 8, 8, 0, 1)) for _ in range(3)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert most == [1, 1, 1]
+
+
 def make(N, H, V, dt, seed):
     g = torch.Generator().manual_seed(seed)
     return (torch.randn(N, H, generator=g).to(dt).cuda(), (torch.randn(V, H, generator=g) * 0.1).to(dt).cuda(),
@@ -105,6 +132,29 @@ def test_two_threads_on_one_stream(dt):
         assert len(got[k]) == 100
         for out in got[k]:
             assert all(torch.equal(a, b) for a, b in zip(want[k], out))
+
+
+@pytest.mark.gpu
+def test_two_threads_copy_operands_on_one_stream():
+    # Variants that copy unaligned operands into the scratch first.
+    variant = next(v["name"] for v in tilec._lib.variants() if v["dtype"] == tilec._lib.BF16 and ext.pad_variant(v))
+    inputs = [(make(201, 333, 257, torch.bfloat16, s)[:2]) for s in (8, 9)]
+    inputs = [(x, w.t()) for x, w in inputs]
+    want = [ext.matrix_mul(*i, variant) for i in inputs]
+    got = [[], []]
+    start = threading.Barrier(2, timeout=20)
+
+    def work(k):
+        start.wait()
+        got[k] = [ext.matrix_mul(*inputs[k], variant) for _ in range(200)]
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    assert all(len(g) == 200 and all(torch.equal(out, w) for out in g) for g, w in zip(got, want))
 
 
 def replay_after_a_larger_call(call, small, large, replaced=()):

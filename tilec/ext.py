@@ -22,6 +22,7 @@ present.  The legacy config-space helpers of the reference (`plan`,
 
 import ctypes
 import re
+import threading
 from functools import lru_cache
 
 import torch
@@ -329,6 +330,12 @@ _SCRATCH = {}
 _COUNTERS = {}
 _CAPTURED = {}  # by address
 
+# Held while a product that uses its stream's scratch is enqueued: variants that
+# copy their operands first (*_pad, *_kc) pass the copies to the product through
+# it, and the C call gives up the interpreter's lock, so another thread's call
+# could write its own copies in between.
+_ENQUEUE = threading.Lock()
+
 
 def _capturing(device):
     return device.type == "cuda" and torch._C._cuda_isCurrentStreamCapturing()
@@ -438,15 +445,14 @@ def _launch(x1, x2, M, K, N, variant, split_k, ops=None):
     if M == 0 or N == 0:
         return out
     stream = _raw_stream(x1.device)
-    ws_ptr, ws_bytes, cnt_ptr, cnt_bytes = None, 0, None, 0
     need, need_cnt = _scratch_sizes(M, N, K, lda, ldb, layout, dtype, variant, split_k)
+    args = (a.data_ptr(), b.data_ptr(), out.data_ptr(), M, N, K, lda, ldb, N, layout, dtype, variant, split_k)
     if need:
-        ws = workspace_for(x1.device, stream, need)
-        ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
-        cnt = counters_for(x1.device, stream, need_cnt)
-        cnt_ptr, cnt_bytes = cnt.data_ptr(), cnt.numel()
-    rc = _lib.lib().tilec_matmul(a.data_ptr(), b.data_ptr(), out.data_ptr(), M, N, K, lda, ldb, N, layout,
-                                 dtype, variant, split_k, ws_ptr, ws_bytes, cnt_ptr, cnt_bytes, stream)
+        with _ENQUEUE:
+            ws, cnt = workspace_for(x1.device, stream, need), counters_for(x1.device, stream, need_cnt)
+            rc = _lib.lib().tilec_matmul(*args, ws.data_ptr(), ws.numel(), cnt.data_ptr(), cnt.numel(), stream)
+    else:
+        rc = _lib.lib().tilec_matmul(*args, None, 0, None, 0, stream)
     if rc:
         _lib.check(rc)
     return out
