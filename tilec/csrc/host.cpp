@@ -1,17 +1,18 @@
 // tilec._host: host code that reads torch tensors, where reading them from Python
 // costs more than the kernels they are for.
 //
-//   adamw_table(params, grads, exp_avg, exp_avg_sq, copies)
-//       -> None (nothing to do) or (table, count, bits, device, kept)
+//   adamw_step(params, grads, exp_avg, exp_avg_sq, copies, step, lr, beta1, beta2,
+//              eps, weight_decay, grad_scale, stream_of) -> None
 //   adamw_values_table(states)
 //       -> None or (table, count, device, outputs)
 //
-// The first checks the lists and packs a tilec_adamw_tensor (include/tilec.h)
-// for each parameter with a gradient into the bytes `table`.  The same checks
-// attribute by attribute in Python take 1.1 us a tensor (80 us for 72 tensors,
-// whose kernels take 12); these take 0.05.  `kept`: contiguous copies of gradients
-// that were not, to be held until the launch.  The second does the same for
-// tilec_adamw_values, whose float32 outputs it allocates, views of one storage.
+// The first checks the lists, packs a tilec_adamw_tensor (include/tilec.h) for
+// each parameter with a gradient and enqueues the step on stream_of(device), the
+// handle of the current stream of the tensors' device.  The same checks attribute
+// by attribute in Python take 1.1 us a tensor (80 us for 72 tensors, whose kernels
+// take 12); these take 0.05.  What the step writes counts as modified in place
+// for autograd.  The second packs the descriptions of tilec_adamw_values, whose
+// float32 outputs it allocates, views of one storage.
 //
 //   layer_norm(x, weight, bias, eps, dtype, stream) -> (y, mean, rstd)
 //   layer_norm_backward(dy, x, mean, rstd, weight, param_grads, stream)
@@ -29,6 +30,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
 
 #include <algorithm>
 #include <string>
@@ -88,70 +90,35 @@ struct Reader {
 
 int32_t code(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? TILEC_BF16 : TILEC_F32; }
 
+// Tensors that are written past torch: each is a new version of itself, so that a
+// backward pass that saved the old one raises instead of reading the new.
+// (Inference tensors have no versions.)
+struct Written {
+  std::vector<const at::Tensor*> all;
+  void* add(const at::Tensor& t) {
+    all.push_back(&t);
+    return t.data_ptr();
+  }
+  void bump() const {
+    for (const at::Tensor* t : all)
+      if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  }
+};
+
 // A state: its values or codes, and the scales of codes (bits 8).
-void read_state(Reader& r, const char* name, PyObject* o, int64_t n, at::ScalarType codes, int& bits, void*& values,
-                float*& scales) {
+void read_state(Reader& r, Written& w, const char* name, PyObject* o, int64_t n, at::ScalarType codes, int& bits,
+                void*& values, float*& scales) {
   const bool pair = PyTuple_Check(o) || PyList_Check(o);
   if (bits == 0) bits = pair ? 8 : 32;
   if ((bits == 8) != pair) bad_value("states of 32 and of 8 bits are mixed");
   if (!pair) {
-    values = r.read(name, o, n, at::kFloat, at::kFloat).data_ptr();
+    values = w.add(r.read(name, o, n, at::kFloat, at::kFloat));
     return;
   }
   const List both(o);
   if (both.size() != 2) bad_value(std::string(name) + ": an 8-bit state is a pair (codes, scales)");
-  values = r.read(name, both[0], n, codes, codes).data_ptr();
-  scales = static_cast<float*>(r.read("scales", both[1], (n + kBlock - 1) / kBlock, at::kFloat, at::kFloat).data_ptr());
-}
-
-PyObject* build(PyObject* const* args) {
-  const List params(args[0]), grads(args[1]), m(args[2]), v(args[3]);
-  const bool copied = args[4] != Py_None;
-  const List copies(copied ? args[4] : args[0]);
-  const Py_ssize_t count = params.size();
-  if (grads.size() != count || m.size() != count || v.size() != count || copies.size() != count)
-    bad_value(std::to_string(count) + " params, " + std::to_string(grads.size()) + " grads, " +
-              std::to_string(m.size()) + " and " + std::to_string(v.size()) + " states, " +
-              std::to_string(copied ? copies.size() : count) + " copies");
-  Reader r;
-  int bits = 0;
-  std::vector<tilec_adamw_tensor> table;
-  std::vector<at::Tensor> kept;
-  table.reserve(count);
-  for (Py_ssize_t i = 0; i < count; ++i) {
-    if (grads[i] == Py_None) continue;
-    tilec_adamw_tensor d{};
-    const at::Tensor& p = r.read("params", params[i], -1, at::kFloat, at::kBFloat16);
-    const int64_t n = p.numel();
-    const at::Tensor* g = &r.read("grads", grads[i], n, at::kFloat, at::kBFloat16, false);
-    if (!g->is_contiguous()) {
-      kept.push_back(g->contiguous());
-      g = &kept.back();
-    }
-    d.param = p.data_ptr();
-    d.grad = g->const_data_ptr();
-    d.param_dtype = code(p);
-    d.grad_dtype = code(*g);
-    d.n = n;
-    read_state(r, "exp_avg", m[i], n, at::kChar, bits, d.exp_avg, d.exp_avg_scale);
-    read_state(r, "exp_avg_sq", v[i], n, at::kByte, bits, d.exp_avg_sq, d.exp_avg_sq_scale);
-    if (copied && copies[i] != Py_None) d.copy = r.read("copies", copies[i], n, at::kBFloat16, at::kBFloat16).data_ptr();
-    table.push_back(d);
-  }
-  if (table.empty()) Py_RETURN_NONE;
-  // One memory for two parameters (a tied weight given twice) would be a race.
-  std::vector<void*> starts;
-  starts.reserve(table.size());
-  for (const auto& d : table)
-    if (d.n > 0) starts.push_back(d.param);
-  std::sort(starts.begin(), starts.end());
-  if (std::adjacent_find(starts.begin(), starts.end()) != starts.end()) bad_value("two params share their memory");
-  PyObject* held = PyList_New((Py_ssize_t)kept.size());
-  if (held == nullptr) throw python_error();
-  for (size_t i = 0; i < kept.size(); ++i) PyList_SET_ITEM(held, (Py_ssize_t)i, THPVariable_Wrap(kept[i]));
-  return Py_BuildValue("(y#iiLN)", reinterpret_cast<const char*>(table.data()),
-                       (Py_ssize_t)(table.size() * sizeof(tilec_adamw_tensor)), (int)table.size(), bits,
-                       (long long)r.device, held);
+  values = w.add(r.read(name, both[0], n, codes, codes));
+  scales = static_cast<float*>(w.add(r.read("scales", both[1], (n + kBlock - 1) / kBlock, at::kFloat, at::kFloat)));
 }
 
 PyObject* build_values(PyObject* const* args) {
@@ -267,6 +234,12 @@ void* stream_of(PyObject* o) {
   return s;
 }
 
+double number(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+
 PyObject* three(const at::Tensor& a, const at::Tensor& b, const at::Tensor& c) {
   PyObject* t = PyTuple_New(3);
   if (t == nullptr) throw python_error();
@@ -279,14 +252,77 @@ PyObject* three(const at::Tensor& a, const at::Tensor& b, const at::Tensor& c) {
   return t;
 }
 
+PyObject* build_adamw(PyObject* const* args) {
+  const List params(args[0]), grads(args[1]), m(args[2]), v(args[3]);
+  const bool copied = args[4] != Py_None;
+  const List copies(copied ? args[4] : params.seq);  // (an iterator gives its tensors once)
+  const Py_ssize_t count = params.size();
+  if (grads.size() != count || m.size() != count || v.size() != count || copies.size() != count)
+    bad_value(std::to_string(count) + " params, " + std::to_string(grads.size()) + " grads, " +
+              std::to_string(m.size()) + " and " + std::to_string(v.size()) + " states, " +
+              std::to_string(copied ? copies.size() : count) + " copies");
+  Reader r;
+  Written w;
+  int bits = 0;
+  std::vector<tilec_adamw_tensor> table;
+  std::vector<at::Tensor> kept;
+  table.reserve(count);
+  w.all.reserve(6 * count);
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    if (grads[i] == Py_None) continue;
+    tilec_adamw_tensor d{};
+    const at::Tensor& p = r.read("params", params[i], -1, at::kFloat, at::kBFloat16);
+    const int64_t n = p.numel();
+    const at::Tensor* g = &r.read("grads", grads[i], n, at::kFloat, at::kBFloat16, false);
+    if (!g->is_contiguous()) {
+      kept.push_back(g->contiguous());
+      g = &kept.back();
+    }
+    d.param = w.add(p);
+    d.grad = g->const_data_ptr();
+    d.param_dtype = code(p);
+    d.grad_dtype = code(*g);
+    d.n = n;
+    read_state(r, w, "exp_avg", m[i], n, at::kChar, bits, d.exp_avg, d.exp_avg_scale);
+    read_state(r, w, "exp_avg_sq", v[i], n, at::kByte, bits, d.exp_avg_sq, d.exp_avg_sq_scale);
+    if (copied && copies[i] != Py_None) d.copy = w.add(r.read("copies", copies[i], n, at::kBFloat16, at::kBFloat16));
+    table.push_back(d);
+  }
+  if (table.empty()) Py_RETURN_NONE;
+  // One memory for two parameters (a tied weight given twice) would be a race.
+  std::vector<void*> starts;
+  starts.reserve(table.size());
+  for (const auto& d : table)
+    if (d.n > 0) starts.push_back(d.param);
+  std::sort(starts.begin(), starts.end());
+  if (std::adjacent_find(starts.begin(), starts.end()) != starts.end()) bad_value("two params share their memory");
+  const int64_t step = PyLong_AsLongLong(args[5]);
+  if (step == -1 && PyErr_Occurred()) throw python_error();
+  const double lr = number(args[6]), beta1 = number(args[7]), beta2 = number(args[8]), eps = number(args[9]),
+               decay = number(args[10]);
+  const float* grad_scale = nullptr;
+  if (args[11] != Py_None) {
+    const at::Tensor& t = r.read("grad_scale", args[11], -1, at::kFloat, at::kFloat, false);
+    if (t.numel() != 1) bad_value("grad_scale has shape " + shape(t) + ", expected one value");
+    grad_scale = static_cast<const float*>(t.const_data_ptr());
+  }
+  PyObject* stream = PyObject_CallFunction(args[12], "L", (long long)r.device);
+  if (stream == nullptr) throw python_error();
+  const THPObjectPtr held(stream);
+  const c10::DeviceGuard guard(c10::Device(at::kCUDA, (c10::DeviceIndex)r.device));
+  check(tilec_adamw(table.data(), (int32_t)table.size(), bits, step, lr, beta1, beta2, eps, decay, grad_scale,
+                    stream_of(stream)));
+  w.bump();
+  Py_RETURN_NONE;
+}
+
 PyObject* build_norm(PyObject* const* args) {
   const at::Tensor& x = tensor("x", args[0]);
   OneGpu gpu;
   const int32_t x_code = gpu.code("x", x);
   const Rows r("x", x);
   const Params p(gpu, args[1], args[2], r.D);
-  const double eps = PyFloat_AsDouble(args[3]);
-  if (eps == -1.0 && PyErr_Occurred()) throw python_error();
+  const double eps = number(args[3]);
   at::ScalarType type = x.scalar_type();
   if (args[4] != Py_None) {
     if (!THPDtype_Check(args[4])) bad_type("dtype is no torch.dtype");
@@ -338,7 +374,7 @@ PyObject* build_norm_backward(PyObject* const* args) {
   return three(dx, dw, db);
 }
 
-constexpr char kAdamw[] = "adamw", kNorm[] = "layer_norm", kNormBackward[] = "layer_norm_backward";
+constexpr char kAdamw[] = "adamw_step", kValues[] = "adamw_values", kNorm[] = "layer_norm", kNormBackward[] = "layer_norm_backward";
 
 template <PyObject* (*BUILD)(PyObject* const*), int ARGS, const char* NAME>
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t count) {
@@ -362,9 +398,10 @@ PyCFunction function() {
 }
 
 PyMethodDef kMethods[] = {
-    {"adamw_table", function<build, 5, kAdamw>(), METH_FASTCALL,
-     "adamw_table(params, grads, exp_avg, exp_avg_sq, copies) -> None or (table, count, bits, device, kept)"},
-    {"adamw_values_table", function<build_values, 1, kAdamw>(), METH_FASTCALL,
+    {"adamw_step", function<build_adamw, 13, kAdamw>(), METH_FASTCALL,
+     "adamw_step(params, grads, exp_avg, exp_avg_sq, copies, step, lr, beta1, beta2, eps, weight_decay, grad_scale, "
+     "stream_of)"},
+    {"adamw_values_table", function<build_values, 1, kValues>(), METH_FASTCALL,
      "adamw_values_table(states) -> None or (table, count, device, outputs)"},
     {"layer_norm", function<build_norm, 6, kNorm>(), METH_FASTCALL,
      "layer_norm(x, weight, bias, eps, dtype, stream) -> (y, mean, rstd)"},

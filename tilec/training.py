@@ -259,24 +259,14 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     from 1.  grad_scale: a float32 value on the GPU that multiplies every
     gradient (a clipping coefficient).  copies: bfloat16 tensors that get the
     new parameters, rounded (None, or None for some: none).  All arithmetic is
-    float32; many tensors share a launch.
+    float32; many tensors share a launch.  To autograd, what is written has been
+    modified in place: a backward pass through a graph that saved a parameter
+    before the step raises.
     """
-    what = "adamw_step"
     if step < 1:
-        raise ValueError(f"{what}: steps count from 1 (got {step})")
-    packed = _lib.host().adamw_table(params, grads, exp_avg, exp_avg_sq, copies)
-    if packed is None:
-        return
-    table, count, bits, device, kept = packed
-    if grad_scale is not None:
-        if grad_scale.dtype != torch.float32 or grad_scale.get_device() != device:
-            raise TypeError(f"{what}: grad_scale must be float32 on the params' GPU (got {grad_scale.dtype}, "
-                            f"{grad_scale.device})")
-        if grad_scale.numel() != 1:
-            raise ValueError(f"{what}: grad_scale has shape {tuple(grad_scale.shape)}, expected one value")
-    with _on(device):
-        _lib.check(_lib.lib().tilec_adamw(table, count, bits, step, lr, betas[0], betas[1], eps, weight_decay,
-                                          _ptr(grad_scale), _raw_stream(device)))
+        raise ValueError(f"adamw_step: steps count from 1 (got {step})")
+    _lib.host().adamw_step(params, grads, exp_avg, exp_avg_sq, copies, step, lr, betas[0], betas[1], eps, weight_decay,
+                           grad_scale, _raw_stream)
 
 
 def adamw_values(states):
