@@ -258,8 +258,10 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     `adamw_state` makes them, 32-bit or 8-bit (codes, scales).  step counts
     from 1.  grad_scale: a float32 value on the GPU that multiplies every
     gradient (a clipping coefficient).  copies: bfloat16 tensors that get the
-    new parameters, rounded (None, or None for some: none).  All arithmetic is
-    float32; many tensors share a launch.  To autograd, what is written has been
+    new parameters, rounded (None, or None for some: none).  What is written may
+    not overlap anything else in the lists (ValueError), but a result may go
+    where it was read from.  All arithmetic is float32; many tensors share a
+    launch.  To autograd, what is written has been
     modified in place: a backward pass through a graph that saved a parameter
     before the step raises.
     """
