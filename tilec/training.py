@@ -18,7 +18,7 @@ from functools import lru_cache
 import torch
 
 from . import _lib
-from .ext import _tuned, counters_for
+from .ext import _current_device, _raw_stream, _tuned, counters_for
 
 __all__ = ["layer_norm", "layer_norm_backward", "linear_cross_entropy", "linear_cross_entropy_grad",
            "adamw_state", "adamw_step", "adamw_values", "ADAMW_BLOCK"]
@@ -61,11 +61,6 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-# Per call these cost less than torch.cuda.current_stream and current_device,
-# which build objects and check for initialisation (a GPU tensor is at hand).
-_raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
-
-
 def _stream_of(x):
     """The current stream of the GPU that x is on (0 elsewhere: x is refused)."""
     return _raw_stream(x.get_device()) if x.is_cuda else 0
@@ -84,7 +79,7 @@ _HERE = _Here()
 
 def _on(index):
     """The GPU of that index as the current one, where it is not."""
-    return _HERE if index == _current() else torch.cuda.device(index)
+    return _HERE if index == _current_device() else torch.cuda.device(index)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, dtype=None):
