@@ -278,8 +278,9 @@ size_t tilec_layer_norm_backward_workspace_bytes(int64_t R, int64_t D, int32_t x
  *   loss_r = log(sum_v exp(logits[r, v])) - logits[r, target_r]
  * float32: `loss` [N] with TILEC_REDUCE_NONE, else one value, the sum or the
  * mean over the rows that count.  Rows whose target is ignore_index do not:
- * their loss and gradients are 0 whatever x holds there, and a mean over no
- * rows is 0.  A target that is neither that nor a class in [0, V) makes its
+ * their loss and gradients are 0 whatever x holds there and whatever grad_loss
+ * is (dx of float32 inputs: where weight is finite), and a mean over no rows is
+ * 0.  A target that is neither that nor a class in [0, V) makes its
  * loss, and every gradient it reaches, NaN.
  *
  * grad != 0 also writes the gradients dx [N, H] and dweight [V, H],

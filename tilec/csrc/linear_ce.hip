@@ -160,11 +160,20 @@ struct CeGrad {
   int64_t ld32, split;  // split: elements of one
   bool add;             // to what acc32 holds
   const float* scale;   // applied when out is written
+  // dx: the rows' targets.  Ignored rows get zeros by choice, not by a product:
+  // their sums are zeros, but the scalar factor may be infinite or a NaN.
+  const int64_t* target;  // NULL: dW
+  int64_t ignore;
 
   template <class P, int MF>
   __device__ __forceinline__ void run(const TileOut<P, MF>& t, typename P::Acc (&acc)[P::TM][P::TN], int H,
                                       int N) const {
     const float f = out != nullptr ? *scale : 1.f;
+    bool skip[P::TN] = {};
+    if (out != nullptr && target != nullptr) {
+#pragma unroll
+      for (int j = 0; j < P::TN; ++j) skip[j] = target[min(t.col(j), N - 1)] == ignore;
+    }
 #pragma unroll
     for (int j = 0; j < P::TN; ++j)
 #pragma unroll
@@ -177,9 +186,11 @@ struct CeGrad {
             if (add) v += *p;
             if (out == nullptr) *p = v;
           }
-          if (out != nullptr)
-            t.put(i, q, j, (int)(bf16_bits(v[0] * f) | (uint32_t)bf16_bits(v[1] * f) << 16),
-                  (int)(bf16_bits(v[2] * f) | (uint32_t)bf16_bits(v[3] * f) << 16));
+          if (out != nullptr) {
+            const int lo = (int)(bf16_bits(v[0] * f) | (uint32_t)bf16_bits(v[1] * f) << 16);
+            const int hi = (int)(bf16_bits(v[2] * f) | (uint32_t)bf16_bits(v[3] * f) << 16);
+            t.put(i, q, j, skip[j] ? 0 : lo, skip[j] ? 0 : hi);
+          }
         }
     if (out == nullptr) return;
     t.store_all([&](int n, int h, i32x4 x) {
@@ -239,6 +250,7 @@ struct CePrepare {
         float f = 1.f;
         if (reduction != kNone && grad_loss != nullptr) f = *grad_loss;
         if (reduction == kMean) f /= (float)max(count[0], 1);
+        if (count[0] == 0) f = 0.f;  // zeros, whatever grad_loss is
         *scale = f;
       }
       return;
@@ -445,6 +457,8 @@ struct CeJoin {
   float* acc;
   bool add;
   const float* scale;
+  const int64_t* target;  // as CeGrad's
+  int64_t ignore;
 
   // Workgroup `block` of `blocks`: each thread every lanes-th split, then those
   // sums in order.
@@ -455,6 +469,8 @@ struct CeJoin {
     for (int64_t i0 = block * per; i0 < rows * per_row; i0 += blocks * per) {
       const int64_t i = i0 + mine;
       const bool live = i < rows * per_row;
+      const int64_t r = live ? i / per_row : 0, c = 4 * (i - r * per_row);
+      const bool skip = target != nullptr && target[r] == ignore;
       f32x4 v = {0.f, 0.f, 0.f, 0.f};
       if (live) {
         const float* p = part + 4 * i;
@@ -468,7 +484,6 @@ struct CeJoin {
         for (int k = 1; k < lanes && lane == 0; ++k) v += share[k * per + mine];
       }
       if (!live || lane != 0) continue;
-      const int64_t r = i / per_row, c = 4 * (i - r * per_row);
       f32x4* to = reinterpret_cast<f32x4*>(acc + 4 * i);
       if (add) v += *to;
       if (out == nullptr) {
@@ -477,7 +492,7 @@ struct CeJoin {
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (c + k < cols) out[r * cols + c + k] = bf16_bits(v[k] * f);
+        if (c + k < cols) out[r * cols + c + k] = skip ? (u16)0 : bf16_bits(v[k] * f);
     }
   }
 };
@@ -929,13 +944,13 @@ hipError_t run_finish(const CeFinish& f, hipStream_t stream) {
 // last.
 template <bool CB>
 hipError_t run_grad(const CeArgs& a, const CePlan& p, char* ws, const Operands& o, const CeProduct& c, u16* out,
-                    float* acc, bool add, CeJoin* join, hipStream_t stream) {
+                    float* acc, bool add, const int64_t* target, CeJoin* join, hipStream_t stream) {
   const float* scale = reinterpret_cast<const float*>(ws + p.scale);
   float* part = reinterpret_cast<float*>(ws + p.split);
   const int64_t ld = sum_ld(a.H);
   const int64_t splits = gemm_split_geom(o.K, 64, c.splits).splits;
-  CeGrad g{out, a.H, acc, ld, 0, add, scale};
-  if (splits > 1) g = CeGrad{nullptr, 0, part, ld, o.N * ld, false, nullptr};
+  CeGrad g{out, a.H, acc, ld, 0, add, scale, target, a.ignore};
+  if (splits > 1) g = CeGrad{nullptr, 0, part, ld, o.N * ld, false, nullptr, nullptr, 0};
   Operands main = o;
   if (c.main < o.N) {  // CB false: d's rows, N the vocabulary
     Operands rest = o;
@@ -948,7 +963,7 @@ hipError_t run_grad(const CeArgs& a, const CePlan& p, char* ws, const Operands& 
     main.N = c.main;
   }
   CE_TRY((run_product<kKRows, true, CB>(main, g, c.tile, c.splits, stream)));
-  if (splits > 1) *join = CeJoin{part, (int)splits, 1, o.N, a.H, ld, out, acc, add, scale};
+  if (splits > 1) *join = CeJoin{part, (int)splits, 1, o.N, a.H, ld, out, acc, add, scale, target, a.ignore};
   return hipSuccess;
 }
 
@@ -997,7 +1012,7 @@ hipError_t run_bf16(const CeArgs& a, const CePlan& p, char* ws, hipStream_t stre
     // whole K steps, W ends with its rows.
     CeJoin jx{}, jw{};
     CE_TRY(run_grad<true>(a, p, ws, Operands{w, keep, ldw, p.Vp, a.H, R, a.V}, p.p2,
-                          static_cast<u16*>(a.dx) + r0 * a.H, nullptr, false, &jx, stream));
+                          static_cast<u16*>(a.dx) + r0 * a.H, nullptr, false, a.target + r0, &jx, stream));
     const CeFinish f = finish_of(a, p, ws, jx, last);
     // dW^T [H, V] = x^T d over the chunk's rows.  Its kernel of few rows joins
     // dx and the losses beside it (7 x 1024 x 32768: 52.5 -> 48.9 us for all);
@@ -1015,7 +1030,7 @@ hipError_t run_bf16(const CeArgs& a, const CePlan& p, char* ws, hipStream_t stre
     }
     CE_TRY(run_finish(f, stream));
     CE_TRY(run_grad<false>(a, p, ws, Operands{xs, keep, p.Hp, p.Vp, a.H, a.V, R}, p.p3, last ? dw : nullptr,
-                           p.chunks > 1 ? reinterpret_cast<float*>(ws + p.acc) : nullptr, c > 0, &jw, stream));
+                           p.chunks > 1 ? reinterpret_cast<float*>(ws + p.acc) : nullptr, c > 0, nullptr, &jw, stream));
     CE_TRY(run_finish(finish_of(a, p, ws, jw, false), stream));
   }
   return hipSuccess;

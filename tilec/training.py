@@ -209,8 +209,9 @@ def linear_cross_entropy_grad(x, weight, target, reduction="mean", ignore_index=
         d[r, v] = g_r * (softmax(logits)[r, v] - [v = target_r]);  dx = d @ weight;  dweight = d.T @ x
 
     grad_loss: the gradient of the loss on the GPU, float32: one value for
-    "mean" and "sum", [N] for "none"; None: ones.  Ignored rows add nothing,
-    whatever x holds there, and get a dx of zeros.
+    "mean" and "sum", [N] for "none"; None: ones.  Ignored rows add nothing
+    and get a dx of zeros, whatever x holds there and whatever grad_loss is
+    (float32: where weight is finite).
 
     Of the logits, one 16-bit value each (float32 inputs: 32-bit) is kept for
     a chunk of rows at a time, `chunk_rows` of them, or by default as many as
