@@ -77,6 +77,30 @@ def test_buffers_and_captures(monkeypatch, get):
     assert unrecorded() is None
 
 
+def test_counters_outlive_the_call_they_are_for(monkeypatch):
+    # The host code alone, on CPU tensors: another thread's call that needs more
+    # counters replaces the buffer while this call is inside the library.
+    held = []
+
+    class Library:
+        @staticmethod
+        def tilec_linear_ce(*args):
+            buffer = weakref.ref(ext._COUNTERS[None, 987654319].untyped_storage())
+            ext.counters_for(torch.device("cpu"), 987654319, 1 << 20)
+            gc.collect()
+            held.append(buffer() is not None)
+            return 0
+
+    monkeypatch.setattr(training._lib, "lib", lambda: Library)
+    monkeypatch.setattr(training, "_on_gpu", lambda *a: 0)
+    monkeypatch.setattr(training, "_on", lambda index: contextlib.nullcontext())
+    monkeypatch.setattr(training, "_raw_stream", lambda index: 987654319)
+    monkeypatch.setattr(training, "_ce_plan", lambda *a: (4096, 256, None))
+    x, w, t = torch.zeros(4, 8), torch.zeros(5, 8), torch.zeros(4, dtype=torch.int64)
+    tilec.ext.linear_cross_entropy_grad(x, w, t)
+    assert held == [True]
+
+
 def test_products_that_share_scratch_are_enqueued_one_by_one(monkeypatch):
     # The host code alone, on CPU tensors: while one call is inside the library
     # another does not get there.

@@ -177,11 +177,11 @@ def _linear_ce(what, x, weight, target, reduction, ignore_index, grad, grad_loss
         ws, cnt, configs = _ce_plan(at, N, H, V, ldx, ldw, dtype, code, grad, chunk_rows, x.data_ptr() % 16,
                                     weight.data_ptr() % 16)
         scratch = torch.empty(ws, dtype=torch.uint8, device=x.device) if ws else None
-        cnt_ptr = counters_for(x.device, stream, cnt).data_ptr() if cnt else None
+        counters = counters_for(x.device, stream, cnt) if cnt else None  # held until all is enqueued
         _lib.check(_lib.lib().tilec_linear_ce(x.data_ptr(), weight.data_ptr(), target.data_ptr(), loss.data_ptr(),
                                               _ptr(grad_loss), _ptr(dx), _ptr(dw), N, H, V, ldx, ldw, dtype, code,
-                                              int(ignore_index), grad, chunk_rows, configs, _ptr(scratch), ws, cnt_ptr, cnt,
-                                              stream))
+                                              int(ignore_index), grad, chunk_rows, configs, _ptr(scratch), ws,
+                                              _ptr(counters), cnt, stream))
     return loss, dx, dw
 
 
