@@ -20,7 +20,8 @@
  *     input row-major contiguous first (`.contiguous()`, tilec/ext.py:59-60;
  *     then ld == the number of columns); strided and transposed views skip
  *     that copy here.
- *   - Outputs are float32.  Inputs are float32, or bfloat16 (fp32 accumulate).
+ *   - Outputs of products and sums are float32 (the training operators say
+ *     their own types).  Inputs are float32, or bfloat16 (fp32 accumulate).
  *   - Nothing here allocates device memory, synchronizes, or reads the device
  *     back: work is enqueued on `stream` (a hipStream_t; NULL = the legacy
  *     default stream) and returns at once, like the reference's asynchronous
@@ -49,7 +50,7 @@ extern "C" {
 #define TILEC_ERR_WORKSPACE 4   /* workspace missing or too small         */
 #define TILEC_ERR_HIP 5         /* HIP runtime error at launch            */
 
-/* Element types of x1 / x2 (the output is always float32). */
+/* Element types (the output of a product or a sum is always float32). */
 #define TILEC_F32 0
 #define TILEC_BF16 1
 
@@ -272,9 +273,9 @@ int tilec_layer_norm_backward(const void* dy, const void* x, const float* mean, 
 size_t tilec_layer_norm_backward_workspace_bytes(int64_t R, int64_t D, int32_t x_dtype);
 
 /*
- * Cross entropy of logits = x weight^T, which are not kept: x [N, H], weight
- * [V, H] (both float32 or both bfloat16, row-major with row strides ldx, ldw
- * >= H), target [N] int64.
+ * Cross entropy of logits = x weight^T, which are not given out: x [N, H],
+ * weight [V, H] (both float32 or both bfloat16, row-major with row strides ldx,
+ * ldw >= H), target [N] int64.
  *   loss_r = log(sum_v exp(logits[r, v])) - logits[r, target_r]
  * float32: `loss` [N] with TILEC_REDUCE_NONE, else one value, the sum or the
  * mean over the rows that count.  Rows whose target is ignore_index do not:
@@ -288,8 +289,11 @@ size_t tilec_layer_norm_backward_workspace_bytes(int64_t R, int64_t D, int32_t x
  *   TILEC_REDUCE_NONE:       sum_r grad_loss[r] loss_r  (grad_loss [N] float32, NULL: ones)
  *   TILEC_REDUCE_SUM, _MEAN: grad_loss[0] loss          (one float32 on the device, NULL: 1)
  * Rows are worked through in chunks of chunk_rows (0: as many as keep the
- * chunk's 16-bit (float32: 32-bit) values, one per row and class, within 2
- * GiB); more than one chunk adds a float32 [V, H] to the workspace.
+ * chunk's values, one per row and class, within 2 GiB); more than one chunk
+ * adds a float32 [V, H] to the workspace.  Those values are 16-bit ones that
+ * gradients of bfloat16 inputs need, or the float32 logits of float32 inputs,
+ * losses alone included; losses alone of bfloat16 inputs keep 8 bytes per row
+ * and 64 classes.
  *
  * tilec_linear_ce_scratch_bytes gives the workspace (any contents, 16-byte
  * aligned) and counters (zeroed once, left zero) for exactly these arguments;
@@ -321,8 +325,9 @@ int tilec_linear_ce_scratch_bytes(const void* x, const void* weight, int64_t N, 
  *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   p = p - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
  * with `step` counted from 1 and grad_scale one float32 on the device (NULL:
- * 1).  The descriptions in `tensors` (host memory) are read before the call
- * returns.  Every tensor is contiguous, of n elements, at any alignment of
+ * 1).  `step` and the other numbers are read on the host: a HIP graph repeats
+ * those it was recorded with.  The descriptions in `tensors` (host memory) are
+ * read before the call returns.  Every tensor is contiguous, of n elements, at any alignment of
  * its element type; no two of them may overlap.
  *
  * state_bits 32: exp_avg and exp_avg_sq are float32 [n].  state_bits 8: they

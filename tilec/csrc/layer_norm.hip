@@ -539,7 +539,9 @@ constexpr int kMaxGrid = 1 << 20;  // workgroups of the passes over long rows; t
 // Waves a CU of the forward pass, whose workgroups walk over rows with their
 // parameters in registers: read again for every row, from the caches, they made
 // 8192 x 4096 bf16 35 us instead of 28, 4099 x 3001 fp32 22 instead of 20 (16,
-// 24 and 32 waves: 28, 30 and 31 us).
+// 24 and 32 waves: 28, 30 and 31 us).  As many whole workgroups as fit into
+// them: rows of 576 to 960 threads (of many rows, fp32 from 8193 values on, bf16
+// from 16385) have one a CU, 9 to 15 waves.
 constexpr int kWaves = 16;
 
 template <typename TX, typename TY>

@@ -187,7 +187,7 @@ def _linear_ce(what, x, weight, target, reduction, ignore_index, grad, grad_loss
 
 def linear_cross_entropy(x, weight, target, reduction="mean", ignore_index=-100):
     """Cross entropy of the logits x @ weight.T against `target`, without
-    keeping the logits.
+    giving out the logits.
 
         loss_r = log(sum_v exp(logits[r, v])) - logits[r, target_r]
 
@@ -198,6 +198,10 @@ def linear_cross_entropy(x, weight, target, reduction="mean", ignore_index=-100)
     holds there, and a mean over no rows is 0.  A target that is neither that
     nor a class makes its loss NaN (nothing here reads the device back to
     raise for it).
+
+    Of bfloat16 inputs' logits nothing is kept but a maximum and a sum for every
+    64 classes of a row; those of float32 inputs are written to a workspace, for
+    as many rows at a time as fit 2 GiB.
     """
     return _linear_ce("linear_cross_entropy", x, weight, target, reduction, ignore_index, 0, None, 0)[0]
 
@@ -217,6 +221,9 @@ def linear_cross_entropy_grad(x, weight, target, reduction="mean", ignore_index=
     a chunk of rows at a time, `chunk_rows` of them, or by default as many as
     fit 2 GiB of workspace; with more than one chunk, dweight is added up in a
     float32 workspace of its size.
+
+    For bfloat16 inputs d itself is rounded to bfloat16 before the products,
+    beside the rounding of dx and dweight.
     """
     return _linear_ce("linear_cross_entropy_grad", x, weight, target, reduction, ignore_index, 1, grad_loss,
                       chunk_rows)
@@ -260,6 +267,9 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     launch.  To autograd, what is written has been
     modified in place: a backward pass through a graph that saved a parameter
     before the step raises.
+
+    `step`, `lr` and the other numbers are read on the host: a HIP graph of this
+    call repeats the step it was recorded with, bias correction included.
     """
     if step < 1:
         raise ValueError(f"adamw_step: steps count from 1 (got {step})")
