@@ -127,6 +127,29 @@ def test_products_that_share_scratch_are_enqueued_one_by_one(monkeypatch):
     assert most == [1, 1, 1]
 
 
+def test_a_product_in_a_signal_handler_does_not_wait_for_the_call_it_interrupts(monkeypatch):
+    # The host code alone: the handler runs while this thread's call is being
+    # enqueued.
+    calls = []
+
+    class Library:
+        @staticmethod
+        def tilec_matmul(*args):
+            calls.append(args[13])
+            if len(calls) == 1:  # what a handler would do here
+                ext._launch(x, x, 8, 8, 8, 0, 1)
+            return 0
+
+    monkeypatch.setattr(ext._lib, "lib", lambda: Library)
+    monkeypatch.setattr(ext, "_raw_stream", lambda index: 987654318)
+    monkeypatch.setattr(ext, "_scratch_sizes", lambda *a: (4096, 64))
+    x = torch.zeros(8, 8)
+    outer = threading.Thread(target=ext._launch, args=(x, x, 8, 8, 8, 0, 1), daemon=True)
+    outer.start()
+    outer.join(timeout=10)
+    assert not outer.is_alive() and len(calls) == 2
+
+
 def make(N, H, V, dt, seed):
     g = torch.Generator().manual_seed(seed)
     return (torch.randn(N, H, generator=g).to(dt).cuda(), (torch.randn(V, H, generator=g) * 0.1).to(dt).cuda(),

@@ -333,8 +333,9 @@ _CAPTURED = {}  # by address
 # Held while a product that uses its stream's scratch is enqueued: variants that
 # copy their operands first (*_pad, *_kc) pass the copies to the product through
 # it, and the C call gives up the interpreter's lock, so another thread's call
-# could write its own copies in between.
-_ENQUEUE = threading.Lock()
+# could write its own copies in between.  (Re-entrant: a signal handler or a
+# finaliser may multiply too, and is done before the call it interrupts goes on.)
+_ENQUEUE = threading.RLock()
 
 
 # Of torch's own functions for a GPU's state, with a tensor on it at hand: the
