@@ -53,6 +53,9 @@ extern "C" {
 /* Element types (the output of a product or a sum is always float32). */
 #define TILEC_F32 0
 #define TILEC_BF16 1
+/* 8-bit floating point, for operands with scales (below). */
+#define TILEC_F8E4M3 2 /* 4 bits of exponent, largest 448, no infinities */
+#define TILEC_F8E5M2 3 /* 5 bits of exponent, largest 57344              */
 
 /* Kernel families (tilec_variant_info, info[0]). */
 #define TILEC_FAMILY_SKINNY 0 /* output-stationary streaming kernel, split K:   */
@@ -356,6 +359,109 @@ int tilec_adamw(const tilec_adamw_tensor* tensors, int32_t count, int32_t state_
  * exp_avg_sq.
  */
 int tilec_adamw_values(const tilec_adamw_tensor* tensors, int32_t count, void* stream);
+
+/*
+ * Operators of 8-bit linear layers.  An 8-bit operand is a matrix of codes
+ * [R, C] (TILEC_F8E4M3 or TILEC_F8E5M2, row-major, row stride >= C) and float32
+ * scales of its blocks of `block` x 128 values, block 1 or 128:
+ *   value[r, c] = code[r, c] * scale[r / block, c / 128]
+ * The scales [ceil(R / block), ceil(C / 128)] are contiguous; a matrix's last
+ * blocks may be smaller.
+ *
+ * out [M, N] = x weight^T over the values, x [M, K], weight [N, K]:
+ *   out[m, n] = sum_g scale_x[m, g] scale_w[n, g] sum over k of group g of x[m, k] weight[n, k]
+ * out is float32 or bfloat16 with row stride ldo >= N.  The sums over groups are
+ * float32.  For a float32 out so are those within a group, of exact products;
+ * for a bfloat16 out they are the 8-bit matrix instructions', which cut every
+ * product at 2^-13 of the largest among eight consecutive k (1.5e-5 of the result
+ * for normal values).  The product of two scales is rounded to float32.  The same bits on every call on one device.
+ * K <= 2^22; K == 0 writes zeros.
+ *
+ * Operands are read in place where their rows begin at multiples of 16 bytes,
+ * and otherwise copied into the workspace first.  `workspace`:
+ * tilec_linear_fp8_workspace_bytes for the same arguments (of x and weight it
+ * reads the addresses' alignment only), any contents, 16-byte aligned.
+ */
+int tilec_linear_fp8(const void* x, const float* x_scale, const void* weight, const float* w_scale, void* out,
+                     int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldo, int32_t x_dtype,
+                     int32_t w_dtype, int32_t out_dtype, int32_t x_block, int32_t w_block, void* workspace,
+                     size_t workspace_bytes, void* stream);
+size_t tilec_linear_fp8_workspace_bytes(const void* x, const void* weight, int64_t M, int64_t N, int64_t K, int64_t ldx,
+                                        int64_t ldw, int32_t x_dtype, int32_t w_dtype, int32_t out_dtype,
+                                        int32_t x_block, int32_t w_block);
+
+/*
+ * 8-bit operands.  A block's scale and codes, each operation a float32 one that
+ * rounds to nearest, L the largest value of the type (448 or 57344):
+ *   a = max(largest magnitude, 2^-100);  scale = a / L;  code = round(x * (L / a))
+ * A block that holds a NaN or an infinity has a NaN for its scale and its codes.
+ *
+ * x [R, C], float32 or bfloat16, is row-major with row stride ldx (>= C) or, with
+ * layout TILEC_X1_COL_MAJOR, column-major (column stride ldx >= R): the transpose
+ * of a row-major matrix, quantised in blocks of its own columns.  Rows of codes
+ * begin at multiples of 16 bytes (codes 16-byte aligned, ldq a multiple of 16);
+ * the bytes from C to the next multiple of 16 are set to zero.
+ */
+int tilec_quantize_fp8(const void* x, void* codes, float* scales, int64_t R, int64_t C, int64_t ldx, int64_t ldq,
+                       int32_t layout, int32_t x_dtype, int32_t q_dtype, int32_t block, void* stream);
+
+/* The values that codes stand for, in float32 or bfloat16: out[r, c] = code[r, c] * scale. */
+int tilec_dequantize_fp8(const void* codes, const float* scales, void* out, int64_t R, int64_t C, int64_t ldq,
+                         int64_t ldo, int32_t q_dtype, int32_t out_dtype, int32_t block, void* stream);
+
+/*
+ * Root mean square norm over the rows of h [R, D], D >= 1:
+ *   h = x + residual, rounded to the residual's type (residual NULL: h = x, not written)
+ *   rstd = 1 / sqrt(sum(h^2) / D + eps);  y = h rstd weight
+ * x, residual and weight [D] (NULL: ones) are float32 or bfloat16 each, h has the
+ * residual's type.  y is float32, bfloat16, or 8-bit codes with y_scale
+ * [R, ceil(D / 128)] for blocks of 1 x 128, as tilec_quantize_fp8 writes them of
+ * the float32 y.  rstd [R] float32 is written where not NULL.  h may be the
+ * residual; otherwise outputs must not overlap inputs.
+ */
+int tilec_rms_norm(const void* x, const void* residual, const void* weight, void* y, float* y_scale, void* h,
+                   float* rstd, int64_t R, int64_t D, int64_t ldx, int64_t ldr, int64_t ldy, int64_t ldh,
+                   int32_t x_dtype, int32_t r_dtype, int32_t y_dtype, int32_t w_dtype, float eps, void* stream);
+
+/*
+ * Its gradients, hhat = h rstd:
+ *   dx = rstd (dy weight - hhat mean(dy weight hhat)) + dh;  dweight = sum over rows of dy hhat
+ * dx is the gradient of x and of the residual alike; dh (NULL: zeros) is that of h
+ * from its other reader.  dx has dh's type, or dy's without it; dweight [D],
+ * float32, may be NULL and is added in a fixed order.  `workspace`:
+ * tilec_rms_norm_backward_workspace_bytes, any contents, 16-byte aligned.  dx may
+ * be dy or dh where it has that type.
+ */
+int tilec_rms_norm_backward(const void* dy, const void* h, const float* rstd, const void* weight, const void* dh,
+                            void* dx, float* dweight, int64_t R, int64_t D, int64_t lddy, int64_t ldh, int64_t lddh,
+                            int64_t lddx, int32_t dy_dtype, int32_t h_dtype, int32_t dh_dtype, int32_t w_dtype,
+                            void* workspace, size_t workspace_bytes, void* stream);
+size_t tilec_rms_norm_backward_workspace_bytes(int64_t R, int64_t D, int32_t h_dtype);
+
+/*
+ * The norm of a list of gradients and the factor that clips it to max_norm
+ * (negative: no limit), both one float32 on the device:
+ *   norm = |grad_scale| sqrt(sum of all g^2);  scale = grad_scale min(1, max_norm / (norm + 1e-6))
+ * grad_scale: one float32 on the device (NULL: 1); scale may be NULL.  Squares
+ * and sums are float64, in a fixed order.  An infinite norm gives a scale of 0, a
+ * NaN one NaN.  Tensors are contiguous, at any alignment of their type; the
+ * descriptions (host memory) are read before the call returns.  `workspace`:
+ * tilec_grad_norm_workspace_bytes, any contents, 16-byte aligned.  `counter`: 4
+ * bytes, zero before the call and left zero; concurrent calls need their own.
+ *
+ * tilec_scale_grads multiplies every value by *scale in place, rounding once; it
+ * touches none where *scale is 1.  No two tensors may overlap.
+ */
+typedef struct tilec_grad {
+  void* data; /* float32 or bfloat16 [n] */
+  int64_t n;
+  int32_t dtype;
+} tilec_grad;
+int tilec_grad_norm(const tilec_grad* grads, int32_t count, const float* grad_scale, double max_norm, float* norm,
+                    float* scale, void* workspace, size_t workspace_bytes, void* counter, size_t counter_bytes,
+                    void* stream);
+size_t tilec_grad_norm_workspace_bytes(const tilec_grad* grads, int32_t count);
+int tilec_scale_grads(const tilec_grad* grads, int32_t count, const float* scale, void* stream);
 
 /* Message describing the last failure on this thread ("" if none). */
 const char* tilec_last_error(void);

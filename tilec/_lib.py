@@ -16,7 +16,7 @@ LIB_PATH = os.path.join(HERE, "libtilec_hip.so")
 
 # Status codes and enums (include/tilec.h).
 OK, ERR_VALUE, ERR_TYPE, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_HIP = 0, 1, 2, 3, 4, 5
-F32, BF16 = 0, 1
+F32, BF16, F8E4M3, F8E5M2 = 0, 1, 2, 3
 FAMILY_SKINNY, FAMILY_GEMM, FAMILY_DIRECT = 0, 1, 2
 X1_COL_MAJOR, X2_COL_MAJOR = 1, 2  # layout bits
 VARIANT_AUTO = -1
@@ -54,6 +54,19 @@ SIGNATURES = {
                                                      ctypes.POINTER(_i64)]),
     "tilec_adamw": (ctypes.c_int, [_vp, _i32, _i32, _i64, _f64, _f64, _f64, _f64, _f64, _vp, _vp]),
     "tilec_adamw_values": (ctypes.c_int, [_vp, _i32, _vp]),
+    "tilec_linear_fp8": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32,
+                                        _i32, _i32, _vp, _sz, _vp]),
+    "tilec_linear_fp8_workspace_bytes": (_sz, [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32]),
+    "tilec_quantize_fp8": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _vp]),
+    "tilec_dequantize_fp8": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _vp]),
+    "tilec_rms_norm": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32,
+                                      _i32, _i32, ctypes.c_float, _vp]),
+    "tilec_rms_norm_backward": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
+                                               _i32, _i32, _i32, _i32, _vp, _sz, _vp]),
+    "tilec_rms_norm_backward_workspace_bytes": (_sz, [_i64, _i64, _i32]),
+    "tilec_grad_norm": (ctypes.c_int, [_vp, _i32, _vp, _f64, _vp, _vp, _vp, _sz, _vp, _sz, _vp]),
+    "tilec_grad_norm_workspace_bytes": (_sz, [_vp, _i32]),
+    "tilec_scale_grads": (ctypes.c_int, [_vp, _i32, _vp, _vp]),
     "tilec_last_error": (ctypes.c_char_p, []),
     "tilec_version": (_i32, []),
 }

@@ -1,0 +1,315 @@
+// The norm of a list of gradients and the factor that clips it:
+//   norm = |grad_scale| sqrt(sum over all values of g^2)
+//   scale = grad_scale min(1, max_norm / (norm + 1e-6))
+// and the gradients multiplied by that factor in place.
+//
+// Bound by HBM: every value is read once (clipping: once more, and written).  One
+// launch serves up to kMaxTensors tensors, whose descriptions travel as kernel
+// arguments; a workgroup adds up one chunk of one tensor.  Squares and sums are
+// float64: nothing overflows, whatever the gradients, and nothing is lost; at two
+// float64 operations a value the memory still sets the pace.  Every chunk's sum is
+// a value of its own; the last workgroup of the call to finish (a counter, left
+// zero) adds them in order, so the same bits come out every time, and writes both
+// results: a second launch for that would cost a small model's norm half again.
+#include <algorithm>
+#include <cmath>
+
+#include "abi.h"
+#include "common.h"
+#include "../../include/tilec.h"
+
+namespace tilec {
+
+namespace {
+
+typedef unsigned short u16;
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+
+constexpr int kMaxTensors = 120;  // per launch: 3.8 KiB of arguments
+constexpr int kUnit = 4096;       // chunks are a multiple of this
+
+struct Tensor {
+  void* data;
+  int64_t n;
+  int first;  // the tensor's first workgroup
+  int bf16;
+};
+
+struct GradArgs {
+  int count, chunk;
+  int64_t base, total;  // this launch's first chunk among `total`; the last launch has base + grid == total
+  double* partial;
+  unsigned* counter;
+  const float *grad_scale, *scale_in;
+  float *norm, *scale;
+  float max_norm;  // negative: none
+  Tensor t[kMaxTensors];
+};
+
+// The tensor of workgroup b: the last whose first is not past it.
+__device__ __forceinline__ const Tensor& tensor_of(const GradArgs& a, int b) {
+  int lo = 0, hi = a.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.t[mid].first <= b) lo = mid;
+    else hi = mid - 1;
+  }
+  return a.t[lo];
+}
+
+// Sum over a workgroup of 256, in thread order within a wave and wave order.
+__device__ __forceinline__ double block_sum(double s, double* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  s = ((red[0] + red[1]) + red[2]) + red[3];
+  __syncthreads();
+  return s;
+}
+
+template <bool BF16>
+__device__ __forceinline__ void add_squares(u32x4 v, double (&s)[4]) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    if constexpr (BF16) {
+      const double a = (double)__uint_as_float(v[d] << 16), b = (double)__uint_as_float(v[d] & 0xffff0000u);
+      s[d] = fma(a, a, s[d]);
+      s[d] = fma(b, b, s[d]);
+    } else {
+      const double a = (double)__uint_as_float(v[d]);
+      s[d] = fma(a, a, s[d]);
+    }
+  }
+}
+
+// Squares of n values at p (at most a chunk), the thread's share.
+template <bool BF16>
+__device__ __forceinline__ double squares(const void* p, int n) {
+  constexpr int E = BF16 ? 8 : 4, U = 4;
+  typedef std::conditional_t<BF16, u16, float> T;
+  const T* const x = static_cast<const T*>(p);
+  double s[4] = {0., 0., 0., 0.};
+  int i = E * (int)threadIdx.x;
+  for (; i + (U - 1) * 256 * E + E <= n; i += U * 256 * E) {
+    u32x4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const u32x4_any*>(x + i + u * 256 * E);
+#pragma unroll
+    for (int u = 0; u < U; ++u) add_squares<BF16>(v[u], s);
+  }
+  for (; i < n; i += 256 * E) {
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (i + E <= n) {
+      v = *reinterpret_cast<const u32x4_any*>(x + i);
+    } else {
+      for (int e = 0; i + e < n; ++e) {
+        if constexpr (BF16) v[e >> 1] |= (uint32_t)x[i + e] << (16 * (e & 1));
+        else v[e] = __float_as_uint(x[i + e]);
+      }
+    }
+    add_squares<BF16>(v, s);
+  }
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+__global__ __launch_bounds__(256) void grad_norm_kernel(GradArgs a) {
+  __shared__ double red[4];
+  __shared__ int last;
+  if (a.count > 0) {
+    const Tensor& t = tensor_of(a, blockIdx.x);
+    const int64_t at = (int64_t)((int)blockIdx.x - t.first) * a.chunk;
+    const int n = (int)min((int64_t)a.chunk, t.n - at);
+    double s = t.bf16 ? squares<true>(static_cast<const u16*>(t.data) + at, n)
+                      : squares<false>(static_cast<const float*>(t.data) + at, n);
+    s = block_sum(s, red);
+    if (threadIdx.x == 0)
+      __hip_atomic_store(&a.partial[a.base + blockIdx.x], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (a.base + gridDim.x < a.total) return;
+    // The sum is at the device's coherence point before the arrival is counted.
+    __builtin_amdgcn_s_waitcnt(0);
+    if (threadIdx.x == 0)
+      last = __hip_atomic_fetch_add(a.counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    if (threadIdx.x == 0) __hip_atomic_store(a.counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  double s = 0.;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < a.total; i += 256)
+    s += __hip_atomic_load(&a.partial[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  s = block_sum(s, red);
+  if (threadIdx.x != 0) return;
+  const double gs = a.grad_scale != nullptr ? (double)*a.grad_scale : 1.;
+  const double norm = fabs(gs) * sqrt(s);
+  double clip = 1.;
+  if (a.max_norm >= 0.f) {
+    clip = (double)a.max_norm / (norm + 1e-6);
+    clip = clip > 1. ? 1. : clip;  // a NaN stays one
+  }
+  *a.norm = (float)norm;
+  if (a.scale != nullptr) *a.scale = (float)(gs * clip);
+}
+
+// Values multiplied by a factor in place; none is touched where it is 1.
+__global__ __launch_bounds__(256) void grad_scale_kernel(GradArgs a) {
+  const float f = *a.scale_in;
+  if (f == 1.f) return;
+  const Tensor& t = tensor_of(a, blockIdx.x);
+  const int64_t at = (int64_t)((int)blockIdx.x - t.first) * a.chunk;
+  const int n = (int)min((int64_t)a.chunk, t.n - at);
+  auto go = [&](auto* x, auto bf16) {
+    constexpr bool BF16 = decltype(bf16)::value;
+    constexpr int E = BF16 ? 8 : 4, U = 4;
+    auto times = [&](u32x4 v) {
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        if constexpr (BF16) {
+          const __bf16 lo = (__bf16)(__uint_as_float(v[d] << 16) * f), hi = (__bf16)(__uint_as_float(v[d] & 0xffff0000u) * f);
+          v[d] = (uint32_t)__builtin_bit_cast(u16, lo) | (uint32_t)__builtin_bit_cast(u16, hi) << 16;
+        } else {
+          v[d] = __float_as_uint(__uint_as_float(v[d]) * f);
+        }
+      }
+      return v;
+    };
+    int i = E * (int)threadIdx.x;
+    for (; i + (U - 1) * 256 * E + E <= n; i += U * 256 * E) {
+      u32x4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const u32x4_any*>(x + i + u * 256 * E);
+#pragma unroll
+      for (int u = 0; u < U; ++u) *reinterpret_cast<u32x4_any*>(x + i + u * 256 * E) = times(v[u]);
+    }
+    for (; i < n; i += 256 * E) {
+      if (i + E <= n) {
+        *reinterpret_cast<u32x4_any*>(x + i) = times(*reinterpret_cast<const u32x4_any*>(x + i));
+        continue;
+      }
+      for (int e = 0; i + e < n; ++e) {
+        if constexpr (BF16) x[i + e] = __builtin_bit_cast(u16, (__bf16)(__uint_as_float((uint32_t)x[i + e] << 16) * f));
+        else x[i + e] *= f;
+      }
+    }
+  };
+  if (t.bf16) go(static_cast<u16*>(t.data) + at, std::true_type{});
+  else go(static_cast<float*>(t.data) + at, std::false_type{});
+}
+
+// Values a workgroup takes: enough workgroups to fill the chip, then up to 64 Ki
+// values each, so that few sums are left to add.
+int chunk_of(const tilec_grad* grads, int32_t count) {
+  int64_t n = 0;
+  for (int i = 0; i < count; ++i) n += grads[i].n;
+  const int64_t each = n / (8 * (int64_t)device_cus());
+  return kUnit * (int)std::max<int64_t>(1, std::min<int64_t>(16, each / kUnit));
+}
+
+int64_t chunks_of(const tilec_grad* grads, int32_t count, int chunk) {
+  int64_t n = 0;
+  for (int i = 0; i < count; ++i) n += cdiv(grads[i].n, chunk);
+  return n;
+}
+
+// f(workgroups) for the tensors in groups of up to kMaxTensors, with at most 2^22
+// workgroups each; a.base counts them.
+template <typename F>
+hipError_t in_groups(GradArgs& a, const tilec_grad* grads, int32_t count, F f) {
+  constexpr int64_t kMaxBlocks = int64_t(1) << 22;
+  int64_t blocks = 0;
+  a.count = 0, a.base = 0;
+  auto flush = [&]() -> hipError_t {
+    if (a.count == 0) return hipSuccess;
+    f((unsigned)blocks);
+    a.base += blocks;
+    a.count = 0, blocks = 0;
+    return hipGetLastError();
+  };
+  for (int i = 0; i < count; ++i) {
+    const int64_t esz = grads[i].dtype == TILEC_BF16 ? 2 : 4;
+    for (int64_t at = 0; at < grads[i].n; at += kMaxBlocks * a.chunk) {
+      const int64_t n = std::min(grads[i].n - at, kMaxBlocks * a.chunk), need = cdiv(n, a.chunk);
+      if (a.count == kMaxTensors || blocks + need > kMaxBlocks) {
+        const hipError_t e = flush();
+        if (e != hipSuccess) return e;
+      }
+      a.t[a.count++] = {static_cast<char*>(grads[i].data) + at * esz, n, (int)blocks, esz == 2};
+      blocks += need;
+    }
+  }
+  return flush();
+}
+
+int check_grads(const char* what, const tilec_grad* grads, int32_t count) {
+  if (count < 0 || (count > 0 && grads == nullptr))
+    return fail(TILEC_ERR_VALUE, "tilec: %s: no tensors (count %d)", what, count);
+  for (int i = 0; i < count; ++i) {
+    if (grads[i].dtype != TILEC_F32 && grads[i].dtype != TILEC_BF16)
+      return fail(TILEC_ERR_TYPE, "tilec: %s: tensor %d: unsupported dtype code %d (use float32 or bfloat16)", what, i,
+                  grads[i].dtype);
+    if (grads[i].n < 0 || (grads[i].n > 0 && grads[i].data == nullptr))
+      return fail(TILEC_ERR_VALUE, "tilec: %s: tensor %d has a NULL pointer or %lld elements", what, i,
+                  (long long)grads[i].n);
+  }
+  return TILEC_OK;
+}
+
+}  // namespace
+
+}  // namespace tilec
+
+using namespace tilec;
+
+extern "C" {
+
+size_t tilec_grad_norm_workspace_bytes(const tilec_grad* grads, int32_t count) {
+  if (check_grads("grad_norm", grads, count) != TILEC_OK) return 0;
+  return (size_t)chunks_of(grads, count, chunk_of(grads, count)) * sizeof(double);
+}
+
+int tilec_grad_norm(const tilec_grad* grads, int32_t count, const float* grad_scale, double max_norm, float* norm,
+                    float* scale, void* workspace, size_t workspace_bytes, void* counter, size_t counter_bytes,
+                    void* stream) {
+  clear_error();
+  const int rc = check_grads("grad_norm", grads, count);
+  if (rc != TILEC_OK) return rc;
+  if (norm == nullptr) return fail(TILEC_ERR_VALUE, "tilec: grad_norm: norm is NULL");
+  if (max_norm != max_norm) return fail(TILEC_ERR_VALUE, "tilec: grad_norm: max_norm is not a number");
+  GradArgs a{};
+  a.chunk = chunk_of(grads, count);
+  a.total = chunks_of(grads, count, a.chunk);
+  const size_t need = (size_t)a.total * sizeof(double);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || counter == nullptr || counter_bytes < sizeof(unsigned)))
+    return fail(TILEC_ERR_WORKSPACE, "tilec: grad_norm needs %zu workspace bytes and 4 bytes of counter (got %zu and %zu)",
+                need, workspace == nullptr ? (size_t)0 : workspace_bytes, counter == nullptr ? (size_t)0 : counter_bytes);
+  a.partial = static_cast<double*>(workspace), a.counter = static_cast<unsigned*>(counter);
+  a.grad_scale = grad_scale, a.norm = norm, a.scale = scale, a.max_norm = max_norm < 0 ? -1.f : (float)max_norm;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  hipError_t e;
+  if (a.total == 0) {  // the norm of nothing
+    hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(256), 0, st, a);
+    e = hipGetLastError();
+  } else {
+    e = in_groups(a, grads, count,
+                  [&](unsigned blocks) { hipLaunchKernelGGL(grad_norm_kernel, dim3(blocks), dim3(256), 0, st, a); });
+  }
+  if (e != hipSuccess) return fail(TILEC_ERR_HIP, "tilec: launching grad_norm failed: %s", hipGetErrorString(e));
+  return TILEC_OK;
+}
+
+int tilec_scale_grads(const tilec_grad* grads, int32_t count, const float* scale, void* stream) {
+  clear_error();
+  const int rc = check_grads("scale_grads", grads, count);
+  if (rc != TILEC_OK) return rc;
+  if (scale == nullptr) return fail(TILEC_ERR_VALUE, "tilec: scale_grads: scale is NULL");
+  GradArgs a{};
+  a.chunk = chunk_of(grads, count);
+  a.scale_in = scale;
+  const hipError_t e = in_groups(a, grads, count, [&](unsigned blocks) {
+    hipLaunchKernelGGL(grad_scale_kernel, dim3(blocks), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+  });
+  if (e != hipSuccess) return fail(TILEC_ERR_HIP, "tilec: launching scale_grads failed: %s", hipGetErrorString(e));
+  return TILEC_OK;
+}
+
+}  // extern "C"

@@ -21,18 +21,34 @@
 // check their arguments, allocate the outputs and enqueue the kernels on `stream`
 // (the handle of the tensors' device's current stream): one row of 4096 then
 // costs 6 us a call instead of 10.
+//
+//   rms_norm(x, weight, residual, eps, dtype, stream) -> (y, h, rstd)
+//   rms_norm_backward(dy, h, rstd, weight, dh, weight_grad, stream) -> (dx, dweight)
+//   quantize_fp8(x, block, dtype, stream) -> (codes, scales)
+//   dequantize_fp8(q, dtype, stream) -> values
+//   linear_fp8(x, weight, dtype, stream) -> out
+//
+// do the same; 8-bit operands are (codes, scales) pairs.
+//
+//   grad_norm(grads, max_norm, grad_scale, stream_of, counters_for) -> (norm, scale)
+//   clip_grads(grads, max_norm, grad_scale, stream_of, counters_for) -> norm
+//
+// read lists as adamw_step does; counters_for(device, stream, bytes) gives the
+// zeroed counter that the norm's kernel leaves zero.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/Device.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
 #include <algorithm>
+#include <cmath>
 #include <memory>
 #include <string>
 #include <vector>
@@ -241,14 +257,15 @@ double number(PyObject* o) {
   return v;
 }
 
-PyObject* three(const at::Tensor& a, const at::Tensor& b, const at::Tensor& c) {
-  PyObject* t = PyTuple_New(3);
+// A tuple of tensors, None for those that are not defined.
+PyObject* tuple(std::initializer_list<at::Tensor> all) {
+  PyObject* t = PyTuple_New((Py_ssize_t)all.size());
   if (t == nullptr) throw python_error();
-  const at::Tensor* all[3] = {&a, &b, &c};
-  for (int i = 0; i < 3; ++i) {
-    PyObject* o = all[i]->defined() ? THPVariable_Wrap(*all[i]) : nullptr;
+  Py_ssize_t i = 0;
+  for (const at::Tensor& x : all) {
+    PyObject* o = x.defined() ? THPVariable_Wrap(x) : nullptr;
     if (o == nullptr) Py_INCREF(o = Py_None);
-    PyTuple_SET_ITEM(t, i, o);
+    PyTuple_SET_ITEM(t, i++, o);
   }
   return t;
 }
@@ -402,7 +419,7 @@ PyObject* build_norm(PyObject* const* args) {
   check(tilec_layer_norm(r.t.const_data_ptr(), data(p.weight), data(p.bias), y.data_ptr(),
                          static_cast<float*>(mean.data_ptr()), static_cast<float*>(rstd.data_ptr()), r.R, r.D, r.ld,
                          r.D, x_code, code(y), p.code, (float)eps, stream_of(args[5])));
-  return three(y, mean, rstd);
+  return tuple({y, mean, rstd});
 }
 
 PyObject* build_norm_backward(PyObject* const* args) {
@@ -437,10 +454,295 @@ PyObject* build_norm_backward(PyObject* const* args) {
         r.D, d.ld, r.ld, r.D, x_code, y_code, p.code, need > 0 ? scratch.data_ptr() : nullptr, need,
         stream_of(args[6])));
   }
-  return three(dx, dw, db);
+  return tuple({dx, dw, db});
+}
+
+// The type that an argument names; `other` where it is None.
+at::ScalarType dtype(PyObject* o, at::ScalarType other) {
+  if (o == Py_None) return other;
+  if (!THPDtype_Check(o)) bad_type("dtype is no torch.dtype");
+  return reinterpret_cast<THPDtype*>(o)->scalar_type;
+}
+
+bool is_wide(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16; }
+bool is_fp8(at::ScalarType t) { return t == at::kFloat8_e4m3fn || t == at::kFloat8_e5m2; }
+
+int32_t code_of(at::ScalarType t) {
+  return t == at::kFloat ? TILEC_F32 : t == at::kBFloat16 ? TILEC_BF16 : t == at::kFloat8_e4m3fn ? TILEC_F8E4M3 : TILEC_F8E5M2;
+}
+
+constexpr int64_t kGroup = 128;  // values of a row under one scale of an 8-bit operand
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// New codes [R, C], rows at multiples of 16 bytes, and scales of blocks of `block` rows.
+struct NewFp8 {
+  at::Tensor codes, scales;
+  int64_t ld;
+  NewFp8(int64_t R, int64_t C, int64_t block, at::ScalarType type, const at::TensorOptions& options) : ld(cdiv(C, 16) * 16) {
+    codes = at::empty({R, ld}, options.dtype(type));
+    if (ld != C) codes = codes.narrow(1, 0, C);
+    scales = at::empty({cdiv(R, block), cdiv(C, kGroup)}, options.dtype(at::kFloat));
+  }
+};
+
+PyObject* build_rms(PyObject* const* args) {
+  const at::Tensor& x = tensor("x", args[0]);
+  OneGpu gpu;
+  const int32_t x_code = gpu.code("x", x);
+  const Rows r("x", x);
+  const Params p(gpu, args[1], Py_None, r.D);
+  const bool added = args[2] != Py_None;
+  const at::Tensor& res_in = added ? tensor("residual", args[2]) : x;
+  const int32_t r_code = gpu.code("residual", res_in);
+  if (added && res_in.sizes() != x.sizes()) bad_value("residual has shape " + shape(res_in) + ", x " + shape(x));
+  const Rows res("residual", res_in);
+  const double eps = number(args[3]);
+  const at::ScalarType type = dtype(args[4], x.scalar_type());
+  if (!is_wide(type) && !is_fp8(type))
+    bad_type(std::string("unsupported dtype ") + toString(type) +
+             " (use float32, bfloat16, float8_e4m3fn or float8_e5m2)");
+  const c10::DeviceGuard guard(x.device());
+  at::Tensor y, y_scale;
+  int64_t ldy = r.D;
+  if (is_fp8(type)) {
+    const NewFp8 q(r.R, r.D, 1, type, x.options());
+    y = q.codes, y_scale = q.scales, ldy = q.ld;
+  } else {
+    y = at::empty(x.sizes(), x.options().dtype(type));
+  }
+  const at::Tensor h = added ? at::empty(x.sizes(), res_in.options()) : x;
+  const at::Tensor rstd = at::empty({r.R}, x.options().dtype(at::kFloat));
+  check(tilec_rms_norm(r.t.const_data_ptr(), added ? res.t.const_data_ptr() : nullptr, data(p.weight), y.data_ptr(),
+                       y_scale.defined() ? static_cast<float*>(y_scale.data_ptr()) : nullptr,
+                       added ? h.data_ptr() : nullptr, static_cast<float*>(rstd.data_ptr()), r.R, r.D, r.ld, res.ld, ldy,
+                       r.D, x_code, r_code, code_of(type), p.code, (float)eps, stream_of(args[5])));
+  if (!y_scale.defined()) return tuple({y, h, rstd});
+  PyObject* t = PyTuple_New(3);
+  if (t == nullptr) throw python_error();
+  THPObjectPtr held(t);
+  PyTuple_SET_ITEM(t, 0, tuple({y, y_scale}));
+  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(h));
+  PyTuple_SET_ITEM(t, 2, THPVariable_Wrap(rstd));
+  return held.release();
+}
+
+PyObject* build_rms_backward(PyObject* const* args) {
+  const at::Tensor &dy = tensor("dy", args[0]), &h = tensor("h", args[1]), &rstd_in = tensor("rstd", args[2]);
+  OneGpu gpu;
+  const int32_t dy_code = gpu.code("dy", dy), h_code = gpu.code("h", h);
+  if (dy.sizes() != h.sizes()) bad_value("dy has shape " + shape(dy) + ", h " + shape(h));
+  const Rows d("dy", dy), r("h", h);
+  gpu.code("rstd", rstd_in);
+  if (rstd_in.scalar_type() != at::kFloat) bad_type("rstd is float32");
+  const at::Tensor rstd = vector("rstd", rstd_in, r.R);
+  const Params p(gpu, args[3], Py_None, r.D);
+  const bool added = args[4] != Py_None;
+  const at::Tensor& dh_in = added ? tensor("dh", args[4]) : dy;
+  const int32_t dh_code = gpu.code("dh", dh_in);
+  if (dh_in.sizes() != h.sizes()) bad_value("dh has shape " + shape(dh_in) + ", h " + shape(h));
+  const Rows dh("dh", dh_in);
+  const int sums = PyObject_IsTrue(args[5]);
+  if (sums < 0) throw python_error();
+  const c10::DeviceGuard guard(dy.device());
+  const at::Tensor dx = at::empty(dh_in.sizes(), dh_in.options());
+  at::Tensor dw, scratch;
+  if (sums) dw = at::empty({r.D}, dy.options().dtype(at::kFloat));
+  if (sums || r.R > 0) {
+    const size_t need = tilec_rms_norm_backward_workspace_bytes(r.R, r.D, h_code);
+    if (need > 0) scratch = at::empty({(int64_t)need}, dy.options().dtype(at::kByte));
+    check(tilec_rms_norm_backward(
+        d.t.const_data_ptr(), r.t.const_data_ptr(), static_cast<const float*>(rstd.const_data_ptr()), data(p.weight),
+        added ? dh.t.const_data_ptr() : nullptr, dx.data_ptr(), sums ? static_cast<float*>(dw.data_ptr()) : nullptr, r.R,
+        r.D, d.ld, r.ld, dh.ld, r.D, dy_code, h_code, dh_code, p.code, need > 0 ? scratch.data_ptr() : nullptr, need,
+        stream_of(args[6])));
+  }
+  return tuple({dx, dw});
+}
+
+// A (codes, scales) pair: codes whose rows are contiguous (copied if they are
+// not), contiguous scales of blocks of 1 or 128 rows.
+struct Fp8 {
+  at::Tensor codes, scales;
+  int64_t R, C, ld;
+  int32_t code, block;
+  Fp8(OneGpu& gpu, const char* name, PyObject* o) {
+    const std::string of(name);
+    if (!PyTuple_Check(o) && !PyList_Check(o)) bad_type(of + " is no pair (codes, scales)");
+    const List both(o);
+    if (both.size() != 2) bad_value(of + " is no pair (codes, scales)");
+    const at::Tensor &c = tensor(name, both[0]), &s = tensor(name, both[1]);
+    if (!c.is_cuda() || !s.is_cuda())
+      bad_type("needs tensors on a ROCm GPU (" + of + " is on " + (c.is_cuda() ? s : c).device().str() + ")");
+    if (gpu.device < 0) gpu.device = c.get_device();
+    if (c.get_device() != gpu.device || s.get_device() != gpu.device)
+      bad_type("needs all tensors on one GPU (" + of + " is on another)");
+    if (c.layout() != at::kStrided || s.layout() != at::kStrided) bad_type(of + " is not a dense tensor");
+    if (!is_fp8(c.scalar_type()) || s.scalar_type() != at::kFloat)
+      bad_type(of + " has codes of dtype " + toString(c.scalar_type()) + " and scales of dtype " + toString(s.scalar_type()) +
+               " (use float8_e4m3fn or float8_e5m2, and float32)");
+    if (c.dim() != 2) bad_value("expected 2-D codes of " + of + ", got shape " + shape(c));
+    R = c.size(0), C = c.size(1);
+    const int64_t G = cdiv(C, kGroup);
+    if (s.dim() != 2 || s.size(1) != G || (s.size(0) != R && s.size(0) != cdiv(R, kGroup)))
+      bad_value(of + " has codes of shape " + shape(c) + " and scales of shape " + shape(s) + ", expected (" +
+                std::to_string(R) + ", " + std::to_string(G) + ") or (" + std::to_string(cdiv(R, kGroup)) + ", " +
+                std::to_string(G) + ")");
+    block = s.size(0) == R ? 1 : kGroup;
+    codes = (C > 1 && c.stride(1) != 1) || (R > 1 && c.stride(0) < C) ? c.contiguous() : c;
+    scales = s.contiguous();
+    ld = R > 1 ? codes.stride(0) : C;
+    code = code_of(c.scalar_type());
+  }
+};
+
+PyObject* build_quantize(PyObject* const* args) {
+  const at::Tensor& x = tensor("x", args[0]);
+  OneGpu gpu;
+  const int32_t x_code = gpu.code("x", x);
+  if (x.dim() != 2) bad_value("expected a 2-D x, got shape " + shape(x));
+  long long b[2] = {0, 0};
+  if (!PyTuple_Check(args[1]) || !PyArg_ParseTuple(args[1], "LL", &b[0], &b[1])) {
+    PyErr_Clear();
+    bad_value("block is (1, 128) or (128, 128)");
+  }
+  if ((b[0] != 1 && b[0] != kGroup) || b[1] != kGroup) bad_value("block is (1, 128) or (128, 128)");
+  const at::ScalarType type = dtype(args[2], at::kFloat8_e4m3fn);
+  if (!is_fp8(type)) bad_type(std::string("unsupported dtype ") + toString(type) + " (use float8_e4m3fn or float8_e5m2)");
+  const int64_t R = x.size(0), C = x.size(1);
+  at::Tensor t = x;
+  const bool rows = (C <= 1 || x.stride(1) == 1) && (R <= 1 || x.stride(0) >= C);
+  const bool cols = !rows && (R <= 1 || x.stride(0) == 1) && (C <= 1 || x.stride(1) >= R);
+  const c10::DeviceGuard guard(x.device());
+  if (!rows && !cols) t = x.contiguous();
+  const NewFp8 q(R, C, b[0], type, x.options());
+  const int64_t ld = cols ? (C > 1 ? t.stride(1) : R) : (R > 1 ? t.stride(0) : C);
+  check(tilec_quantize_fp8(t.const_data_ptr(), q.codes.data_ptr(), static_cast<float*>(q.scales.data_ptr()), R, C, ld,
+                           q.ld, cols ? TILEC_X1_COL_MAJOR : 0, x_code, code_of(type), (int32_t)b[0], stream_of(args[3])));
+  return tuple({q.codes, q.scales});
+}
+
+PyObject* build_dequantize(PyObject* const* args) {
+  OneGpu gpu;
+  const Fp8 q(gpu, "q", args[0]);
+  const at::ScalarType type = dtype(args[1], at::kFloat);
+  if (!is_wide(type)) bad_type(std::string("unsupported dtype ") + toString(type) + " (use float32 or bfloat16)");
+  const c10::DeviceGuard guard(q.codes.device());
+  const at::Tensor out = at::empty({q.R, q.C}, q.scales.options().dtype(type));
+  check(tilec_dequantize_fp8(q.codes.const_data_ptr(), static_cast<const float*>(q.scales.const_data_ptr()), out.data_ptr(),
+                             q.R, q.C, q.ld, q.C, q.code, code_of(type), q.block, stream_of(args[2])));
+  return THPVariable_Wrap(out);
+}
+
+PyObject* build_linear(PyObject* const* args) {
+  OneGpu gpu;
+  const Fp8 x(gpu, "x", args[0]), w(gpu, "weight", args[1]);
+  if (x.C != w.C)
+    bad_value("expected x [M, K] and weight [N, K], got shapes " + shape(x.codes) + " and " + shape(w.codes));
+  const at::ScalarType type = dtype(args[2], at::kFloat);
+  if (!is_wide(type)) bad_type(std::string("unsupported dtype ") + toString(type) + " (use float32 or bfloat16)");
+  const c10::DeviceGuard guard(x.codes.device());
+  const at::Tensor out = at::empty({x.R, w.R}, x.scales.options().dtype(type));
+  const void *xp = x.codes.const_data_ptr(), *wp = w.codes.const_data_ptr();
+  const size_t need = tilec_linear_fp8_workspace_bytes(xp, wp, x.R, w.R, x.C, x.ld, w.ld, x.code, w.code, code_of(type),
+                                                       x.block, w.block);
+  at::Tensor scratch;
+  if (need > 0) scratch = at::empty({(int64_t)need}, x.scales.options().dtype(at::kByte));
+  check(tilec_linear_fp8(xp, static_cast<const float*>(x.scales.const_data_ptr()), wp,
+                         static_cast<const float*>(w.scales.const_data_ptr()), out.data_ptr(), x.R, w.R, x.C, x.ld, w.ld,
+                         w.R, x.code, w.code, code_of(type), x.block, w.block, need > 0 ? scratch.data_ptr() : nullptr, need,
+                         stream_of(args[3])));
+  return THPVariable_Wrap(out);
+}
+
+// The gradients of a list, None for those that have none.  Values whose order in
+// memory is another than their index's (a transposed gradient) are as good.
+struct Grads {
+  std::vector<tilec_grad> table;
+  std::vector<at::Tensor> kept;
+  Reader r;
+  Written w;
+  at::Device device = at::kCPU;
+  Grads(PyObject* list, bool write) {
+    const List grads(list);
+    table.reserve(grads.size());
+    for (Py_ssize_t i = 0; i < grads.size(); ++i) {
+      if (grads[i] == Py_None) continue;
+      const at::Tensor* g = &r.read("grads", grads[i], -1, at::kFloat, at::kBFloat16, false);
+      device = g->device();
+      if (!g->is_non_overlapping_and_dense()) {
+        if (write) bad_value("grads has a tensor whose values do not lie side by side");
+        kept.push_back(g->contiguous());
+        g = &kept.back();
+      }
+      table.push_back({write ? w.add(*g) : const_cast<void*>(g->const_data_ptr()), g->numel(), code(*g)});
+    }
+    if (r.device < 0) bad_value("no gradients");
+    if (write) refuse_shared();
+  }
+  // Memory that is multiplied twice would be a race between workgroups.
+  void refuse_shared() const {
+    std::vector<std::pair<uintptr_t, uintptr_t>> ranges;
+    ranges.reserve(table.size());
+    for (const tilec_grad& g : table) {
+      const uintptr_t lo = reinterpret_cast<uintptr_t>(g.data);
+      if (g.n > 0) ranges.emplace_back(lo, lo + (uintptr_t)g.n * (g.dtype == TILEC_BF16 ? 2 : 4));
+    }
+    std::sort(ranges.begin(), ranges.end());
+    for (size_t i = 1; i < ranges.size(); ++i)
+      if (ranges[i].first < ranges[i - 1].second) bad_value("two grads share their memory");
+  }
+};
+
+// Enqueues the norm; {norm, scale}.  args: grads, max_norm, grad_scale, stream_of, counters_for.
+std::pair<at::Tensor, at::Tensor> norm_of(Grads& g, PyObject* const* args, void*& stream) {
+  const double max_norm = args[1] == Py_None ? -1. : number(args[1]);
+  if (args[1] != Py_None && !(max_norm >= 0)) bad_value("max_norm is negative or not a number");
+  const float* grad_scale = nullptr;
+  if (args[2] != Py_None) {
+    const at::Tensor& t = g.r.read("grad_scale", args[2], -1, at::kFloat, at::kFloat, false);
+    if (t.numel() != 1) bad_value("grad_scale has shape " + shape(t) + ", expected one value");
+    grad_scale = static_cast<const float*>(t.const_data_ptr());
+  }
+  THPObjectPtr handle(PyObject_CallFunction(args[3], "L", (long long)g.r.device));
+  if (!handle) throw python_error();
+  stream = stream_of(handle.get());
+  THPObjectPtr where(THPDevice_New(g.device));
+  THPObjectPtr held(PyObject_CallFunction(args[4], "OOi", where.get(), handle.get(), 4));
+  if (!held) throw python_error();
+  const at::Tensor counter = tensor("counters", held.get());
+  const auto options = at::TensorOptions().device(g.device);
+  const at::Tensor both = at::empty({2}, options.dtype(at::kFloat));
+  float* const out = static_cast<float*>(both.data_ptr());
+  const size_t need = tilec_grad_norm_workspace_bytes(g.table.data(), (int32_t)g.table.size());
+  at::Tensor scratch;
+  if (need > 0) scratch = at::empty({(int64_t)need}, options.dtype(at::kByte));
+  check(tilec_grad_norm(g.table.data(), (int32_t)g.table.size(), grad_scale, max_norm, out, out + 1,
+                        need > 0 ? scratch.data_ptr() : nullptr, need, counter.data_ptr(), (size_t)counter.numel(), stream));
+  return {both.select(0, 0), both.select(0, 1)};
+}
+
+PyObject* build_grad_norm(PyObject* const* args) {
+  Grads g(args[0], false);
+  const c10::DeviceGuard guard(g.device);
+  void* stream;
+  const auto got = norm_of(g, args, stream);
+  return tuple({got.first, got.second});
+}
+
+PyObject* build_clip(PyObject* const* args) {
+  Grads g(args[0], true);
+  const c10::DeviceGuard guard(g.device);
+  void* stream;
+  const auto got = norm_of(g, args, stream);
+  check(tilec_scale_grads(g.table.data(), (int32_t)g.table.size(), static_cast<const float*>(got.second.const_data_ptr()),
+                          stream));
+  g.w.bump();
+  return THPVariable_Wrap(got.first);
 }
 
 constexpr char kAdamw[] = "adamw_step", kValues[] = "adamw_values", kNorm[] = "layer_norm", kNormBackward[] = "layer_norm_backward";
+constexpr char kRms[] = "rms_norm", kRmsBackward[] = "rms_norm_backward", kQuantize[] = "quantize_fp8",
+               kDequantize[] = "dequantize_fp8", kLinear[] = "linear_fp8", kGradNorm[] = "grad_norm", kClip[] = "clip_grads";
 
 template <PyObject* (*BUILD)(PyObject* const*), int ARGS, const char* NAME>
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t count) {
@@ -473,6 +775,19 @@ PyMethodDef kMethods[] = {
      "layer_norm(x, weight, bias, eps, dtype, stream) -> (y, mean, rstd)"},
     {"layer_norm_backward", function<build_norm_backward, 7, kNormBackward>(), METH_FASTCALL,
      "layer_norm_backward(dy, x, mean, rstd, weight, param_grads, stream) -> (dx, dweight, dbias)"},
+    {"rms_norm", function<build_rms, 6, kRms>(), METH_FASTCALL,
+     "rms_norm(x, weight, residual, eps, dtype, stream) -> (y, h, rstd)"},
+    {"rms_norm_backward", function<build_rms_backward, 7, kRmsBackward>(), METH_FASTCALL,
+     "rms_norm_backward(dy, h, rstd, weight, dh, weight_grad, stream) -> (dx, dweight)"},
+    {"quantize_fp8", function<build_quantize, 4, kQuantize>(), METH_FASTCALL,
+     "quantize_fp8(x, block, dtype, stream) -> (codes, scales)"},
+    {"dequantize_fp8", function<build_dequantize, 3, kDequantize>(), METH_FASTCALL,
+     "dequantize_fp8(q, dtype, stream) -> values"},
+    {"linear_fp8", function<build_linear, 4, kLinear>(), METH_FASTCALL, "linear_fp8(x, weight, dtype, stream) -> out"},
+    {"grad_norm", function<build_grad_norm, 5, kGradNorm>(), METH_FASTCALL,
+     "grad_norm(grads, max_norm, grad_scale, stream_of, counters_for) -> (norm, scale)"},
+    {"clip_grads", function<build_clip, 5, kClip>(), METH_FASTCALL,
+     "clip_grads(grads, max_norm, grad_scale, stream_of, counters_for) -> norm"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

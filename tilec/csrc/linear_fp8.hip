@@ -1,0 +1,160 @@
+// tilec_linear_fp8: the choice of a kernel of linear_fp8.h, operands whose rows do
+// not begin at multiples of 16 bytes, and the sums of split groups.
+#include <algorithm>
+
+#include "abi.h"
+#include "linear_fp8.h"
+
+namespace tilec {
+
+namespace {
+
+typedef unsigned short u16;
+
+struct Plan {
+  int tile;            // -1: the streaming kernel
+  int splits, steps;   // groups of K a split
+  bool copy_x, copy_w;
+  int64_t padded;      // row stride of a copied operand
+  size_t x_bytes, w_bytes, partial_bytes;
+  size_t bytes() const { return x_bytes + w_bytes + partial_bytes; }
+};
+
+size_t round16(int64_t n) { return (size_t)(n + 15) / 16 * 16; }
+
+Plan plan_of(const void* x, const void* w, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, bool f8) {
+  Plan p{};
+  auto aligned = [](const void* q, int64_t rows, int64_t ld) {
+    return reinterpret_cast<uintptr_t>(q) % 16 == 0 && (rows <= 1 || (ld % 16 == 0 && ld <= (int64_t(1) << 22)));
+  };
+  p.copy_x = !aligned(x, M, ldx), p.copy_w = !aligned(w, N, ldw);
+  p.padded = (int64_t)round16(K);
+  p.x_bytes = p.copy_x ? (size_t)(M * p.padded) : 0;
+  p.w_bytes = p.copy_w ? (size_t)(N * p.padded) : 0;
+  const int64_t G = cdiv(K, kGroup), cus = device_cus();
+  p.splits = 1, p.steps = (int)G;
+  if (M <= kFp8StreamRows) {
+    p.tile = -1;
+    return p;
+  }
+  auto tiles = [&](int t) { return cdiv(M, kFp8Tiles[t].bm) * cdiv(N, f8 ? kFp8Tiles[t].bn : kFp8Tiles[t].bn_exact); };
+  p.tile = tiles(0) >= cus ? 0 : tiles(1) >= cus / 2 ? 1 : 2;
+  const int64_t n = tiles(p.tile);
+  int64_t s = std::max<int64_t>(1, std::min(cus / std::max<int64_t>(n, 1), G / 4));
+  if (s > 1) {
+    p.steps = (int)cdiv(G, s);
+    p.splits = (int)cdiv(G, p.steps);
+  }
+  if (p.splits > 1) p.partial_bytes = round16((int64_t)p.splits * M * N * 4);
+  return p;
+}
+
+// out = the sum of the splits' partial sums, in order: a float4 a thread.
+template <typename TO>
+__global__ __launch_bounds__(256) void fp8_join_kernel(const float* __restrict__ partial, TO* __restrict__ out, int64_t n,
+                                                       int64_t ldo, int N, int splits) {
+  for (int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x); i < n; i += 4 * 256 * (int64_t)gridDim.x) {
+    const int live = (int)min((int64_t)4, n - i);
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    typedef f32x4 __attribute__((aligned(4))) f32x4_any;
+    for (int k = 0; k < splits; ++k) {
+      const float* p = partial + k * n + i;
+      if (live == 4) {
+        const f32x4 v = *reinterpret_cast<const f32x4_any*>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += v[e];
+      } else {
+        for (int e = 0; e < live; ++e) s[e] += p[e];
+      }
+    }
+    for (int e = 0; e < live; ++e) {
+      const int64_t m = (i + e) / N, at = m * ldo + (i + e - m * N);
+      if constexpr (sizeof(TO) == 4) out[at] = s[e];
+      else out[at] = __builtin_bit_cast(u16, (__bf16)s[e]);
+    }
+  }
+}
+
+int check_linear(int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int32_t x_dtype, int32_t w_dtype,
+                 int32_t out_dtype, int32_t x_block, int32_t w_block) {
+  if (!is_fp8(x_dtype) || !is_fp8(w_dtype))
+    return fail(TILEC_ERR_TYPE, "tilec: linear_fp8: unsupported dtype codes %d, %d of x and weight (use an 8-bit type)",
+                x_dtype, w_dtype);
+  if (out_dtype != TILEC_F32 && out_dtype != TILEC_BF16)
+    return fail(TILEC_ERR_TYPE, "tilec: linear_fp8: unsupported dtype code %d of out (use float32 or bfloat16)", out_dtype);
+  if (M < 0 || N < 0 || K < 0 || M > kMaxDim || N > kMaxDim || K > (int64_t(1) << 22))
+    return fail(TILEC_ERR_VALUE, "tilec: linear_fp8: bad shape M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
+  if ((M > 1 && (ldx < K || ldx > (int64_t(1) << 40))) || (N > 1 && (ldw < K || ldw > (int64_t(1) << 40))))
+    return fail(TILEC_ERR_VALUE, "tilec: linear_fp8: bad row strides ldx=%lld ldw=%lld for K=%lld", (long long)ldx,
+                (long long)ldw, (long long)K);
+  if ((x_block != 1 && x_block != kGroup) || (w_block != 1 && w_block != kGroup))
+    return fail(TILEC_ERR_VALUE, "tilec: linear_fp8: blocks have 1 or 128 rows (got %d and %d)", x_block, w_block);
+  return TILEC_OK;
+}
+
+}  // namespace
+
+}  // namespace tilec
+
+using namespace tilec;
+
+extern "C" {
+
+size_t tilec_linear_fp8_workspace_bytes(const void* x, const void* weight, int64_t M, int64_t N, int64_t K, int64_t ldx,
+                                        int64_t ldw, int32_t x_dtype, int32_t w_dtype, int32_t out_dtype,
+                                        int32_t x_block, int32_t w_block) {
+  if (check_linear(M, N, K, ldx, ldw, x_dtype, w_dtype, out_dtype, x_block, w_block) != TILEC_OK || M == 0 || N == 0 ||
+      K == 0)
+    return 0;
+  return plan_of(x, weight, M, N, K, ldx, ldw, out_dtype == TILEC_BF16).bytes();
+}
+
+int tilec_linear_fp8(const void* x, const float* x_scale, const void* weight, const float* w_scale, void* out,
+                     int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldo, int32_t x_dtype,
+                     int32_t w_dtype, int32_t out_dtype, int32_t x_block, int32_t w_block, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  clear_error();
+  const int rc = check_linear(M, N, K, ldx, ldw, x_dtype, w_dtype, out_dtype, x_block, w_block);
+  if (rc != TILEC_OK) return rc;
+  if (M == 0 || N == 0) return TILEC_OK;
+  if (M > 1 && (ldo < N || ldo > (int64_t(1) << 40)))
+    return fail(TILEC_ERR_VALUE, "tilec: linear_fp8: bad row stride ldo=%lld for N=%lld", (long long)ldo, (long long)N);
+  if (out == nullptr || (K > 0 && (x == nullptr || weight == nullptr || x_scale == nullptr || w_scale == nullptr)))
+    return fail(TILEC_ERR_VALUE, "tilec: linear_fp8: a pointer is NULL");
+  const bool f8 = out_dtype == TILEC_BF16;
+  const Plan p = K > 0 ? plan_of(x, weight, M, N, K, ldx, ldw, f8) : Plan{1, 1, 0, false, false, 0, 0, 0, 0};
+  if (p.bytes() > 0 && (workspace == nullptr || workspace_bytes < p.bytes()))
+    return fail(TILEC_ERR_WORKSPACE, "tilec: linear_fp8 needs %zu workspace bytes (got %zu)", p.bytes(),
+                workspace == nullptr ? (size_t)0 : workspace_bytes);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  char* const ws = static_cast<char*>(workspace);
+  hipError_t e = hipSuccess;
+  if (p.copy_x || p.copy_w) {
+    e = pad_copy<1>(x, ws, M, K, ldx, p.copy_x ? M : 0, p.padded, weight, ws + p.x_bytes, N, K, ldw,
+                    p.copy_w ? N : 0, p.padded, st);
+    if (e != hipSuccess) return fail(TILEC_ERR_HIP, "tilec: linear_fp8: copying an operand failed: %s", hipGetErrorString(e));
+  }
+  Fp8Args a{};
+  a.x = p.copy_x ? reinterpret_cast<unsigned char*>(ws) : static_cast<const unsigned char*>(x);
+  a.w = p.copy_w ? reinterpret_cast<unsigned char*>(ws + p.x_bytes) : static_cast<const unsigned char*>(weight);
+  a.sx = x_scale, a.sw = w_scale, a.out = out;
+  a.partial = reinterpret_cast<float*>(ws + p.x_bytes + p.w_bytes);
+  // (One row has no stride: one that is not a multiple of 16 is not used.)
+  a.ldx = p.copy_x ? p.padded : M > 1 ? ldx : 0, a.ldw = p.copy_w ? p.padded : N > 1 ? ldw : 0, a.ldo = M > 1 ? ldo : N;
+  a.M = (int)M, a.N = (int)N, a.K = (int)K, a.G = (int)cdiv(K, kGroup);
+  a.xshift = x_block == 1 ? 0 : 7, a.wshift = w_block == 1 ? 0 : 7;
+  a.group_m = 8, a.xcds = device_xcds(), a.split_steps = p.steps;
+  const int fx = x_dtype == TILEC_F8E5M2, fw = w_dtype == TILEC_F8E5M2;
+  e = fx ? (fw ? launch_fp8<1, 1>(a, f8, p.tile, p.splits, st) : launch_fp8<1, 0>(a, f8, p.tile, p.splits, st))
+         : (fw ? launch_fp8<0, 1>(a, f8, p.tile, p.splits, st) : launch_fp8<0, 0>(a, f8, p.tile, p.splits, st));
+  if (e == hipSuccess && p.splits > 1) {
+    const unsigned grid = (unsigned)std::min<int64_t>(cdiv(M * N, 1024), 16 * (int64_t)device_cus());
+    if (f8) hipLaunchKernelGGL(fp8_join_kernel<u16>, dim3(grid), dim3(256), 0, st, a.partial, static_cast<u16*>(out), M * N, a.ldo, a.N, p.splits);
+    else hipLaunchKernelGGL(fp8_join_kernel<float>, dim3(grid), dim3(256), 0, st, a.partial, static_cast<float*>(out), M * N, a.ldo, a.N, p.splits);
+    e = hipGetLastError();
+  }
+  if (e != hipSuccess) return fail(TILEC_ERR_HIP, "tilec: launching linear_fp8 failed: %s", hipGetErrorString(e));
+  return TILEC_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,6 @@
+// x in e5m2, w in e4m3.
+#include "linear_fp8_kernels.h"
+
+namespace tilec {
+template hipError_t launch_fp8<1, 0>(const Fp8Args&, bool, int, int, hipStream_t);
+}

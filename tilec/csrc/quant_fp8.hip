@@ -1,0 +1,329 @@
+// Quantisation to 8-bit floating point in blocks of 128 values of a row or 128 x
+// 128 tiles (fp8.h says what a block's scale and codes are), and back.
+//
+// Bound by HBM: values are read once, 16 bytes or more a load, and stay in
+// registers from the block's maximum to its codes.
+//   Blocks of a row, row-major: 16 threads hold a block, 8 values each.
+//   Tiles, and matrices whose memory runs along their columns: a workgroup of 256
+//   holds 128 x 128 values, 8 x 8 a thread where it transposes: a thread's 8
+//   values of one output row leave as 8 bytes into LDS, and from there in
+//   16-byte pieces of whole 128-byte runs.
+#include <algorithm>
+
+#include "abi.h"
+#include "common.h"
+#include "fp8.h"
+#include "rows.h"
+#include "../../include/tilec.h"
+
+namespace tilec {
+
+namespace {
+
+struct QuantArgs {
+  const void* x;
+  unsigned char* codes;
+  float* scales;
+  int64_t R, C, ldx, ldq;  // of the result; ldx: row stride of x, or of its transpose
+  int64_t G;               // scales of a row
+  int e5m2, lg;            // rows kernel: 2^lg blocks of a row side by side
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t top_of(const Group<T, 8>& g) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(g.get(e)) & 0x7fffffffu);
+  return top;
+}
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+template <typename T>
+__device__ __forceinline__ u32x2 codes_of(const Group<T, 8>& g, float inverse, bool e5m2) {
+  u32x2 q;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    q[i] = to_fp8(g.get(4 * i) * inverse, g.get(4 * i + 1) * inverse, g.get(4 * i + 2) * inverse,
+                  g.get(4 * i + 3) * inverse, e5m2);
+  return q;
+}
+
+// A workgroup takes 2^lg blocks of 16 >> lg rows at a time, U of those in flight.
+template <typename T>
+__global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a) {
+  constexpr int U = 4;
+  const int slot = threadIdx.x >> 4, sub = threadIdx.x & 15;
+  const int64_t g = ((int64_t)blockIdx.x << a.lg) + (slot & ((1 << a.lg) - 1));
+  if (g >= a.G) return;
+  const int rpb = 16 >> a.lg;
+  const int c = (int)(g * kGroup) + 8 * sub, C = (int)a.C;
+  const bool e5m2 = a.e5m2;
+  const int64_t step = (int64_t)gridDim.y * rpb;
+  for (int64_t r0 = (int64_t)blockIdx.y * rpb + (slot >> a.lg); r0 < a.R; r0 += U * step) {
+    Group<T, 8> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = min(r0 + u * step, a.R - 1);
+      v[u].load(static_cast<const T*>(a.x) + r * a.ldx, c, C);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = r0 + u * step;
+      if (r >= a.R) break;
+      uint32_t top = top_of<T>(v[u]);
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+      float scale, inverse;
+      block_scale(top, fp8_largest(e5m2), scale, inverse);
+      if (sub == 0) a.scales[r * a.G + g] = scale;
+      if (c < a.ldq && c / 16 <= (C - 1) / 16)
+        *reinterpret_cast<u32x2*>(a.codes + r * a.ldq + c) = codes_of<T>(v[u], inverse, e5m2);
+    }
+  }
+}
+
+// One 128 x 128 tile of the result a workgroup.  TRANS: x holds its transpose.
+// TILE: one scale; otherwise one a row (with TRANS only).
+template <typename T, bool TRANS, bool TILE>
+__global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a, int tiles_c) {
+  static_assert(TRANS || TILE, "blocks of row-major rows have a kernel of their own");
+  __shared__ uint32_t red[4][TILE ? 1 : 128];
+  __shared__ __align__(16) char out[TRANS ? 128 * 128 : 16];
+  const int tid = threadIdx.x, lo = tid & 15, hi = tid >> 4, wave = tid >> 6;
+  const int tr = (int)blockIdx.x / tiles_c, tc = (int)blockIdx.x - tr * tiles_c;
+  const int64_t r0 = (int64_t)tr * 128;
+  const int c0 = tc * 128, C = (int)a.C;
+  const bool e5m2 = a.e5m2;
+  // TRANS: v[p] is memory row c0 + 8 hi + p (a column of the result), its values
+  // those of the result's rows r0 + 8 lo ..; otherwise row r0 + 16 p + hi, columns
+  // c0 + 8 lo ...
+  Group<T, 8> v[8];
+  uint32_t top[8];
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const int64_t m = TRANS ? c0 + 8 * hi + p : r0 + 16 * p + hi;
+    const bool live = m < (TRANS ? a.C : a.R);
+    const T* row = static_cast<const T*>(a.x) + (live ? m : 0) * a.ldx;
+    v[p].load(row, TRANS ? (int)r0 + 8 * lo : c0 + 8 * lo, live ? (int)(TRANS ? a.R : a.C) : 0);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    top[e] = 0;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) top[e] = max(top[e], __float_as_uint(v[p].get(e)) & 0x7fffffffu);
+  }
+  float inverse[8], scale;
+  if constexpr (TILE) {
+    uint32_t t = top[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) t = max(t, top[e]);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) t = max(t, (uint32_t)__shfl_xor((int)t, o));
+    if ((tid & 63) == 0) red[wave][0] = t;
+    __syncthreads();
+    t = max(max(red[0][0], red[1][0]), max(red[2][0], red[3][0]));
+    block_scale(t, fp8_largest(e5m2), scale, inverse[0]);
+#pragma unroll
+    for (int e = 1; e < 8; ++e) inverse[e] = inverse[0];
+    if (tid == 0) a.scales[(int64_t)tr * a.G + tc] = scale;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      top[e] = max(top[e], (uint32_t)__shfl_xor((int)top[e], 16));
+      top[e] = max(top[e], (uint32_t)__shfl_xor((int)top[e], 32));
+    }
+    if ((hi & 3) == 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) red[wave][8 * lo + e] = top[e];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t t = max(max(red[0][8 * lo + e], red[1][8 * lo + e]), max(red[2][8 * lo + e], red[3][8 * lo + e]));
+      block_scale(t, fp8_largest(e5m2), scale, inverse[e]);
+      if (hi == 0 && r0 + 8 * lo + e < a.R) a.scales[(r0 + 8 * lo + e) * a.G + tc] = scale;
+    }
+  }
+  const int end = (int)std::min<int64_t>(a.ldq, (int64_t)((C - 1) / 16 + 1) * 16);  // of a row, with the bytes that fill its last 16
+  if constexpr (!TRANS) {
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const int64_t r = r0 + 16 * p + hi;
+      if (r < a.R && c0 + 8 * lo < end)
+        *reinterpret_cast<u32x2*>(a.codes + r * a.ldq + c0 + 8 * lo) = codes_of<T>(v[p], inverse[0], e5m2);
+    }
+  } else {
+    // Row 8 lo + e of the tile, columns 8 hi ..: 8-byte piece hi of its 16, at hi ^ lo.
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      u32x2 q;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        q[i] = to_fp8(v[4 * i].get(e) * inverse[e], v[4 * i + 1].get(e) * inverse[e], v[4 * i + 2].get(e) * inverse[e],
+                      v[4 * i + 3].get(e) * inverse[e], e5m2);
+      *reinterpret_cast<u32x2*>(out + 128 * (8 * lo + e) + 8 * (hi ^ lo)) = q;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int row = 32 * k + (tid >> 3), piece = tid & 7, swap = row >> 3;
+      const u32x2 a0 = *reinterpret_cast<const u32x2*>(out + 128 * row + 8 * ((2 * piece) ^ swap));
+      const u32x2 a1 = *reinterpret_cast<const u32x2*>(out + 128 * row + 8 * ((2 * piece + 1) ^ swap));
+      if (r0 + row < a.R && c0 + 16 * piece < end)
+        *reinterpret_cast<u32x4*>(a.codes + (r0 + row) * a.ldq + c0 + 16 * piece) = u32x4{a0.x, a0.y, a1.x, a1.y};
+    }
+  }
+}
+
+struct ValuesArgs {
+  const unsigned char* codes;
+  const float* scales;
+  void* out;
+  int64_t R, C, ldq, ldo, G;
+  int shift, e5m2, lg;
+};
+
+// The values that codes stand for, mapped as in quant_rows_kernel.
+template <typename T>
+__global__ __launch_bounds__(256) void values_kernel(ValuesArgs a) {
+  constexpr int U = 4;
+  const int slot = threadIdx.x >> 4, sub = threadIdx.x & 15;
+  const int64_t g = ((int64_t)blockIdx.x << a.lg) + (slot & ((1 << a.lg) - 1));
+  const int64_t c64 = g * kGroup + 8 * sub;
+  if (c64 >= a.C) return;
+  const int c = (int)c64, C = (int)a.C, rpb = 16 >> a.lg;
+  const int64_t step = (int64_t)gridDim.y * rpb;
+  for (int64_t r0 = (int64_t)blockIdx.y * rpb + (slot >> a.lg); r0 < a.R; r0 += U * step) {
+    u32x2 q[U];
+    float s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = min(r0 + u * step, a.R - 1);
+      const unsigned char* p = a.codes + r * a.ldq + c;
+      s[u] = a.scales[(r >> a.shift) * a.G + g];
+      if (c + 8 <= C) {
+        typedef u32x2 __attribute__((aligned(1))) u32x2_any;
+        q[u] = *reinterpret_cast<const u32x2_any*>(p);
+      } else {
+        q[u] = u32x2{0u, 0u};
+        for (int e = 0; c + e < C; ++e) q[u][e >> 2] |= (uint32_t)p[e] << (8 * (e & 3));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = r0 + u * step;
+      if (r >= a.R) break;
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        const int w = (int)q[u][i];
+        f32x2 x, y;
+        if (a.e5m2) x = __builtin_amdgcn_cvt_pk_f32_bf8(w, false), y = __builtin_amdgcn_cvt_pk_f32_bf8(w, true);
+        else x = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), y = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+        v[4 * i] = x.x * s[u], v[4 * i + 1] = x.y * s[u], v[4 * i + 2] = y.x * s[u], v[4 * i + 3] = y.y * s[u];
+      }
+      store_group<T, 8>(static_cast<T*>(a.out) + r * a.ldo, c, C, v);
+    }
+  }
+}
+
+// The grid over a matrix of G blocks a row, 2^lg of them side by side in a
+// workgroup of 16.
+dim3 rows_grid(int64_t R, int64_t G, int& lg) {
+  lg = 0;
+  while (lg < 4 && (int64_t(1) << lg) < G) ++lg;
+  const int64_t gx = cdiv(G, int64_t(1) << lg);
+  const int64_t full = cdiv(R, 4 * (16 >> lg));  // 4 rows a thread
+  return dim3((unsigned)gx, (unsigned)std::max<int64_t>(1, std::min<int64_t>(full, 65535)));
+}
+
+int check_matrix(const char* what, int64_t R, int64_t C, int32_t wide, int32_t fp8, int32_t block) {
+  if ((wide != TILEC_F32 && wide != TILEC_BF16) || !is_fp8(fp8))
+    return fail(TILEC_ERR_TYPE, "tilec: %s: unsupported dtype codes %d, %d (use float32 or bfloat16, and an 8-bit type)",
+                what, wide, fp8);
+  if (R < 0 || C < 0 || R > kMaxDim || C > kMaxDim)
+    return fail(TILEC_ERR_VALUE, "tilec: %s: bad shape %lld x %lld", what, (long long)R, (long long)C);
+  if (block != 1 && block != kGroup)
+    return fail(TILEC_ERR_VALUE, "tilec: %s: blocks have 1 or 128 rows (got %d)", what, block);
+  return TILEC_OK;
+}
+
+constexpr int64_t kMaxStride = int64_t(1) << 40;
+
+}  // namespace
+
+}  // namespace tilec
+
+using namespace tilec;
+
+extern "C" {
+
+int tilec_quantize_fp8(const void* x, void* codes, float* scales, int64_t R, int64_t C, int64_t ldx, int64_t ldq,
+                       int32_t layout, int32_t x_dtype, int32_t q_dtype, int32_t block, void* stream) {
+  clear_error();
+  const int rc = check_matrix("quantize_fp8", R, C, x_dtype, q_dtype, block);
+  if (rc != TILEC_OK) return rc;
+  if (layout != 0 && layout != TILEC_X1_COL_MAJOR)
+    return fail(TILEC_ERR_VALUE, "tilec: quantize_fp8: bad layout %d", layout);
+  if (R == 0 || C == 0) return TILEC_OK;
+  const bool trans = layout != 0;
+  const int64_t rows = trans ? C : R, cols = trans ? R : C, room = cdiv(C, 16) * 16;
+  if ((rows > 1 && ldx < cols) || ldx > kMaxStride)
+    return fail(TILEC_ERR_VALUE, "tilec: quantize_fp8: bad stride %lld of x", (long long)ldx);
+  if (x == nullptr || codes == nullptr || scales == nullptr)
+    return fail(TILEC_ERR_VALUE, "tilec: quantize_fp8: a pointer is NULL");
+  if (reinterpret_cast<uintptr_t>(codes) % 16 != 0 || (R > 1 && (ldq % 16 != 0 || ldq < room || ldq > kMaxStride)))
+    return fail(TILEC_ERR_VALUE, "tilec: quantize_fp8: rows of codes begin at multiples of 16 bytes (row stride %lld)",
+                (long long)ldq);
+  QuantArgs a{};
+  a.x = x, a.codes = static_cast<unsigned char*>(codes), a.scales = scales;
+  a.R = R, a.C = C, a.ldx = rows > 1 ? ldx : cols, a.ldq = R > 1 ? ldq : room, a.G = cdiv(C, kGroup);
+  a.e5m2 = q_dtype == TILEC_F8E5M2;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  auto by_type = [&](auto t) {
+    using T = decltype(t);
+    if (!trans && block == 1) {
+      const dim3 grid = rows_grid(R, a.G, a.lg);
+      hipLaunchKernelGGL(quant_rows_kernel<T>, grid, dim3(256), 0, st, a);
+      return hipGetLastError();
+    }
+    const int64_t tiles = cdiv(R, 128) * a.G;
+    if (tiles > INT32_MAX) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)tiles);
+    const int tiles_c = (int)a.G;
+    if (!trans) hipLaunchKernelGGL((quant_tile_kernel<T, false, true>), grid, dim3(256), 0, st, a, tiles_c);
+    else if (block == 1) hipLaunchKernelGGL((quant_tile_kernel<T, true, false>), grid, dim3(256), 0, st, a, tiles_c);
+    else hipLaunchKernelGGL((quant_tile_kernel<T, true, true>), grid, dim3(256), 0, st, a, tiles_c);
+    return hipGetLastError();
+  };
+  const hipError_t e = x_dtype == TILEC_F32 ? by_type(float{}) : by_type(u16{});
+  if (e != hipSuccess) return fail(TILEC_ERR_HIP, "tilec: launching quantize_fp8 failed: %s", hipGetErrorString(e));
+  return TILEC_OK;
+}
+
+int tilec_dequantize_fp8(const void* codes, const float* scales, void* out, int64_t R, int64_t C, int64_t ldq,
+                         int64_t ldo, int32_t q_dtype, int32_t out_dtype, int32_t block, void* stream) {
+  clear_error();
+  const int rc = check_matrix("dequantize_fp8", R, C, out_dtype, q_dtype, block);
+  if (rc != TILEC_OK) return rc;
+  if (R == 0 || C == 0) return TILEC_OK;
+  if (R > 1 && (ldq < C || ldo < C || ldq > kMaxStride || ldo > kMaxStride))
+    return fail(TILEC_ERR_VALUE, "tilec: dequantize_fp8: bad row strides %lld, %lld", (long long)ldq, (long long)ldo);
+  if (codes == nullptr || scales == nullptr || out == nullptr)
+    return fail(TILEC_ERR_VALUE, "tilec: dequantize_fp8: a pointer is NULL");
+  ValuesArgs a{};
+  a.codes = static_cast<const unsigned char*>(codes), a.scales = scales, a.out = out;
+  a.R = R, a.C = C, a.ldq = ldq, a.ldo = ldo, a.G = cdiv(C, kGroup);
+  a.shift = block == 1 ? 0 : 7, a.e5m2 = q_dtype == TILEC_F8E5M2;
+  const dim3 grid = rows_grid(R, a.G, a.lg);
+  if (out_dtype == TILEC_F32)
+    hipLaunchKernelGGL(values_kernel<float>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
+  else hipLaunchKernelGGL(values_kernel<u16>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(TILEC_ERR_HIP, "tilec: launching dequantize_fp8 failed: %s", hipGetErrorString(e));
+  return TILEC_OK;
+}
+
+}  // extern "C"

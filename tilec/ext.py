@@ -11,8 +11,8 @@ libtilec_hip.so instead of a JIT-compiled Metal tile kernel.
     out = tilec.ext.matrix_mul(x1, x2)
     rows = tilec.ext.sum(x1, axis=1)       # [512] fp32 row sums
 
-The training operators of training.py (layer norm, linear cross entropy, AdamW)
-are part of this module too.
+The training operators of training.py (norms, linear cross entropy, gradient norm,
+AdamW) and those of 8-bit linear layers (fp8.py) are part of this module too.
 
 Kernel choice per shape comes from `tune.pick` (the shape→config model trained
 on MI355X), falling back to the library's built-in rule when no model is
@@ -569,9 +569,11 @@ def sum(x, axis=1):
     return out
 
 
-# The training operators (training.py) are part of this module's API; they use
-# the buffers above, so they come last.
+# The training operators (training.py) and those of 8-bit linear layers (fp8.py)
+# are part of this module's API; they use the buffers above, so they come last.
+from . import fp8 as _fp8  # noqa: E402
 from . import training as _training  # noqa: E402
+from .fp8 import *  # noqa: E402,F401,F403
 from .training import *  # noqa: E402,F401,F403
 
-__all__ += _training.__all__
+__all__ += _training.__all__ + _fp8.__all__

@@ -1,6 +1,7 @@
 """Training operators on PyTorch-ROCm tensors, reached as `tilec.ext.*`: layer
-norm and its gradients, the cross entropy of a linear layer's outputs and its
-gradients, and an AdamW step over many tensors.
+norm and root mean square norm with their gradients, the cross entropy of a
+linear layer's outputs and its gradients, the norm of a model's gradients with
+clipping, and an AdamW step over many tensors.
 
 They are what a training step needs beside the products (`matrix_mul`) and the
 sums (`sum`) of its linear layers, and follow the same rules: arguments are
@@ -18,10 +19,10 @@ from functools import lru_cache
 import torch
 
 from . import _lib
-from .ext import _current_device, _raw_stream, _tuned, counters_for
+from .ext import _capturing, _current_device, _raw_stream, _tuned, counters_for
 
-__all__ = ["layer_norm", "layer_norm_backward", "linear_cross_entropy", "linear_cross_entropy_grad",
-           "adamw_state", "adamw_step", "adamw_values", "ADAMW_BLOCK"]
+__all__ = ["layer_norm", "layer_norm_backward", "rms_norm", "rms_norm_backward", "linear_cross_entropy", "linear_cross_entropy_grad",
+           "grad_norm", "clip_grads", "adamw_state", "adamw_step", "adamw_values", "ADAMW_BLOCK"]
 
 _CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
@@ -110,6 +111,40 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, param_grads=True):
     same bits on every call).  param_grads=False leaves them out (None).
     """
     return _lib.host().layer_norm_backward(dy, x, mean, rstd, weight, param_grads, _stream_of(dy))
+
+
+def rms_norm(x, weight=None, residual=None, eps=1e-5, dtype=None):
+    """(y, h, rstd): every row of h = x + residual divided by its root mean
+    square, times `weight`.
+
+        rstd = 1 / sqrt(sum(h^2) / D + eps);  y = h * rstd * weight
+
+    x: [R, D] (or [D], one row) float32 or bfloat16, D >= 1; row-strided views are
+    read in place.  weight: [D] or None.  residual: of x's shape, float32 or
+    bfloat16, or None; h has its type (the sum is rounded to it before anything
+    else is computed) and is x itself where there is none.  y has x's shape and
+    its type, or `dtype`.  With dtype float8_e4m3fn or float8_e5m2 y is the 8-bit
+    operand of the next `linear_fp8`, a pair (codes [R, D], scales [R, ceil(D /
+    128)]): the codes and scales that `quantize_fp8` gives of the float32 y.  rstd
+    is float32 [R]; `rms_norm_backward` takes it and h.
+    """
+    return _lib.host().rms_norm(x, weight, residual, eps, dtype, _stream_of(x))
+
+
+def rms_norm_backward(dy, h, rstd, weight=None, dh=None, weight_grad=True):
+    """(dx, dweight) of `rms_norm` for the gradient dy of its y.
+
+        hhat = h * rstd
+        dx = rstd * (dy * weight - hhat * mean(dy * weight * hhat)) + dh
+        dweight = sum over rows of dy * hhat
+
+    h, rstd: the forward pass's (h is x where it had no residual).  dh: the
+    gradient of h from its other reader, the residual stream, of h's shape, or
+    None.  dx is the gradient of x and of the residual alike; it has h's shape and
+    dh's type, without dh dy's.  dweight is float32 [D], added in a fixed order
+    (the same bits on every call); weight_grad=False leaves it out (None).
+    """
+    return _lib.host().rms_norm_backward(dy, h, rstd, weight, dh, weight_grad, _stream_of(dy))
 
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
@@ -227,6 +262,41 @@ def linear_cross_entropy_grad(x, weight, target, reduction="mean", ignore_index=
     """
     return _linear_ce("linear_cross_entropy_grad", x, weight, target, reduction, ignore_index, 1, grad_loss,
                       chunk_rows)
+
+
+def _counter(device, stream, nbytes):
+    """A zeroed counter that its kernel leaves zero: the stream's own, or in a
+    capture one of the graph's, zeroed in every replay (graphs of one stream may be
+    replayed on others at the same time)."""
+    if _capturing(device):
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    return counters_for(device, stream, nbytes)
+
+
+def grad_norm(grads, max_norm=None, grad_scale=None):
+    """(norm, scale): the norm of all values of a list of gradients, and the factor
+    that clips it to max_norm, each one float32 on the GPU.
+
+        norm = |grad_scale| * sqrt(sum of all g^2)
+        scale = grad_scale * min(1, max_norm / (norm + 1e-6))
+
+    `adamw_step` takes the scale as its grad_scale: gradients are clipped without
+    being written.  grads: float32 and bfloat16 tensors on one GPU (None: a
+    parameter without a gradient), at least one.  max_norm: at least 0, or None,
+    no limit.  grad_scale: a float32 value on the GPU that the gradients are to be
+    multiplied by in any case (the inverse of a loss's scale), or None.  Squares
+    and sums are float64, in a fixed order: nothing overflows, and the same bits
+    come out on every call.  An infinite norm gives a scale of 0, a NaN one NaN.
+    """
+    return _lib.host().grad_norm(grads, max_norm, grad_scale, _raw_stream, _counter)
+
+
+def clip_grads(grads, max_norm, grad_scale=None):
+    """The norm of `grad_norm`; the gradients are multiplied in place by its scale
+    (not touched where that is 1).  Two of them may not share memory, and a view
+    whose values do not lie side by side is refused (ValueError).  To autograd they
+    have been modified in place."""
+    return _lib.host().clip_grads(grads, max_norm, grad_scale, _raw_stream, _counter)
 
 
 ADAMW_BLOCK = 256  # values per scale of an 8-bit state
