@@ -192,6 +192,29 @@ def test_products(M, N, K, out, xt, wt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("xt,wt,wb", [("e4m3", "e4m3", 128), ("e5m2", "e4m3", 1)])
+@pytest.mark.parametrize("M,N,K", [(512, 4096, 1030), (1000, 3001, 4097), (1030, 2050, 1000), (2900, 5000, 201),
+                                   (4000, 4100, 901), (520, 1030, 40003), (2048, 2048, 32768)])
+def test_larger_products(M, N, K, xt, wt, wb, out):
+    # Every tile, whole and ragged, with and without splits of K.  (An eight's largest
+    # product is at most the eight's sum of magnitudes.)
+    x, w = operand(M, K, xt, 1, M + K), operand(N, K, wt, wb, N + K + 1)
+    got = tilec.ext.linear_fp8(x, w, dtype=WIDE[out])
+    xv, wv = values(x, 1), values(w, wb).t().contiguous()
+    ref, S = torch.mm(xv, wv), torch.mm(xv.abs_(), wv.abs_())
+    G = -(-K // 128)
+    err = (got.double() - ref).abs()
+    if out == "f32":
+        assert (err <= (128 + G + 16) * E32 * S + 2 * E32 * ref.abs()).all()
+        assert err.norm() <= 8 * E32 * ref.norm()
+    else:
+        assert (err <= (7 * 2.0 ** -13 + (32 + G + 16) * E32) * S + 2.0 ** -8 * ref.abs()).all()
+        assert err.norm() <= 2.0 ** -8 * ref.norm()
+    assert torch.equal(got, tilec.ext.linear_fp8(x, w, dtype=WIDE[out]))
+
+
+@pytest.mark.gpu
 def test_integers_are_exact():
     # Small whole numbers, scales of powers of two: every sum is exact, in either type's reach.
     g = torch.Generator().manual_seed(0)

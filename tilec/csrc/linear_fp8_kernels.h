@@ -83,30 +83,46 @@ __device__ __forceinline__ void store4(TO* __restrict__ row, int n, int N, f32x4
 template <bool F8>
 using Out = std::conditional_t<F8, unsigned short, float>;  // bf16, or float32
 
-template <int BM_, int BN_, int WM_, int WN_>
+template <int BM_, int BN_, int WM_, int WN_, int NBUF_>
 struct TileGeom {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NBUF = NBUF_;
   static constexpr int NW = WM * WN, NT = 64 * NW;
   static constexpr int MT = BM / WM / 16, NB = BN / WN / 16;  // blocks of a wave
   static constexpr int XI = BM * 8 / NT, WI = BN * 8 / NT;    // 16-byte copies a thread and step
   static constexpr int SI = (BM + BN + NT - 1) / NT;          // scales a thread and step
-  static constexpr int W_AT = BM * 128, S_AT = W_AT + BN * 128, STAGE = S_AT + SI * NT * 4;
+  static constexpr int W_AT = BM * 128, S_AT = W_AT + BN * 128, STAGE = S_AT + SI * NT * 4;  // of a stage
   static_assert(BM * 8 % NT == 0 && BN * 8 % NT == 0 && BM % 64 == 0 && BN % 64 == 0, "whole copies");
   static_assert(BN / WN <= 128 && 128 % (BN / WN) == 0, "a wave's columns lie in one tile of w");
-  static_assert(2 * STAGE <= 160 * 1024, "LDS is 160 KiB");
+  static_assert(NBUF * STAGE <= 160 * 1024 && (NBUF == 2 || NBUF == 4), "LDS is 160 KiB");
 };
 
-// BM x BN outputs a workgroup, a group of 128 k a step.  Two stages: a step's
-// codes and scales are copied into one (global to LDS, 16 bytes a lane) while
-// the other is multiplied.  A stage holds rows of 128 bytes whose 16-byte chunks
-// are exchanged by (row / 2) % 8, so that 16 rows' reads spread over the banks.
-// What lies past M, N or K is never read: those copies have an address out of
-// range and leave zeros; where K ends inside a chunk the rest of it is cleared
-// in LDS before the last step.
+// BM x BN outputs a workgroup, a group of 128 k a step, NBUF stages: the codes and
+// scales of up to NBUF steps are on their way (global to LDS, 16 bytes a lane) while
+// one is multiplied, and a wave reads its operands from LDS a step before it
+// multiplies them.  A stage holds rows of 128 bytes whose 16-byte chunks are
+// exchanged by (row / 2) % 8, so that 16 rows' reads spread over the banks.  What
+// lies past M, N or K is never read: those copies have an address out of range and
+// leave zeros; where K ends inside a chunk the rest of it is cleared in LDS before
+// the last step's operands are read.
+//
+// A step of 128 x 128 takes 0.5 us: 8 waves read 96 KiB and the copies write 36 KiB,
+// which LDS passes on at 128 bytes a clock; without any copies it takes as long, and
+// the copies alone take as long too where rows begin at multiples of 128 bytes (1.45
+// times where they do not, two lines a row).
 template <class P, bool F8, int FX, int FW, bool WROWS>
 __global__ __launch_bounds__(P::NT, 1) void fp8_tile_kernel(Fp8Args a) {
+  // Objects of their own, so that the compiler knows which copies a read waits for.
   __shared__ __align__(16) char lds0[P::STAGE];
   __shared__ __align__(16) char lds1[P::STAGE];
+  __shared__ __align__(16) char lds2[P::NBUF > 2 ? P::STAGE : 16];
+  __shared__ __align__(16) char lds3[P::NBUF > 3 ? P::STAGE : 16];
+  auto slot = [&](auto i) -> char* {
+    constexpr int k = decltype(i)::value % P::NBUF;
+    if constexpr (k == 0) return lds0;
+    else if constexpr (k == 1) return lds1;
+    else if constexpr (k == 2) return lds2;
+    else return lds3;
+  };
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / P::WN, wn = wave % P::WN;
@@ -180,42 +196,56 @@ __global__ __launch_bounds__(P::NT, 1) void fp8_tile_kernel(Fp8Args a) {
   // A lane's 32 codes of row lane % 16: chunks lane / 16 and 4 + lane / 16.
   const int row = lane & 15, quad = lane >> 4;
   const int at = 128 * row + 16 * (quad ^ ((row >> 1) & 7));
-  auto frag = [&](auto& f, const char* rows) __attribute__((always_inline)) {
-    f.set(*reinterpret_cast<const i32x4*>(rows + at), *reinterpret_cast<const i32x4*>(rows + (at ^ 64)));
+  // What a wave multiplies in a step, read from LDS a step ahead.
+  struct Operands {
+    i32x4 w[P::NB][2], x[P::MT][2];
+    f32x4 s4[P::NB];
+    float sx[P::MT], sw;
   };
-  auto multiply = [&](const char* st) __attribute__((always_inline)) {
-    const char* const xs = st + 128 * (wm * (P::BM / P::WM));
-    const char* const ws = st + P::W_AT + 128 * (wn * (P::BN / P::WN));
+  Operands ops[2];
+  auto read = [&](const char* st, Operands& o) __attribute__((always_inline)) {
+    const char* const xs = st + 128 * (wm * (P::BM / P::WM)) + at;
+    const char* const ws = st + P::W_AT + 128 * (wn * (P::BN / P::WN)) + at;
+    const char* const xs2 = st + 128 * (wm * (P::BM / P::WM)) + (at ^ 64);
+    const char* const ws2 = st + P::W_AT + 128 * (wn * (P::BN / P::WN)) + (at ^ 64);
     const float* const ssx = reinterpret_cast<const float*>(st + P::S_AT) + wm * (P::BM / P::WM) + row;
     const float* const ssw = reinterpret_cast<const float*>(st + P::S_AT) + P::BM + wn * (P::BN / P::WN);
-    Frag<F8, FW> fw[P::NB];
-    Frag<F8, FX> fx[2];
-    f32x4 s4[P::NB], p[2][P::NB];
-    float s[2], s1 = 1.f;
-    frag(fx[0], xs);
 #pragma unroll
     for (int j = 0; j < P::NB; ++j) {
-      frag(fw[j], ws + 2048 * j);
-      if constexpr (WROWS) s4[j] = *reinterpret_cast<const f32x4*>(ssw + 16 * j + 4 * quad);
+      o.w[j][0] = *reinterpret_cast<const i32x4*>(ws + 2048 * j);
+      o.w[j][1] = *reinterpret_cast<const i32x4*>(ws2 + 2048 * j);
+      if constexpr (WROWS) o.s4[j] = *reinterpret_cast<const f32x4*>(ssw + 16 * j + 4 * quad);
     }
-    if constexpr (!WROWS) s1 = *ssw;
-    s[0] = ssx[0] * s1;
-    __builtin_amdgcn_sched_barrier(0);
-    // Row i's blocks on the matrix core, beside them the multiply-adds of row i - 1.
+    if constexpr (!WROWS) o.sw = *ssw;
 #pragma unroll
-    for (int i = 0; i <= P::MT; ++i) {
-      if (i + 1 < P::MT) frag(fx[(i + 1) & 1], xs + 2048 * (i + 1));
+    for (int i = 0; i < P::MT; ++i) {
+      o.x[i][0] = *reinterpret_cast<const i32x4*>(xs + 2048 * i);
+      o.x[i][1] = *reinterpret_cast<const i32x4*>(xs2 + 2048 * i);
+      o.sx[i] = ssx[16 * i];
+    }
+  };
+  // A block's P_g on the matrix core, beside it the multiply-adds of the one before last.
+  auto multiply = [&](const Operands& o) __attribute__((always_inline)) {
+    constexpr int LAG = 2, BLOCKS = P::MT * P::NB;
+    Frag<F8, FW> fw[P::NB];
+    Frag<F8, FX> fx;
+    f32x4 p[LAG + 1];
 #pragma unroll
-      for (int j = 0; j < P::NB; ++j) {
-        if (i < P::MT) p[i & 1][j] = block<FX, FW>(fw[j], fx[i & 1]);
-        if (i > 0) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            acc[i - 1][j][r] = fmaf(p[(i - 1) & 1][j][r], WROWS ? s[(i - 1) & 1] * s4[j][r] : s[(i - 1) & 1], acc[i - 1][j][r]);
-        }
+    for (int b = 0; b < BLOCKS + LAG; ++b) {
+      if (b < BLOCKS) {
+        const int i = b / P::NB, j = b % P::NB;
+        if (i == 0) fw[j].set(o.w[j][0], o.w[j][1]);
+        if (j == 0) fx.set(o.x[i][0], o.x[i][1]);
+        p[b % (LAG + 1)] = block<FX, FW>(fw[j], fx);
       }
-      if (i + 1 < P::MT) s[(i + 1) & 1] = ssx[16 * (i + 1)] * s1;
-      __builtin_amdgcn_sched_barrier(0);
+      if (b >= LAG) {
+        const int i = (b - LAG) / P::NB, j = (b - LAG) % P::NB;
+        const float s = WROWS ? o.sx[i] : o.sx[i] * o.sw;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          acc[i][j][r] = fmaf(p[(b - LAG) % (LAG + 1)][r], WROWS ? s * o.s4[j][r] : s, acc[i][j][r]);
+      }
+      __builtin_amdgcn_sched_barrier(0);  // (else the multiply-adds move up to their block and wait for it)
     }
   };
   // Clears what the last chunk of every row holds past K.
@@ -230,36 +260,314 @@ __global__ __launch_bounds__(P::NT, 1) void fp8_tile_kernel(Fp8Args a) {
       }
     }
   };
-  auto arrive = [&]() __attribute__((always_inline)) {
-    __builtin_amdgcn_s_waitcnt(0);  // this wave's copies of the step, and its reads of the other stage
+  // This wave's copies are there but for the last `later` steps', and its reads are
+  // done: then everybody's.
+  auto arrive = [&](auto later) __attribute__((always_inline)) {
+    constexpr int n = decltype(later)::value * (P::XI + P::WI + P::SI);
+    static_assert(n < 64, "vmcnt has 6 bits");
+    __builtin_amdgcn_s_waitcnt(0x0070 | (n & 15) | (n >> 4) << 14);
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  auto step = [&](int kt, char* cur, char* next) __attribute__((always_inline)) {
-    arrive();
-    copy(kt + 1, next);
-    multiply(cur);
+  using std::integral_constant;
+  // Step kt, whose operands are in registers; its stage takes the copies of step
+  // kt + NBUF.
+  auto step = [&](auto i, int kt) __attribute__((always_inline)) {
+    constexpr int k = decltype(i)::value;
+    arrive(integral_constant<int, P::NBUF - 2>{});
+    read(slot(integral_constant<int, k + 1>{}), ops[(k + 1) & 1]);
+    copy(kt + P::NBUF, slot(i));
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(ops[k & 1]);
+    __builtin_amdgcn_sched_barrier(0);
   };
   if (nk > 0) {
     copy(0, lds0);
-    int kt = 0;
-#pragma unroll 1
-    for (; kt + 2 < nk; kt += 2) {
-      step(kt, lds0, lds1);
-      step(kt + 1, lds1, lds0);
-    }
-    char* last = lds0;
-    if (kt + 2 == nk) {
-      step(kt, lds0, lds1);
-      last = lds1;
-    }
-    arrive();
-    if ((a.K & 15) != 0 && g0 + nk == a.G) {
-      clear_tail(last);
+    copy(1, lds1);
+    if constexpr (P::NBUF > 2) copy(2, lds2);
+    if constexpr (P::NBUF > 3) copy(3, lds3);
+    arrive(integral_constant<int, P::NBUF - 1>{});
+    const bool tail = (a.K & 15) != 0 && g0 + nk == a.G;
+    if (tail && nk == 1) {
+      clear_tail(lds0);
       __syncthreads();
     }
-    multiply(last);
+    read(lds0, ops[0]);
+    // All steps but the last two, whose operands may need clearing.
+    int kt = 0;
+#pragma unroll 1
+    for (; kt + P::NBUF + 1 < nk; kt += P::NBUF) {
+      step(integral_constant<int, 0>{}, kt);
+      step(integral_constant<int, 1>{}, kt + 1);
+      if constexpr (P::NBUF > 2) step(integral_constant<int, 2>{}, kt + 2);
+      if constexpr (P::NBUF > 3) step(integral_constant<int, 3>{}, kt + 3);
+    }
+    // Up to NBUF + 1 steps are left, of which all copies but one's are on their way.
+    auto rest = [&](auto i) __attribute__((always_inline)) {
+      constexpr int k = decltype(i)::value;
+      if (kt >= nk) return;
+      if (kt + 1 < nk) {
+        arrive(integral_constant<int, k == 0 ? P::NBUF - 2 : 0>{});
+        char* const next = slot(integral_constant<int, k + 1>{});
+        if (tail && kt + 2 == nk) {
+          clear_tail(next);
+          __syncthreads();
+        }
+        read(next, ops[(k + 1) & 1]);
+        if constexpr (k == 0) copy(kt + P::NBUF, slot(i));
+      }
+      multiply(ops[k & 1]);
+      ++kt;
+    };
+    rest(integral_constant<int, 0>{});
+    rest(integral_constant<int, 1>{});
+    rest(integral_constant<int, 2>{});
+    if constexpr (P::NBUF > 2) rest(integral_constant<int, 3>{});
+    if constexpr (P::NBUF > 3) rest(integral_constant<int, 4>{});
+  }
+
+  const bool inside = m0 + P::BM <= a.M && n0 + P::BN <= a.N;
+  auto store = [&](auto* out, int64_t ld) __attribute__((always_inline)) {
+    using T = std::remove_pointer_t<decltype(out)>;
+    const int mw = m0 + wm * (P::BM / P::WM) + row, nw = n0 + wn * (P::BN / P::WN) + 4 * quad;
+    T* const first = out + (int64_t)mw * ld;
+#pragma unroll
+    for (int i = 0; i < P::MT; ++i) {
+      T* const line = first + (int64_t)(16 * i) * ld;
+#pragma unroll
+      for (int j = 0; j < P::NB; ++j)
+        if (inside || mw + 16 * i < a.M) store4<T>(line, nw + 16 * j, inside ? INT32_MAX : a.N, acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  if (gridDim.y > 1) store(a.partial + (int64_t)split * a.M * a.N, a.N);
+  else store(static_cast<Out<F8>*>(a.out), a.ldo);
+}
+
+// The same product for large outputs: 256 rows, and the eight waves in two groups
+// of four, one wave of each on every SIMD.  While one group multiplies, the other
+// reads its next operands from LDS; they change places at a barrier, so the matrix
+// cores are never without a wave whose operands are in registers.  In half step 2 k
+// the first group reads step k and the second multiplies step k - 1, in half step
+// 2 k + 1 the first multiplies step k and the second reads it.
+//
+// Two stages.  A group's own rows of x are read until it has multiplied the step, w
+// and the scales until the second group has read it.  So in half step 2 k the first
+// group may copy w, the scales and its rows of x of step k + 1, in half step 2 k + 1
+// the second group its own rows of x; each wave waits for its copies before the
+// barrier that ends its multiplying, two half steps later.  (Each group has a loop
+// of its own: one loop with a branch around the copies left the compiler without
+// registers.)
+//
+// 8192^3 with tiles of w: 460-470 us, 2340-2390 TFLOP/s, against 540-550 for
+// fp8_tile_kernel with this tile, whose waves all read and then all multiply; a
+// library's plain 8-bit product with one scale takes 399.  Copies after the reads of
+// a half step instead of before: 486 us; w copied by the second group between its
+// multiplications: 500.  The clock is at 1.9 GHz (2.4 without load): what bounds it
+// is power, with the matrix cores busy in 60 % of the cycles.
+template <class P, bool F8, int FX, int FW, bool WROWS>
+__global__ __launch_bounds__(512, 1) void fp8_pair_kernel(Fp8Args a) {
+  static_assert(P::NW == 8, "two groups of four waves");
+  // Copies of a thread: the second group's of its own rows of x, the first's of all else.
+  constexpr int XI = P::BM * 4 / 256, WI = P::BN * 8 / 256, SI = (P::BM + P::BN + 255) / 256;
+  // Rows of x in registers, refilled while multiplying, and blocks whose sums are
+  // under way.
+  constexpr int RING = F8 && WROWS ? 2 : 3, LAG = 2;
+  // Objects of their own, so that the compiler knows which copies a read waits for.
+  __shared__ __align__(16) char x0[P::BM * 128];
+  __shared__ __align__(16) char x1[P::BM * 128];
+  __shared__ __align__(16) char w0[P::BN * 128];
+  __shared__ __align__(16) char w1[P::BN * 128];
+  __shared__ __align__(16) float s0[SI * 256];
+  __shared__ __align__(16) float s1[SI * 256];
+  struct Stage {
+    char *x, *w;
+    float* s;
+  };
+  const Stage st0 = {x0, w0, s0}, st1 = {x1, w1, s1};
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = wave >> 2, w4 = wave & 3;
+  const int wm = wave / P::WN, wn = wave % P::WN;
+  const int tiles_m = (a.M + P::BM - 1) / P::BM, tiles_n = (a.N + P::BN - 1) / P::BN;
+  int tm, tn;
+  tile_of(blockIdx.x, a.xcds, tiles_m, tiles_n, a.group_m, tm, tn);
+  const int m0 = tm * P::BM, n0 = tn * P::BN;
+  const int split = blockIdx.y, g0 = split * a.split_steps, nk = min(a.G, g0 + a.split_steps) - g0;
+
+  const int c0 = (lane & 7) ^ (lane >> 4);
+  const uint32_t row8 = lane >> 3;
+  const uint32_t rx8 = (P::BM / 2 * group + 8u * XI * w4 + row8) * (uint32_t)a.ldx, rw8 = (8u * WI * w4 + row8) * (uint32_t)a.ldw;
+  const uint32_t vx[2] = {rx8 + 16u * c0, rx8 + 16u * (c0 ^ 4)}, vw[2] = {rw8 + 16u * c0, rw8 + 16u * (c0 ^ 4)};
+  const uint32_t sx8 = 8u * (uint32_t)a.ldx, sw8 = 8u * (uint32_t)a.ldw;
+  uint32_t off_s[SI];
+#pragma unroll
+  for (int i = 0; i < SI; ++i) {
+    const int first = 64 * (w4 * SI + i);
+    const bool is_x = first < P::BM;
+    const int e = first + lane - (is_x ? 0 : P::BM), shift = is_x ? a.xshift : a.wshift, r0 = is_x ? m0 : n0;
+    off_s[i] = 4u * (uint32_t)(((r0 + e) >> shift) - (r0 >> shift)) * (uint32_t)a.G | oob_unless(r0 + e < (is_x ? a.M : a.N) && (is_x || e < P::BN));
+  }
+  const unsigned char* const xb = a.x + (int64_t)m0 * a.ldx + (int64_t)g0 * kGroup;
+  const unsigned char* const wb = a.w + (int64_t)n0 * a.ldw + (int64_t)g0 * kGroup;
+  const float* const sxb = a.sx + (int64_t)(m0 >> a.xshift) * a.G + g0;
+  const float* const swb = a.sw + (int64_t)(n0 >> a.wshift) * a.G + g0;
+  // Bytes of the tile's rows: what lies past the last row is past the end.
+  const uint32_t x_bytes = a.M - m0 >= P::BM ? 0x7FFFFFFFu : (uint32_t)(a.M - m0) * (uint32_t)a.ldx;
+  const uint32_t w_bytes = a.N - n0 >= P::BN ? 0x7FFFFFFFu : (uint32_t)(a.N - n0) * (uint32_t)a.ldw;
+  auto past_of = [&](int kt, uint32_t (&past)[2]) __attribute__((always_inline)) {
+    const int left = a.K - (g0 + kt) * kGroup;
+    past[0] = oob_unless(16 * c0 < left), past[1] = oob_unless(16 * (c0 ^ 4) < left);
+  };
+  auto rsrc_of = [&](const unsigned char* base, uint32_t n, int kt) __attribute__((always_inline)) {
+    const uint32_t r = n == 0x7FFFFFFFu ? n : n - (uint32_t)((g0 + kt) * kGroup);
+    return make_rsrc_uniform(base + kt * kGroup, kt < nk ? r : 0u);
+  };
+  // A group's own half of x's rows.
+  auto copy_x = [&](int kt, const Stage& st) __attribute__((always_inline)) {
+    uint32_t past[2];
+    past_of(kt, past);
+    const BufRsrc rx = rsrc_of(xb, x_bytes, kt);
+#pragma unroll
+    for (int i = 0; i < XI; ++i) {
+      const uint32_t off = (vx[i & 1] + i * sx8) | past[i & 1];
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr_t)(st.x + P::BM * 64 * group + 1024 * (w4 * XI + i)), 16, off, 0, 0, 0);
+    }
+  };
+  auto copy_w = [&](const Stage& st, int i, BufRsrc rw, const uint32_t (&past)[2]) __attribute__((always_inline)) {
+    const uint32_t off = (vw[i & 1] + i * sw8) | past[i & 1];
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr_t)(st.w + 1024 * (w4 * WI + i)), 16, off, 0, 0, 0);
+  };
+  auto copy_s = [&](int kt, const Stage& st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < SI; ++i) {
+      const int first = 64 * (w4 * SI + i);
+      const uint32_t off = off_s[i];
+      const BufRsrc rs = make_rsrc_uniform((first < P::BM ? sxb : swb) + kt, kt < nk ? 0x7FFFFFFFu : 0u);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(st.s + first), 4, off, 0, 0, 0);
+    }
+  };
+
+  auto copy = [&](auto first_t, int kt, const Stage& st) __attribute__((always_inline)) {
+    copy_x(kt, st);
+    if constexpr (decltype(first_t)::value) {
+      uint32_t past[2];
+      past_of(kt, past);
+      const BufRsrc rw = rsrc_of(wb, w_bytes, kt);
+#pragma unroll
+      for (int i = 0; i < WI; ++i) copy_w(st, i, rw, past);
+      copy_s(kt, st);
+    }
+  };
+  f32x4 acc[P::MT][P::NB];
+#pragma unroll
+  for (int i = 0; i < P::MT; ++i)
+#pragma unroll
+    for (int j = 0; j < P::NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int row = lane & 15, quad = lane >> 4;
+  const int at = 128 * row + 16 * (quad ^ ((row >> 1) & 7));
+  Frag<F8, FW> fw[P::NB];
+  Frag<F8, FX> fx[RING];
+  f32x4 p[LAG + 1], s4[P::NB];
+  float s[P::MT];
+#pragma unroll
+  for (int j = 0; j <= LAG; ++j) p[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < P::NB; ++j) s4[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < P::MT; ++i) s[i] = 0.f;
+  constexpr int BLOCKS = P::MT * P::NB;
+  auto add = [&](int b) __attribute__((always_inline)) {  // block b's P_g to its sums
+    const int i = b / P::NB, j = b % P::NB;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(p[b % (LAG + 1)][r], WROWS ? s[i] * s4[j][r] : s[i], acc[i][j][r]);
+  };
+  auto change = [&]() __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  auto step = [&](auto first_t, auto last_t, int kt, const Stage& st, const Stage& next) __attribute__((always_inline)) {
+    constexpr bool LAST = decltype(last_t)::value;
+    const int left = a.K - (g0 + kt) * kGroup - 16 * quad;  // LAST: codes of the lane's first 16
+    auto cut = [&](i32x4 v, int n) {
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const int keep = n - 4 * d;
+        v[d] &= keep >= 4 ? ~0 : keep <= 0 ? 0 : (1 << (8 * keep)) - 1;
+      }
+      return v;
+    };
+    auto frag = [&](auto& f, const char* rows) __attribute__((always_inline)) {
+      i32x4 lo = *reinterpret_cast<const i32x4*>(rows + at), hi = *reinterpret_cast<const i32x4*>(rows + (at ^ 64));
+      if constexpr (LAST) lo = cut(lo, left), hi = cut(hi, left - 64);
+      f.set(lo, hi);
+    };
+    const char* const xs = st.x + 128 * (wm * (P::BM / P::WM));
+    const char* const ws = st.w + 128 * (wn * (P::BN / P::WN));
+    const float* const ssx = st.s + wm * (P::BM / P::WM) + row;
+    const float* const ssw = st.s + P::BM + wn * (P::BN / P::WN);
+    // Reading, beside the other group's multiplying.
+    if constexpr (!LAST) copy(first_t, kt + 1, next);
+#pragma unroll
+    for (int b = BLOCKS - LAG; b < BLOCKS; ++b) add(b);
+#pragma unroll
+    for (int j = 0; j < P::NB; ++j) frag(fw[j], ws + 2048 * j);
+#pragma unroll
+    for (int i = 0; i < RING; ++i) frag(fx[i], xs + 2048 * i);
+    float sw1 = 1.f;
+    if constexpr (WROWS) {
+#pragma unroll
+      for (int j = 0; j < P::NB; ++j) s4[j] = *reinterpret_cast<const f32x4*>(ssw + 16 * j + 4 * quad);
+    } else {
+      sw1 = *ssw;
+    }
+#pragma unroll
+    for (int i = 0; i < P::MT; ++i) s[i] = ssx[16 * i] * sw1;
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    change();
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+      const int i = b / P::NB, j = b % P::NB;
+      p[b % (LAG + 1)] = block<FX, FW>(fw[j], fx[i % RING]);
+      if (b >= LAG) add(b - LAG);
+      if (j == P::NB - 1 && i + RING < P::MT) frag(fx[i % RING], xs + 2048 * (i + RING));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_s_waitcnt(0);
+    change();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  using std::integral_constant;
+  if (nk > 0) {
+    if (group == 0) copy(integral_constant<bool, true>{}, 0, st0);
+    else copy(integral_constant<bool, false>{}, 0, st0);
+    __builtin_amdgcn_s_waitcnt(0);
+    change();
+    if (group == 1) change();
+    auto loop = [&](auto first_t) __attribute__((always_inline)) {
+      int kt = 0;
+#pragma unroll 1
+      for (; kt + 2 < nk; kt += 2) {
+        step(first_t, integral_constant<bool, false>{}, kt, st0, st1);
+        step(first_t, integral_constant<bool, false>{}, kt + 1, st1, st0);
+      }
+      Stage last = st0;
+      if (kt + 2 == nk) {
+        step(first_t, integral_constant<bool, false>{}, kt, st0, st1);
+        last = st1;
+      }
+      step(first_t, integral_constant<bool, true>{}, nk - 1, last, last);
+    };
+    if (group == 0) loop(integral_constant<bool, true>{});
+    else loop(integral_constant<bool, false>{});
+    if (group == 0) change();
+#pragma unroll
+    for (int b = BLOCKS - LAG; b < BLOCKS; ++b) add(b);
   }
 
   const bool inside = m0 + P::BM <= a.M && n0 + P::BN <= a.N;
@@ -383,6 +691,14 @@ hipError_t launch_tile(const Fp8Args& a, int splits, hipStream_t stream) {
   return hipGetLastError();
 }
 
+template <class P, bool F8, int FX, int FW>
+hipError_t launch_pair(const Fp8Args& a, int splits, hipStream_t stream) {
+  const dim3 grid((unsigned)(cdiv(a.M, P::BM) * cdiv(a.N, P::BN)), (unsigned)splits);
+  if (a.wshift == 0) hipLaunchKernelGGL((fp8_pair_kernel<P, F8, FX, FW, true>), grid, dim3(P::NT), 0, stream, a);
+  else hipLaunchKernelGGL((fp8_pair_kernel<P, F8, FX, FW, false>), grid, dim3(P::NT), 0, stream, a);
+  return hipGetLastError();
+}
+
 template <int MT, int U, bool F8, int FX, int FW>
 hipError_t launch_stream(const Fp8Args& a, hipStream_t stream) {
   constexpr int NW = 8;
@@ -396,13 +712,12 @@ hipError_t launch_stream(const Fp8Args& a, hipStream_t stream) {
 template <bool F8, int FX, int FW>
 hipError_t launch_kind(const Fp8Args& a, int tile, int splits, hipStream_t stream) {
   if (tile < 0) {
-    if (a.M <= 16) return launch_stream<1, 4, F8, FX, FW>(a, stream);
-    if (a.M <= 32) return launch_stream<2, 2, F8, FX, FW>(a, stream);
-    return launch_stream<4, 2, F8, FX, FW>(a, stream);
+    return a.M <= 16 ? launch_stream<1, 4, F8, FX, FW>(a, stream) : launch_stream<2, 2, F8, FX, FW>(a, stream);
   }
-  if (tile == 0) return launch_tile<TileGeom<256, F8 ? 256 : 128, F8 ? 2 : 4, F8 ? 4 : 2>, F8, FX, FW>(a, splits, stream);
-  if (tile == 1) return launch_tile<TileGeom<128, 128, 2, 2>, F8, FX, FW>(a, splits, stream);
-  return launch_tile<TileGeom<64, 128, 1, 4>, F8, FX, FW>(a, splits, stream);
+  if (tile == 0) return launch_pair<TileGeom<256, F8 ? 256 : 128, F8 ? 2 : 4, F8 ? 4 : 2, 2>, F8, FX, FW>(a, splits, stream);
+  if (tile == 1) return launch_tile<TileGeom<128, 128, 2, 4, 4>, F8, FX, FW>(a, splits, stream);
+  if (tile == 2) return launch_tile<TileGeom<64, 128, 2, 4, 4>, F8, FX, FW>(a, splits, stream);
+  return launch_tile<TileGeom<64, 64, 2, 2, 4>, F8, FX, FW>(a, splits, stream);
 }
 
 }  // namespace
