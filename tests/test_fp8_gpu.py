@@ -175,7 +175,8 @@ def check_product(out, x, w, xb, wb):
 
 PRODUCTS = [(1, 1, 1), (1, 16, 128), (1, 4096, 4096), (5, 7, 130), (16, 33, 1000), (17, 64, 4097), (33, 20, 16),
             (64, 200, 129), (65, 130, 257), (100, 300, 64), (129, 257, 1025), (300, 500, 2048), (256, 256, 128),
-            (700, 513, 640), (80, 128, 8192), (2000, 2100, 272), (72, 5000, 17)]
+            (700, 513, 640), (80, 128, 8192), (2000, 2100, 272), (72, 5000, 17),
+            (3, 13001, 300), (16, 20000, 1290)]
 
 
 @pytest.mark.gpu

@@ -54,6 +54,6 @@ constexpr Fp8Tile kFp8Tiles[] = {
     {64, {64, 64}, {3.6f, 3.1f}, {0.43f, 0.30f}, {0.75f, 0.47f}},
 };
 constexpr int kFp8TileCount = 4;
-constexpr int kFp8StreamRows = 32;  // the most rows of x that the streaming kernel takes
+constexpr int kFp8StreamRows = 16;  // the most rows of x that the streaming kernel takes
 
 }  // namespace tilec

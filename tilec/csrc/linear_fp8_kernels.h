@@ -13,6 +13,8 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
+constexpr int kReadOnce = 2;  // cache policy: non-temporal
+
 // Two 8-bit values as bf16, exactly.
 template <int FMT, bool HIGH>
 __device__ __forceinline__ bf16x2 widen2(int v) {
@@ -588,99 +590,144 @@ __global__ __launch_bounds__(512, 1) void fp8_pair_kernel(Fp8Args a) {
   else store(static_cast<Out<F8>*>(a.out), a.ldo);
 }
 
-// Few rows of x (16 MT of them): bound by reading w, which goes from memory into
-// the matrix core's registers.  A workgroup takes 16 rows of w, its waves every
-// NW-th group each, U of them in flight; the waves' sums meet in LDS, in order.
-template <int MT, int NW, int U, bool F8, int FX, int FW, bool WROWS>
-__global__ __launch_bounds__(64 * NW) void fp8_stream_kernel(Fp8Args a) {
-  __shared__ f32x4 red[NW][MT][64];
+// Few rows of x, up to 8 XR: bound by reading w, once.  Tiles of 16 rows of w,
+// workgroups that walk over tiles; a workgroup's NW waves take every NW-th group of a
+// tile, and their sums meet in LDS, in order.  Every wave copies its own codes and
+// scales through its own LDS, D groups at a time and across the ends of tiles,
+// without a barrier: memory is then read in runs of 128 bytes, where operands loaded
+// straight into registers, a row a lane, come in pieces of 16 (16 rows against 4096 x
+// 4096 and 16384 x 4096, w from memory: 7.8 and 22.3 us so, 6.6 and 16.2 by way of
+// LDS; one row: 6.2 and 15.5, 6.0 and 14.2).
+template <int XR, int NW, int D, bool F8, int FX, int FW, bool WROWS>
+__global__ __launch_bounds__(64 * NW, 1) void fp8_stream_kernel(Fp8Args a) {
+  static_assert(XR == 1 || XR == 2, "one block of the matrix core");
+  // A group's codes of w and x, then 64 scales of each.
+  constexpr int X_AT = 2048, S_AT = X_AT + XR * 1024, SLOT = S_AT + 512, COPIES = 2 + XR + 2;
+  static_assert((D - 1) * COPIES < 64, "vmcnt has 6 bits");
+  __shared__ __align__(16) char ring[NW][D][SLOT];
+  __shared__ f32x4 red[2][NW][64];
   const int tid = threadIdx.x, lane = tid & 63, row = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n0 = blockIdx.x * 16;
-  const BufRsrc rw = make_rsrc(a.w + (int64_t)n0 * a.ldw), rx = make_rsrc(a.x);
-  const BufRsrc rsx = make_rsrc(a.sx), rsw = make_rsrc(a.sw + (int64_t)(n0 >> a.wshift) * a.G);
-  const uint32_t w_row = (uint32_t)row * (uint32_t)a.ldw | oob_unless(n0 + row < a.N);
-  uint32_t x_row[MT], sx_row[MT], sw_row[4];
+  const int tiles = (a.N + 15) / 16, mine = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+  const int turns = (a.G + NW - 1) / NW, items = mine * turns;  // groups of a wave: a tile's, and all (some past the last)
+
+  const int c0 = (lane & 7) ^ (lane >> 4);
+  uint32_t off_w[2], off_x[XR];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int m = 16 * i + row;
-    x_row[i] = (uint32_t)m * (uint32_t)a.ldx | oob_unless(m < a.M);
-    sx_row[i] = 4u * (uint32_t)(m >> a.xshift) * (uint32_t)a.G | oob_unless(m < a.M);
-  }
+  for (int i = 0; i < 2; ++i) off_w[i] = (8 * i + (lane >> 3)) * (uint32_t)a.ldw + 16u * (c0 ^ 4 * i);
 #pragma unroll
-  for (int r = 0; r < 4; ++r) sw_row[r] = 4u * (4 * quad + r) * (uint32_t)a.G | oob_unless(n0 + 4 * quad + r < a.N);
-  auto load = [&](BufRsrc r, uint32_t off) {
-    return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
+  for (int i = 0; i < XR; ++i) off_x[i] = (8 * i + (lane >> 3)) * (uint32_t)a.ldx + 16u * (c0 ^ 4 * i);
+  const uint32_t off_sx = 4u * (uint32_t)(lane >> a.xshift) * (uint32_t)a.G | oob_unless(lane < a.M);
+  const uint32_t off_sw = 4u * (uint32_t)(lane >> a.wshift) * (uint32_t)a.G | oob_unless(lane < 16);
+
+  int tile = blockIdx.x, g = wave, left = items, to = 0;  // of the next copies
+  auto copy = [&]() __attribute__((always_inline)) {
+    const bool live = left > 0 && g < a.G;
+    const int n0 = 16 * tile, skip = g * kGroup, rest = a.K - skip;
+    const uint32_t past[2] = {oob_unless(16 * c0 < rest), oob_unless(16 * (c0 ^ 4) < rest)};
+    const int64_t w_rows = a.N - n0 < 16 ? a.N - n0 : 16;
+    const BufRsrc rw = make_rsrc_uniform(a.w + (int64_t)n0 * a.ldw + skip, live ? (uint32_t)(w_rows * a.ldw - skip) : 0u);
+    const BufRsrc rx = make_rsrc_uniform(a.x + skip, live ? (uint32_t)(a.M * a.ldx - skip) : 0u);
+    const BufRsrc rsx = make_rsrc_uniform(a.sx + g, live ? 0x7FFFFFFFu : 0u);
+    const BufRsrc rsw = make_rsrc_uniform(a.sw + (int64_t)(n0 >> a.wshift) * a.G + g,
+                                          live ? (WROWS ? 4u * (uint32_t)(w_rows * a.G - g) : 4u) : 0u);
+    char* const at = ring[wave][to];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t off = off_w[j] | past[j];
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr_t)(at + 1024 * j), 16, off, 0, 0, kReadOnce);
+    }
+#pragma unroll
+    for (int j = 0; j < XR; ++j) {
+      const uint32_t off = off_x[j] | past[j];
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr_t)(at + X_AT + 1024 * j), 16, off, 0, 0, 0);
+    }
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsx, (lds_ptr_t)(at + S_AT), 4, off_sx, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsw, (lds_ptr_t)(at + S_AT + 256), 4, off_sw, 0, 0, 0);
+    --left;
+    to = to + 1 == D ? 0 : to + 1;
+    g += NW;
+    if (g >= turns * NW) g = wave, tile += gridDim.x;
   };
-  auto load_once = [&](BufRsrc r, uint32_t off) {
-    return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 2));
-  };
-  auto cut = [&](i32x4 v, int left) {  // the first `left` bytes
+  auto cut = [&](i32x4 v, int n) {  // the first n bytes
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
-      const int keep = left - 4 * d;
+      const int keep = n - 4 * d;
       v[d] &= keep >= 4 ? ~0 : keep <= 0 ? 0 : (1 << (8 * keep)) - 1;
     }
     return v;
   };
-  f32x4 acc[MT];
+  auto lds_of = [](const void* q) __attribute__((always_inline)) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)q;
+  };
+  // Where a lane reads in a slot.
+  const uint32_t w_at = 128 * row + 16 * (quad ^ ((row >> 1) & 7));
+  const int xr = XR == 2 ? row : row & 7;  // eight rows stand for themselves twice
+  const uint32_t x_at = X_AT + 128 * xr + 16 * (quad ^ ((xr >> 1) & 7));
+  const uint32_t sx_at = S_AT + 4 * xr, sw_at = S_AT + 256 + (WROWS ? 16 * quad : 0);
+
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  int at_tile = blockIdx.x, at_g = wave, from = 0, half = 0;  // of the next group to multiply
 #pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int first = wave; first < a.G; first += NW * U) {
-    i32x4 w[U][2], x[U][MT][2];
-    float sx[U][MT], sw[U][4];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int g = first + NW * u, k = kGroup * g + 16 * quad;
-      const uint32_t lo = (uint32_t)k | oob_unless(k < a.K), hi = (uint32_t)(k + 64) | oob_unless(k + 64 < a.K);
-      const uint32_t live = oob_unless(g < a.G);
-      w[u][0] = load_once(rw, (w_row + lo) | ((w_row | lo) & kOob));
-      w[u][1] = load_once(rw, (w_row + hi) | ((w_row | hi) & kOob));
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        x[u][i][0] = load(rx, (x_row[i] + lo) | ((x_row[i] | lo) & kOob));
-        x[u][i][1] = load(rx, (x_row[i] + hi) | ((x_row[i] | hi) & kOob));
-        sx[u][i] = load_f32(rsx, (sx_row[i] + 4u * g) | ((sx_row[i] | live) & kOob));
-      }
-      if constexpr (WROWS) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sw[u][r] = load_f32(rsw, (sw_row[r] + 4u * g) | ((sw_row[r] | live) & kOob));
-      } else {
-        sw[u][0] = load_f32(rsw, 4u * g | live);
-      }
+  for (int i = 0; i < D; ++i) copy();
+  // `items` is the same for every wave of the workgroup: so are its barriers.
+#pragma unroll 1
+  for (int i = 0; i < items; ++i) {
+    // The group's copies are there, those of the D - 1 after it may be under way.
+    // (LDS is read in assembly, wait included: before reads of its own the compiler
+    // waits for every copy.)
+    constexpr int n = (D - 1) * COPIES;
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (n & 15) | (n >> 4) << 14);
+    const uint32_t base = lds_of(ring[wave][from]);
+    i32x4 w0, w1, x0, x1;
+    float sx;
+    f32x4 sw;
+    asm volatile(
+        "ds_read_b128 %0, %6\n\tds_read_b128 %1, %7\n\tds_read_b128 %2, %8\n\tds_read_b128 %3, %9\n\t"
+        "ds_read_b32 %4, %10\n\tds_read_b128 %5, %11\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(w0), "=&v"(w1), "=&v"(x0), "=&v"(x1), "=&v"(sx), "=&v"(sw)
+        : "v"(base + w_at), "v"(base + (w_at ^ 64)), "v"(base + x_at), "v"(base + (x_at ^ 64)), "v"(base + sx_at),
+          "v"(base + sw_at)
+        : "memory");
+    copy();
+    from = from + 1 == D ? 0 : from + 1;
+    if ((a.K & 15) != 0 && at_g == a.G - 1) {
+      const int m = a.K - kGroup * at_g - 16 * quad;
+      w0 = cut(w0, m), w1 = cut(w1, m - 64), x0 = cut(x0, m), x1 = cut(x1, m - 64);
     }
+    Frag<F8, FW> fw;
+    Frag<F8, FX> fx;
+    fw.set(w0, w1);
+    fx.set(x0, x1);
+    const f32x4 p = block<FX, FW>(fw, fx);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int g = first + NW * u;
-      if (g >= a.G) break;  // wave-uniform
-      if (g == a.G - 1 && (a.K & 15) != 0) {
-        const int left = a.K - kGroup * g - 16 * quad;
-        w[u][0] = cut(w[u][0], left), w[u][1] = cut(w[u][1], left - 64);
+    for (int r = 0; r < 4; ++r) acc[r] = fmaf(p[r], sx * sw[WROWS ? r : 0], acc[r]);
+    at_g += NW;
+    if (at_g < turns * NW) continue;
+    // The tile's last group.
+    red[half][wave][lane] = acc;
+    acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): copies go on
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (wave == at_tile % NW) {
+      f32x4 part[NW];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) x[u][i][0] = cut(x[u][i][0], left), x[u][i][1] = cut(x[u][i][1], left - 64);
+      for (int v = 0; v < NW; ++v) {
+        const uint32_t q = lds_of(&red[half][v][lane]);
+        asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(part[v]) : "v"(q) : "memory");
       }
-      Frag<F8, FW> fw;
-      fw.set(w[u][0], w[u][1]);
+      f32x4 s = part[0];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        Frag<F8, FX> fx;
-        fx.set(x[u][i][0], x[u][i][1]);
-        const f32x4 p = block<FX, FW>(fw, fx);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][r] = fmaf(p[r], sx[u][i] * sw[u][WROWS ? r : 0], acc[i][r]);
-      }
+      for (int v = 1; v < NW; ++v) s += part[v];
+      if (row < a.M)
+        store4<Out<F8>>(static_cast<Out<F8>*>(a.out) + (int64_t)row * a.ldo, 16 * at_tile + 4 * quad, a.N, s);
     }
+    half ^= 1;
+    at_g = wave, at_tile += gridDim.x;
   }
-#pragma unroll
-  for (int i = 0; i < MT; ++i) red[wave][i][lane] = acc[i];
-  __syncthreads();
-  for (int t = tid; t < MT * 64; t += 64 * NW) {
-    const int i = t >> 6, l = t & 63, m = 16 * i + (l & 15);
-    f32x4 s = red[0][i][l];
-#pragma unroll
-    for (int v = 1; v < NW; ++v) s += red[v][i][l];
-    if (m < a.M) store4<Out<F8>>(static_cast<Out<F8>*>(a.out) + (int64_t)m * a.ldo, n0 + 4 * (l >> 4), a.N, s);
-  }
+  __builtin_amdgcn_s_waitcnt(0);  // copies past the end leave zeros: not after the workgroup's LDS is another's
 }
 
 template <class P, bool F8, int FX, int FW>
@@ -699,21 +746,27 @@ hipError_t launch_pair(const Fp8Args& a, int splits, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <int MT, int U, bool F8, int FX, int FW>
-hipError_t launch_stream(const Fp8Args& a, hipStream_t stream) {
-  constexpr int NW = 8;
-  const dim3 grid((unsigned)cdiv(a.N, 16));
-  if (a.wshift == 0)
-    hipLaunchKernelGGL((fp8_stream_kernel<MT, NW, U, F8, FX, FW, true>), grid, dim3(64 * NW), 0, stream, a);
-  else hipLaunchKernelGGL((fp8_stream_kernel<MT, NW, U, F8, FX, FW, false>), grid, dim3(64 * NW), 0, stream, a);
+template <int XR, int NW, bool F8, int FX, int FW>
+hipError_t launch_stream(const Fp8Args& a, int64_t most, hipStream_t stream) {
+  const dim3 grid((unsigned)std::min<int64_t>(cdiv(a.N, 16), most));
+  if (a.wshift == 0) hipLaunchKernelGGL((fp8_stream_kernel<XR, NW, 2, F8, FX, FW, true>), grid, dim3(64 * NW), 0, stream, a);
+  else hipLaunchKernelGGL((fp8_stream_kernel<XR, NW, 2, F8, FX, FW, false>), grid, dim3(64 * NW), 0, stream, a);
   return hipGetLastError();
+}
+
+// Eight waves a tile while every workgroup has one tile (4096 x 4096, one row: 5.3
+// us, 5.8 with four), four and three workgroups a CU where they have several (16384 x
+// 4096: 13.5 us, 14.2 with eight; 16 rows: 15.8 and 18.6).
+template <int XR, bool F8, int FX, int FW>
+hipError_t launch_stream(const Fp8Args& a, hipStream_t stream) {
+  const int64_t cus = device_cus();
+  return cdiv(a.N, 16) <= 2 * cus ? launch_stream<XR, 8, F8, FX, FW>(a, 2 * cus, stream)
+                                  : launch_stream<XR, 4, F8, FX, FW>(a, 3 * cus, stream);
 }
 
 template <bool F8, int FX, int FW>
 hipError_t launch_kind(const Fp8Args& a, int tile, int splits, hipStream_t stream) {
-  if (tile < 0) {
-    return a.M <= 16 ? launch_stream<1, 4, F8, FX, FW>(a, stream) : launch_stream<2, 2, F8, FX, FW>(a, stream);
-  }
+  if (tile < 0) return a.M <= 8 ? launch_stream<1, F8, FX, FW>(a, stream) : launch_stream<2, F8, FX, FW>(a, stream);
   if (tile == 0) return launch_pair<TileGeom<256, F8 ? 256 : 128, F8 ? 2 : 4, F8 ? 4 : 2, 2>, F8, FX, FW>(a, splits, stream);
   if (tile == 1) return launch_tile<TileGeom<128, 128, 2, 4, 4>, F8, FX, FW>(a, splits, stream);
   if (tile == 2) return launch_tile<TileGeom<64, 128, 2, 4, 4>, F8, FX, FW>(a, splits, stream);
