@@ -365,8 +365,9 @@ int tilec_adamw_values(const tilec_adamw_tensor* tensors, int32_t count, void* s
  * [R, C] (TILEC_F8E4M3 or TILEC_F8E5M2, row-major, row stride >= C) and float32
  * scales of its blocks of `block` x 128 values, block 1 or 128:
  *   value[r, c] = code[r, c] * scale[r / block, c / 128]
- * The scales [ceil(R / block), ceil(C / 128)] are contiguous; a matrix's last
- * blocks may be smaller.
+ * The scales [ceil(R / block), ceil(C / 128)] have strides of their own, *_row and
+ * *_group elements (in a product *_row <= 2^21); a matrix's last blocks may be
+ * smaller.
  *
  * out [M, N] = x weight^T over the values, x [M, K], weight [N, K]:
  *   out[m, n] = sum_g scale_x[m, g] scale_w[n, g] sum over k of group g of x[m, k] weight[n, k]
@@ -378,17 +379,18 @@ int tilec_adamw_values(const tilec_adamw_tensor* tensors, int32_t count, void* s
  * K <= 2^22; K == 0 writes zeros.
  *
  * Operands are read in place where their rows begin at multiples of 16 bytes,
- * and otherwise copied into the workspace first.  `workspace`:
- * tilec_linear_fp8_workspace_bytes for the same arguments (of x and weight it
- * reads the addresses' alignment only), any contents, 16-byte aligned.
+ * and otherwise copied into the workspace first; scales of rows are read fastest
+ * with a row stride of 1 (8192^3: 2 %).  `workspace`: tilec_linear_fp8_workspace_bytes for the
+ * same arguments (of x and weight it reads the addresses' alignment only), any
+ * contents, 16-byte aligned.
  */
 int tilec_linear_fp8(const void* x, const float* x_scale, const void* weight, const float* w_scale, void* out,
-                     int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldo, int32_t x_dtype,
-                     int32_t w_dtype, int32_t out_dtype, int32_t x_block, int32_t w_block, void* workspace,
-                     size_t workspace_bytes, void* stream);
+                     int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldo, int64_t x_scale_row,
+                     int64_t x_scale_group, int64_t w_scale_row, int64_t w_scale_group, int32_t x_dtype, int32_t w_dtype,
+                     int32_t out_dtype, int32_t x_block, int32_t w_block, void* workspace, size_t workspace_bytes,
+                     void* stream);
 size_t tilec_linear_fp8_workspace_bytes(const void* x, const void* weight, int64_t M, int64_t N, int64_t K, int64_t ldx,
-                                        int64_t ldw, int32_t x_dtype, int32_t w_dtype, int32_t out_dtype,
-                                        int32_t x_block, int32_t w_block);
+                                        int64_t ldw, int32_t x_dtype, int32_t w_dtype, int32_t out_dtype);
 
 /*
  * 8-bit operands.  A block's scale and codes, each operation a float32 one that
@@ -403,11 +405,13 @@ size_t tilec_linear_fp8_workspace_bytes(const void* x, const void* weight, int64
  * the bytes from C to the next multiple of 16 are set to zero.
  */
 int tilec_quantize_fp8(const void* x, void* codes, float* scales, int64_t R, int64_t C, int64_t ldx, int64_t ldq,
-                       int32_t layout, int32_t x_dtype, int32_t q_dtype, int32_t block, void* stream);
+                       int64_t scale_row, int64_t scale_group, int32_t layout, int32_t x_dtype, int32_t q_dtype,
+                       int32_t block, void* stream);
 
 /* The values that codes stand for, in float32 or bfloat16: out[r, c] = code[r, c] * scale. */
 int tilec_dequantize_fp8(const void* codes, const float* scales, void* out, int64_t R, int64_t C, int64_t ldq,
-                         int64_t ldo, int32_t q_dtype, int32_t out_dtype, int32_t block, void* stream);
+                         int64_t ldo, int64_t scale_row, int64_t scale_group, int32_t q_dtype, int32_t out_dtype,
+                         int32_t block, void* stream);
 
 /*
  * Root mean square norm over the rows of h [R, D], D >= 1:
@@ -421,7 +425,8 @@ int tilec_dequantize_fp8(const void* codes, const float* scales, void* out, int6
  */
 int tilec_rms_norm(const void* x, const void* residual, const void* weight, void* y, float* y_scale, void* h,
                    float* rstd, int64_t R, int64_t D, int64_t ldx, int64_t ldr, int64_t ldy, int64_t ldh,
-                   int32_t x_dtype, int32_t r_dtype, int32_t y_dtype, int32_t w_dtype, float eps, void* stream);
+                   int64_t scale_row, int64_t scale_group, int32_t x_dtype, int32_t r_dtype, int32_t y_dtype,
+                   int32_t w_dtype, float eps, void* stream);
 
 /*
  * Its gradients, hhat = h rstd:

@@ -471,7 +471,8 @@ int32_t code_of(at::ScalarType t) {
   return t == at::kFloat ? TILEC_F32 : t == at::kBFloat16 ? TILEC_BF16 : t == at::kFloat8_e4m3fn ? TILEC_F8E4M3 : TILEC_F8E5M2;
 }
 
-constexpr int64_t kGroup = 128;  // values of a row under one scale of an 8-bit operand
+constexpr int64_t kGroup = 128;                      // values of a row under one scale of an 8-bit operand
+constexpr int64_t kMaxScaleRow = int64_t(1) << 21;  // the largest row stride of scales in a product
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // New codes [R, C], rows at multiples of 16 bytes, and scales of blocks of `block` rows.
@@ -515,7 +516,7 @@ PyObject* build_rms(PyObject* const* args) {
   check(tilec_rms_norm(r.t.const_data_ptr(), added ? res.t.const_data_ptr() : nullptr, data(p.weight), y.data_ptr(),
                        y_scale.defined() ? static_cast<float*>(y_scale.data_ptr()) : nullptr,
                        added ? h.data_ptr() : nullptr, static_cast<float*>(rstd.data_ptr()), r.R, r.D, r.ld, res.ld, ldy,
-                       r.D, x_code, r_code, code_of(type), p.code, (float)eps, stream_of(args[5])));
+                       r.D, y_scale.defined() ? y_scale.stride(0) : 0, y_scale.defined() ? y_scale.stride(1) : 0, x_code, r_code, code_of(type), p.code, (float)eps, stream_of(args[5])));
   if (!y_scale.defined()) return tuple({y, h, rstd});
   PyObject* t = PyTuple_New(3);
   if (t == nullptr) throw python_error();
@@ -560,7 +561,7 @@ PyObject* build_rms_backward(PyObject* const* args) {
 }
 
 // A (codes, scales) pair: codes whose rows are contiguous (copied if they are
-// not), contiguous scales of blocks of 1 or 128 rows.
+// not), scales of blocks of 1 or 128 rows.
 struct Fp8 {
   at::Tensor codes, scales;
   int64_t R, C, ld;
@@ -589,7 +590,7 @@ struct Fp8 {
                 std::to_string(G) + ")");
     block = s.size(0) == R ? 1 : kGroup;
     codes = (C > 1 && c.stride(1) != 1) || (R > 1 && c.stride(0) < C) ? c.contiguous() : c;
-    scales = s.contiguous();
+    scales = R > 1 && s.stride(0) > kMaxScaleRow ? s.contiguous() : s;
     ld = R > 1 ? codes.stride(0) : C;
     code = code_of(c.scalar_type());
   }
@@ -617,7 +618,7 @@ PyObject* build_quantize(PyObject* const* args) {
   const NewFp8 q(R, C, b[0], type, x.options());
   const int64_t ld = cols ? (C > 1 ? t.stride(1) : R) : (R > 1 ? t.stride(0) : C);
   check(tilec_quantize_fp8(t.const_data_ptr(), q.codes.data_ptr(), static_cast<float*>(q.scales.data_ptr()), R, C, ld,
-                           q.ld, cols ? TILEC_X1_COL_MAJOR : 0, x_code, code_of(type), (int32_t)b[0], stream_of(args[3])));
+                           q.ld, q.scales.stride(0), q.scales.stride(1), cols ? TILEC_X1_COL_MAJOR : 0, x_code, code_of(type), (int32_t)b[0], stream_of(args[3])));
   return tuple({q.codes, q.scales});
 }
 
@@ -629,7 +630,7 @@ PyObject* build_dequantize(PyObject* const* args) {
   const c10::DeviceGuard guard(q.codes.device());
   const at::Tensor out = at::empty({q.R, q.C}, q.scales.options().dtype(type));
   check(tilec_dequantize_fp8(q.codes.const_data_ptr(), static_cast<const float*>(q.scales.const_data_ptr()), out.data_ptr(),
-                             q.R, q.C, q.ld, q.C, q.code, code_of(type), q.block, stream_of(args[2])));
+                             q.R, q.C, q.ld, q.C, q.scales.stride(0), q.scales.stride(1), q.code, code_of(type), q.block, stream_of(args[2])));
   return THPVariable_Wrap(out);
 }
 
@@ -643,13 +644,13 @@ PyObject* build_linear(PyObject* const* args) {
   const c10::DeviceGuard guard(x.codes.device());
   const at::Tensor out = at::empty({x.R, w.R}, x.scales.options().dtype(type));
   const void *xp = x.codes.const_data_ptr(), *wp = w.codes.const_data_ptr();
-  const size_t need = tilec_linear_fp8_workspace_bytes(xp, wp, x.R, w.R, x.C, x.ld, w.ld, x.code, w.code, code_of(type),
-                                                       x.block, w.block);
+  const size_t need =
+      tilec_linear_fp8_workspace_bytes(xp, wp, x.R, w.R, x.C, x.ld, w.ld, x.code, w.code, code_of(type));
   at::Tensor scratch;
   if (need > 0) scratch = at::empty({(int64_t)need}, x.scales.options().dtype(at::kByte));
   check(tilec_linear_fp8(xp, static_cast<const float*>(x.scales.const_data_ptr()), wp,
                          static_cast<const float*>(w.scales.const_data_ptr()), out.data_ptr(), x.R, w.R, x.C, x.ld, w.ld,
-                         w.R, x.code, w.code, code_of(type), x.block, w.block, need > 0 ? scratch.data_ptr() : nullptr, need,
+                         w.R, x.scales.stride(0), x.scales.stride(1), w.scales.stride(0), w.scales.stride(1), x.code, w.code, code_of(type), x.block, w.block, need > 0 ? scratch.data_ptr() : nullptr, need,
                          stream_of(args[3])));
   return THPVariable_Wrap(out);
 }

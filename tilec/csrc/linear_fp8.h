@@ -30,6 +30,7 @@ struct Fp8Args {
   void* out;
   float* partial;  // [splits][M][N], where there are several
   int64_t ldx, ldw, ldo;
+  int64_t sx_row, sx_group, sw_row, sw_group;  // strides of the scales
   int M, N, K, G;      // G: groups of K
   int xshift, wshift;  // rows of a scale: 1 << shift
   int group_m, xcds, split_steps;

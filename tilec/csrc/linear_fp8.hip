@@ -11,6 +11,8 @@ namespace {
 
 typedef unsigned short u16;
 
+constexpr int64_t kMaxScaleRow = int64_t(1) << 21, kMaxScaleGroup = int64_t(1) << 40;
+
 struct Plan {
   int tile;            // -1: the streaming kernel
   int splits, steps;   // groups of K a split
@@ -21,6 +23,11 @@ struct Plan {
 };
 
 size_t round16(int64_t n) { return (size_t)(n + 15) / 16 * 16; }
+
+struct Scales {
+  int block;
+  int64_t row, group;  // strides
+};
 
 Plan plan_of(const void* x, const void* w, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, bool f8) {
   Plan p{};
@@ -86,7 +93,7 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(const float* __restrict__
 }
 
 int check_linear(int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int32_t x_dtype, int32_t w_dtype,
-                 int32_t out_dtype, int32_t x_block, int32_t w_block) {
+                 int32_t out_dtype, Scales sx, Scales sw) {
   if (!is_fp8(x_dtype) || !is_fp8(w_dtype))
     return fail(TILEC_ERR_TYPE, "tilec: linear_fp8: unsupported dtype codes %d, %d of x and weight (use an 8-bit type)",
                 x_dtype, w_dtype);
@@ -97,8 +104,12 @@ int check_linear(int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int3
   if ((M > 1 && (ldx < K || ldx > (int64_t(1) << 40))) || (N > 1 && (ldw < K || ldw > (int64_t(1) << 40))))
     return fail(TILEC_ERR_VALUE, "tilec: linear_fp8: bad row strides ldx=%lld ldw=%lld for K=%lld", (long long)ldx,
                 (long long)ldw, (long long)K);
-  if ((x_block != 1 && x_block != kGroup) || (w_block != 1 && w_block != kGroup))
-    return fail(TILEC_ERR_VALUE, "tilec: linear_fp8: blocks have 1 or 128 rows (got %d and %d)", x_block, w_block);
+  if ((sx.block != 1 && sx.block != kGroup) || (sw.block != 1 && sw.block != kGroup))
+    return fail(TILEC_ERR_VALUE, "tilec: linear_fp8: blocks have 1 or 128 rows (got %d and %d)", sx.block, sw.block);
+  // (256 rows' scales lie within 2^31 bytes.)
+  for (const Scales& s : {sx, sw})
+    if (s.row < 0 || s.group < 0 || s.row > kMaxScaleRow || s.group > kMaxScaleGroup)
+      return fail(TILEC_ERR_VALUE, "tilec: linear_fp8: bad strides %lld, %lld of scales", (long long)s.row, (long long)s.group);
   return TILEC_OK;
 }
 
@@ -111,20 +122,20 @@ using namespace tilec;
 extern "C" {
 
 size_t tilec_linear_fp8_workspace_bytes(const void* x, const void* weight, int64_t M, int64_t N, int64_t K, int64_t ldx,
-                                        int64_t ldw, int32_t x_dtype, int32_t w_dtype, int32_t out_dtype,
-                                        int32_t x_block, int32_t w_block) {
-  if (check_linear(M, N, K, ldx, ldw, x_dtype, w_dtype, out_dtype, x_block, w_block) != TILEC_OK || M == 0 || N == 0 ||
-      K == 0)
-    return 0;
+                                        int64_t ldw, int32_t x_dtype, int32_t w_dtype, int32_t out_dtype) {
+  const Scales sx{1, 0, 0}, sw{1, 0, 0};
+  if (check_linear(M, N, K, ldx, ldw, x_dtype, w_dtype, out_dtype, sx, sw) != TILEC_OK || M == 0 || N == 0 || K == 0) return 0;
   return plan_of(x, weight, M, N, K, ldx, ldw, out_dtype == TILEC_BF16).bytes();
 }
 
 int tilec_linear_fp8(const void* x, const float* x_scale, const void* weight, const float* w_scale, void* out,
-                     int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldo, int32_t x_dtype,
-                     int32_t w_dtype, int32_t out_dtype, int32_t x_block, int32_t w_block, void* workspace,
-                     size_t workspace_bytes, void* stream) {
+                     int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldo, int64_t x_scale_row,
+                     int64_t x_scale_group, int64_t w_scale_row, int64_t w_scale_group, int32_t x_dtype, int32_t w_dtype,
+                     int32_t out_dtype, int32_t x_block, int32_t w_block, void* workspace, size_t workspace_bytes,
+                     void* stream) {
   clear_error();
-  const int rc = check_linear(M, N, K, ldx, ldw, x_dtype, w_dtype, out_dtype, x_block, w_block);
+  const Scales sx{x_block, x_scale_row, x_scale_group}, sw{w_block, w_scale_row, w_scale_group};
+  const int rc = check_linear(M, N, K, ldx, ldw, x_dtype, w_dtype, out_dtype, sx, sw);
   if (rc != TILEC_OK) return rc;
   if (M == 0 || N == 0) return TILEC_OK;
   if (M > 1 && (ldo < N || ldo > (int64_t(1) << 40)))
@@ -132,7 +143,9 @@ int tilec_linear_fp8(const void* x, const float* x_scale, const void* weight, co
   if (out == nullptr || (K > 0 && (x == nullptr || weight == nullptr || x_scale == nullptr || w_scale == nullptr)))
     return fail(TILEC_ERR_VALUE, "tilec: linear_fp8: a pointer is NULL");
   const bool f8 = out_dtype == TILEC_BF16;
-  const Plan p = K > 0 ? plan_of(x, weight, M, N, K, ldx, ldw, f8) : Plan{3, 1, 0, false, false, 0, 0, 0, 0};
+  Plan none{};
+  none.tile = kFp8TileCount - 1, none.splits = 1;
+  const Plan p = K > 0 ? plan_of(x, weight, M, N, K, ldx, ldw, f8) : none;
   if (p.bytes() > 0 && (workspace == nullptr || workspace_bytes < p.bytes()))
     return fail(TILEC_ERR_WORKSPACE, "tilec: linear_fp8 needs %zu workspace bytes (got %zu)", p.bytes(),
                 workspace == nullptr ? (size_t)0 : workspace_bytes);
@@ -148,6 +161,7 @@ int tilec_linear_fp8(const void* x, const float* x_scale, const void* weight, co
   a.x = p.copy_x ? reinterpret_cast<unsigned char*>(ws) : static_cast<const unsigned char*>(x);
   a.w = p.copy_w ? reinterpret_cast<unsigned char*>(ws + p.x_bytes) : static_cast<const unsigned char*>(weight);
   a.sx = x_scale, a.sw = w_scale, a.out = out;
+  a.sx_row = sx.row, a.sx_group = sx.group, a.sw_row = sw.row, a.sw_group = sw.group;
   a.partial = reinterpret_cast<float*>(ws + p.x_bytes + p.w_bytes);
   // (One row has no stride; its length stands in.)
   a.ldx = p.copy_x || M == 1 ? p.padded : ldx, a.ldw = p.copy_w || N == 1 ? p.padded : ldw, a.ldo = M > 1 ? ldo : N;

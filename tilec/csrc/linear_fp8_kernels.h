@@ -154,13 +154,13 @@ __global__ __launch_bounds__(P::NT, 1) void fp8_tile_kernel(Fp8Args a) {
     const int first = 64 * (wave * P::SI + i);  // wave-uniform
     const bool is_x = first < P::BM;
     const int e = first + lane - (is_x ? 0 : P::BM), shift = is_x ? a.xshift : a.wshift, r0 = is_x ? m0 : n0;
-    off_s[i] = 4u * (uint32_t)(((r0 + e) >> shift) - (r0 >> shift)) * (uint32_t)a.G |
+    off_s[i] = 4u * (uint32_t)(((r0 + e) >> shift) - (r0 >> shift)) * (uint32_t)(is_x ? a.sx_row : a.sw_row) |
                oob_unless(r0 + e < (is_x ? a.M : a.N) && (is_x || e < P::BN));
   }
   const unsigned char* const xb = a.x + (int64_t)m0 * a.ldx + (int64_t)g0 * kGroup;
   const unsigned char* const wb = a.w + (int64_t)n0 * a.ldw + (int64_t)g0 * kGroup;
-  const float* const sxb = a.sx + (int64_t)(m0 >> a.xshift) * a.G + g0;
-  const float* const swb = a.sw + (int64_t)(n0 >> a.wshift) * a.G + g0;
+  const float* const sxb = a.sx + (int64_t)(m0 >> a.xshift) * a.sx_row + (int64_t)g0 * a.sx_group;
+  const float* const swb = a.sw + (int64_t)(n0 >> a.wshift) * a.sw_row + (int64_t)g0 * a.sw_group;
   // A step past the last has resources without records: nothing is read.
   auto copy = [&](int kt, char* st) __attribute__((always_inline)) {
     const uint32_t records = kt < nk ? 0x7FFFFFFFu : 0u;
@@ -184,7 +184,7 @@ __global__ __launch_bounds__(P::NT, 1) void fp8_tile_kernel(Fp8Args a) {
     for (int i = 0; i < P::SI; ++i) {
       const int first = 64 * (wave * P::SI + i);
       const uint32_t off = off_s[i];
-      const BufRsrc rs = make_rsrc_uniform((first < P::BM ? sxb : swb) + kt, records);
+      const BufRsrc rs = make_rsrc_uniform(first < P::BM ? sxb + kt * a.sx_group : swb + kt * a.sw_group, records);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(st + P::S_AT + 4 * first), 4, off, 0, 0, 0);
     }
   };
@@ -408,12 +408,13 @@ __global__ __launch_bounds__(512, 1) void fp8_pair_kernel(Fp8Args a) {
     const int first = 64 * (w4 * SI + i);
     const bool is_x = first < P::BM;
     const int e = first + lane - (is_x ? 0 : P::BM), shift = is_x ? a.xshift : a.wshift, r0 = is_x ? m0 : n0;
-    off_s[i] = 4u * (uint32_t)(((r0 + e) >> shift) - (r0 >> shift)) * (uint32_t)a.G | oob_unless(r0 + e < (is_x ? a.M : a.N) && (is_x || e < P::BN));
+    off_s[i] = 4u * (uint32_t)(((r0 + e) >> shift) - (r0 >> shift)) * (uint32_t)(is_x ? a.sx_row : a.sw_row) |
+               oob_unless(r0 + e < (is_x ? a.M : a.N) && (is_x || e < P::BN));
   }
   const unsigned char* const xb = a.x + (int64_t)m0 * a.ldx + (int64_t)g0 * kGroup;
   const unsigned char* const wb = a.w + (int64_t)n0 * a.ldw + (int64_t)g0 * kGroup;
-  const float* const sxb = a.sx + (int64_t)(m0 >> a.xshift) * a.G + g0;
-  const float* const swb = a.sw + (int64_t)(n0 >> a.wshift) * a.G + g0;
+  const float* const sxb = a.sx + (int64_t)(m0 >> a.xshift) * a.sx_row + (int64_t)g0 * a.sx_group;
+  const float* const swb = a.sw + (int64_t)(n0 >> a.wshift) * a.sw_row + (int64_t)g0 * a.sw_group;
   // Bytes of the tile's rows: what lies past the last row is past the end.
   const uint32_t x_bytes = a.M - m0 >= P::BM ? 0x7FFFFFFFu : (uint32_t)(a.M - m0) * (uint32_t)a.ldx;
   const uint32_t w_bytes = a.N - n0 >= P::BN ? 0x7FFFFFFFu : (uint32_t)(a.N - n0) * (uint32_t)a.ldw;
@@ -445,7 +446,7 @@ __global__ __launch_bounds__(512, 1) void fp8_pair_kernel(Fp8Args a) {
     for (int i = 0; i < SI; ++i) {
       const int first = 64 * (w4 * SI + i);
       const uint32_t off = off_s[i];
-      const BufRsrc rs = make_rsrc_uniform((first < P::BM ? sxb : swb) + kt, kt < nk ? 0x7FFFFFFFu : 0u);
+      const BufRsrc rs = make_rsrc_uniform(first < P::BM ? sxb + kt * a.sx_group : swb + kt * a.sw_group, kt < nk ? 0x7FFFFFFFu : 0u);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(st.s + first), 4, off, 0, 0, 0);
     }
   };
@@ -617,8 +618,8 @@ __global__ __launch_bounds__(64 * NW, 1) void fp8_stream_kernel(Fp8Args a) {
   for (int i = 0; i < 2; ++i) off_w[i] = (8 * i + (lane >> 3)) * (uint32_t)a.ldw + 16u * (c0 ^ 4 * i);
 #pragma unroll
   for (int i = 0; i < XR; ++i) off_x[i] = (8 * i + (lane >> 3)) * (uint32_t)a.ldx + 16u * (c0 ^ 4 * i);
-  const uint32_t off_sx = 4u * (uint32_t)(lane >> a.xshift) * (uint32_t)a.G | oob_unless(lane < a.M);
-  const uint32_t off_sw = 4u * (uint32_t)(lane >> a.wshift) * (uint32_t)a.G | oob_unless(lane < 16);
+  const uint32_t off_sx = 4u * (uint32_t)(lane >> a.xshift) * (uint32_t)a.sx_row | oob_unless(lane < a.M);
+  const uint32_t sw_step = 4u * (uint32_t)(lane >> a.wshift) * (uint32_t)a.sw_row;
 
   int tile = blockIdx.x, g = wave, left = items, to = 0;  // of the next copies
   auto copy = [&]() __attribute__((always_inline)) {
@@ -628,9 +629,9 @@ __global__ __launch_bounds__(64 * NW, 1) void fp8_stream_kernel(Fp8Args a) {
     const int64_t w_rows = a.N - n0 < 16 ? a.N - n0 : 16;
     const BufRsrc rw = make_rsrc_uniform(a.w + (int64_t)n0 * a.ldw + skip, live ? (uint32_t)(w_rows * a.ldw - skip) : 0u);
     const BufRsrc rx = make_rsrc_uniform(a.x + skip, live ? (uint32_t)(a.M * a.ldx - skip) : 0u);
-    const BufRsrc rsx = make_rsrc_uniform(a.sx + g, live ? 0x7FFFFFFFu : 0u);
-    const BufRsrc rsw = make_rsrc_uniform(a.sw + (int64_t)(n0 >> a.wshift) * a.G + g,
-                                          live ? (WROWS ? 4u * (uint32_t)(w_rows * a.G - g) : 4u) : 0u);
+    const BufRsrc rsx = make_rsrc_uniform(a.sx + g * a.sx_group, live ? 0x7FFFFFFFu : 0u);
+    const BufRsrc rsw = make_rsrc_uniform(a.sw + (int64_t)(n0 >> a.wshift) * a.sw_row + g * a.sw_group, live ? 0x7FFFFFFFu : 0u);
+    const uint32_t off_sw = sw_step | oob_unless(lane < w_rows);
     char* const at = ring[wave][to];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {

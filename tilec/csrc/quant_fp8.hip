@@ -26,6 +26,7 @@ struct QuantArgs {
   float* scales;
   int64_t R, C, ldx, ldq;  // of the result; ldx: row stride of x, or of its transpose
   int64_t G;               // scales of a row
+  int64_t s_row, s_group;  // strides of the scales
   int e5m2, lg;            // rows kernel: 2^lg blocks of a row side by side
 };
 
@@ -76,7 +77,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a) {
       for (int o = 1; o < 16; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
       float scale, inverse;
       block_scale(top, fp8_largest(e5m2), scale, inverse);
-      if (sub == 0) a.scales[r * a.G + g] = scale;
+      if (sub == 0) a.scales[r * a.s_row + g * a.s_group] = scale;
       if (c < a.ldq && c / 16 <= (C - 1) / 16)
         *reinterpret_cast<u32x2*>(a.codes + r * a.ldq + c) = codes_of<T>(v[u], inverse, e5m2);
     }
@@ -126,7 +127,7 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a, int tiles_
     block_scale(t, fp8_largest(e5m2), scale, inverse[0]);
 #pragma unroll
     for (int e = 1; e < 8; ++e) inverse[e] = inverse[0];
-    if (tid == 0) a.scales[(int64_t)tr * a.G + tc] = scale;
+    if (tid == 0) a.scales[tr * a.s_row + tc * a.s_group] = scale;
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -142,7 +143,7 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a, int tiles_
     for (int e = 0; e < 8; ++e) {
       const uint32_t t = max(max(red[0][8 * lo + e], red[1][8 * lo + e]), max(red[2][8 * lo + e], red[3][8 * lo + e]));
       block_scale(t, fp8_largest(e5m2), scale, inverse[e]);
-      if (hi == 0 && r0 + 8 * lo + e < a.R) a.scales[(r0 + 8 * lo + e) * a.G + tc] = scale;
+      if (hi == 0 && r0 + 8 * lo + e < a.R) a.scales[(r0 + 8 * lo + e) * a.s_row + tc * a.s_group] = scale;
     }
   }
   const int end = (int)std::min<int64_t>(a.ldq, (int64_t)((C - 1) / 16 + 1) * 16);  // of a row, with the bytes that fill its last 16
@@ -180,7 +181,7 @@ struct ValuesArgs {
   const unsigned char* codes;
   const float* scales;
   void* out;
-  int64_t R, C, ldq, ldo, G;
+  int64_t R, C, ldq, ldo, G, s_row, s_group;
   int shift, e5m2, lg;
 };
 
@@ -201,7 +202,7 @@ __global__ __launch_bounds__(256) void values_kernel(ValuesArgs a) {
     for (int u = 0; u < U; ++u) {
       const int64_t r = min(r0 + u * step, a.R - 1);
       const unsigned char* p = a.codes + r * a.ldq + c;
-      s[u] = a.scales[(r >> a.shift) * a.G + g];
+      s[u] = a.scales[(r >> a.shift) * a.s_row + g * a.s_group];
       if (c + 8 <= C) {
         typedef u32x2 __attribute__((aligned(1))) u32x2_any;
         q[u] = *reinterpret_cast<const u32x2_any*>(p);
@@ -261,7 +262,8 @@ using namespace tilec;
 extern "C" {
 
 int tilec_quantize_fp8(const void* x, void* codes, float* scales, int64_t R, int64_t C, int64_t ldx, int64_t ldq,
-                       int32_t layout, int32_t x_dtype, int32_t q_dtype, int32_t block, void* stream) {
+                       int64_t scale_row, int64_t scale_group, int32_t layout, int32_t x_dtype, int32_t q_dtype,
+                       int32_t block, void* stream) {
   clear_error();
   const int rc = check_matrix("quantize_fp8", R, C, x_dtype, q_dtype, block);
   if (rc != TILEC_OK) return rc;
@@ -274,13 +276,15 @@ int tilec_quantize_fp8(const void* x, void* codes, float* scales, int64_t R, int
     return fail(TILEC_ERR_VALUE, "tilec: quantize_fp8: bad stride %lld of x", (long long)ldx);
   if (x == nullptr || codes == nullptr || scales == nullptr)
     return fail(TILEC_ERR_VALUE, "tilec: quantize_fp8: a pointer is NULL");
+  if (scale_row < 0 || scale_group < 0 || scale_row > kMaxStride || scale_group > kMaxStride)
+    return fail(TILEC_ERR_VALUE, "tilec: quantize_fp8: bad strides %lld, %lld of scales", (long long)scale_row, (long long)scale_group);
   if (reinterpret_cast<uintptr_t>(codes) % 16 != 0 || (R > 1 && (ldq % 16 != 0 || ldq < room || ldq > kMaxStride)))
     return fail(TILEC_ERR_VALUE, "tilec: quantize_fp8: rows of codes begin at multiples of 16 bytes (row stride %lld)",
                 (long long)ldq);
   QuantArgs a{};
   a.x = x, a.codes = static_cast<unsigned char*>(codes), a.scales = scales;
   a.R = R, a.C = C, a.ldx = rows > 1 ? ldx : cols, a.ldq = R > 1 ? ldq : room, a.G = cdiv(C, kGroup);
-  a.e5m2 = q_dtype == TILEC_F8E5M2;
+  a.s_row = scale_row, a.s_group = scale_group, a.e5m2 = q_dtype == TILEC_F8E5M2;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   auto by_type = [&](auto t) {
     using T = decltype(t);
@@ -304,7 +308,8 @@ int tilec_quantize_fp8(const void* x, void* codes, float* scales, int64_t R, int
 }
 
 int tilec_dequantize_fp8(const void* codes, const float* scales, void* out, int64_t R, int64_t C, int64_t ldq,
-                         int64_t ldo, int32_t q_dtype, int32_t out_dtype, int32_t block, void* stream) {
+                         int64_t ldo, int64_t scale_row, int64_t scale_group, int32_t q_dtype, int32_t out_dtype,
+                         int32_t block, void* stream) {
   clear_error();
   const int rc = check_matrix("dequantize_fp8", R, C, out_dtype, q_dtype, block);
   if (rc != TILEC_OK) return rc;
@@ -313,10 +318,12 @@ int tilec_dequantize_fp8(const void* codes, const float* scales, void* out, int6
     return fail(TILEC_ERR_VALUE, "tilec: dequantize_fp8: bad row strides %lld, %lld", (long long)ldq, (long long)ldo);
   if (codes == nullptr || scales == nullptr || out == nullptr)
     return fail(TILEC_ERR_VALUE, "tilec: dequantize_fp8: a pointer is NULL");
+  if (scale_row < 0 || scale_group < 0 || scale_row > kMaxStride || scale_group > kMaxStride)
+    return fail(TILEC_ERR_VALUE, "tilec: dequantize_fp8: bad strides %lld, %lld of scales", (long long)scale_row, (long long)scale_group);
   ValuesArgs a{};
   a.codes = static_cast<const unsigned char*>(codes), a.scales = scales, a.out = out;
   a.R = R, a.C = C, a.ldq = ldq, a.ldo = ldo, a.G = cdiv(C, kGroup);
-  a.shift = block == 1 ? 0 : 7, a.e5m2 = q_dtype == TILEC_F8E5M2;
+  a.s_row = scale_row, a.s_group = scale_group, a.shift = block == 1 ? 0 : 7, a.e5m2 = q_dtype == TILEC_F8E5M2;
   const dim3 grid = rows_grid(R, a.G, a.lg);
   if (out_dtype == TILEC_F32)
     hipLaunchKernelGGL(values_kernel<float>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);

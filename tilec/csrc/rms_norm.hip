@@ -38,6 +38,7 @@ struct RmsArgs {
   const float* rstd_in;
   float *dw, *partial;    // backward: dw NULL where not wanted
   int64_t ldx, ldr, ldy, ldh, lddh, lddx;  // ldy: of y, or of dy; ldh: of h written; ldx: of h read
+  int64_t s_row, s_group;  // strides of y's scales
   int64_t R;
   int D, Dp;  // Dp: columns of a partial row
   int y_type, w_bf16, tpr, groups;  // groups: scales of a row of y
@@ -91,7 +92,7 @@ __device__ __forceinline__ void store_y(const RmsArgs& a, int64_t r, int c, cons
   uint32_t* const out = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(a.y) + r * a.ldy + c);
 #pragma unroll
   for (int i = 0; i < E / 4; ++i) out[i] = q[i];
-  if (c % kGroup == 0) a.y_scale[r * a.groups + c / kGroup] = scale;
+  if (c % kGroup == 0) a.y_scale[r * a.s_row + c / kGroup * a.s_group] = scale;
 }
 
 template <typename TX, typename TR, int NV, int NT>
@@ -489,7 +490,7 @@ extern "C" {
 
 int tilec_rms_norm(const void* x, const void* residual, const void* weight, void* y, float* y_scale, void* h,
                    float* rstd, int64_t R, int64_t D, int64_t ldx, int64_t ldr, int64_t ldy, int64_t ldh,
-                   int32_t x_dtype, int32_t r_dtype, int32_t y_dtype, int32_t w_dtype, float eps, void* stream) {
+                   int64_t scale_row, int64_t scale_group, int32_t x_dtype, int32_t r_dtype, int32_t y_dtype, int32_t w_dtype, float eps, void* stream) {
   clear_error();
   if (!is_wide(x_dtype) || (residual != nullptr && !is_wide(r_dtype)) || !is_wide(w_dtype) ||
       (!is_wide(y_dtype) && !is_fp8(y_dtype)))
@@ -505,8 +506,11 @@ int tilec_rms_norm(const void* x, const void* residual, const void* weight, void
   if (is_fp8(y_dtype) && (y_scale == nullptr || reinterpret_cast<uintptr_t>(y) % 16 != 0 ||
                           (R > 1 && (ldy % 16 != 0 || ldy < room))))
     return fail(TILEC_ERR_VALUE, "tilec: RMS norm: 8-bit codes need scales and rows at multiples of 16 bytes");
+  if (is_fp8(y_dtype) && (scale_row < 0 || scale_group < 0 || scale_row > (int64_t(1) << 40) || scale_group > (int64_t(1) << 40)))
+    return fail(TILEC_ERR_VALUE, "tilec: RMS norm: bad strides %lld, %lld of scales", (long long)scale_row, (long long)scale_group);
   RmsArgs a{};
   a.x = x, a.res = residual, a.w = weight, a.y = y, a.y_scale = y_scale, a.h = h, a.rstd = rstd;
+  a.s_row = scale_row, a.s_group = scale_group;
   a.ldx = ldx, a.ldr = ldr, a.ldy = is_fp8(y_dtype) && R == 1 ? room : ldy, a.ldh = ldh;
   a.R = R, a.D = (int)D, a.y_type = y_dtype, a.w_bf16 = w_dtype == TILEC_BF16, a.groups = (int)cdiv(D, kGroup);
   a.eps = eps, a.inv_d = 1.f / (float)D;
