@@ -59,7 +59,7 @@ def _host():
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-I" + sysconfig.get_paths()["include"], *("-isystem" + p for p in cpp_extension.include_paths()),
            os.path.join(CSRC, "host.cpp"), "-o", tmp, "-L" + torch_lib, "-Wl,-rpath," + torch_lib,
-           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-L" + HERE, "-Wl,-rpath,$ORIGIN", "-ltilec_hip"]
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-L" + HERE, "-Wl,-rpath,$ORIGIN", "-ltilec_hip"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"building {HOST} failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")

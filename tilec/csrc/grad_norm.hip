@@ -25,14 +25,23 @@ namespace {
 typedef unsigned short u16;
 typedef u32x4 __attribute__((aligned(2))) u32x4_any;
 
-constexpr int kMaxTensors = 120;  // per launch: 3.8 KiB of arguments
+constexpr int kMaxTensors = 128;  // per launch: 2.1 KiB of arguments
 constexpr int kUnit = 4096;       // chunks are a multiple of this
 
+constexpr int64_t kMaxBlocks = int64_t(1) << 22;  // workgroups of a launch
+constexpr int64_t kMaxPiece = int64_t(1) << 38;   // values of a piece of a tensor: at most kMaxBlocks chunks
+
+// A tensor, or a piece of one: 16 bytes, since a launch takes the longer the more
+// its arguments are.
 struct Tensor {
   void* data;
-  int64_t n;
-  int first;  // the tensor's first workgroup
-  int bf16;
+  uint64_t packed;  // n (39 bits), the first workgroup (23), bf16 (1)
+  __host__ __device__ int64_t n() const { return (int64_t)(packed & ((uint64_t(1) << 39) - 1)); }
+  __host__ __device__ int first() const { return (int)(packed >> 39 & ((1 << 23) - 1)); }
+  __host__ __device__ bool bf16() const { return packed >> 62 != 0; }
+  static Tensor of(void* data, int64_t n, int64_t first, bool bf16) {
+    return {data, (uint64_t)n | (uint64_t)first << 39 | (uint64_t)bf16 << 62};
+  }
 };
 
 struct GradArgs {
@@ -51,7 +60,7 @@ __device__ __forceinline__ const Tensor& tensor_of(const GradArgs& a, int b) {
   int lo = 0, hi = a.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (a.t[mid].first <= b) lo = mid;
+    if (a.t[mid].first() <= b) lo = mid;
     else hi = mid - 1;
   }
   return a.t[lo];
@@ -118,9 +127,9 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(GradArgs a) {
   __shared__ int last;
   if (a.count > 0) {
     const Tensor& t = tensor_of(a, blockIdx.x);
-    const int64_t at = (int64_t)((int)blockIdx.x - t.first) * a.chunk;
-    const int n = (int)min((int64_t)a.chunk, t.n - at);
-    double s = t.bf16 ? squares<true>(static_cast<const u16*>(t.data) + at, n)
+    const int64_t at = (int64_t)((int)blockIdx.x - t.first()) * a.chunk;
+    const int n = (int)min((int64_t)a.chunk, t.n() - at);
+    double s = t.bf16() ? squares<true>(static_cast<const u16*>(t.data) + at, n)
                       : squares<false>(static_cast<const float*>(t.data) + at, n);
     s = block_sum(s, red);
     if (threadIdx.x == 0)
@@ -156,8 +165,8 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(GradArgs a) {
   const float f = *a.scale_in;
   if (f == 1.f) return;
   const Tensor& t = tensor_of(a, blockIdx.x);
-  const int64_t at = (int64_t)((int)blockIdx.x - t.first) * a.chunk;
-  const int n = (int)min((int64_t)a.chunk, t.n - at);
+  const int64_t at = (int64_t)((int)blockIdx.x - t.first()) * a.chunk;
+  const int n = (int)min((int64_t)a.chunk, t.n() - at);
   auto go = [&](auto* x, auto bf16) {
     constexpr bool BF16 = decltype(bf16)::value;
     constexpr int E = BF16 ? 8 : 4, U = 4;
@@ -192,7 +201,7 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(GradArgs a) {
       }
     }
   };
-  if (t.bf16) go(static_cast<u16*>(t.data) + at, std::true_type{});
+  if (t.bf16()) go(static_cast<u16*>(t.data) + at, std::true_type{});
   else go(static_cast<float*>(t.data) + at, std::false_type{});
 }
 
@@ -215,7 +224,6 @@ int64_t chunks_of(const tilec_grad* grads, int32_t count, int chunk) {
 // workgroups each; a.base counts them.
 template <typename F>
 hipError_t in_groups(GradArgs& a, const tilec_grad* grads, int32_t count, F f) {
-  constexpr int64_t kMaxBlocks = int64_t(1) << 22;
   int64_t blocks = 0;
   a.count = 0, a.base = 0;
   auto flush = [&]() -> hipError_t {
@@ -227,13 +235,14 @@ hipError_t in_groups(GradArgs& a, const tilec_grad* grads, int32_t count, F f) {
   };
   for (int i = 0; i < count; ++i) {
     const int64_t esz = grads[i].dtype == TILEC_BF16 ? 2 : 4;
+    static_assert(kMaxBlocks * 16 * kUnit <= kMaxPiece, "a piece's size fits its bits");
     for (int64_t at = 0; at < grads[i].n; at += kMaxBlocks * a.chunk) {
       const int64_t n = std::min(grads[i].n - at, kMaxBlocks * a.chunk), need = cdiv(n, a.chunk);
       if (a.count == kMaxTensors || blocks + need > kMaxBlocks) {
         const hipError_t e = flush();
         if (e != hipSuccess) return e;
       }
-      a.t[a.count++] = {static_cast<char*>(grads[i].data) + at * esz, n, (int)blocks, esz == 2};
+      a.t[a.count++] = Tensor::of(static_cast<char*>(grads[i].data) + at * esz, n, blocks, esz == 2);
       blocks += need;
     }
   }

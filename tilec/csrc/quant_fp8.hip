@@ -30,25 +30,45 @@ struct QuantArgs {
   int e5m2, lg;            // rows kernel: 2^lg blocks of a row side by side
 };
 
-template <typename T>
-__device__ __forceinline__ uint32_t top_of(const Group<T, 8>& g) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(g.get(e)) & 0x7fffffffu);
-  return top;
-}
-
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
+// The 8 of 128 neighbouring values that one of 16 threads holds: in 16-byte pieces,
+// so that a load or store of the 16 threads is one run of 256 bytes (8 fp32 values
+// side by side instead: 35.8 us for 4099 x 3001, transposed and back; 32.1 so).
 template <typename T>
-__device__ __forceinline__ u32x2 codes_of(const Group<T, 8>& g, float inverse, bool e5m2) {
-  u32x2 q;
+struct Eight {
+  static constexpr int V = 16 / (int)sizeof(T), PIECES = 8 / V;
+  Group<T, V> g[PIECES];
+  __device__ __forceinline__ static int at(int sub, int e) { return V * sub + 128 / PIECES * (e / V) + e % V; }
+  __device__ __forceinline__ float get(int e) const { return g[e / V].get(e % V); }
+  __device__ __forceinline__ void load(const T* row, int c, int sub, int D) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    q[i] = to_fp8(g.get(4 * i) * inverse, g.get(4 * i + 1) * inverse, g.get(4 * i + 2) * inverse,
-                  g.get(4 * i + 3) * inverse, e5m2);
-  return q;
-}
+    for (int i = 0; i < PIECES; ++i) g[i].load(row, c + at(sub, V * i), D);
+  }
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t t = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t = max(t, __float_as_uint(get(e)) & 0x7fffffffu);
+    return t;
+  }
+  // The codes at columns c + .. of a row, up to column `end` (a multiple of 16).
+  __device__ __forceinline__ void store(unsigned char* row, int c, int sub, int end, float inverse, bool e5m2) const {
+    uint32_t q[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      q[i] = to_fp8(get(4 * i) * inverse, get(4 * i + 1) * inverse, get(4 * i + 2) * inverse, get(4 * i + 3) * inverse, e5m2);
+    if constexpr (PIECES == 1) {
+      if (c + at(sub, 0) < end) *reinterpret_cast<u32x2*>(row + c + at(sub, 0)) = u32x2{q[0], q[1]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (c + at(sub, 4 * i) < end) *reinterpret_cast<uint32_t*>(row + c + at(sub, 4 * i)) = q[i];
+    }
+  }
+};
+
+// Where a row of codes ends: with the bytes that fill its last 16.
+__device__ __forceinline__ int row_end(int C) { return (C + 15) / 16 * 16; }
 
 // A workgroup takes 2^lg blocks of 16 >> lg rows at a time, U of those in flight.
 template <typename T>
@@ -58,28 +78,27 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a) {
   const int64_t g = ((int64_t)blockIdx.x << a.lg) + (slot & ((1 << a.lg) - 1));
   if (g >= a.G) return;
   const int rpb = 16 >> a.lg;
-  const int c = (int)(g * kGroup) + 8 * sub, C = (int)a.C;
+  const int c = (int)(g * kGroup), C = (int)a.C;
   const bool e5m2 = a.e5m2;
   const int64_t step = (int64_t)gridDim.y * rpb;
   for (int64_t r0 = (int64_t)blockIdx.y * rpb + (slot >> a.lg); r0 < a.R; r0 += U * step) {
-    Group<T, 8> v[U];
+    Eight<T> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t r = min(r0 + u * step, a.R - 1);
-      v[u].load(static_cast<const T*>(a.x) + r * a.ldx, c, C);
+      v[u].load(static_cast<const T*>(a.x) + r * a.ldx, c, sub, C);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t r = r0 + u * step;
       if (r >= a.R) break;
-      uint32_t top = top_of<T>(v[u]);
+      uint32_t top = v[u].top();
 #pragma unroll
       for (int o = 1; o < 16; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
       float scale, inverse;
       block_scale(top, fp8_largest(e5m2), scale, inverse);
       if (sub == 0) a.scales[r * a.s_row + g * a.s_group] = scale;
-      if (c < a.ldq && c / 16 <= (C - 1) / 16)
-        *reinterpret_cast<u32x2*>(a.codes + r * a.ldq + c) = codes_of<T>(v[u], inverse, e5m2);
+      v[u].store(a.codes + r * a.ldq, c, sub, row_end(C), inverse, e5m2);
     }
   }
 }
@@ -96,17 +115,18 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a, int tiles_
   const int64_t r0 = (int64_t)tr * 128;
   const int c0 = tc * 128, C = (int)a.C;
   const bool e5m2 = a.e5m2;
-  // TRANS: v[p] is memory row c0 + 8 hi + p (a column of the result), its values
-  // those of the result's rows r0 + 8 lo ..; otherwise row r0 + 16 p + hi, columns
-  // c0 + 8 lo ...
-  Group<T, 8> v[8];
+  // TRANS: v[p] is of memory row c0 + 8 hi + p (a column of the result), its values
+  // those of eight of the result's rows from r0 on; otherwise of row r0 + 16 p + hi,
+  // eight columns from c0 on.
+  auto mine = [&](int e) { return Eight<T>::at(lo, e); };
+  Eight<T> v[8];
   uint32_t top[8];
 #pragma unroll
   for (int p = 0; p < 8; ++p) {
     const int64_t m = TRANS ? c0 + 8 * hi + p : r0 + 16 * p + hi;
     const bool live = m < (TRANS ? a.C : a.R);
     const T* row = static_cast<const T*>(a.x) + (live ? m : 0) * a.ldx;
-    v[p].load(row, TRANS ? (int)r0 + 8 * lo : c0 + 8 * lo, live ? (int)(TRANS ? a.R : a.C) : 0);
+    v[p].load(row, TRANS ? (int)r0 : c0, lo, live ? (int)(TRANS ? a.R : a.C) : 0);
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -136,26 +156,28 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a, int tiles_
     }
     if ((hi & 3) == 0) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) red[wave][8 * lo + e] = top[e];
+      for (int e = 0; e < 8; ++e) red[wave][mine(e)] = top[e];
     }
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const uint32_t t = max(max(red[0][8 * lo + e], red[1][8 * lo + e]), max(red[2][8 * lo + e], red[3][8 * lo + e]));
+      const int r = mine(e);
+      const uint32_t t = max(max(red[0][r], red[1][r]), max(red[2][r], red[3][r]));
       block_scale(t, fp8_largest(e5m2), scale, inverse[e]);
-      if (hi == 0 && r0 + 8 * lo + e < a.R) a.scales[(r0 + 8 * lo + e) * a.s_row + tc * a.s_group] = scale;
+      if (hi == 0 && r0 + r < a.R) a.scales[(r0 + r) * a.s_row + tc * a.s_group] = scale;
     }
   }
-  const int end = (int)std::min<int64_t>(a.ldq, (int64_t)((C - 1) / 16 + 1) * 16);  // of a row, with the bytes that fill its last 16
+  const int end = row_end(C);
   if constexpr (!TRANS) {
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
       const int64_t r = r0 + 16 * p + hi;
-      if (r < a.R && c0 + 8 * lo < end)
-        *reinterpret_cast<u32x2*>(a.codes + r * a.ldq + c0 + 8 * lo) = codes_of<T>(v[p], inverse[0], e5m2);
+      if (r < a.R) v[p].store(a.codes + r * a.ldq, c0, lo, end, inverse[0], e5m2);
     }
   } else {
-    // Row 8 lo + e of the tile, columns 8 hi ..: 8-byte piece hi of its 16, at hi ^ lo.
+    // Row mine(e) of the tile, columns 8 hi ..: 8-byte piece hi of its 16, exchanged
+    // by rows (by lo).
+    constexpr int ROWS = Eight<T>::V;  // side by side in one thread
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       u32x2 q;
@@ -163,12 +185,12 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a, int tiles_
       for (int i = 0; i < 2; ++i)
         q[i] = to_fp8(v[4 * i].get(e) * inverse[e], v[4 * i + 1].get(e) * inverse[e], v[4 * i + 2].get(e) * inverse[e],
                       v[4 * i + 3].get(e) * inverse[e], e5m2);
-      *reinterpret_cast<u32x2*>(out + 128 * (8 * lo + e) + 8 * (hi ^ lo)) = q;
+      *reinterpret_cast<u32x2*>(out + 128 * mine(e) + 8 * (hi ^ lo)) = q;
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int row = 32 * k + (tid >> 3), piece = tid & 7, swap = row >> 3;
+      const int row = 32 * k + (tid >> 3), piece = tid & 7, swap = row / ROWS & 15;
       const u32x2 a0 = *reinterpret_cast<const u32x2*>(out + 128 * row + 8 * ((2 * piece) ^ swap));
       const u32x2 a1 = *reinterpret_cast<const u32x2*>(out + 128 * row + 8 * ((2 * piece + 1) ^ swap));
       if (r0 + row < a.R && c0 + 16 * piece < end)
@@ -188,34 +210,49 @@ struct ValuesArgs {
 // The values that codes stand for, mapped as in quant_rows_kernel.
 template <typename T>
 __global__ __launch_bounds__(256) void values_kernel(ValuesArgs a) {
-  constexpr int U = 4;
+  constexpr int U = 4, V = Eight<T>::V, PIECES = Eight<T>::PIECES;
   const int slot = threadIdx.x >> 4, sub = threadIdx.x & 15;
   const int64_t g = ((int64_t)blockIdx.x << a.lg) + (slot & ((1 << a.lg) - 1));
-  const int64_t c64 = g * kGroup + 8 * sub;
-  if (c64 >= a.C) return;
-  const int c = (int)c64, C = (int)a.C, rpb = 16 >> a.lg;
+  if (g >= a.G) return;
+  const int c = (int)(g * kGroup), C = (int)a.C, rpb = 16 >> a.lg;
   const int64_t step = (int64_t)gridDim.y * rpb;
   for (int64_t r0 = (int64_t)blockIdx.y * rpb + (slot >> a.lg); r0 < a.R; r0 += U * step) {
-    u32x2 q[U];
+    uint32_t q[U][2];
     float s[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t r = min(r0 + u * step, a.R - 1);
-      const unsigned char* p = a.codes + r * a.ldq + c;
       s[u] = a.scales[(r >> a.shift) * a.s_row + g * a.s_group];
-      if (c + 8 <= C) {
-        typedef u32x2 __attribute__((aligned(1))) u32x2_any;
-        q[u] = *reinterpret_cast<const u32x2_any*>(p);
-      } else {
-        q[u] = u32x2{0u, 0u};
-        for (int e = 0; c + e < C; ++e) q[u][e >> 2] |= (uint32_t)p[e] << (8 * (e & 3));
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int k = c + Eight<T>::at(sub, V * i);
+        const unsigned char* p = a.codes + r * a.ldq + k;
+        uint32_t* const to = q[u] + i;  // V codes
+        if (k + V <= C) {
+          typedef u32x2 __attribute__((aligned(1))) u32x2_any;
+          typedef uint32_t __attribute__((aligned(1))) u32_any;
+          if constexpr (V == 8) {
+            const u32x2 w = *reinterpret_cast<const u32x2_any*>(p);
+            to[0] = w.x, to[1] = w.y;
+          } else {
+            to[0] = *reinterpret_cast<const u32_any*>(p);
+          }
+        } else {
+#pragma unroll
+          for (int w = 0; w < V / 4; ++w) {
+            to[w] = 0u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (k + 4 * w + e < C) to[w] |= (uint32_t)p[4 * w + e] << (8 * e);
+          }
+        }
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t r = r0 + u * step;
       if (r >= a.R) break;
-      float v[8];
+      float v[PIECES][V];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -223,9 +260,14 @@ __global__ __launch_bounds__(256) void values_kernel(ValuesArgs a) {
         f32x2 x, y;
         if (a.e5m2) x = __builtin_amdgcn_cvt_pk_f32_bf8(w, false), y = __builtin_amdgcn_cvt_pk_f32_bf8(w, true);
         else x = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), y = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
-        v[4 * i] = x.x * s[u], v[4 * i + 1] = x.y * s[u], v[4 * i + 2] = y.x * s[u], v[4 * i + 3] = y.y * s[u];
+        float* const to = v[4 * i / V] + 4 * i % V;
+        to[0] = x.x * s[u], to[1] = x.y * s[u], to[2] = y.x * s[u], to[3] = y.y * s[u];
       }
-      store_group<T, 8>(static_cast<T*>(a.out) + r * a.ldo, c, C, v);
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int k = c + Eight<T>::at(sub, V * i);
+        if (k < C) store_group<T, V>(static_cast<T*>(a.out) + r * a.ldo, k, C, v[i]);
+      }
     }
   }
 }
