@@ -29,17 +29,13 @@ scratch is each call's own, and there is no autograd.
 import torch
 
 from . import _lib
-from .ext import _raw_stream
+from .training import _stream_of
 
 __all__ = ["quantize_fp8", "dequantize_fp8", "linear_fp8"]
 
 
-def _stream_of(x):
-    """The current stream of the GPU that x is on (0 elsewhere: x is refused)."""
-    return _raw_stream(x.get_device()) if isinstance(x, torch.Tensor) and x.is_cuda else 0
-
-
 def _stream_of_pair(q):
+    """The same for a (codes, scales) pair."""
     return _stream_of(q[0]) if isinstance(q, (tuple, list)) and q else 0
 
 

@@ -64,7 +64,7 @@ def _ptr(t):
 
 def _stream_of(x):
     """The current stream of the GPU that x is on (0 elsewhere: x is refused)."""
-    return _raw_stream(x.get_device()) if x.is_cuda else 0
+    return _raw_stream(x.get_device()) if isinstance(x, torch.Tensor) and x.is_cuda else 0
 
 
 class _Here:
