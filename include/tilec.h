@@ -445,7 +445,7 @@ size_t tilec_rms_norm_backward_workspace_bytes(int64_t R, int64_t D, int32_t h_d
 
 /*
  * The norm of a list of gradients and the factor that clips it to max_norm
- * (negative: no limit), both one float32 on the device:
+ * (negative or infinite: no limit), both one float32 on the device:
  *   norm = |grad_scale| sqrt(sum of all g^2);  scale = grad_scale min(1, max_norm / (norm + 1e-6))
  * grad_scale: one float32 on the device (NULL: 1); scale may be NULL.  Squares
  * and sums are float64, in a fixed order.  An infinite norm gives a scale of 0, a

@@ -362,3 +362,32 @@ def test_cpu_tensors_are_refused():
     for call in (lambda: tilec.ext.quantize_fp8(x), lambda: tilec.ext.dequantize_fp8(q), lambda: tilec.ext.linear_fp8(q, q)):
         with pytest.raises(TypeError):
             call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 100])
+def test_scales_far_apart(rows):
+    # One row's scales, or one tile row's, have no row stride, whatever their view says;
+    # several rows' may lie farther apart than the kernels index.
+    x, w = (tilec.ext.quantize_fp8(normal(r, 256, "f32", seed=r)) for r in (rows, 40))
+    far = (1 << 21) + 7
+    store = torch.zeros(rows * far + 2, device="cuda")
+    scales = store.as_strided(x[1].shape, (far, 1))
+    scales.copy_(x[1])
+    want = tilec.ext.linear_fp8(x, w), tilec.ext.dequantize_fp8(x)
+    assert torch.equal(tilec.ext.linear_fp8((x[0], scales), w), want[0])
+    assert torch.equal(tilec.ext.linear_fp8(w, (x[0], scales)), tilec.ext.linear_fp8(w, x))
+    assert torch.equal(tilec.ext.dequantize_fp8((x[0], scales)), want[1])
+
+
+@pytest.mark.gpu
+def test_more_rows_than_small_tiles_have_grids_for():
+    M = (1 << 30) + 5  # 2^24 tiles of 64 rows
+    codes = torch.zeros(M, 16, dtype=torch.uint8, device="cuda")
+    codes[0], codes[1 << 29], codes[M - 1] = 0x38, 0x40, 0x48  # 1, 2 and 4
+    one = torch.ones(1, 1, device="cuda")
+    x = codes.view(torch.float8_e4m3fn), one.expand(M, 1)
+    w = codes[:1].view(torch.float8_e4m3fn), one
+    out = tilec.ext.linear_fp8(x, w, dtype=torch.bfloat16)
+    assert out[0].item() == 16 and out[1 << 29].item() == 32 and out[M - 1].item() == 64
+    assert out.count_nonzero().item() == 3

@@ -164,3 +164,9 @@ def test_wrong_arguments_raise():
         tilec.ext.quantize_fp8("x")
     with pytest.raises(TypeError):
         tilec.ext.rms_norm([1.0])
+
+
+def test_more_outputs_than_a_grid_has():
+    most = (1 << 31) - 1024
+    assert linear(M=most, N=most) == VALUE and "too many" in _lib.last_error()
+    assert linear_bytes(most, 1, 16) == 0

@@ -198,3 +198,14 @@ def test_cpu_tensors_are_refused():
         tilec.ext.grad_norm([x])
     with pytest.raises(TypeError):
         tilec.ext.clip_grads([x], 1.0)
+
+
+@pytest.mark.gpu
+def test_an_infinite_limit_is_none():
+    x = torch.ones(1000, device="cuda")
+    x[7] = float("inf")
+    norm, scale = tilec.ext.grad_norm([x], math.inf, grad_scale=torch.tensor(0.5, device="cuda"))
+    assert norm.item() == math.inf and scale.item() == 0.5
+    x[8] = float("nan")
+    norm, scale = tilec.ext.grad_norm([x], math.inf)
+    assert math.isnan(norm.item()) and scale.item() == 1

@@ -51,7 +51,7 @@ struct GradArgs {
   unsigned* counter;
   const float *grad_scale, *scale_in;
   float *norm, *scale;
-  float max_norm;  // negative: none
+  double max_norm;  // negative: none
   Tensor t[kMaxTensors];
 };
 
@@ -152,8 +152,8 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(GradArgs a) {
   const double gs = a.grad_scale != nullptr ? (double)*a.grad_scale : 1.;
   const double norm = fabs(gs) * sqrt(s);
   double clip = 1.;
-  if (a.max_norm >= 0.f) {
-    clip = (double)a.max_norm / (norm + 1e-6);
+  if (a.max_norm >= 0.) {
+    clip = a.max_norm / (norm + 1e-6);
     clip = clip > 1. ? 1. : clip;  // a NaN stays one
   }
   *a.norm = (float)norm;
@@ -292,7 +292,8 @@ int tilec_grad_norm(const tilec_grad* grads, int32_t count, const float* grad_sc
     return fail(TILEC_ERR_WORKSPACE, "tilec: grad_norm needs %zu workspace bytes and 4 bytes of counter (got %zu and %zu)",
                 need, workspace == nullptr ? (size_t)0 : workspace_bytes, counter == nullptr ? (size_t)0 : counter_bytes);
   a.partial = static_cast<double*>(workspace), a.counter = static_cast<unsigned*>(counter);
-  a.grad_scale = grad_scale, a.norm = norm, a.scale = scale, a.max_norm = max_norm < 0 ? -1.f : (float)max_norm;
+  a.grad_scale = grad_scale, a.norm = norm, a.scale = scale;
+  a.max_norm = max_norm < 0 || std::isinf(max_norm) ? -1. : max_norm;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   hipError_t e;
   if (a.total == 0) {  // the norm of nothing

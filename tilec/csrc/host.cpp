@@ -526,7 +526,8 @@ PyObject* build_rms(PyObject* const* args) {
   check(tilec_rms_norm(r.t.const_data_ptr(), added ? res.t.const_data_ptr() : nullptr, data(p.weight), y.data_ptr(),
                        y_scale.defined() ? static_cast<float*>(y_scale.data_ptr()) : nullptr,
                        added ? h.data_ptr() : nullptr, static_cast<float*>(rstd.data_ptr()), r.R, r.D, r.ld, res.ld, ldy,
-                       r.D, y_scale.defined() ? y_scale.stride(0) : 0, y_scale.defined() ? y_scale.stride(1) : 0, x_code, r_code, code_of(type), p.code, (float)eps, stream_of(args[5])));
+                       r.D, y_scale.defined() ? y_scale.stride(0) : 0, y_scale.defined() ? y_scale.stride(1) : 0, x_code,
+                       r_code, code_of(type), p.code, (float)eps, stream_of(args[5])));
   if (!y_scale.defined()) return tuple({y, h, rstd});
   PyObject* t = PyTuple_New(3);
   if (t == nullptr) throw python_error();
@@ -574,7 +575,7 @@ PyObject* build_rms_backward(PyObject* const* args) {
 // not), scales of blocks of 1 or 128 rows.
 struct Fp8 {
   at::Tensor codes, scales;
-  int64_t R, C, ld;
+  int64_t R, C, ld, s_row, s_group;  // strides of the rows of codes and of the scales
   int32_t code, block;
   Fp8(OneGpu& gpu, const char* name, PyObject* o) {
     const std::string of(name);
@@ -600,7 +601,8 @@ struct Fp8 {
                 std::to_string(G) + ")");
     block = s.size(0) == R ? 1 : kGroup;
     codes = (C > 1 && c.stride(1) != 1) || (R > 1 && c.stride(0) < C) ? c.contiguous() : c;
-    scales = R > 1 && s.stride(0) > kMaxScaleRow ? s.contiguous() : s;
+    scales = s.size(0) > 1 && s.stride(0) > kMaxScaleRow ? s.contiguous() : s;
+    s_row = s.size(0) > 1 ? scales.stride(0) : 0, s_group = G > 1 ? scales.stride(1) : 0;
     ld = R > 1 ? codes.stride(0) : C;
     code = code_of(c.scalar_type());
   }
@@ -628,7 +630,8 @@ PyObject* build_quantize(PyObject* const* args) {
   const NewFp8 q(R, C, b[0], type, x.device());
   const int64_t ld = cols ? (C > 1 ? t.stride(1) : R) : (R > 1 ? t.stride(0) : C);
   check(tilec_quantize_fp8(t.const_data_ptr(), q.codes.data_ptr(), static_cast<float*>(q.scales.data_ptr()), R, C, ld,
-                           q.ld, q.scales.stride(0), q.scales.stride(1), cols ? TILEC_X1_COL_MAJOR : 0, x_code, code_of(type), (int32_t)b[0], stream_of(args[3])));
+                           q.ld, q.scales.stride(0), q.scales.stride(1), cols ? TILEC_X1_COL_MAJOR : 0, x_code,
+                           code_of(type), (int32_t)b[0], stream_of(args[3])));
   return tuple({q.codes, q.scales});
 }
 
@@ -639,8 +642,9 @@ PyObject* build_dequantize(PyObject* const* args) {
   if (!is_wide(type)) bad_type(std::string("unsupported dtype ") + toString(type) + " (use float32 or bfloat16)");
   const c10::DeviceGuard guard(q.codes.device());
   const at::Tensor out = make({q.R, q.C}, type, q.codes.device());
-  check(tilec_dequantize_fp8(q.codes.const_data_ptr(), static_cast<const float*>(q.scales.const_data_ptr()), out.data_ptr(),
-                             q.R, q.C, q.ld, q.C, q.scales.stride(0), q.scales.stride(1), q.code, code_of(type), q.block, stream_of(args[2])));
+  check(tilec_dequantize_fp8(q.codes.const_data_ptr(), static_cast<const float*>(q.scales.const_data_ptr()),
+                             out.data_ptr(),
+                             q.R, q.C, q.ld, q.C, q.s_row, q.s_group, q.code, code_of(type), q.block, stream_of(args[2])));
   return THPVariable_Wrap(out);
 }
 
@@ -660,8 +664,8 @@ PyObject* build_linear(PyObject* const* args) {
   if (need > 0) scratch = make({(int64_t)need}, at::kByte, x.codes.device());
   check(tilec_linear_fp8(xp, static_cast<const float*>(x.scales.const_data_ptr()), wp,
                          static_cast<const float*>(w.scales.const_data_ptr()), out.data_ptr(), x.R, w.R, x.C, x.ld, w.ld,
-                         w.R, x.scales.stride(0), x.scales.stride(1), w.scales.stride(0), w.scales.stride(1), x.code, w.code, code_of(type), x.block, w.block, need > 0 ? scratch.data_ptr() : nullptr, need,
-                         stream_of(args[3])));
+                         w.R, x.s_row, x.s_group, w.s_row, w.s_group, x.code, w.code, code_of(type), x.block, w.block,
+                         need > 0 ? scratch.data_ptr() : nullptr, need, stream_of(args[3])));
   return THPVariable_Wrap(out);
 }
 

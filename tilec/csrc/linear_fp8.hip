@@ -1,6 +1,7 @@
 // tilec_linear_fp8: the choice of a kernel of linear_fp8.h, operands whose rows do
 // not begin at multiples of 16 bytes, and the sums of split groups.
 #include <algorithm>
+#include <type_traits>
 
 #include "abi.h"
 #include "linear_fp8.h"
@@ -12,6 +13,7 @@ namespace {
 typedef unsigned short u16;
 
 constexpr int64_t kMaxScaleRow = int64_t(1) << 21, kMaxScaleGroup = int64_t(1) << 40;
+constexpr int64_t kMaxTiles = (int64_t(1) << 23) - 1;  // of up to 512 threads: a grid has less than 2^32
 
 struct Plan {
   int tile;            // -1: the streaming kernel
@@ -47,10 +49,12 @@ Plan plan_of(const void* x, const void* w, int64_t M, int64_t N, int64_t K, int6
   // The tile and the splits of K that are estimated to be done first: whole turns
   // over the chip, and with splits the partial sums written, read and joined by a
   // kernel of its own (2 us, 4.5 TB/s).
+  p.tile = kFp8TileCount;
   double best = 1e30;
   for (int t = 0; t < kFp8TileCount; ++t) {
     const Fp8Tile& g = kFp8Tiles[t];
     const int64_t n = cdiv(M, g.bm) * cdiv(N, g.bn[f8]);
+    if (n > kMaxTiles) continue;
     for (int64_t s = 1; s <= std::min<int64_t>(G, 64); ++s) {
       const int64_t steps = cdiv(G, s), splits = cdiv(G, steps);
       if (splits != s) continue;
@@ -146,6 +150,9 @@ int tilec_linear_fp8(const void* x, const float* x_scale, const void* weight, co
   Plan none{};
   none.tile = kFp8TileCount - 1, none.splits = 1;
   const Plan p = K > 0 ? plan_of(x, weight, M, N, K, ldx, ldw, f8) : none;
+  if (p.tile == kFp8TileCount)
+    return fail(TILEC_ERR_VALUE, "tilec: linear_fp8: %lld x %lld outputs are too many for one launch", (long long)M,
+                (long long)N);
   if (p.bytes() > 0 && (workspace == nullptr || workspace_bytes < p.bytes()))
     return fail(TILEC_ERR_WORKSPACE, "tilec: linear_fp8 needs %zu workspace bytes (got %zu)", p.bytes(),
                 workspace == nullptr ? (size_t)0 : workspace_bytes);
@@ -173,8 +180,12 @@ int tilec_linear_fp8(const void* x, const float* x_scale, const void* weight, co
          : (fw ? launch_fp8<0, 1>(a, f8, p.tile, p.splits, st) : launch_fp8<0, 0>(a, f8, p.tile, p.splits, st));
   if (e == hipSuccess && p.splits > 1) {
     const unsigned grid = (unsigned)std::min<int64_t>(cdiv(M * N, 1024), 16 * (int64_t)device_cus());
-    if (f8) hipLaunchKernelGGL(fp8_join_kernel<u16>, dim3(grid), dim3(256), 0, st, a.partial, static_cast<u16*>(out), M * N, a.ldo, a.N, p.splits);
-    else hipLaunchKernelGGL(fp8_join_kernel<float>, dim3(grid), dim3(256), 0, st, a.partial, static_cast<float*>(out), M * N, a.ldo, a.N, p.splits);
+    auto join = [&](auto* to) {
+      hipLaunchKernelGGL(fp8_join_kernel<std::remove_pointer_t<decltype(to)>>, dim3(grid), dim3(256), 0, st, a.partial, to,
+                         M * N, a.ldo, a.N, p.splits);
+    };
+    if (f8) join(static_cast<u16*>(out));
+    else join(static_cast<float*>(out));
     e = hipGetLastError();
   }
   if (e != hipSuccess) return fail(TILEC_ERR_HIP, "tilec: launching linear_fp8 failed: %s", hipGetErrorString(e));

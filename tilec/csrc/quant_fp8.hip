@@ -319,7 +319,8 @@ int tilec_quantize_fp8(const void* x, void* codes, float* scales, int64_t R, int
   if (x == nullptr || codes == nullptr || scales == nullptr)
     return fail(TILEC_ERR_VALUE, "tilec: quantize_fp8: a pointer is NULL");
   if (scale_row < 0 || scale_group < 0 || scale_row > kMaxStride || scale_group > kMaxStride)
-    return fail(TILEC_ERR_VALUE, "tilec: quantize_fp8: bad strides %lld, %lld of scales", (long long)scale_row, (long long)scale_group);
+    return fail(TILEC_ERR_VALUE, "tilec: quantize_fp8: bad strides %lld, %lld of scales",
+                (long long)scale_row, (long long)scale_group);
   if (reinterpret_cast<uintptr_t>(codes) % 16 != 0 || (R > 1 && (ldq % 16 != 0 || ldq < room || ldq > kMaxStride)))
     return fail(TILEC_ERR_VALUE, "tilec: quantize_fp8: rows of codes begin at multiples of 16 bytes (row stride %lld)",
                 (long long)ldq);
@@ -361,7 +362,8 @@ int tilec_dequantize_fp8(const void* codes, const float* scales, void* out, int6
   if (codes == nullptr || scales == nullptr || out == nullptr)
     return fail(TILEC_ERR_VALUE, "tilec: dequantize_fp8: a pointer is NULL");
   if (scale_row < 0 || scale_group < 0 || scale_row > kMaxStride || scale_group > kMaxStride)
-    return fail(TILEC_ERR_VALUE, "tilec: dequantize_fp8: bad strides %lld, %lld of scales", (long long)scale_row, (long long)scale_group);
+    return fail(TILEC_ERR_VALUE, "tilec: dequantize_fp8: bad strides %lld, %lld of scales",
+                (long long)scale_row, (long long)scale_group);
   ValuesArgs a{};
   a.codes = static_cast<const unsigned char*>(codes), a.scales = scales, a.out = out;
   a.R = R, a.C = C, a.ldq = ldq, a.ldo = ldo, a.G = cdiv(C, kGroup);

@@ -501,7 +501,8 @@ extern "C" {
 
 int tilec_rms_norm(const void* x, const void* residual, const void* weight, void* y, float* y_scale, void* h,
                    float* rstd, int64_t R, int64_t D, int64_t ldx, int64_t ldr, int64_t ldy, int64_t ldh,
-                   int64_t scale_row, int64_t scale_group, int32_t x_dtype, int32_t r_dtype, int32_t y_dtype, int32_t w_dtype, float eps, void* stream) {
+                   int64_t scale_row, int64_t scale_group, int32_t x_dtype, int32_t r_dtype, int32_t y_dtype,
+                   int32_t w_dtype, float eps, void* stream) {
   clear_error();
   if (!is_wide(x_dtype) || (residual != nullptr && !is_wide(r_dtype)) || !is_wide(w_dtype) ||
       (!is_wide(y_dtype) && !is_fp8(y_dtype)))
@@ -517,8 +518,10 @@ int tilec_rms_norm(const void* x, const void* residual, const void* weight, void
   if (is_fp8(y_dtype) && (y_scale == nullptr || reinterpret_cast<uintptr_t>(y) % 16 != 0 ||
                           (R > 1 && (ldy % 16 != 0 || ldy < room))))
     return fail(TILEC_ERR_VALUE, "tilec: RMS norm: 8-bit codes need scales and rows at multiples of 16 bytes");
-  if (is_fp8(y_dtype) && (scale_row < 0 || scale_group < 0 || scale_row > (int64_t(1) << 40) || scale_group > (int64_t(1) << 40)))
-    return fail(TILEC_ERR_VALUE, "tilec: RMS norm: bad strides %lld, %lld of scales", (long long)scale_row, (long long)scale_group);
+  constexpr int64_t most = int64_t(1) << 40;
+  if (is_fp8(y_dtype) && (scale_row < 0 || scale_group < 0 || scale_row > most || scale_group > most))
+    return fail(TILEC_ERR_VALUE, "tilec: RMS norm: bad strides %lld, %lld of scales", (long long)scale_row,
+                (long long)scale_group);
   RmsArgs a{};
   a.x = x, a.res = residual, a.w = weight, a.y = y, a.y_scale = y_scale, a.h = h, a.rstd = rstd;
   a.s_row = scale_row, a.s_group = scale_group;

@@ -21,8 +21,8 @@ import torch
 from . import _lib
 from .ext import _capturing, _current_device, _raw_stream, _tuned, counters_for
 
-__all__ = ["layer_norm", "layer_norm_backward", "rms_norm", "rms_norm_backward", "linear_cross_entropy", "linear_cross_entropy_grad",
-           "grad_norm", "clip_grads", "adamw_state", "adamw_step", "adamw_values", "ADAMW_BLOCK"]
+__all__ = ["layer_norm", "layer_norm_backward", "rms_norm", "rms_norm_backward", "linear_cross_entropy",
+           "linear_cross_entropy_grad", "grad_norm", "clip_grads", "adamw_state", "adamw_step", "adamw_values", "ADAMW_BLOCK"]
 
 _CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
@@ -126,7 +126,9 @@ def rms_norm(x, weight=None, residual=None, eps=1e-5, dtype=None):
     its type, or `dtype`.  With dtype float8_e4m3fn or float8_e5m2 y is the 8-bit
     operand of the next `linear_fp8`, a pair (codes [R, D], scales [R, ceil(D /
     128)]): the codes and scales that `quantize_fp8` gives of the float32 y.  rstd
-    is float32 [R]; `rms_norm_backward` takes it and h.
+    is float32 [R]; `rms_norm_backward` takes it and h.  The sum of squares is
+    float32: it overflows (rstd 0) for rows of a norm above 2^64, and squares of
+    values below 2^-75 are lost.
     """
     return _lib.host().rms_norm(x, weight, residual, eps, dtype, _stream_of(x))
 
@@ -282,8 +284,8 @@ def grad_norm(grads, max_norm=None, grad_scale=None):
 
     `adamw_step` takes the scale as its grad_scale: gradients are clipped without
     being written.  grads: float32 and bfloat16 tensors on one GPU (None: a
-    parameter without a gradient), at least one.  max_norm: at least 0, or None,
-    no limit.  grad_scale: a float32 value on the GPU that the gradients are to be
+    parameter without a gradient), at least one.  max_norm: at least 0; None or
+    infinite: no limit.  grad_scale: a float32 value on the GPU that the gradients are to be
     multiplied by in any case (the inverse of a loss's scale), or None.  Squares
     and sums are float64, in a fixed order: nothing overflows, and the same bits
     come out on every call.  An infinite norm gives a scale of 0, a NaN one NaN.
