@@ -54,12 +54,15 @@ def _host():
     import torch
     from torch.utils import cpp_extension
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    rocm = os.path.dirname(os.path.dirname(os.path.realpath(hipcc())))
     tmp = HOST + ".tmp"
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-D__HIP_PLATFORM_AMD__=1", "-isystem" + os.path.join(rocm, "include"),
            "-I" + sysconfig.get_paths()["include"], *("-isystem" + p for p in cpp_extension.include_paths()),
            os.path.join(CSRC, "host.cpp"), "-o", tmp, "-L" + torch_lib, "-Wl,-rpath," + torch_lib,
-           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-L" + HERE, "-Wl,-rpath,$ORIGIN", "-ltilec_hip"]
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
+           "-L" + HERE, "-Wl,-rpath,$ORIGIN", "-ltilec_hip"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"building {HOST} failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")

@@ -16,6 +16,7 @@
 
 #include "abi.h"
 #include "common.h"
+#include "enqueue.h"
 #include "../../include/tilec.h"
 
 namespace tilec {
@@ -44,6 +45,7 @@ struct Tensor {
   }
 };
 
+template <int MAX>
 struct GradArgs {
   int count, chunk;
   int64_t base, total;  // this launch's first chunk among `total`; the last launch has base + grid == total
@@ -52,18 +54,35 @@ struct GradArgs {
   const float *grad_scale, *scale_in;
   float *norm, *scale;
   double max_norm;  // negative: none
-  Tensor t[kMaxTensors];
+  Tensor t[MAX];
 };
+using Args = GradArgs<kMaxTensors>;
 
-// The tensor of workgroup b: the last whose first is not past it.
-__device__ __forceinline__ const Tensor& tensor_of(const GradArgs& a, int b) {
-  int lo = 0, hi = a.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.t[mid].first() <= b) lo = mid;
-    else hi = mid - 1;
+// The tensor of workgroup b: the last whose first is not past it.  Every lane looks
+// at one in 64: arguments lie in the host's memory, and this is one trip there where
+// a search is one a step.
+template <int MAX>
+__device__ __forceinline__ Tensor tensor_of(const GradArgs<MAX>& a, int b) {
+  const int lane = threadIdx.x & 63;
+  constexpr int N = (MAX + 63) / 64;
+  uint64_t data[N], packed[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const Tensor& t = a.t[min(lane + 64 * i, a.count - 1)];
+    data[i] = reinterpret_cast<uint64_t>(t.data), packed[i] = t.packed;
   }
-  return a.t[lo];
+  int at = -1;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    at += __popcll(__ballot(lane + 64 * i < a.count && Tensor{nullptr, packed[i]}.first() <= b));
+#pragma unroll
+  for (int i = 1; i < N; ++i)
+    if (at >= 64 * i) data[0] = data[i], packed[0] = packed[i];
+  auto from = [&](uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)v, at & 63), hi = __builtin_amdgcn_readlane((int)(v >> 32), at & 63);
+    return (uint64_t)hi << 32 | lo;
+  };
+  return {reinterpret_cast<void*>(from(data[0])), from(packed[0])};
 }
 
 // Sum over a workgroup of 256, in thread order within a wave and wave order.
@@ -122,11 +141,12 @@ __device__ __forceinline__ double squares(const void* p, int n) {
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-__global__ __launch_bounds__(256) void grad_norm_kernel(GradArgs a) {
+template <int MAX>
+__global__ __launch_bounds__(256) void grad_norm_kernel(GradArgs<MAX> a) {
   __shared__ double red[4];
   __shared__ int last;
   if (a.count > 0) {
-    const Tensor& t = tensor_of(a, blockIdx.x);
+    const Tensor t = tensor_of(a, blockIdx.x);
     const int64_t at = (int64_t)((int)blockIdx.x - t.first()) * a.chunk;
     const int n = (int)min((int64_t)a.chunk, t.n() - at);
     double s = t.bf16() ? squares<true>(static_cast<const u16*>(t.data) + at, n)
@@ -161,10 +181,11 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(GradArgs a) {
 }
 
 // Values multiplied by a factor in place; none is touched where it is 1.
-__global__ __launch_bounds__(256) void grad_scale_kernel(GradArgs a) {
+template <int MAX>
+__global__ __launch_bounds__(256) void grad_scale_kernel(GradArgs<MAX> a) {
   const float f = *a.scale_in;
   if (f == 1.f) return;
-  const Tensor& t = tensor_of(a, blockIdx.x);
+  const Tensor t = tensor_of(a, blockIdx.x);
   const int64_t at = (int64_t)((int)blockIdx.x - t.first()) * a.chunk;
   const int n = (int)min((int64_t)a.chunk, t.n() - at);
   auto go = [&](auto* x, auto bf16) {
@@ -223,15 +244,15 @@ int64_t chunks_of(const tilec_grad* grads, int32_t count, int chunk) {
 // f(workgroups) for the tensors in groups of up to kMaxTensors, with at most 2^22
 // workgroups each; a.base counts them.
 template <typename F>
-hipError_t in_groups(GradArgs& a, const tilec_grad* grads, int32_t count, F f) {
+hipError_t in_groups(Args& a, const tilec_grad* grads, int32_t count, F f) {
   int64_t blocks = 0;
   a.count = 0, a.base = 0;
   auto flush = [&]() -> hipError_t {
     if (a.count == 0) return hipSuccess;
-    f((unsigned)blocks);
+    const hipError_t e = f((unsigned)blocks);
     a.base += blocks;
     a.count = 0, blocks = 0;
-    return hipGetLastError();
+    return e;
   };
   for (int i = 0; i < count; ++i) {
     const int64_t esz = grads[i].dtype == TILEC_BF16 ? 2 : 4;
@@ -248,6 +269,24 @@ hipError_t in_groups(GradArgs& a, const tilec_grad* grads, int32_t count, F f) {
   }
   return flush();
 }
+
+// Launches the kernel that takes no more arguments than it has to: a launch copies
+// them to memory that the GPU reads over the bus.  Theirs are the beginning of `a`.
+template <template <int> class KERNEL, int MAX = 32>
+hipError_t launch(const Args& a, unsigned blocks, hipStream_t stream) {
+  if constexpr (MAX < kMaxTensors) {
+    if (a.count > MAX) return launch<KERNEL, MAX + 32>(a, blocks, stream);
+  }
+  return enqueue(KERNEL<MAX>::get(), dim3(blocks), dim3(256), stream, reinterpret_cast<const GradArgs<MAX>&>(a));
+}
+template <int MAX>
+struct NormKernel {
+  static auto get() { return grad_norm_kernel<MAX>; }
+};
+template <int MAX>
+struct ScaleKernel {
+  static auto get() { return grad_scale_kernel<MAX>; }
+};
 
 int check_grads(const char* what, const tilec_grad* grads, int32_t count) {
   if (count < 0 || (count > 0 && grads == nullptr))
@@ -284,7 +323,7 @@ int tilec_grad_norm(const tilec_grad* grads, int32_t count, const float* grad_sc
   if (rc != TILEC_OK) return rc;
   if (norm == nullptr) return fail(TILEC_ERR_VALUE, "tilec: grad_norm: norm is NULL");
   if (max_norm != max_norm) return fail(TILEC_ERR_VALUE, "tilec: grad_norm: max_norm is not a number");
-  GradArgs a{};
+  Args a{};
   a.chunk = chunk_of(grads, count);
   a.total = chunks_of(grads, count, a.chunk);
   const size_t need = (size_t)a.total * sizeof(double);
@@ -297,11 +336,9 @@ int tilec_grad_norm(const tilec_grad* grads, int32_t count, const float* grad_sc
   const hipStream_t st = static_cast<hipStream_t>(stream);
   hipError_t e;
   if (a.total == 0) {  // the norm of nothing
-    hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(256), 0, st, a);
-    e = hipGetLastError();
+    e = launch<NormKernel>(a, 1, st);
   } else {
-    e = in_groups(a, grads, count,
-                  [&](unsigned blocks) { hipLaunchKernelGGL(grad_norm_kernel, dim3(blocks), dim3(256), 0, st, a); });
+    e = in_groups(a, grads, count, [&](unsigned blocks) { return launch<NormKernel>(a, blocks, st); });
   }
   if (e != hipSuccess) return fail(TILEC_ERR_HIP, "tilec: launching grad_norm failed: %s", hipGetErrorString(e));
   return TILEC_OK;
@@ -312,11 +349,11 @@ int tilec_scale_grads(const tilec_grad* grads, int32_t count, const float* scale
   const int rc = check_grads("scale_grads", grads, count);
   if (rc != TILEC_OK) return rc;
   if (scale == nullptr) return fail(TILEC_ERR_VALUE, "tilec: scale_grads: scale is NULL");
-  GradArgs a{};
+  Args a{};
   a.chunk = chunk_of(grads, count);
   a.scale_in = scale;
   const hipError_t e = in_groups(a, grads, count, [&](unsigned blocks) {
-    hipLaunchKernelGGL(grad_scale_kernel, dim3(blocks), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    return launch<ScaleKernel>(a, blocks, static_cast<hipStream_t>(stream));
   });
   if (e != hipSuccess) return fail(TILEC_ERR_HIP, "tilec: launching scale_grads failed: %s", hipGetErrorString(e));
   return TILEC_OK;

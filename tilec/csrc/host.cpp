@@ -22,19 +22,20 @@
 // (the handle of the tensors' device's current stream): one row of 4096 then
 // costs 6 us a call instead of 10.
 //
-//   rms_norm(x, weight, residual, eps, dtype, stream) -> (y, h, rstd)
-//   rms_norm_backward(dy, h, rstd, weight, dh, weight_grad, stream) -> (dx, dweight)
-//   quantize_fp8(x, block, dtype, stream) -> (codes, scales)
-//   dequantize_fp8(q, dtype, stream) -> values
-//   linear_fp8(x, weight, dtype, stream) -> out
+//   rms_norm(x, weight, residual, eps, dtype) -> (y, h, rstd)
+//   rms_norm_backward(dy, h, rstd, weight, dh, weight_grad) -> (dx, dweight)
+//   quantize_fp8(x, block, dtype) -> (codes, scales)
+//   dequantize_fp8(q, dtype) -> values
+//   linear_fp8(x, weight, dtype) -> out
 //
-// do the same; 8-bit operands are (codes, scales) pairs.
+// do the same and find the stream themselves; 8-bit operands are (codes, scales)
+// pairs.
 //
-//   grad_norm(grads, max_norm, grad_scale, stream_of, counters_for) -> (norm, scale)
-//   clip_grads(grads, max_norm, grad_scale, stream_of, counters_for) -> norm
+//   grad_norm(grads, max_norm, grad_scale, counter_of) -> (norm, scale)
+//   clip_grads(grads, max_norm, grad_scale, counter_of) -> norm
 //
-// read lists as adamw_step does; counters_for(device, stream, bytes) gives the
-// zeroed counter that the norm's kernel leaves zero.
+// read lists as adamw_step does; counter_of(device index, stream) gives the zeroed
+// counter that the norm's kernel leaves zero.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -46,7 +47,7 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <c10/core/DeviceGuard.h>
-#include <torch/csrc/Device.h>
+#include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -480,6 +481,9 @@ constexpr int64_t kGroup = 128;                      // values of a row under on
 constexpr int64_t kMaxScaleRow = int64_t(1) << 21;  // the largest row stride of scales in a product
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// The current stream of a GPU.
+void* stream_on(at::Device device) { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
+
 // A new tensor on a GPU, past the dispatcher: 0.5 us instead of 0.75.
 at::Tensor make(at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
   return at::Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
@@ -527,7 +531,7 @@ PyObject* build_rms(PyObject* const* args) {
                        y_scale.defined() ? static_cast<float*>(y_scale.data_ptr()) : nullptr,
                        added ? h.data_ptr() : nullptr, static_cast<float*>(rstd.data_ptr()), r.R, r.D, r.ld, res.ld, ldy,
                        r.D, y_scale.defined() ? y_scale.stride(0) : 0, y_scale.defined() ? y_scale.stride(1) : 0, x_code,
-                       r_code, code_of(type), p.code, (float)eps, stream_of(args[5])));
+                       r_code, code_of(type), p.code, (float)eps, stream_on(x.device())));
   if (!y_scale.defined()) return tuple({y, h, rstd});
   PyObject* t = PyTuple_New(3);
   if (t == nullptr) throw python_error();
@@ -566,7 +570,7 @@ PyObject* build_rms_backward(PyObject* const* args) {
         d.t.const_data_ptr(), r.t.const_data_ptr(), static_cast<const float*>(rstd.const_data_ptr()), data(p.weight),
         added ? dh.t.const_data_ptr() : nullptr, dx.data_ptr(), sums ? static_cast<float*>(dw.data_ptr()) : nullptr, r.R,
         r.D, d.ld, r.ld, dh.ld, r.D, dy_code, h_code, dh_code, p.code, need > 0 ? scratch.data_ptr() : nullptr, need,
-        stream_of(args[6])));
+        stream_on(dy.device())));
   }
   return tuple({dx, dw});
 }
@@ -631,7 +635,7 @@ PyObject* build_quantize(PyObject* const* args) {
   const int64_t ld = cols ? (C > 1 ? t.stride(1) : R) : (R > 1 ? t.stride(0) : C);
   check(tilec_quantize_fp8(t.const_data_ptr(), q.codes.data_ptr(), static_cast<float*>(q.scales.data_ptr()), R, C, ld,
                            q.ld, q.scales.stride(0), q.scales.stride(1), cols ? TILEC_X1_COL_MAJOR : 0, x_code,
-                           code_of(type), (int32_t)b[0], stream_of(args[3])));
+                           code_of(type), (int32_t)b[0], stream_on(x.device())));
   return tuple({q.codes, q.scales});
 }
 
@@ -644,7 +648,8 @@ PyObject* build_dequantize(PyObject* const* args) {
   const at::Tensor out = make({q.R, q.C}, type, q.codes.device());
   check(tilec_dequantize_fp8(q.codes.const_data_ptr(), static_cast<const float*>(q.scales.const_data_ptr()),
                              out.data_ptr(),
-                             q.R, q.C, q.ld, q.C, q.s_row, q.s_group, q.code, code_of(type), q.block, stream_of(args[2])));
+                             q.R, q.C, q.ld, q.C, q.s_row, q.s_group, q.code, code_of(type), q.block,
+                             stream_on(q.codes.device())));
   return THPVariable_Wrap(out);
 }
 
@@ -665,7 +670,7 @@ PyObject* build_linear(PyObject* const* args) {
   check(tilec_linear_fp8(xp, static_cast<const float*>(x.scales.const_data_ptr()), wp,
                          static_cast<const float*>(w.scales.const_data_ptr()), out.data_ptr(), x.R, w.R, x.C, x.ld, w.ld,
                          w.R, x.s_row, x.s_group, w.s_row, w.s_group, x.code, w.code, code_of(type), x.block, w.block,
-                         need > 0 ? scratch.data_ptr() : nullptr, need, stream_of(args[3])));
+                         need > 0 ? scratch.data_ptr() : nullptr, need, stream_on(x.codes.device())));
   return THPVariable_Wrap(out);
 }
 
@@ -708,7 +713,7 @@ struct Grads {
   }
 };
 
-// Enqueues the norm; {norm, scale}.  args: grads, max_norm, grad_scale, stream_of, counters_for.
+// Enqueues the norm; {norm, scale}.  args: grads, max_norm, grad_scale, counter_of.
 std::pair<at::Tensor, at::Tensor> norm_of(Grads& g, PyObject* const* args, void*& stream) {
   const double max_norm = args[1] == Py_None ? -1. : number(args[1]);
   if (args[1] != Py_None && !(max_norm >= 0)) bad_value("max_norm is negative or not a number");
@@ -718,11 +723,10 @@ std::pair<at::Tensor, at::Tensor> norm_of(Grads& g, PyObject* const* args, void*
     if (t.numel() != 1) bad_value("grad_scale has shape " + shape(t) + ", expected one value");
     grad_scale = static_cast<const float*>(t.const_data_ptr());
   }
-  THPObjectPtr handle(PyObject_CallFunction(args[3], "L", (long long)g.r.device));
+  stream = stream_on(g.device);
+  THPObjectPtr handle(PyLong_FromVoidPtr(stream));
   if (!handle) throw python_error();
-  stream = stream_of(handle.get());
-  THPObjectPtr where(THPDevice_New(g.device));
-  THPObjectPtr held(PyObject_CallFunction(args[4], "OOi", where.get(), handle.get(), 4));
+  THPObjectPtr held(PyObject_CallFunction(args[3], "iO", (int)g.device.index(), handle.get()));
   if (!held) throw python_error();
   const at::Tensor counter = tensor("counters", held.get());
   const at::Tensor norm = make({}, at::kFloat, g.device), scale = make({}, at::kFloat, g.device);
@@ -789,19 +793,19 @@ PyMethodDef kMethods[] = {
      "layer_norm(x, weight, bias, eps, dtype, stream) -> (y, mean, rstd)"},
     {"layer_norm_backward", function<build_norm_backward, 7, kNormBackward>(), METH_FASTCALL,
      "layer_norm_backward(dy, x, mean, rstd, weight, param_grads, stream) -> (dx, dweight, dbias)"},
-    {"rms_norm", function<build_rms, 6, kRms>(), METH_FASTCALL,
-     "rms_norm(x, weight, residual, eps, dtype, stream) -> (y, h, rstd)"},
-    {"rms_norm_backward", function<build_rms_backward, 7, kRmsBackward>(), METH_FASTCALL,
-     "rms_norm_backward(dy, h, rstd, weight, dh, weight_grad, stream) -> (dx, dweight)"},
-    {"quantize_fp8", function<build_quantize, 4, kQuantize>(), METH_FASTCALL,
-     "quantize_fp8(x, block, dtype, stream) -> (codes, scales)"},
-    {"dequantize_fp8", function<build_dequantize, 3, kDequantize>(), METH_FASTCALL,
-     "dequantize_fp8(q, dtype, stream) -> values"},
-    {"linear_fp8", function<build_linear, 4, kLinear>(), METH_FASTCALL, "linear_fp8(x, weight, dtype, stream) -> out"},
-    {"grad_norm", function<build_grad_norm, 5, kGradNorm>(), METH_FASTCALL,
-     "grad_norm(grads, max_norm, grad_scale, stream_of, counters_for) -> (norm, scale)"},
-    {"clip_grads", function<build_clip, 5, kClip>(), METH_FASTCALL,
-     "clip_grads(grads, max_norm, grad_scale, stream_of, counters_for) -> norm"},
+    {"rms_norm", function<build_rms, 5, kRms>(), METH_FASTCALL,
+     "rms_norm(x, weight, residual, eps, dtype) -> (y, h, rstd)"},
+    {"rms_norm_backward", function<build_rms_backward, 6, kRmsBackward>(), METH_FASTCALL,
+     "rms_norm_backward(dy, h, rstd, weight, dh, weight_grad) -> (dx, dweight)"},
+    {"quantize_fp8", function<build_quantize, 3, kQuantize>(), METH_FASTCALL,
+     "quantize_fp8(x, block, dtype) -> (codes, scales)"},
+    {"dequantize_fp8", function<build_dequantize, 2, kDequantize>(), METH_FASTCALL,
+     "dequantize_fp8(q, dtype) -> values"},
+    {"linear_fp8", function<build_linear, 3, kLinear>(), METH_FASTCALL, "linear_fp8(x, weight, dtype) -> out"},
+    {"grad_norm", function<build_grad_norm, 4, kGradNorm>(), METH_FASTCALL,
+     "grad_norm(grads, max_norm, grad_scale, counter_of) -> (norm, scale)"},
+    {"clip_grads", function<build_clip, 4, kClip>(), METH_FASTCALL,
+     "clip_grads(grads, max_norm, grad_scale, counter_of) -> norm"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,9 +1,9 @@
 // tilec_linear_fp8: the choice of a kernel of linear_fp8.h, operands whose rows do
 // not begin at multiples of 16 bytes, and the sums of split groups.
 #include <algorithm>
-#include <type_traits>
 
 #include "abi.h"
+#include "enqueue.h"
 #include "linear_fp8.h"
 
 namespace tilec {
@@ -180,13 +180,10 @@ int tilec_linear_fp8(const void* x, const float* x_scale, const void* weight, co
          : (fw ? launch_fp8<0, 1>(a, f8, p.tile, p.splits, st) : launch_fp8<0, 0>(a, f8, p.tile, p.splits, st));
   if (e == hipSuccess && p.splits > 1) {
     const unsigned grid = (unsigned)std::min<int64_t>(cdiv(M * N, 1024), 16 * (int64_t)device_cus());
-    auto join = [&](auto* to) {
-      hipLaunchKernelGGL(fp8_join_kernel<std::remove_pointer_t<decltype(to)>>, dim3(grid), dim3(256), 0, st, a.partial, to,
-                         M * N, a.ldo, a.N, p.splits);
-    };
-    if (f8) join(static_cast<u16*>(out));
-    else join(static_cast<float*>(out));
-    e = hipGetLastError();
+    e = f8 ? enqueue(fp8_join_kernel<u16>, dim3(grid), dim3(256), st, a.partial, static_cast<u16*>(out), M * N, a.ldo, a.N,
+                     p.splits)
+           : enqueue(fp8_join_kernel<float>, dim3(grid), dim3(256), st, a.partial, static_cast<float*>(out), M * N, a.ldo,
+                     a.N, p.splits);
   }
   if (e != hipSuccess) return fail(TILEC_ERR_HIP, "tilec: launching linear_fp8 failed: %s", hipGetErrorString(e));
   return TILEC_OK;

@@ -3,6 +3,7 @@
 
 #include <type_traits>
 
+#include "enqueue.h"
 #include "linear_fp8.h"
 
 namespace tilec {
@@ -734,25 +735,22 @@ __global__ __launch_bounds__(64 * NW, 1) void fp8_stream_kernel(Fp8Args a) {
 template <class P, bool F8, int FX, int FW>
 hipError_t launch_tile(const Fp8Args& a, int splits, hipStream_t stream) {
   const dim3 grid((unsigned)(cdiv(a.M, P::BM) * cdiv(a.N, P::BN)), (unsigned)splits);
-  if (a.wshift == 0) hipLaunchKernelGGL((fp8_tile_kernel<P, F8, FX, FW, true>), grid, dim3(P::NT), 0, stream, a);
-  else hipLaunchKernelGGL((fp8_tile_kernel<P, F8, FX, FW, false>), grid, dim3(P::NT), 0, stream, a);
-  return hipGetLastError();
+  const auto kernel = a.wshift == 0 ? fp8_tile_kernel<P, F8, FX, FW, true> : fp8_tile_kernel<P, F8, FX, FW, false>;
+  return enqueue(kernel, grid, dim3(P::NT), stream, a);
 }
 
 template <class P, bool F8, int FX, int FW>
 hipError_t launch_pair(const Fp8Args& a, int splits, hipStream_t stream) {
   const dim3 grid((unsigned)(cdiv(a.M, P::BM) * cdiv(a.N, P::BN)), (unsigned)splits);
-  if (a.wshift == 0) hipLaunchKernelGGL((fp8_pair_kernel<P, F8, FX, FW, true>), grid, dim3(P::NT), 0, stream, a);
-  else hipLaunchKernelGGL((fp8_pair_kernel<P, F8, FX, FW, false>), grid, dim3(P::NT), 0, stream, a);
-  return hipGetLastError();
+  const auto kernel = a.wshift == 0 ? fp8_pair_kernel<P, F8, FX, FW, true> : fp8_pair_kernel<P, F8, FX, FW, false>;
+  return enqueue(kernel, grid, dim3(P::NT), stream, a);
 }
 
 template <int XR, int NW, bool F8, int FX, int FW>
 hipError_t launch_stream(const Fp8Args& a, int64_t most, hipStream_t stream) {
   const dim3 grid((unsigned)std::min<int64_t>(cdiv(a.N, 16), most));
-  if (a.wshift == 0) hipLaunchKernelGGL((fp8_stream_kernel<XR, NW, 2, F8, FX, FW, true>), grid, dim3(64 * NW), 0, stream, a);
-  else hipLaunchKernelGGL((fp8_stream_kernel<XR, NW, 2, F8, FX, FW, false>), grid, dim3(64 * NW), 0, stream, a);
-  return hipGetLastError();
+  const auto kernel = a.wshift == 0 ? fp8_stream_kernel<XR, NW, 2, F8, FX, FW, true> : fp8_stream_kernel<XR, NW, 2, F8, FX, FW, false>;
+  return enqueue(kernel, grid, dim3(64 * NW), stream, a);
 }
 
 // Eight waves a tile while every workgroup has one tile (4096 x 4096, one row: 5.3

@@ -12,6 +12,7 @@
 
 #include "abi.h"
 #include "common.h"
+#include "enqueue.h"
 #include "fp8.h"
 #include "rows.h"
 #include "../../include/tilec.h"
@@ -333,17 +334,16 @@ int tilec_quantize_fp8(const void* x, void* codes, float* scales, int64_t R, int
     using T = decltype(t);
     if (!trans && block == 1) {
       const dim3 grid = rows_grid(R, a.G, a.lg);
-      hipLaunchKernelGGL(quant_rows_kernel<T>, grid, dim3(256), 0, st, a);
-      return hipGetLastError();
+      return enqueue(quant_rows_kernel<T>, grid, dim3(256), st, a);
     }
     const int64_t tiles = cdiv(R, 128) * a.G;
     if (tiles > INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid((unsigned)tiles);
     const int tiles_c = (int)a.G;
-    if (!trans) hipLaunchKernelGGL((quant_tile_kernel<T, false, true>), grid, dim3(256), 0, st, a, tiles_c);
-    else if (block == 1) hipLaunchKernelGGL((quant_tile_kernel<T, true, false>), grid, dim3(256), 0, st, a, tiles_c);
-    else hipLaunchKernelGGL((quant_tile_kernel<T, true, true>), grid, dim3(256), 0, st, a, tiles_c);
-    return hipGetLastError();
+    const auto kernel = !trans       ? quant_tile_kernel<T, false, true>
+                        : block == 1 ? quant_tile_kernel<T, true, false>
+                                     : quant_tile_kernel<T, true, true>;
+    return enqueue(kernel, grid, dim3(256), st, a, tiles_c);
   };
   const hipError_t e = x_dtype == TILEC_F32 ? by_type(float{}) : by_type(u16{});
   if (e != hipSuccess) return fail(TILEC_ERR_HIP, "tilec: launching quantize_fp8 failed: %s", hipGetErrorString(e));
@@ -369,10 +369,8 @@ int tilec_dequantize_fp8(const void* codes, const float* scales, void* out, int6
   a.R = R, a.C = C, a.ldq = ldq, a.ldo = ldo, a.G = cdiv(C, kGroup);
   a.s_row = scale_row, a.s_group = scale_group, a.shift = block == 1 ? 0 : 7, a.e5m2 = q_dtype == TILEC_F8E5M2;
   const dim3 grid = rows_grid(R, a.G, a.lg);
-  if (out_dtype == TILEC_F32)
-    hipLaunchKernelGGL(values_kernel<float>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
-  else hipLaunchKernelGGL(values_kernel<u16>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
-  const hipError_t e = hipGetLastError();
+  const auto kernel = out_dtype == TILEC_F32 ? values_kernel<float> : values_kernel<u16>;
+  const hipError_t e = enqueue(kernel, grid, dim3(256), static_cast<hipStream_t>(stream), a);
   if (e != hipSuccess) return fail(TILEC_ERR_HIP, "tilec: launching dequantize_fp8 failed: %s", hipGetErrorString(e));
   return TILEC_OK;
 }

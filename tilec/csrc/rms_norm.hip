@@ -21,6 +21,7 @@
 
 #include "abi.h"
 #include "common.h"
+#include "enqueue.h"
 #include "fp8.h"
 #include "rows.h"
 #include "../../include/tilec.h"
@@ -402,15 +403,13 @@ hipError_t launch_rms(RmsArgs a, hipStream_t stream) {
   const NormGeom g = norm_geom(a.R, a.D, E, 4, is_fp8(a.y_type) ? kGroup / E : 1);
   if (g.nv == 0) {
     const unsigned grid = (unsigned)std::min<int64_t>(a.R, kMaxGrid);
-    hipLaunchKernelGGL((rms_long_kernel<TX, TR>), dim3(grid), dim3(1024), 0, stream, a);
-    return hipGetLastError();
+    return enqueue(rms_long_kernel<TX, TR>, dim3(grid), dim3(1024), stream, a);
   }
   a.tpr = g.tpr;
   const int64_t most = kWaves * 64 / g.nt * (int64_t)device_cus();
   const dim3 grid((unsigned)std::min<int64_t>(cdiv(a.R, g.nt / g.tpr), most)), block(g.nt);
   return by_geom<4>(g, [&](auto nv, auto nt) {
-    hipLaunchKernelGGL((rms_kernel<TX, TR, decltype(nv)::value, decltype(nt)::value>), grid, block, 0, stream, a);
-    return hipGetLastError();
+    return enqueue(rms_kernel<TX, TR, decltype(nv)::value, decltype(nt)::value>, grid, block, stream, a);
   });
 }
 
@@ -447,23 +446,19 @@ hipError_t launch_rms_grad(RmsArgs a, const GradGeom& q, float* cs, hipStream_t 
   hipError_t e = hipSuccess;
   if (a.R > 0 && q.g.nv == 0) {
     const unsigned grid = (unsigned)std::min<int64_t>(a.R, kMaxGrid);
-    hipLaunchKernelGGL((rms_grad_rows_kernel<TX, TY>), dim3(grid), dim3(1024), 0, stream, a, cs);
-    e = hipGetLastError();
+    e = enqueue(rms_grad_rows_kernel<TX, TY>, dim3(grid), dim3(1024), stream, a, cs);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((rms_grad_cols_kernel<TX, TY, TD>), dim3((unsigned)cdiv(a.D, 256 * E), (unsigned)q.parts),
-                       dim3(256), 0, stream, a, cs);
-    e = hipGetLastError();
+    e = enqueue(rms_grad_cols_kernel<TX, TY, TD>, dim3((unsigned)cdiv(a.D, 256 * E), (unsigned)q.parts), dim3(256), stream,
+                a, cs);
   } else if (a.R > 0) {
     a.tpr = q.g.tpr;
     e = by_geom<16 / E>(q.g, [&](auto nv, auto nt) {
-      hipLaunchKernelGGL((rms_grad_kernel<TX, TY, TD, decltype(nv)::value, decltype(nt)::value>),
-                         dim3((unsigned)q.parts), dim3(q.g.nt), 0, stream, a);
-      return hipGetLastError();
+      return enqueue(rms_grad_kernel<TX, TY, TD, decltype(nv)::value, decltype(nt)::value>, dim3((unsigned)q.parts),
+                     dim3(q.g.nt), stream, a);
     });
   }
   if (e != hipSuccess || !a.dw || q.parts == 1) return e;
-  hipLaunchKernelGGL(rms_grad_sum_kernel, dim3((unsigned)cdiv(a.D, 16)), dim3(1024), 0, stream, a, (int)q.parts);
-  return hipGetLastError();
+  return enqueue(rms_grad_sum_kernel, dim3((unsigned)cdiv(a.D, 16)), dim3(1024), stream, a, (int)q.parts);
 }
 
 bool is_wide(int32_t t) { return t == TILEC_F32 || t == TILEC_BF16; }

@@ -29,14 +29,8 @@ scratch is each call's own, and there is no autograd.
 import torch
 
 from . import _lib
-from .training import _stream_of
 
 __all__ = ["quantize_fp8", "dequantize_fp8", "linear_fp8"]
-
-
-def _stream_of_pair(q):
-    """The same for a (codes, scales) pair."""
-    return _stream_of(q[0]) if isinstance(q, (tuple, list)) and q else 0
 
 
 def quantize_fp8(x, block=(1, 128), dtype=torch.float8_e4m3fn):
@@ -53,13 +47,13 @@ def quantize_fp8(x, block=(1, 128), dtype=torch.float8_e4m3fn):
     read in place.  The codes' rows begin at multiples of 16 bytes: where C is not
     a multiple of 16 the codes are a view of wider rows.  The last blocks may be smaller.
     """
-    return _lib.host().quantize_fp8(x, tuple(block), dtype, _stream_of(x))
+    return _lib.host().quantize_fp8(x, tuple(block), dtype)
 
 
 def dequantize_fp8(q, dtype=torch.float32):
     """The values that an 8-bit matrix (codes, scales) stands for, as a float32 or
     bfloat16 [R, C]: codes * scales, in float32, rounded once."""
-    return _lib.host().dequantize_fp8(q, dtype, _stream_of_pair(q))
+    return _lib.host().dequantize_fp8(q, dtype)
 
 
 def linear_fp8(x, weight, dtype=torch.float32):
@@ -82,4 +76,4 @@ def linear_fp8(x, weight, dtype=torch.float32):
     have any strides (transposes, with a group's scales of all rows side by side, are
     read 2 % faster at 8192^3, and written 4 % slower).
     """
-    return _lib.host().linear_fp8(x, weight, dtype, _stream_of_pair(x))
+    return _lib.host().linear_fp8(x, weight, dtype)

@@ -19,7 +19,7 @@ from functools import lru_cache
 import torch
 
 from . import _lib
-from .ext import _capturing, _current_device, _raw_stream, _tuned, counters_for
+from .ext import _current_device, _raw_stream, _stream_captured, _tuned, counters_for
 
 __all__ = ["layer_norm", "layer_norm_backward", "rms_norm", "rms_norm_backward", "linear_cross_entropy",
            "linear_cross_entropy_grad", "grad_norm", "clip_grads", "adamw_state", "adamw_step", "adamw_values", "ADAMW_BLOCK"]
@@ -64,7 +64,7 @@ def _ptr(t):
 
 def _stream_of(x):
     """The current stream of the GPU that x is on (0 elsewhere: x is refused)."""
-    return _raw_stream(x.get_device()) if isinstance(x, torch.Tensor) and x.is_cuda else 0
+    return _raw_stream(x.get_device()) if x.is_cuda else 0
 
 
 class _Here:
@@ -130,7 +130,7 @@ def rms_norm(x, weight=None, residual=None, eps=1e-5, dtype=None):
     float32: it overflows (rstd 0) for rows of a norm above 2^64, and squares of
     values below 2^-75 are lost.
     """
-    return _lib.host().rms_norm(x, weight, residual, eps, dtype, _stream_of(x))
+    return _lib.host().rms_norm(x, weight, residual, eps, dtype)
 
 
 def rms_norm_backward(dy, h, rstd, weight=None, dh=None, weight_grad=True):
@@ -146,7 +146,7 @@ def rms_norm_backward(dy, h, rstd, weight=None, dh=None, weight_grad=True):
     dh's type, without dh dy's.  dweight is float32 [D], added in a fixed order
     (the same bits on every call); weight_grad=False leaves it out (None).
     """
-    return _lib.host().rms_norm_backward(dy, h, rstd, weight, dh, weight_grad, _stream_of(dy))
+    return _lib.host().rms_norm_backward(dy, h, rstd, weight, dh, weight_grad)
 
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
@@ -266,13 +266,20 @@ def linear_cross_entropy_grad(x, weight, target, reduction="mean", ignore_index=
                       chunk_rows)
 
 
-def _counter(device, stream, nbytes):
-    """A zeroed counter that its kernel leaves zero: the stream's own, or in a
-    capture one of the graph's, zeroed in every replay (graphs of one stream may be
-    replayed on others at the same time)."""
-    if _capturing(device):
-        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
-    return counters_for(device, stream, nbytes)
+_NORM_COUNTERS = {}  # by device index and stream
+
+
+def _counter(index, stream):
+    """A zeroed counter that the norm's kernel leaves zero: the stream's, in no
+    graph, or in a capture one of the graph's own, zeroed in every replay (a graph may
+    be replayed beside its stream's other work).  `index`: the current device's."""
+    capturing = _stream_captured()
+    kept = None if capturing else _NORM_COUNTERS.get((index, stream))
+    if kept is None:
+        kept = torch.zeros(4, dtype=torch.uint8, device=torch.device("cuda", index))
+        if not capturing:
+            _NORM_COUNTERS[index, stream] = kept
+    return kept
 
 
 def grad_norm(grads, max_norm=None, grad_scale=None):
@@ -290,7 +297,7 @@ def grad_norm(grads, max_norm=None, grad_scale=None):
     and sums are float64, in a fixed order: nothing overflows, and the same bits
     come out on every call.  An infinite norm gives a scale of 0, a NaN one NaN.
     """
-    return _lib.host().grad_norm(grads, max_norm, grad_scale, _raw_stream, _counter)
+    return _lib.host().grad_norm(grads, max_norm, grad_scale, _counter)
 
 
 def clip_grads(grads, max_norm, grad_scale=None):
@@ -298,7 +305,7 @@ def clip_grads(grads, max_norm, grad_scale=None):
     (not touched where that is 1).  Two of them may not share memory, and a view
     whose values do not lie side by side is refused (ValueError).  To autograd they
     have been modified in place."""
-    return _lib.host().clip_grads(grads, max_norm, grad_scale, _raw_stream, _counter)
+    return _lib.host().clip_grads(grads, max_norm, grad_scale, _counter)
 
 
 ADAMW_BLOCK = 256  # values per scale of an 8-bit state
