@@ -266,3 +266,30 @@ def test_cpu_tensors_are_refused():
         tilec.ext.rms_norm(x)
     with pytest.raises(TypeError):
         tilec.ext.rms_norm_backward(x, x, torch.ones(2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ht,dt", [("f32", ""), ("f32", "f32"), ("bf16", ""), ("bf16", "bf16")])
+@pytest.mark.parametrize("R,D", [(2, 4096), (130, 1600), (1023, 1009), (1024, 1009), (1025, 1009), (700, 2049), (1000, 40),
+                                 (64, 16384), (257, 8200), (3, 15)])
+def test_backward_of_few_rows(R, D, ht, dt):
+    # Both gradients in one launch, several rows a workgroup, and just past that.
+    h, dh, w = make(R, D, ht, dt, ht, seed=R * D)
+    dy = torch.randn(R, D, generator=torch.Generator().manual_seed(R)).to(TYPES[ht]).cuda()
+    rstd = tilec.ext.rms_norm(h, w)[2]
+    dx, dw = tilec.ext.rms_norm_backward(dy, h, rstd, w, dh=dh)
+    check_backward(dy, h, rstd, w, dh, dx, dw)
+    again = tilec.ext.rms_norm_backward(dy, h, rstd, w, dh=dh)
+    assert torch.equal(dx, again[0]) and torch.equal(dw, again[1])
+
+
+@pytest.mark.gpu
+def test_backward_of_few_rows_keeps_a_nan_to_its_row_and_column():
+    h, _, w = make(300, 500, "f32", "", "f32", seed=8)
+    dy = torch.randn(300, 500, generator=torch.Generator().manual_seed(9)).cuda()
+    rstd = tilec.ext.rms_norm(h, w)[2]
+    good = tilec.ext.rms_norm_backward(dy, h, rstd, w)
+    dy[299, 499] = float("nan")
+    dx, dw = tilec.ext.rms_norm_backward(dy, h, rstd, w)
+    assert torch.equal(dx[:299], good[0][:299]) and dx[299].isnan().all()
+    assert torch.equal(dw[:499], good[1][:499]) and dw[499].isnan()

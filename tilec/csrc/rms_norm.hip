@@ -15,7 +15,8 @@
 // registers of the threads that serve it, and the backward pass keeps each
 // thread's columns fixed while its workgroup walks over rows, so that dw leaves
 // once, a partial row per workgroup, added in order by a second kernel (no
-// atomics: the same bits every time).
+// atomics: the same bits every time).  Where launches cost more than reading, some
+// workgroups take dx's rows and others dw's columns, in one launch.
 #include <algorithm>
 #include <type_traits>
 
@@ -194,23 +195,19 @@ __device__ __forceinline__ void store_dw(const RmsArgs& a, int part, int parts, 
   else store_group<float, E>(a.partial + (int64_t)part * a.Dp, c, a.Dp, dw);
 }
 
-template <typename TX, typename TY, typename TD, int NV, int NT>
-__global__ __launch_bounds__(NT) void rms_grad_kernel(RmsArgs a) {
-  constexpr int E = 16 / (int)sizeof(TX);
+// dx of the rows that workgroup `block` of `blocks` takes, and its share of dw where
+// DW says so.
+template <typename TX, typename TY, typename TD, bool DW, int NV, int E>
+__device__ __forceinline__ void grad_rows(const RmsArgs& a, int block, int blocks, float (&dw)[NV][E]) {
   __shared__ float red[2][16][1];
-  __shared__ float sums[NT == 256 ? 256 * E : 1];
   int slot = 0;
   const int tpr = a.tpr, D = a.D;
   const int rpb = blockDim.x / tpr;
-  const int sub = rpb == 1 ? threadIdx.x : threadIdx.x & (tpr - 1);
-  float w[NV][E], dw[NV][E];
+  const int sub = rpb == 1 ? threadIdx.x : threadIdx.x % tpr;
+  float w[NV][E];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    load_params<E>(a.w, a.w_bf16, E * (sub + i * tpr), D, 1.f, w[i]);
-#pragma unroll
-    for (int e = 0; e < E; ++e) dw[i][e] = 0.f;
-  }
-  for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < a.R; r0 += (int64_t)gridDim.x * rpb) {
+  for (int i = 0; i < NV; ++i) load_params<E>(a.w, a.w_bf16, E * (sub + i * tpr), D, 1.f, w[i]);
+  for (int64_t r0 = (int64_t)block * rpb; r0 < a.R; r0 += (int64_t)blocks * rpb) {
     const int64_t r = r0 + (rpb == 1 ? 0 : threadIdx.x / tpr);
     const bool live = r < a.R;
     const int64_t rr = live ? r : a.R - 1;
@@ -232,7 +229,9 @@ __global__ __launch_bounds__(NT) void rms_grad_kernel(RmsArgs a) {
       for (int e = 0; e < E; ++e) {
         const float t = dy[i].get(e), h = x[i].get(e) * rstd;
         s[0] = fmaf(t * w[i][e], h, s[0]);
-        if (live) dw[i][e] = fmaf(t, h, dw[i][e]);
+        if constexpr (DW) {
+          if (live) dw[i][e] = fmaf(t, h, dw[i][e]);
+        }
       }
     row_sums(s, tpr, red, slot);
     if (!live) continue;
@@ -250,6 +249,20 @@ __global__ __launch_bounds__(NT) void rms_grad_kernel(RmsArgs a) {
       store_group<TO, E>(out, c, D, v);
     }
   }
+}
+
+template <typename TX, typename TY, typename TD, int NV, int NT>
+__global__ __launch_bounds__(NT) void rms_grad_kernel(RmsArgs a) {
+  constexpr int E = 16 / (int)sizeof(TX);
+  __shared__ float sums[NT == 256 ? 256 * E : 1];
+  const int tpr = a.tpr, D = a.D, rpb = blockDim.x / tpr;
+  const int sub = rpb == 1 ? threadIdx.x : threadIdx.x & (tpr - 1);
+  float dw[NV][E];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < E; ++e) dw[i][e] = 0.f;
+  grad_rows<TX, TY, TD, true>(a, blockIdx.x, gridDim.x, dw);
   if (!a.dw) return;
   // The rows that ran side by side: within a wave by shuffles, then the waves
   // in order through LDS.
@@ -283,6 +296,62 @@ __global__ __launch_bounds__(NT) void rms_grad_kernel(RmsArgs a) {
   for (int i = 0; i < NV; ++i) {
     const int c = E * (sub + i * tpr);
     if (c < D) store_dw<E>(a, blockIdx.x, gridDim.x, c, dw[i]);
+  }
+}
+
+// dw of 4 E columns by one workgroup: four threads across them, the others each a
+// share of the rows, which meet by shuffles and then, waves in order, in LDS.
+template <typename TX, typename TY>
+__device__ __forceinline__ void grad_columns(const RmsArgs& a, int block) {
+  constexpr int E = 16 / (int)sizeof(TX), ACROSS = 4, U = 4;
+  __shared__ float sums[16][ACROSS * E];
+  const int tid = threadIdx.x, c = E * (ACROSS * block + tid % ACROSS), R = (int)a.R, rows = blockDim.x / ACROSS;
+  float dw[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) dw[e] = 0.f;
+  for (int r0 = tid / ACROSS; r0 < R; r0 += U * rows) {
+    Group<TX, E> x[U];
+    Group<TY, E> dy[U];
+    float rstd[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = min(r0 + u * rows, R - 1);
+      x[u].load(static_cast<const TX*>(a.x) + r * a.ldx, c, a.D);
+      dy[u].load(static_cast<const TY*>(a.dy) + r * a.ldy, c, a.D);
+      rstd[u] = a.rstd_in[r];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (r0 + u * rows >= R) break;
+#pragma unroll
+      for (int e = 0; e < E; ++e) dw[e] = fmaf(dy[u].get(e), x[u].get(e) * rstd[u], dw[e]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+#pragma unroll
+    for (int o = ACROSS; o < 64; o <<= 1) dw[e] += __shfl_xor(dw[e], o);
+    if ((tid & 63) < ACROSS) sums[tid >> 6][E * (tid & 3) + e] = dw[e];
+  }
+  __syncthreads();
+  if (tid < ACROSS * E && ACROSS * E * block + tid < a.D) {
+    float t = sums[0][tid];
+    for (int v = 1; v < (int)blockDim.x / 64; ++v) t += sums[v][tid];
+    a.dw[ACROSS * E * block + tid] = t;
+  }
+}
+
+// Both gradients in one launch: the first workgroups take columns, the others rows.
+// dw needs nothing that the rows compute, so no workgroup waits for another; h and dy
+// are read twice, the second time from the caches.
+template <typename TX, typename TY, typename TD, int NV>
+__global__ __launch_bounds__(1024) void rms_grad_small_kernel(RmsArgs a, int column_blocks) {
+  constexpr int E = 16 / (int)sizeof(TX);
+  if ((int)blockIdx.x < column_blocks) {
+    grad_columns<TX, TY>(a, blockIdx.x);
+  } else {
+    float none[NV][E];
+    grad_rows<TX, TY, TD, false>(a, (int)blockIdx.x - column_blocks, (int)gridDim.x - column_blocks, none);
   }
 }
 
@@ -382,19 +451,22 @@ __global__ __launch_bounds__(1024) void rms_grad_sum_kernel(RmsArgs a, int parts
 constexpr int kMaxGrid = 1 << 20;  // workgroups of the passes over long rows; their loops stride over the rest
 constexpr int kWaves = 16;         // a CU, of the forward pass
 
-// f of the kernel's groups a thread and threads a workgroup, as constants.
+// f of the kernel's groups a thread, and (by_geom) threads a workgroup, as constants.
+template <int MAX_NV, typename F>
+hipError_t by_nv(const NormGeom& g, F f) {
+  if constexpr (MAX_NV == 4) {
+    if (g.nv == 4) return f(std::integral_constant<int, 4>{});
+  }
+  return g.nv == 1 ? f(std::integral_constant<int, 1>{}) : f(std::integral_constant<int, 2>{});
+}
 template <int MAX_NV, typename F>
 hipError_t by_geom(const NormGeom& g, F f) {
   using std::integral_constant;
-  auto by_nv = [&](auto nt) {
-    if constexpr (MAX_NV == 4) {
-      if (g.nv == 4) return f(integral_constant<int, 4>{}, nt);
-    }
-    return g.nv == 1 ? f(integral_constant<int, 1>{}, nt) : f(integral_constant<int, 2>{}, nt);
-  };
-  return g.nt <= 256   ? by_nv(integral_constant<int, 256>{})
-         : g.nt <= 512 ? by_nv(integral_constant<int, 512>{})
-                       : by_nv(integral_constant<int, 1024>{});
+  return by_nv<MAX_NV>(g, [&](auto nv) {
+    return g.nt <= 256   ? f(nv, integral_constant<int, 256>{})
+           : g.nt <= 512 ? f(nv, integral_constant<int, 512>{})
+                         : f(nv, integral_constant<int, 1024>{});
+  });
 }
 
 template <typename TX, typename TR>
@@ -416,12 +488,13 @@ hipError_t launch_rms(RmsArgs a, hipStream_t stream) {
 // The backward pass holds 16 columns a thread: their sum, w, h, dy and dh.
 struct GradGeom {
   NormGeom g;
-  int64_t parts;  // partial rows of dw
+  bool small;     // both gradients in one launch
+  int64_t parts;  // partial rows of dw, or workgroups that take rows
   int64_t Dp;
   size_t partial_bytes, c_bytes;
 };
 
-GradGeom grad_geom(int64_t R, int64_t D, int hsz) {
+GradGeom grad_geom(int64_t R, int64_t D, int hsz, bool dw) {
   const int e = 16 / hsz;
   GradGeom q{};
   q.g = norm_geom(R, D, e, 16 / e);
@@ -436,7 +509,16 @@ GradGeom grad_geom(int64_t R, int64_t D, int hsz) {
     q.parts = std::min<int64_t>(R, std::max<int64_t>(1, cdiv(4 * (int64_t)device_cus(), cdiv(D, 256 * e))));
     q.c_bytes = (size_t)(R * sizeof(float) + 15) / 16 * 16;
   }
-  q.partial_bytes = q.parts > 1 ? (size_t)(q.parts * q.Dp) * sizeof(float) : 0;
+  // Up to 1024 rows of 8 MiB in all: one launch instead of two, though h and dy are
+  // read twice (fp32, 64 x 4096 7.1 us and 4.5, 1000 x 1009 9.7 and 8.5, 1024 x 2048
+  // 12.3 and 10.7, but 2048 x 512 7.9 and 11.6, 1024 x 4096 16.1 and 20.3; bf16, 512 x
+  // 2048 8.4 and 6.3, 1024 x 4096 14.8 and 11.4, 2048 x 2048 16.0 and 14.4).
+  q.small = dw && q.g.nv > 0 && q.parts > 1 && R <= 1024 && R * D * hsz <= (int64_t(8) << 20);
+  if (q.small) {
+    q.g.nt = 1024 / q.g.tpr * q.g.tpr;
+    q.parts = cdiv(R, q.g.nt / q.g.tpr);
+  }
+  q.partial_bytes = dw && !q.small && q.parts > 1 ? (size_t)(q.parts * q.Dp) * sizeof(float) : 0;
   return q;
 }
 
@@ -452,6 +534,13 @@ hipError_t launch_rms_grad(RmsArgs a, const GradGeom& q, float* cs, hipStream_t 
                 a, cs);
   } else if (a.R > 0) {
     a.tpr = q.g.tpr;
+    if (q.small) {
+      const int columns = (int)cdiv(a.D, 4 * E);
+      return by_nv<16 / E>(q.g, [&](auto nv) {
+        return enqueue(rms_grad_small_kernel<TX, TY, TD, decltype(nv)::value>, dim3((unsigned)(columns + q.parts)),
+                       dim3(q.g.nt), stream, a, columns);
+      });
+    }
     e = by_geom<16 / E>(q.g, [&](auto nv, auto nt) {
       return enqueue(rms_grad_kernel<TX, TY, TD, decltype(nv)::value, decltype(nt)::value>, dim3((unsigned)q.parts),
                      dim3(q.g.nt), stream, a);
@@ -534,7 +623,7 @@ int tilec_rms_norm(const void* x, const void* residual, const void* weight, void
 
 size_t tilec_rms_norm_backward_workspace_bytes(int64_t R, int64_t D, int32_t h_dtype) {
   if (!is_wide(h_dtype) || check_shape(R, D) != TILEC_OK) return 0;
-  const GradGeom q = grad_geom(R, D, h_dtype == TILEC_F32 ? 4 : 2);
+  const GradGeom q = grad_geom(R, D, h_dtype == TILEC_F32 ? 4 : 2, true);
   return q.c_bytes + q.partial_bytes;
 }
 
@@ -553,7 +642,7 @@ int tilec_rms_norm_backward(const void* dy, const void* h, const float* rstd, co
   if (rc == TILEC_OK) rc = check_rows("dx", dx, lddx, R, D);
   if (rc != TILEC_OK) return rc;
   if (R > 0 && rstd == nullptr) return fail(TILEC_ERR_VALUE, "tilec: RMS norm: rstd is NULL");
-  const GradGeom q = grad_geom(R, D, h_dtype == TILEC_F32 ? 4 : 2);
+  const GradGeom q = grad_geom(R, D, h_dtype == TILEC_F32 ? 4 : 2, dweight != nullptr);
   const size_t need = q.c_bytes + q.partial_bytes;
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(TILEC_ERR_WORKSPACE, "tilec: RMS norm's backward pass needs %zu workspace bytes (got %zu)", need,

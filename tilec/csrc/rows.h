@@ -117,15 +117,16 @@ __device__ __forceinline__ void row_sums(float (&s)[NS], int tpr, float (*red)[1
     for (int i = 0; i < NS; ++i) s[i] += __shfl_xor(s[i], o);
   }
   if (tpr <= 64) return;
-  const int wave = threadIdx.x >> 6, waves = tpr >> 6;  // past a wave a row has the workgroup to itself
+  const int wave = threadIdx.x >> 6, waves = tpr >> 6;
+  const int first = tpr == (int)blockDim.x ? 0 : wave / waves * waves;  // of the row
   if ((threadIdx.x & 63) == 0) {
 #pragma unroll
     for (int i = 0; i < NS; ++i) red[slot][wave][i] = s[i];
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < NS; ++i) s[i] = red[slot][0][i];
-  for (int w = 1; w < waves; ++w) {
+  for (int i = 0; i < NS; ++i) s[i] = red[slot][first][i];
+  for (int w = first + 1; w < first + waves; ++w) {
 #pragma unroll
     for (int i = 0; i < NS; ++i) s[i] += red[slot][w][i];
   }
