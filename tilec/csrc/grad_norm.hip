@@ -26,7 +26,7 @@ namespace {
 typedef unsigned short u16;
 typedef u32x4 __attribute__((aligned(2))) u32x4_any;
 
-constexpr int kMaxTensors = 128;  // per launch: 2.1 KiB of arguments
+constexpr int kMaxTensors = 224;  // per launch: 3.6 KiB of arguments, of at most 4
 constexpr int kUnit = 4096;       // chunks are a multiple of this
 
 constexpr int64_t kMaxBlocks = int64_t(1) << 22;  // workgroups of a launch
