@@ -375,22 +375,24 @@ int tilec_adamw_values(const tilec_adamw_tensor* tensors, int32_t count, void* s
  * float32.  For a float32 out so are those within a group, of exact products;
  * for a bfloat16 out they are the 8-bit matrix instructions', which cut every
  * product at 2^-13 of the largest among eight consecutive k (1.5e-5 of the result
- * for normal values).  The product of two scales is rounded to float32.  The same bits on every call on one device.
- * K <= 2^22; K == 0 writes zeros.
+ * for normal values).  The product of two scales is rounded to float32.  The
+ * same bits on every call on one device.  K <= 2^22; K == 0 writes zeros.
  *
  * Operands are read in place where their rows begin at multiples of 16 bytes,
  * and otherwise copied into the workspace first; scales of rows are read fastest
- * with a row stride of 1 (8192^3: 2 %).  `workspace`: tilec_linear_fp8_workspace_bytes for the
- * same arguments (of x and weight it reads the addresses' alignment only), any
- * contents, 16-byte aligned.
+ * with a row stride of 1 (8192^3: 2 %).  tilec_linear_fp8_scratch_bytes says for
+ * the same arguments (of x and weight it reads the addresses' alignment only) how
+ * much `workspace` (any contents, 16-byte aligned) and `counters` (4-byte aligned,
+ * zero before the call and left zero) it takes; concurrent calls need their own.
  */
 int tilec_linear_fp8(const void* x, const float* x_scale, const void* weight, const float* w_scale, void* out,
                      int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldo, int64_t x_scale_row,
                      int64_t x_scale_group, int64_t w_scale_row, int64_t w_scale_group, int32_t x_dtype, int32_t w_dtype,
                      int32_t out_dtype, int32_t x_block, int32_t w_block, void* workspace, size_t workspace_bytes,
-                     void* stream);
-size_t tilec_linear_fp8_workspace_bytes(const void* x, const void* weight, int64_t M, int64_t N, int64_t K, int64_t ldx,
-                                        int64_t ldw, int32_t x_dtype, int32_t w_dtype, int32_t out_dtype);
+                     void* counters, size_t counter_bytes, void* stream);
+int tilec_linear_fp8_scratch_bytes(const void* x, const void* weight, int64_t M, int64_t N, int64_t K, int64_t ldx,
+                                   int64_t ldw, int32_t x_dtype, int32_t w_dtype, int32_t out_dtype,
+                                   size_t* workspace_bytes, size_t* counter_bytes);
 
 /*
  * 8-bit operands.  A block's scale and codes, each operation a float32 one that
@@ -435,7 +437,7 @@ int tilec_rms_norm(const void* x, const void* residual, const void* weight, void
  * from its other reader.  dx has dh's type, or dy's without it; dweight [D],
  * float32, may be NULL and is added in a fixed order.  `workspace`:
  * tilec_rms_norm_backward_workspace_bytes, any contents, 16-byte aligned.  dx may
- * be dy or dh where it has that type.
+ * be dh where it has that type, and overlaps nothing else.
  */
 int tilec_rms_norm_backward(const void* dy, const void* h, const float* rstd, const void* weight, const void* dh,
                             void* dx, float* dweight, int64_t R, int64_t D, int64_t lddy, int64_t ldh, int64_t lddh,

@@ -18,15 +18,19 @@ OK, VALUE, TYPE, WORKSPACE = _lib.OK, _lib.ERR_VALUE, _lib.ERR_TYPE, _lib.ERR_WO
 
 
 def linear(M=4, N=8, K=256, x=16, sx=16, w=16, sw=16, out=16, ldx=None, ldw=None, ldo=None, srow=2, sgroup=1, xd=E4, wd=E5,
-           od=F32, xb=1, wb=128, ws=None, ws_bytes=0):
+           od=F32, xb=1, wb=128, ws=None, ws_bytes=0, cnt=None, cnt_bytes=0):
     # Non-null dummy pointers: every case must fail (or finish) before launch.
     return _lib.lib().tilec_linear_fp8(x, sx, w, sw, out, M, N, K, K if ldx is None else ldx, K if ldw is None else ldw,
-                                       N if ldo is None else ldo, srow, sgroup, 2, 1, xd, wd, od, xb, wb, ws, ws_bytes, None)
+                                       N if ldo is None else ldo, srow, sgroup, 2, 1, xd, wd, od, xb, wb, ws, ws_bytes, cnt,
+                                       cnt_bytes, None)
 
 
 def linear_bytes(M, N, K, x=16, w=16, ldx=None, ldw=None, od=F32):
-    return _lib.lib().tilec_linear_fp8_workspace_bytes(x, w, M, N, K, K if ldx is None else ldx, K if ldw is None else ldw,
-                                                       E4, E4, od)
+    ws, cnt = ctypes.c_size_t(), ctypes.c_size_t()
+    rc = _lib.lib().tilec_linear_fp8_scratch_bytes(x, w, M, N, K, K if ldx is None else ldx, K if ldw is None else ldw, E4, E4,
+                                                   od, ctypes.byref(ws), ctypes.byref(cnt))
+    assert rc == OK and cnt.value % 256 == 0 and (cnt.value == 0 or ws.value > 0)
+    return ws.value
 
 
 def test_linear_refusals():
@@ -41,6 +45,9 @@ def test_linear_refusals():
     # An unaligned operand is copied, split sums are kept.
     assert linear(x=17) == WORKSPACE and linear(ldw=257) == WORKSPACE
     assert linear(M=100, N=100, K=8192) == WORKSPACE and linear(M=100, N=100, K=8192, ws=16, ws_bytes=1000) == WORKSPACE
+    need = linear_bytes(100, 100, 8192)
+    assert linear(M=100, N=100, K=8192, ws=16, ws_bytes=need) == WORKSPACE and "counter" in _lib.last_error()
+    assert linear(M=100, N=100, K=8192, ws=16, ws_bytes=need, cnt=16, cnt_bytes=255) == WORKSPACE
 
 
 def test_linear_workspace():
@@ -50,8 +57,9 @@ def test_linear_workspace():
     assert linear_bytes(5, 7, 130, x=17, ldw=144) == 5 * 144
     assert linear_bytes(1, 7, 128, ldx=3) == 0  # one row has no stride
     assert linear_bytes(5, 7, 128, w=24) == 7 * 128
-    assert linear_bytes(100, 100, 8192) % (100 * 100 * 4) == 0 and linear_bytes(100, 100, 8192) >= 2 * 100 * 100 * 4
-    assert linear_bytes(0, 7, 130, x=17) == linear_bytes(5, 7, 0) == linear_bytes(-1, 7, 130) == 0
+    assert linear_bytes(100, 100, 8192) % (128 * 128 * 4) == 0 and linear_bytes(100, 100, 8192) >= 2 * 100 * 100 * 4
+    assert linear_bytes(0, 7, 130, x=17) == linear_bytes(5, 7, 0) == 0
+    assert _lib.lib().tilec_linear_fp8_scratch_bytes(16, 16, -1, 7, 130, 130, 130, E4, E4, F32, None, None) == VALUE
 
 
 def test_quantize_refusals():
@@ -87,12 +95,13 @@ def test_rms_refusals():
     assert f(R=0, x=None, y=None) == OK
     L = _lib.lib()
 
-    def b(R=4, D=64, dy=16, h=16, rstd=16, dh=None, dx=16, dw=16, ld=64, lddh=64, yd=F32, hd=F32, dd=F32, wd=F32, ws=None, n=0):
+    def b(R=4, D=64, dy=16, h=16, rstd=16, dh=None, dx=32, dw=16, ld=64, lddh=64, yd=F32, hd=F32, dd=F32, wd=F32, ws=None, n=0):
         return L.tilec_rms_norm_backward(dy, h, rstd, None, dh, dx, dw, R, D, ld, ld, lddh, ld, yd, hd, dd, wd, ws, n, None)
 
     for kw in ({"yd": E4}, {"hd": E4}, {"wd": 9}, {"dh": 16, "dd": E5}):
         assert b(**kw) == TYPE, kw
-    for kw in ({"R": -1}, {"D": 0}, {"dy": None}, {"h": None}, {"rstd": None}, {"dx": None}, {"ld": 63}, {"dh": 16, "lddh": 63}):
+    for kw in ({"R": -1}, {"D": 0}, {"dy": None}, {"h": None}, {"rstd": None}, {"dx": None}, {"ld": 63}, {"dh": 16, "lddh": 63},
+               {"dx": 16}):  # dx in dy's place
         assert b(**kw) == VALUE, kw
     assert L.tilec_rms_norm_backward_workspace_bytes(1, 64, F32) == 0
     assert L.tilec_rms_norm_backward_workspace_bytes(3000, 64, F32) > 0

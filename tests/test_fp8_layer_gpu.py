@@ -153,3 +153,56 @@ def test_two_threads_on_one_stream():
     for th in threads:
         th.join()
     assert not bad
+
+
+def split_operands(M, N, K):
+    g = torch.Generator().manual_seed(M + N)
+    return tuple(tilec.ext.quantize_fp8(torch.randn(r, K, generator=g).cuda()) for r in (M, N))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_split_products_on_two_streams_and_in_graphs(dt):
+    # Workgroups that share a tile count themselves in: counts of two streams, of a
+    # graph and of the stream that it was recorded on are apart, and zero afterwards.
+    f = tilec.ext.linear_fp8
+    operands = [split_operands(*s) for s in ((70, 192, 9088), (38, 3584, 4800), (300, 100, 3000))]
+    want = [f(*o, dtype=dt) for o in operands]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        inside = [f(*o, dtype=dt) for o in operands]
+    for _ in range(4):
+        out = []
+        for s in streams[:2]:
+            with torch.cuda.stream(s):
+                out.append([f(*o, dtype=dt) for _ in range(5) for o in operands])
+        with torch.cuda.stream(streams[2]):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want[i % 3]) for got in out for i, o in enumerate(got))
+        assert all(torch.equal(o, w) for o, w in zip(inside, want))
+        for o in inside:
+            o.zero_()
+
+
+@pytest.mark.gpu
+def test_split_products_of_two_threads_on_one_stream():
+    f = tilec.ext.linear_fp8
+    operands = [split_operands(*s) for s in ((70, 192, 9088), (33, 4096, 2048))]
+    want = [f(*o) for o in operands]
+    got = [[], []]
+    start = threading.Barrier(2, timeout=20)
+
+    def work(k):
+        start.wait()
+        got[k] = [f(*operands[k]) for _ in range(100)]
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    assert all(len(g) == 100 and all(torch.equal(o, w) for o in g) for g, w in zip(got, want))

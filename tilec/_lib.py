@@ -54,8 +54,9 @@ SIGNATURES = {
                                                      ctypes.POINTER(_i64)]),
     "tilec_adamw": (ctypes.c_int, [_vp, _i32, _i32, _i64, _f64, _f64, _f64, _f64, _f64, _vp, _vp]),
     "tilec_adamw_values": (ctypes.c_int, [_vp, _i32, _vp]),
-    "tilec_linear_fp8": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, *[_i64] * 10, _i32, _i32, _i32, _i32, _i32, _vp, _sz, _vp]),
-    "tilec_linear_fp8_workspace_bytes": (_sz, [_vp, _vp, *[_i64] * 5, _i32, _i32, _i32]),
+    "tilec_linear_fp8": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, *[_i64] * 10, _i32, _i32, _i32, _i32, _i32, _vp, _sz, _vp, _sz,
+                                       _vp]),
+    "tilec_linear_fp8_scratch_bytes": (ctypes.c_int, [_vp, _vp, *[_i64] * 5, _i32, _i32, _i32, _vp, _vp]),
     "tilec_quantize_fp8": (ctypes.c_int, [_vp, _vp, _vp, *[_i64] * 6, _i32, _i32, _i32, _i32, _vp]),
     "tilec_dequantize_fp8": (ctypes.c_int, [_vp, _vp, _vp, *[_i64] * 6, _i32, _i32, _i32, _vp]),
     "tilec_rms_norm": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, *[_i64] * 8, _i32, _i32, _i32, _i32,

@@ -26,16 +26,16 @@
 //   rms_norm_backward(dy, h, rstd, weight, dh, weight_grad) -> (dx, dweight)
 //   quantize_fp8(x, block, dtype) -> (codes, scales)
 //   dequantize_fp8(q, dtype) -> values
-//   linear_fp8(x, weight, dtype) -> out
+//   linear_fp8(x, weight, dtype, counters_of) -> out
 //
 // do the same and find the stream themselves; 8-bit operands are (codes, scales)
 // pairs.
 //
-//   grad_norm(grads, max_norm, grad_scale, counter_of) -> (norm, scale)
-//   clip_grads(grads, max_norm, grad_scale, counter_of) -> norm
+//   grad_norm(grads, max_norm, grad_scale, counters_of) -> (norm, scale)
+//   clip_grads(grads, max_norm, grad_scale, counters_of) -> norm
 //
-// read lists as adamw_step does; counter_of(device index, stream) gives the zeroed
-// counter that the norm's kernel leaves zero.
+// read lists as adamw_step does; counters_of(device index, stream, bytes) gives the
+// zeroed counters that kernels leave zero.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -484,6 +484,15 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // The current stream of a GPU.
 void* stream_on(at::Device device) { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
 
+// The zeroed counters, which kernels leave zero, that `counters_of` gives.
+at::Tensor zeroed(PyObject* counters_of, at::Device device, void* stream, size_t bytes) {
+  THPObjectPtr handle(PyLong_FromVoidPtr(stream));
+  if (!handle) throw python_error();
+  THPObjectPtr held(PyObject_CallFunction(counters_of, "iOn", (int)device.index(), handle.get(), (Py_ssize_t)bytes));
+  if (!held) throw python_error();
+  return tensor("counters", held.get());
+}
+
 // A new tensor on a GPU, past the dispatcher: 0.5 us instead of 0.75.
 at::Tensor make(at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
   return at::Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
@@ -663,14 +672,17 @@ PyObject* build_linear(PyObject* const* args) {
   const c10::DeviceGuard guard(x.codes.device());
   const at::Tensor out = make({x.R, w.R}, type, x.codes.device());
   const void *xp = x.codes.const_data_ptr(), *wp = w.codes.const_data_ptr();
-  const size_t need =
-      tilec_linear_fp8_workspace_bytes(xp, wp, x.R, w.R, x.C, x.ld, w.ld, x.code, w.code, code_of(type));
-  at::Tensor scratch;
+  size_t need = 0, counts = 0;
+  check(tilec_linear_fp8_scratch_bytes(xp, wp, x.R, w.R, x.C, x.ld, w.ld, x.code, w.code, code_of(type), &need, &counts));
+  void* const stream = stream_on(x.codes.device());
+  at::Tensor scratch, counters;
   if (need > 0) scratch = make({(int64_t)need}, at::kByte, x.codes.device());
+  if (counts > 0) counters = zeroed(args[3], x.codes.device(), stream, counts);
   check(tilec_linear_fp8(xp, static_cast<const float*>(x.scales.const_data_ptr()), wp,
                          static_cast<const float*>(w.scales.const_data_ptr()), out.data_ptr(), x.R, w.R, x.C, x.ld, w.ld,
                          w.R, x.s_row, x.s_group, w.s_row, w.s_group, x.code, w.code, code_of(type), x.block, w.block,
-                         need > 0 ? scratch.data_ptr() : nullptr, need, stream_on(x.codes.device())));
+                         need > 0 ? scratch.data_ptr() : nullptr, need, counts > 0 ? counters.data_ptr() : nullptr,
+                         counts, stream));
   return THPVariable_Wrap(out);
 }
 
@@ -713,7 +725,7 @@ struct Grads {
   }
 };
 
-// Enqueues the norm; {norm, scale}.  args: grads, max_norm, grad_scale, counter_of.
+// Enqueues the norm; {norm, scale}.  args: grads, max_norm, grad_scale, counters_of.
 std::pair<at::Tensor, at::Tensor> norm_of(Grads& g, PyObject* const* args, void*& stream) {
   const double max_norm = args[1] == Py_None ? -1. : number(args[1]);
   if (args[1] != Py_None && !(max_norm >= 0)) bad_value("max_norm is negative or not a number");
@@ -724,11 +736,7 @@ std::pair<at::Tensor, at::Tensor> norm_of(Grads& g, PyObject* const* args, void*
     grad_scale = static_cast<const float*>(t.const_data_ptr());
   }
   stream = stream_on(g.device);
-  THPObjectPtr handle(PyLong_FromVoidPtr(stream));
-  if (!handle) throw python_error();
-  THPObjectPtr held(PyObject_CallFunction(args[3], "iO", (int)g.device.index(), handle.get()));
-  if (!held) throw python_error();
-  const at::Tensor counter = tensor("counters", held.get());
+  const at::Tensor counter = zeroed(args[3], g.device, stream, sizeof(unsigned));
   const at::Tensor norm = make({}, at::kFloat, g.device), scale = make({}, at::kFloat, g.device);
   const size_t need = tilec_grad_norm_workspace_bytes(g.table.data(), (int32_t)g.table.size());
   at::Tensor scratch;
@@ -801,11 +809,12 @@ PyMethodDef kMethods[] = {
      "quantize_fp8(x, block, dtype) -> (codes, scales)"},
     {"dequantize_fp8", function<build_dequantize, 2, kDequantize>(), METH_FASTCALL,
      "dequantize_fp8(q, dtype) -> values"},
-    {"linear_fp8", function<build_linear, 3, kLinear>(), METH_FASTCALL, "linear_fp8(x, weight, dtype) -> out"},
+    {"linear_fp8", function<build_linear, 4, kLinear>(), METH_FASTCALL,
+     "linear_fp8(x, weight, dtype, counters_of) -> out"},
     {"grad_norm", function<build_grad_norm, 4, kGradNorm>(), METH_FASTCALL,
-     "grad_norm(grads, max_norm, grad_scale, counter_of) -> (norm, scale)"},
+     "grad_norm(grads, max_norm, grad_scale, counters_of) -> (norm, scale)"},
     {"clip_grads", function<build_clip, 4, kClip>(), METH_FASTCALL,
-     "clip_grads(grads, max_norm, grad_scale, counter_of) -> norm"},
+     "clip_grads(grads, max_norm, grad_scale, counters_of) -> norm"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

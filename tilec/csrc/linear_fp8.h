@@ -28,7 +28,8 @@ struct Fp8Args {
   const unsigned char *x, *w;
   const float *sx, *sw;
   void* out;
-  float* partial;  // [splits][M][N], where there are several
+  float* partial;      // of splits, where there are several, and
+  unsigned* counters;  // their tiles' counts
   int64_t ldx, ldw, ldo;
   int64_t sx_row, sx_group, sw_row, sw_group;  // strides of the scales
   int M, N, K, G;      // G: groups of K
@@ -41,18 +42,19 @@ struct Fp8Args {
 template <int FX, int FW>
 hipError_t launch_fp8(const Fp8Args& a, bool f8, int tile, int splits, hipStream_t stream);
 
-// A tile and what it takes, in us on an MI355X: a workgroup's start and end, and a
+// A tile, how many splits of K its last workgroup adds up at a time, and what it takes, in us on an MI355X: a workgroup's start and end, and a
 // step of 128 k, of bfloat16 outputs ([1]) and float32 ones ([0]); step2: with two
 // workgroups on a CU, where that many fit.
 struct Fp8Tile {
   int bm, bn[2];
+  int batch;
   float fixed[2], step[2], step2[2];
 };
 constexpr Fp8Tile kFp8Tiles[] = {
-    {256, {128, 256}, {9.0f, 9.7f}, {1.6f, 1.7f}, {0.f, 0.f}},
-    {128, {128, 128}, {7.0f, 5.5f}, {1.05f, 0.58f}, {0.f, 0.f}},
-    {64, {128, 128}, {4.3f, 3.6f}, {0.70f, 0.37f}, {0.f, 0.f}},
-    {64, {64, 64}, {3.6f, 3.1f}, {0.43f, 0.30f}, {0.75f, 0.47f}},
+    {256, {128, 256}, 0, {9.0f, 9.7f}, {1.6f, 1.7f}, {0.f, 0.f}},
+    {128, {128, 128}, 2, {7.0f, 5.5f}, {1.05f, 0.58f}, {0.f, 0.f}},
+    {64, {128, 128}, 4, {4.3f, 3.6f}, {0.70f, 0.37f}, {0.f, 0.f}},
+    {64, {64, 64}, 4, {3.6f, 3.1f}, {0.43f, 0.30f}, {0.75f, 0.47f}},
 };
 constexpr int kFp8TileCount = 4;
 constexpr int kFp8StreamRows = 16;  // the most rows of x that the streaming kernel takes

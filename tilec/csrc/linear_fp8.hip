@@ -3,14 +3,11 @@
 #include <algorithm>
 
 #include "abi.h"
-#include "enqueue.h"
 #include "linear_fp8.h"
 
 namespace tilec {
 
 namespace {
-
-typedef unsigned short u16;
 
 constexpr int64_t kMaxScaleRow = int64_t(1) << 21, kMaxScaleGroup = int64_t(1) << 40;
 constexpr int64_t kMaxTiles = (int64_t(1) << 23) - 1;  // of up to 512 threads: a grid has less than 2^32
@@ -20,7 +17,7 @@ struct Plan {
   int splits, steps;   // groups of K a split
   bool copy_x, copy_w;
   int64_t padded;      // row stride of a copied operand
-  size_t x_bytes, w_bytes, partial_bytes;
+  size_t x_bytes, w_bytes, partial_bytes, counter_bytes;
   size_t bytes() const { return x_bytes + w_bytes + partial_bytes; }
 };
 
@@ -47,53 +44,35 @@ Plan plan_of(const void* x, const void* w, int64_t M, int64_t N, int64_t K, int6
     return p;
   }
   // The tile and the splits of K that are estimated to be done first: whole turns
-  // over the chip, and with splits the partial sums written, read and joined by a
-  // kernel of its own (2 us, 4.5 TB/s).
+  // over the chip, and with splits the partial sums, added up by the last of a tile's
+  // workgroups `batch` splits at a time (measured 1.5 to 2.2 us for one batch, 3.5 and
+  // 5.3 for two and three; a kernel of its own took 4 to 13: 38 x 3584 x 4800 bf16 13.0
+  // us so, 8.3 now, 70 x 192 x 9088 17.5 and 9.1).
   p.tile = kFp8TileCount;
   double best = 1e30;
   for (int t = 0; t < kFp8TileCount; ++t) {
     const Fp8Tile& g = kFp8Tiles[t];
     const int64_t n = cdiv(M, g.bm) * cdiv(N, g.bn[f8]);
     if (n > kMaxTiles) continue;
-    for (int64_t s = 1; s <= std::min<int64_t>(G, 64); ++s) {
+    const int64_t most = t == 0 ? 1 : std::min<int64_t>(G, 64);
+    for (int64_t s = 1; s <= most; ++s) {
       const int64_t steps = cdiv(G, s), splits = cdiv(G, steps);
       if (splits != s) continue;
       const int64_t groups = n * splits;
-      if (s > 1 && groups > 2 * cus) break;
+      if (s > 1 && (groups > 2 * cus || groups * g.bm * g.bn[f8] >= (int64_t(1) << 29))) break;
       const bool two = g.step2[f8] > 0.f && groups > cus;
       double time = (double)cdiv(groups, two ? 2 * cus : cus) * (g.fixed[f8] + (double)steps * (two ? g.step2 : g.step)[f8]);
-      if (s > 1) time += 2. + (double)M * (double)N * (4. * (double)s + (f8 ? 2. : 4.)) / 4.5e6;
+      if (s > 1) time += 0.2 + 1.6 * (double)cdiv(s, g.batch) + (double)M * (double)N * 8. * (double)s / 12e6;
       if (time < best) best = time, p.tile = t, p.splits = (int)splits, p.steps = (int)steps;
     }
   }
-  if (p.splits > 1) p.partial_bytes = round16((int64_t)p.splits * M * N * 4);
-  return p;
-}
-
-// out = the sum of the splits' partial sums, in order: a float4 a thread.
-template <typename TO>
-__global__ __launch_bounds__(256) void fp8_join_kernel(const float* __restrict__ partial, TO* __restrict__ out, int64_t n,
-                                                       int64_t ldo, int N, int splits) {
-  for (int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x); i < n; i += 4 * 256 * (int64_t)gridDim.x) {
-    const int live = (int)min((int64_t)4, n - i);
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    typedef f32x4 __attribute__((aligned(4))) f32x4_any;
-    for (int k = 0; k < splits; ++k) {
-      const float* p = partial + k * n + i;
-      if (live == 4) {
-        const f32x4 v = *reinterpret_cast<const f32x4_any*>(p);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += v[e];
-      } else {
-        for (int e = 0; e < live; ++e) s[e] += p[e];
-      }
-    }
-    for (int e = 0; e < live; ++e) {
-      const int64_t m = (i + e) / N, at = m * ldo + (i + e - m * N);
-      if constexpr (sizeof(TO) == 4) out[at] = s[e];
-      else out[at] = __builtin_bit_cast(u16, (__bf16)s[e]);
-    }
+  if (p.splits > 1) {
+    const Fp8Tile& g = kFp8Tiles[p.tile];
+    const int64_t n = cdiv(M, g.bm) * cdiv(N, g.bn[f8]);
+    p.partial_bytes = (size_t)(p.splits * n * g.bm * g.bn[f8] * 4);
+    p.counter_bytes = (size_t)n * kSplitCounterStride * sizeof(unsigned);
   }
+  return p;
 }
 
 int check_linear(int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int32_t x_dtype, int32_t w_dtype,
@@ -125,18 +104,24 @@ using namespace tilec;
 
 extern "C" {
 
-size_t tilec_linear_fp8_workspace_bytes(const void* x, const void* weight, int64_t M, int64_t N, int64_t K, int64_t ldx,
-                                        int64_t ldw, int32_t x_dtype, int32_t w_dtype, int32_t out_dtype) {
+int tilec_linear_fp8_scratch_bytes(const void* x, const void* weight, int64_t M, int64_t N, int64_t K, int64_t ldx,
+                                   int64_t ldw, int32_t x_dtype, int32_t w_dtype, int32_t out_dtype,
+                                   size_t* workspace_bytes, size_t* counter_bytes) {
+  clear_error();
   const Scales sx{1, 0, 0}, sw{1, 0, 0};
-  if (check_linear(M, N, K, ldx, ldw, x_dtype, w_dtype, out_dtype, sx, sw) != TILEC_OK || M == 0 || N == 0 || K == 0) return 0;
-  return plan_of(x, weight, M, N, K, ldx, ldw, out_dtype == TILEC_BF16).bytes();
+  const int rc = check_linear(M, N, K, ldx, ldw, x_dtype, w_dtype, out_dtype, sx, sw);
+  if (rc != TILEC_OK) return rc;
+  const Plan p = M > 0 && N > 0 && K > 0 ? plan_of(x, weight, M, N, K, ldx, ldw, out_dtype == TILEC_BF16) : Plan{};
+  if (workspace_bytes != nullptr) *workspace_bytes = p.bytes();
+  if (counter_bytes != nullptr) *counter_bytes = p.counter_bytes;
+  return TILEC_OK;
 }
 
 int tilec_linear_fp8(const void* x, const float* x_scale, const void* weight, const float* w_scale, void* out,
                      int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldo, int64_t x_scale_row,
                      int64_t x_scale_group, int64_t w_scale_row, int64_t w_scale_group, int32_t x_dtype, int32_t w_dtype,
                      int32_t out_dtype, int32_t x_block, int32_t w_block, void* workspace, size_t workspace_bytes,
-                     void* stream) {
+                     void* counters, size_t counter_bytes, void* stream) {
   clear_error();
   const Scales sx{x_block, x_scale_row, x_scale_group}, sw{w_block, w_scale_row, w_scale_group};
   const int rc = check_linear(M, N, K, ldx, ldw, x_dtype, w_dtype, out_dtype, sx, sw);
@@ -156,6 +141,9 @@ int tilec_linear_fp8(const void* x, const float* x_scale, const void* weight, co
   if (p.bytes() > 0 && (workspace == nullptr || workspace_bytes < p.bytes()))
     return fail(TILEC_ERR_WORKSPACE, "tilec: linear_fp8 needs %zu workspace bytes (got %zu)", p.bytes(),
                 workspace == nullptr ? (size_t)0 : workspace_bytes);
+  if (p.counter_bytes > 0 && (counters == nullptr || counter_bytes < p.counter_bytes))
+    return fail(TILEC_ERR_WORKSPACE, "tilec: linear_fp8 needs %zu counter bytes (got %zu)", p.counter_bytes,
+                counters == nullptr ? (size_t)0 : counter_bytes);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   char* const ws = static_cast<char*>(workspace);
   hipError_t e = hipSuccess;
@@ -170,6 +158,7 @@ int tilec_linear_fp8(const void* x, const float* x_scale, const void* weight, co
   a.sx = x_scale, a.sw = w_scale, a.out = out;
   a.sx_row = sx.row, a.sx_group = sx.group, a.sw_row = sw.row, a.sw_group = sw.group;
   a.partial = reinterpret_cast<float*>(ws + p.x_bytes + p.w_bytes);
+  a.counters = static_cast<unsigned*>(counters);
   // (One row has no stride; its length stands in.)
   a.ldx = p.copy_x || M == 1 ? p.padded : ldx, a.ldw = p.copy_w || N == 1 ? p.padded : ldw, a.ldo = M > 1 ? ldo : N;
   a.M = (int)M, a.N = (int)N, a.K = (int)K, a.G = (int)cdiv(K, kGroup);
@@ -178,13 +167,6 @@ int tilec_linear_fp8(const void* x, const float* x_scale, const void* weight, co
   const int fx = x_dtype == TILEC_F8E5M2, fw = w_dtype == TILEC_F8E5M2;
   e = fx ? (fw ? launch_fp8<1, 1>(a, f8, p.tile, p.splits, st) : launch_fp8<1, 0>(a, f8, p.tile, p.splits, st))
          : (fw ? launch_fp8<0, 1>(a, f8, p.tile, p.splits, st) : launch_fp8<0, 0>(a, f8, p.tile, p.splits, st));
-  if (e == hipSuccess && p.splits > 1) {
-    const unsigned grid = (unsigned)std::min<int64_t>(cdiv(M * N, 1024), 16 * (int64_t)device_cus());
-    e = f8 ? enqueue(fp8_join_kernel<u16>, dim3(grid), dim3(256), st, a.partial, static_cast<u16*>(out), M * N, a.ldo, a.N,
-                     p.splits)
-           : enqueue(fp8_join_kernel<float>, dim3(grid), dim3(256), st, a.partial, static_cast<float*>(out), M * N, a.ldo,
-                     a.N, p.splits);
-  }
   if (e != hipSuccess) return fail(TILEC_ERR_HIP, "tilec: launching linear_fp8 failed: %s", hipGetErrorString(e));
   return TILEC_OK;
 }

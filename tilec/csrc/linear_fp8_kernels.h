@@ -330,22 +330,31 @@ __global__ __launch_bounds__(P::NT, 1) void fp8_tile_kernel(Fp8Args a) {
     if constexpr (P::NBUF > 3) rest(integral_constant<int, 4>{});
   }
 
-  const bool inside = m0 + P::BM <= a.M && n0 + P::BN <= a.N;
-  auto store = [&](auto* out, int64_t ld) __attribute__((always_inline)) {
-    using T = std::remove_pointer_t<decltype(out)>;
-    const int mw = m0 + wm * (P::BM / P::WM) + row, nw = n0 + wn * (P::BN / P::WN) + 4 * quad;
-    T* const first = out + (int64_t)mw * ld;
+  const int mw = m0 + wm * (P::BM / P::WM) + row, nw = n0 + wn * (P::BN / P::WN) + 4 * quad;
+  if (gridDim.y > 1) {  // the split that comes last adds them all up, in order
+    __shared__ int last;
+    constexpr int NV = P::MT * P::NB;
+    f32x4 v[NV];
+    bool live[NV];
 #pragma unroll
-    for (int i = 0; i < P::MT; ++i) {
-      T* const line = first + (int64_t)(16 * i) * ld;
-#pragma unroll
-      for (int j = 0; j < P::NB; ++j)
-        if (inside || mw + 16 * i < a.M) store4<T>(line, nw + 16 * j, inside ? INT32_MAX : a.N, acc[i][j]);
-      __builtin_amdgcn_sched_barrier(0);
+    for (int b = 0; b < NV; ++b) {
+      v[b] = acc[b / P::NB][b % P::NB];
+      live[b] = (mw + 16 * (b / P::NB) < a.M) & (nw + 16 * (b % P::NB) < a.N);
     }
-  };
-  if (gridDim.y > 1) store(a.partial + (int64_t)split * a.M * a.N, a.N);
-  else store(static_cast<Out<F8>*>(a.out), a.ldo);
+    if (!splitk_combine<P::NT, NV>(v, live, split, gridDim.y, blockIdx.x, gridDim.x, a.partial, a.counters, &last)) return;
+#pragma unroll
+    for (int b = 0; b < NV; ++b) acc[b / P::NB][b % P::NB] = v[b];
+  }
+  const bool inside = m0 + P::BM <= a.M && n0 + P::BN <= a.N;
+  Out<F8>* const first = static_cast<Out<F8>*>(a.out) + (int64_t)mw * a.ldo;
+#pragma unroll
+  for (int i = 0; i < P::MT; ++i) {
+    Out<F8>* const line = first + (int64_t)(16 * i) * a.ldo;
+#pragma unroll
+    for (int j = 0; j < P::NB; ++j)
+      if (inside || mw + 16 * i < a.M) store4<Out<F8>>(line, nw + 16 * j, inside ? INT32_MAX : a.N, acc[i][j]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
 // The same product for large outputs: 256 rows, and the eight waves in two groups
@@ -396,7 +405,7 @@ __global__ __launch_bounds__(512, 1) void fp8_pair_kernel(Fp8Args a) {
   int tm, tn;
   tile_of(blockIdx.x, a.xcds, tiles_m, tiles_n, a.group_m, tm, tn);
   const int m0 = tm * P::BM, n0 = tn * P::BN;
-  const int split = blockIdx.y, g0 = split * a.split_steps, nk = min(a.G, g0 + a.split_steps) - g0;
+  const int nk = a.G;
 
   const int c0 = (lane & 7) ^ (lane >> 4);
   const uint32_t row8 = lane >> 3;
@@ -412,19 +421,19 @@ __global__ __launch_bounds__(512, 1) void fp8_pair_kernel(Fp8Args a) {
     off_s[i] = 4u * (uint32_t)(((r0 + e) >> shift) - (r0 >> shift)) * (uint32_t)(is_x ? a.sx_row : a.sw_row) |
                oob_unless(r0 + e < (is_x ? a.M : a.N) && (is_x || e < P::BN));
   }
-  const unsigned char* const xb = a.x + (int64_t)m0 * a.ldx + (int64_t)g0 * kGroup;
-  const unsigned char* const wb = a.w + (int64_t)n0 * a.ldw + (int64_t)g0 * kGroup;
-  const float* const sxb = a.sx + (int64_t)(m0 >> a.xshift) * a.sx_row + (int64_t)g0 * a.sx_group;
-  const float* const swb = a.sw + (int64_t)(n0 >> a.wshift) * a.sw_row + (int64_t)g0 * a.sw_group;
+  const unsigned char* const xb = a.x + (int64_t)m0 * a.ldx;
+  const unsigned char* const wb = a.w + (int64_t)n0 * a.ldw;
+  const float* const sxb = a.sx + (int64_t)(m0 >> a.xshift) * a.sx_row;
+  const float* const swb = a.sw + (int64_t)(n0 >> a.wshift) * a.sw_row;
   // Bytes of the tile's rows: what lies past the last row is past the end.
   const uint32_t x_bytes = a.M - m0 >= P::BM ? 0x7FFFFFFFu : (uint32_t)(a.M - m0) * (uint32_t)a.ldx;
   const uint32_t w_bytes = a.N - n0 >= P::BN ? 0x7FFFFFFFu : (uint32_t)(a.N - n0) * (uint32_t)a.ldw;
   auto past_of = [&](int kt, uint32_t (&past)[2]) __attribute__((always_inline)) {
-    const int left = a.K - (g0 + kt) * kGroup;
+    const int left = a.K - kt * kGroup;
     past[0] = oob_unless(16 * c0 < left), past[1] = oob_unless(16 * (c0 ^ 4) < left);
   };
   auto rsrc_of = [&](const unsigned char* base, uint32_t n, int kt) __attribute__((always_inline)) {
-    const uint32_t r = n == 0x7FFFFFFFu ? n : n - (uint32_t)((g0 + kt) * kGroup);
+    const uint32_t r = n == 0x7FFFFFFFu ? n : n - (uint32_t)(kt * kGroup);
     return make_rsrc_uniform(base + kt * kGroup, kt < nk ? r : 0u);
   };
   // A group's own half of x's rows.
@@ -493,7 +502,7 @@ __global__ __launch_bounds__(512, 1) void fp8_pair_kernel(Fp8Args a) {
   };
   auto step = [&](auto first_t, auto last_t, int kt, const Stage& st, const Stage& next) __attribute__((always_inline)) {
     constexpr bool LAST = decltype(last_t)::value;
-    const int left = a.K - (g0 + kt) * kGroup - 16 * quad;  // LAST: codes of the lane's first 16
+    const int left = a.K - kt * kGroup - 16 * quad;  // LAST: codes of the lane's first 16
     auto cut = [&](i32x4 v, int n) {
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
@@ -575,21 +584,16 @@ __global__ __launch_bounds__(512, 1) void fp8_pair_kernel(Fp8Args a) {
   }
 
   const bool inside = m0 + P::BM <= a.M && n0 + P::BN <= a.N;
-  auto store = [&](auto* out, int64_t ld) __attribute__((always_inline)) {
-    using T = std::remove_pointer_t<decltype(out)>;
-    const int mw = m0 + wm * (P::BM / P::WM) + row, nw = n0 + wn * (P::BN / P::WN) + 4 * quad;
-    T* const first = out + (int64_t)mw * ld;
+  const int mw = m0 + wm * (P::BM / P::WM) + row, nw = n0 + wn * (P::BN / P::WN) + 4 * quad;
+  Out<F8>* const first = static_cast<Out<F8>*>(a.out) + (int64_t)mw * a.ldo;
 #pragma unroll
-    for (int i = 0; i < P::MT; ++i) {
-      T* const line = first + (int64_t)(16 * i) * ld;
+  for (int i = 0; i < P::MT; ++i) {
+    Out<F8>* const line = first + (int64_t)(16 * i) * a.ldo;
 #pragma unroll
-      for (int j = 0; j < P::NB; ++j)
-        if (inside || mw + 16 * i < a.M) store4<T>(line, nw + 16 * j, inside ? INT32_MAX : a.N, acc[i][j]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
-  if (gridDim.y > 1) store(a.partial + (int64_t)split * a.M * a.N, a.N);
-  else store(static_cast<Out<F8>*>(a.out), a.ldo);
+    for (int j = 0; j < P::NB; ++j)
+      if (inside || mw + 16 * i < a.M) store4<Out<F8>>(line, nw + 16 * j, inside ? INT32_MAX : a.N, acc[i][j]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
 // Few rows of x, up to 8 XR: bound by reading w, once.  Tiles of 16 rows of w,
@@ -740,8 +744,8 @@ hipError_t launch_tile(const Fp8Args& a, int splits, hipStream_t stream) {
 }
 
 template <class P, bool F8, int FX, int FW>
-hipError_t launch_pair(const Fp8Args& a, int splits, hipStream_t stream) {
-  const dim3 grid((unsigned)(cdiv(a.M, P::BM) * cdiv(a.N, P::BN)), (unsigned)splits);
+hipError_t launch_pair(const Fp8Args& a, hipStream_t stream) {
+  const dim3 grid((unsigned)(cdiv(a.M, P::BM) * cdiv(a.N, P::BN)));
   const auto kernel = a.wshift == 0 ? fp8_pair_kernel<P, F8, FX, FW, true> : fp8_pair_kernel<P, F8, FX, FW, false>;
   return enqueue(kernel, grid, dim3(P::NT), stream, a);
 }
@@ -766,7 +770,7 @@ hipError_t launch_stream(const Fp8Args& a, hipStream_t stream) {
 template <bool F8, int FX, int FW>
 hipError_t launch_kind(const Fp8Args& a, int tile, int splits, hipStream_t stream) {
   if (tile < 0) return a.M <= 8 ? launch_stream<1, F8, FX, FW>(a, stream) : launch_stream<2, F8, FX, FW>(a, stream);
-  if (tile == 0) return launch_pair<TileGeom<256, F8 ? 256 : 128, F8 ? 2 : 4, F8 ? 4 : 2, 2>, F8, FX, FW>(a, splits, stream);
+  if (tile == 0) return launch_pair<TileGeom<256, F8 ? 256 : 128, F8 ? 2 : 4, F8 ? 4 : 2, 2>, F8, FX, FW>(a, stream);
   if (tile == 1) return launch_tile<TileGeom<128, 128, 2, 4, 4>, F8, FX, FW>(a, splits, stream);
   if (tile == 2) return launch_tile<TileGeom<64, 128, 2, 4, 4>, F8, FX, FW>(a, splits, stream);
   return launch_tile<TileGeom<64, 64, 2, 2, 4>, F8, FX, FW>(a, splits, stream);

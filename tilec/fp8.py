@@ -29,6 +29,7 @@ scratch is each call's own, and there is no autograd.
 import torch
 
 from . import _lib
+from .training import _counters
 
 __all__ = ["quantize_fp8", "dequantize_fp8", "linear_fp8"]
 
@@ -76,4 +77,4 @@ def linear_fp8(x, weight, dtype=torch.float32):
     have any strides (transposes, with a group's scales of all rows side by side, are
     read 2 % faster at 8192^3, and written 4 % slower).
     """
-    return _lib.host().linear_fp8(x, weight, dtype)
+    return _lib.host().linear_fp8(x, weight, dtype, _counters)

@@ -266,19 +266,20 @@ def linear_cross_entropy_grad(x, weight, target, reduction="mean", ignore_index=
                       chunk_rows)
 
 
-_NORM_COUNTERS = {}  # by device index and stream
+_OWN_COUNTERS = {}  # by device index and stream
 
 
-def _counter(index, stream):
-    """A zeroed counter that the norm's kernel leaves zero: the stream's, in no
-    graph, or in a capture one of the graph's own, zeroed in every replay (a graph may
-    be replayed beside its stream's other work).  `index`: the current device's."""
+def _counters(index, stream, nbytes):
+    """Zeroed counters that kernels leave zero: the stream's, in no graph, or in a
+    capture the graph's own, zeroed in every replay (a graph may be replayed beside
+    its stream's other work).  `index`: the current device's."""
     capturing = _stream_captured()
-    kept = None if capturing else _NORM_COUNTERS.get((index, stream))
-    if kept is None:
-        kept = torch.zeros(4, dtype=torch.uint8, device=torch.device("cuda", index))
+    kept = None if capturing else _OWN_COUNTERS.get((index, stream))
+    if kept is None or kept.numel() < nbytes:
+        kept = torch.zeros(nbytes if capturing else max(nbytes, 1 << 17), dtype=torch.uint8,
+                           device=torch.device("cuda", index))
         if not capturing:
-            _NORM_COUNTERS[index, stream] = kept
+            _OWN_COUNTERS[index, stream] = kept
     return kept
 
 
@@ -297,7 +298,7 @@ def grad_norm(grads, max_norm=None, grad_scale=None):
     and sums are float64, in a fixed order: nothing overflows, and the same bits
     come out on every call.  An infinite norm gives a scale of 0, a NaN one NaN.
     """
-    return _lib.host().grad_norm(grads, max_norm, grad_scale, _counter)
+    return _lib.host().grad_norm(grads, max_norm, grad_scale, _counters)
 
 
 def clip_grads(grads, max_norm, grad_scale=None):
@@ -305,7 +306,7 @@ def clip_grads(grads, max_norm, grad_scale=None):
     (not touched where that is 1).  Two of them may not share memory, and a view
     whose values do not lie side by side is refused (ValueError).  To autograd they
     have been modified in place."""
-    return _lib.host().clip_grads(grads, max_norm, grad_scale, _counter)
+    return _lib.host().clip_grads(grads, max_norm, grad_scale, _counters)
 
 
 ADAMW_BLOCK = 256  # values per scale of an 8-bit state
