@@ -42,9 +42,10 @@ struct Fp8Args {
 template <int FX, int FW>
 hipError_t launch_fp8(const Fp8Args& a, bool f8, int tile, int splits, hipStream_t stream);
 
-// A tile, how many splits of K its last workgroup adds up at a time, and what it takes, in us on an MI355X: a workgroup's start and end, and a
-// step of 128 k, of bfloat16 outputs ([1]) and float32 ones ([0]); step2: with two
-// workgroups on a CU, where that many fit.
+// A tile, how many splits of K its last workgroup adds up at a time, and what it
+// takes, in us on an MI355X: a workgroup's start and end, and a step of 128 k, of
+// bfloat16 outputs ([1]) and float32 ones ([0]); step2: with two workgroups on a CU,
+// where that many fit.
 struct Fp8Tile {
   int bm, bn[2];
   int batch;
