@@ -293,3 +293,19 @@ def test_backward_of_few_rows_keeps_a_nan_to_its_row_and_column():
     dx, dw = tilec.ext.rms_norm_backward(dy, h, rstd, w)
     assert torch.equal(dx[:299], good[0][:299]) and dx[299].isnan().all()
     assert torch.equal(dw[:499], good[1][:499]) and dw[499].isnan()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,D,ht", [(1024, 4096, "f32"), (1024, 8192, "bf16"), (1000, 4001, "bf16"), (500, 512, "f32")])
+def test_backward_of_the_largest_in_one_launch(R, D, ht):
+    # Rows of whole lines, as a matrix of its own and as columns of a wider one.
+    h, dh, w = make(R, D, ht, ht, ht, seed=R + D)
+    dy = torch.randn(R, D, generator=torch.Generator().manual_seed(R)).to(TYPES[ht]).cuda()
+    rstd = tilec.ext.rms_norm(h, w)[2]
+    dx, dw = tilec.ext.rms_norm_backward(dy, h, rstd, w, dh=dh)
+    check_backward(dy, h, rstd, w, dh, dx, dw)
+    wide = torch.empty((R, D + 3), dtype=dy.dtype, device="cuda")
+    wide[:, 2:D + 2] = dy
+    again = tilec.ext.rms_norm_backward(wide[:, 2:D + 2], h, rstd, w, dh=dh)
+    assert torch.equal(again[0], dx)
+    check_backward(dy, h, rstd, w, dh, *again)

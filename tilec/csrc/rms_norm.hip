@@ -299,13 +299,14 @@ __global__ __launch_bounds__(NT) void rms_grad_kernel(RmsArgs a) {
   }
 }
 
-// dw of 4 E columns by one workgroup: four threads across them, the others each a
+// dw of E ACROSS columns by one workgroup: ACROSS threads across them, the others each a
 // share of the rows, which meet by shuffles and then, waves in order, in LDS.
-template <typename TX, typename TY>
+template <typename TX, typename TY, int ACROSS>
 __device__ __forceinline__ void grad_columns(const RmsArgs& a, int block) {
-  constexpr int E = 16 / (int)sizeof(TX), ACROSS = 4, U = 4;
+  constexpr int E = 16 / (int)sizeof(TX), U = 4;
   __shared__ float sums[16][ACROSS * E];
-  const int tid = threadIdx.x, c = E * (ACROSS * block + tid % ACROSS), R = (int)a.R, rows = blockDim.x / ACROSS;
+  const int tid = threadIdx.x, first = E * ACROSS * block, at = tid % ACROSS, c = first + E * at;
+  const int R = (int)a.R, rows = blockDim.x / ACROSS;
   float dw[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) dw[e] = 0.f;
@@ -331,13 +332,13 @@ __device__ __forceinline__ void grad_columns(const RmsArgs& a, int block) {
   for (int e = 0; e < E; ++e) {
 #pragma unroll
     for (int o = ACROSS; o < 64; o <<= 1) dw[e] += __shfl_xor(dw[e], o);
-    if ((tid & 63) < ACROSS) sums[tid >> 6][E * (tid & 3) + e] = dw[e];
+    if ((tid & 63) == at) sums[tid >> 6][E * at + e] = dw[e];
   }
   __syncthreads();
-  if (tid < ACROSS * E && ACROSS * E * block + tid < a.D) {
+  if (tid < E * ACROSS && first + tid < a.D) {
     float t = sums[0][tid];
     for (int v = 1; v < (int)blockDim.x / 64; ++v) t += sums[v][tid];
-    a.dw[ACROSS * E * block + tid] = t;
+    a.dw[first + tid] = t;
   }
 }
 
@@ -345,10 +346,11 @@ __device__ __forceinline__ void grad_columns(const RmsArgs& a, int block) {
 // dw needs nothing that the rows compute, so no workgroup waits for another; h and dy
 // are read twice, the second time from the caches.
 template <typename TX, typename TY, typename TD, int NV>
-__global__ __launch_bounds__(1024) void rms_grad_small_kernel(RmsArgs a, int column_blocks) {
+__global__ __launch_bounds__(1024) void rms_grad_small_kernel(RmsArgs a, int column_blocks, bool lines) {
   constexpr int E = 16 / (int)sizeof(TX);
   if ((int)blockIdx.x < column_blocks) {
-    grad_columns<TX, TY>(a, blockIdx.x);
+    if (lines) grad_columns<TX, TY, 8>(a, blockIdx.x);
+    else grad_columns<TX, TY, 4>(a, blockIdx.x);
   } else {
     float none[NV][E];
     grad_rows<TX, TY, TD, false>(a, (int)blockIdx.x - column_blocks, (int)gridDim.x - column_blocks, none);
@@ -509,11 +511,14 @@ GradGeom grad_geom(int64_t R, int64_t D, int hsz, bool dw) {
     q.parts = std::min<int64_t>(R, std::max<int64_t>(1, cdiv(4 * (int64_t)device_cus(), cdiv(D, 256 * e))));
     q.c_bytes = (size_t)(R * sizeof(float) + 15) / 16 * 16;
   }
-  // Up to 1024 rows of 8 MiB in all: one launch instead of two, though h and dy are
-  // read twice (fp32, 64 x 4096 7.1 us and 4.5, 1000 x 1009 9.7 and 8.5, 1024 x 2048
-  // 12.3 and 10.7, but 2048 x 512 7.9 and 11.6, 1024 x 4096 16.1 and 20.3; bf16, 512 x
-  // 2048 8.4 and 6.3, 1024 x 4096 14.8 and 11.4, 2048 x 2048 16.0 and 14.4).
-  q.small = dw && q.g.nv > 0 && q.parts > 1 && R <= 1024 && R * D * hsz <= (int64_t(8) << 20);
+  // Up to 1024 rows of 16 MiB in all, 8 where rows are not whole lines: one launch
+  // instead of two, though h and dy are read twice (fp32, 64 x 4096 7.4 us and 4.7, 512
+  // x 4096 12.0 and 9.1, 1024 x 4096 16.2 and 14.7, 1000 x 1009 9.7 and 8.5, but 1000 x
+  // 4001 17.9 and 25.1, 2048 x 512 7.9 and 11.1, 1024 x 8192 24.4 and 26.1; bf16, 512 x
+  // 2048 8.3 and 4.8, 1024 x 8192 19.7 and 15.3, 1000 x 4001 16.6 and 12.8, 2048 x 1024
+  // 9.2 and 12.0).
+  const int64_t most = int64_t(D * hsz % 128 == 0 ? 16 : 8) << 20;
+  q.small = dw && q.g.nv > 0 && q.parts > 1 && R <= 1024 && R * D * hsz <= most;
   if (q.small) {
     q.g.nt = 1024 / q.g.tpr * q.g.tpr;
     q.parts = cdiv(R, q.g.nt / q.g.tpr);
@@ -535,10 +540,13 @@ hipError_t launch_rms_grad(RmsArgs a, const GradGeom& q, float* cs, hipStream_t 
   } else if (a.R > 0) {
     a.tpr = q.g.tpr;
     if (q.small) {
-      const int columns = (int)cdiv(a.D, 4 * E);
+      // Lines of 128 bytes where rows begin at them (512 x 4096 fp32 12.1 us and 9.2),
+      // elsewhere half as much and twice the workgroups (1000 x 1009 fp32 10.2 and 8.5).
+      const bool lines = a.ldx * sizeof(TX) % 128 == 0 && a.ldy * sizeof(TY) % 128 == 0;
+      const int columns = (int)cdiv(a.D, lines ? 8 * E : 4 * E);
       return by_nv<16 / E>(q.g, [&](auto nv) {
         return enqueue(rms_grad_small_kernel<TX, TY, TD, decltype(nv)::value>, dim3((unsigned)(columns + q.parts)),
-                       dim3(q.g.nt), stream, a, columns);
+                       dim3(q.g.nt), stream, a, columns, lines);
       });
     }
     e = by_geom<16 / E>(q.g, [&](auto nv, auto nt) {
