@@ -8,17 +8,21 @@ torch.float8_e5m2, and float32 scales of blocks of a row's 128 values,
 
     value[r, c] = codes[r, c] * scales[r or r // 128, c // 128]
 
-A layer in 8 bits, with `rms_norm` of training.py before it:
+A layer in 8 bits, y = n @ weight.T with n the norm of h = x + residual:
 
     x8, h, rstd = tilec.ext.rms_norm(x, w, residual, dtype=torch.float8_e4m3fn)
     w8 = tilec.ext.quantize_fp8(weight, block=(128, 128))         # once a step
-    y = tilec.ext.linear_fp8(x8, w8, dtype=torch.bfloat16)        # x @ weight.T
+    y = tilec.ext.linear_fp8(x8, w8, dtype=torch.bfloat16)
 
-and its gradients for dy, each product summed over the axis its operands' blocks
-run along:
+and its gradients for dy, with dh that of h from its other reader.  Each product is
+summed over the axis its operands' blocks run along, and the weight's reads what the
+forward product read, which is n and not x:
 
-    dx = linear_fp8(quantize_fp8(dy), quantize_fp8(weight.t(), block=(128, 128)))
-    dweight = linear_fp8(quantize_fp8(dy.t()), quantize_fp8(x.t()))
+    dn = tilec.ext.linear_fp8(tilec.ext.quantize_fp8(dy), tilec.ext.quantize_fp8(weight.t(), block=(128, 128)),
+                              dtype=torch.bfloat16)
+    dx, dw = tilec.ext.rms_norm_backward(dn, h, rstd, w, dh=dh)   # dx: of x and of residual
+    n = tilec.ext.dequantize_fp8(x8, torch.bfloat16)
+    dweight = tilec.ext.linear_fp8(tilec.ext.quantize_fp8(dy.t()), tilec.ext.quantize_fp8(n.t()))
 
 The rules are those of training.py's operators: arguments are checked before
 anything is enqueued (ValueError for shapes, TypeError for types and devices),
