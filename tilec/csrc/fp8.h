@@ -40,4 +40,9 @@ __device__ __forceinline__ uint32_t to_fp8(float a, float b, float c, float d, b
   return (uint32_t)v;
 }
 
+// The bits of a word of four codes that are those of the `left` (any number) of a row.
+__device__ __forceinline__ uint32_t code_bits(int left) {
+  return left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+}
+
 }  // namespace tilec

@@ -54,12 +54,15 @@ struct Eight {
     for (int e = 0; e < 8; ++e) t = max(t, __float_as_uint(get(e)) & 0x7fffffffu);
     return t;
   }
-  // The codes at columns c + .. of a row, up to column `end` (a multiple of 16).
-  __device__ __forceinline__ void store(unsigned char* row, int c, int sub, int end, float inverse, bool e5m2) const {
+  // The codes at columns c + .. of a row, up to column `end` (a multiple of 16); `bits`
+  // of them, zeros elsewhere (past a row, where zero times the inverse may be a NaN).
+  __device__ __forceinline__ void store(unsigned char* row, int c, int sub, int end, float inverse, bool e5m2,
+                                        const uint32_t (&bits)[2]) const {
     uint32_t q[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      q[i] = to_fp8(get(4 * i) * inverse, get(4 * i + 1) * inverse, get(4 * i + 2) * inverse, get(4 * i + 3) * inverse, e5m2);
+      q[i] = bits[i] &
+             to_fp8(get(4 * i) * inverse, get(4 * i + 1) * inverse, get(4 * i + 2) * inverse, get(4 * i + 3) * inverse, e5m2);
     if constexpr (PIECES == 1) {
       if (c + at(sub, 0) < end) *reinterpret_cast<u32x2*>(row + c + at(sub, 0)) = u32x2{q[0], q[1]};
     } else {
@@ -84,6 +87,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a) {
   const int c = (int)(g * kGroup), C = (int)a.C;
   const bool e5m2 = a.e5m2;
   const int64_t step = (int64_t)gridDim.y * rpb;
+  const uint32_t bits[2] = {code_bits(C - c - Eight<T>::at(sub, 0)), code_bits(C - c - Eight<T>::at(sub, 4))};
   for (int64_t r0 = (int64_t)blockIdx.y * rpb + (slot >> a.lg); r0 < a.R; r0 += U * step) {
     Eight<T> v[U];
 #pragma unroll
@@ -101,7 +105,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a) {
       float scale, inverse;
       block_scale(top, fp8_largest(e5m2), scale, inverse);
       if (sub == 0) a.scales[r * a.s_row + g * a.s_group] = scale;
-      v[u].store(a.codes + r * a.ldq, c, sub, row_end(C), inverse, e5m2);
+      v[u].store(a.codes + r * a.ldq, c, sub, row_end(C), inverse, e5m2, bits);
     }
   }
 }
@@ -173,22 +177,24 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a, int tiles_
   }
   const int end = row_end(C);
   if constexpr (!TRANS) {
+    const uint32_t bits[2] = {code_bits(C - c0 - mine(0)), code_bits(C - c0 - mine(4))};
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
       const int64_t r = r0 + 16 * p + hi;
-      if (r < a.R) v[p].store(a.codes + r * a.ldq, c0, lo, end, inverse[0], e5m2);
+      if (r < a.R) v[p].store(a.codes + r * a.ldq, c0, lo, end, inverse[0], e5m2, bits);
     }
   } else {
     // Row mine(e) of the tile, columns 8 hi ..: 8-byte piece hi of its 16, exchanged
     // by rows (by lo).
     constexpr int ROWS = Eight<T>::V;  // side by side in one thread
+    const uint32_t bits[2] = {code_bits(C - c0 - 8 * hi), code_bits(C - c0 - 8 * hi - 4)};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       u32x2 q;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        q[i] = to_fp8(v[4 * i].get(e) * inverse[e], v[4 * i + 1].get(e) * inverse[e], v[4 * i + 2].get(e) * inverse[e],
-                      v[4 * i + 3].get(e) * inverse[e], e5m2);
+        q[i] = bits[i] & to_fp8(v[4 * i].get(e) * inverse[e], v[4 * i + 1].get(e) * inverse[e],
+                                v[4 * i + 2].get(e) * inverse[e], v[4 * i + 3].get(e) * inverse[e], e5m2);
       *reinterpret_cast<u32x2*>(out + 128 * mine(e) + 8 * (hi ^ lo)) = q;
     }
     __syncthreads();
