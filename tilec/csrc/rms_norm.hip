@@ -649,8 +649,8 @@ int tilec_rms_norm_backward(const void* dy, const void* h, const float* rstd, co
   if (rc == TILEC_OK && dh != nullptr) rc = check_rows("dh", dh, lddh, R, D);
   if (rc == TILEC_OK) rc = check_rows("dx", dx, lddx, R, D);
   if (rc != TILEC_OK) return rc;
-  if (R > 0 && dx == dy)  // (dy is read again after rows of dx are written)
-    return fail(TILEC_ERR_VALUE, "tilec: RMS norm: dx is dy");
+  if (R > 0 && (dx == dy || dx == h))  // (both are read again after rows of dx are written)
+    return fail(TILEC_ERR_VALUE, "tilec: RMS norm: dx is %s", dx == dy ? "dy" : "h");
   if (R > 0 && rstd == nullptr) return fail(TILEC_ERR_VALUE, "tilec: RMS norm: rstd is NULL");
   const GradGeom q = grad_geom(R, D, h_dtype == TILEC_F32 ? 4 : 2, dweight != nullptr);
   const size_t need = q.c_bytes + q.partial_bytes;
