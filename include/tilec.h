@@ -423,7 +423,7 @@ int tilec_dequantize_fp8(const void* codes, const float* scales, void* out, int6
  * residual's type.  y is float32, bfloat16, or 8-bit codes with y_scale
  * [R, ceil(D / 128)] for blocks of 1 x 128, as tilec_quantize_fp8 writes them of
  * the float32 y.  rstd [R] float32 is written where not NULL.  h may be the
- * residual; otherwise outputs must not overlap inputs.
+ * residual, rows and all (ldh == ldr); otherwise outputs must not overlap inputs.
  */
 int tilec_rms_norm(const void* x, const void* residual, const void* weight, void* y, float* y_scale, void* h,
                    float* rstd, int64_t R, int64_t D, int64_t ldx, int64_t ldr, int64_t ldy, int64_t ldh,
@@ -437,7 +437,7 @@ int tilec_rms_norm(const void* x, const void* residual, const void* weight, void
  * from its other reader.  dx has dh's type, or dy's without it; dweight [D],
  * float32, may be NULL and is added in a fixed order.  `workspace`:
  * tilec_rms_norm_backward_workspace_bytes, any contents, 16-byte aligned.  dx may
- * be dh where it has that type, and overlaps nothing else.
+ * be dh, rows and all (lddx == lddh), and overlaps nothing else.
  */
 int tilec_rms_norm_backward(const void* dy, const void* h, const float* rstd, const void* weight, const void* dh,
                             void* dx, float* dweight, int64_t R, int64_t D, int64_t lddy, int64_t ldh, int64_t lddh,

@@ -24,3 +24,16 @@ def test_dx_in_the_place_of_dy_or_h(R, D, t, dw):
     assert backward(dx=2 << 20, **ld) == _lib.ERR_VALUE and "dx is h" in _lib.last_error()
     assert backward(dx=2 << 20, dh=6 << 20, **ld) == _lib.ERR_VALUE and "dx is h" in _lib.last_error()
     assert dw is not None or backward(dx=2 << 20, R=0, dw=None) == _lib.OK  # no rows: nothing is written
+
+
+def test_in_the_place_of_an_input_but_with_other_rows():
+    both = dict(dx=6 << 20, dh=6 << 20)
+    assert backward(lddx=64, lddh=65, **both) == _lib.ERR_VALUE and "dx is dh" in _lib.last_error()
+    assert backward(lddx=80, lddh=64, **both) == _lib.ERR_VALUE and "dx is dh" in _lib.last_error()
+
+    def forward(ldr, ldh):
+        return _lib.lib().tilec_rms_norm(1 << 20, 2 << 20, None, 3 << 20, None, 2 << 20, None, 4, 64, 64, ldr, 64, ldh, 0, 0, F32,
+                                         F32, F32, F32, 1e-5, None)
+
+    for ldr, ldh in ((64, 65), (80, 64)):
+        assert forward(ldr, ldh) == _lib.ERR_VALUE and "h is the residual" in _lib.last_error()

@@ -606,6 +606,9 @@ int tilec_rms_norm(const void* x, const void* residual, const void* weight, void
   if (rc == TILEC_OK && residual != nullptr) rc = check_rows("h", h, ldh, R, D);
   if (rc == TILEC_OK) rc = check_rows("y", y, ldy, R, D);
   if (rc != TILEC_OK || R == 0) return rc;
+  if (R > 1 && residual != nullptr && h == residual && ldh != ldr)
+    return fail(TILEC_ERR_VALUE, "tilec: RMS norm: h is the residual, with rows %lld apart instead of %lld", (long long)ldh,
+                (long long)ldr);
   const int64_t room = cdiv(D, 16) * 16;
   if (is_fp8(y_dtype) && (y_scale == nullptr || reinterpret_cast<uintptr_t>(y) % 16 != 0 ||
                           (R > 1 && (ldy % 16 != 0 || ldy < room))))
@@ -651,6 +654,9 @@ int tilec_rms_norm_backward(const void* dy, const void* h, const float* rstd, co
   if (rc != TILEC_OK) return rc;
   if (R > 0 && (dx == dy || dx == h))  // (both are read again after rows of dx are written)
     return fail(TILEC_ERR_VALUE, "tilec: RMS norm: dx is %s", dx == dy ? "dy" : "h");
+  if (R > 1 && dx == dh && lddx != lddh)  // (a row of dx would be another's dh)
+    return fail(TILEC_ERR_VALUE, "tilec: RMS norm: dx is dh, with rows %lld apart instead of %lld", (long long)lddx,
+                (long long)lddh);
   if (R > 0 && rstd == nullptr) return fail(TILEC_ERR_VALUE, "tilec: RMS norm: rstd is NULL");
   const GradGeom q = grad_geom(R, D, h_dtype == TILEC_F32 ? 4 : 2, dweight != nullptr);
   const size_t need = q.c_bytes + q.partial_bytes;
