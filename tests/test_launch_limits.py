@@ -1,0 +1,90 @@
+"""Grids of the calls with the most rows, columns or nothing at all, on the host: the
+library is loaded beside a small one whose hipLaunchKernel writes the launches down
+instead of enqueueing them, so no memory of these sizes and no GPU is needed.  A grid
+has fewer than 2^32 threads along an axis, and at most 2^16 workgroups along y and z."""
+
+import json
+import os
+import subprocess
+import sys
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+RECORDER = r"""
+#include <cstddef>
+struct Dim3 { unsigned x, y, z; };
+static unsigned kept[6 * 1024];
+static int count;
+extern "C" {
+int hipLaunchKernel(const void*, Dim3 grid, Dim3 block, void**, size_t, void*) {
+  const unsigned all[6] = {grid.x, grid.y, grid.z, block.x, block.y, block.z};
+  for (int i = 0; count < 1024 && i < 6; ++i) kept[6 * count + i] = all[i];
+  ++count;
+  return 0;
+}
+int hipGetLastError() { return 0; }
+int recorded(unsigned* out) {
+  const int n = count;
+  for (int i = 0; i < 6 * n && i < 6 * 1024; ++i) out[i] = kept[i];
+  count = 0;
+  return n;
+}
+}
+"""
+
+# (The package itself would load torch, and with it the runtime's library first.)
+PROGRAM = """
+import ctypes, importlib.util, json, sys
+recorder = ctypes.CDLL(sys.argv[1], mode=ctypes.RTLD_GLOBAL)
+spec = importlib.util.spec_from_file_location("binding", sys.argv[2])
+binding = importlib.util.module_from_spec(spec)
+spec.loader.exec_module(binding)
+L = binding.lib()
+out = (ctypes.c_uint32 * (6 * 1024))()
+answers = []
+for name, args in json.load(sys.stdin):
+    rc = getattr(L, name)(*args)
+    n = recorder.recorded(out)
+    answers.append([rc, [list(out[6 * i:6 * i + 6]) for i in range(n)]])
+print("ANSWERS" + json.dumps(answers))
+"""
+
+F32, BF16, E4 = 0, 1, 2
+AT, ROOM = 1 << 20, 1 << 60  # an address, and room for anything: nothing reads or writes there
+MOST = (1 << 31) - 1024
+TINY = 1e-5
+
+
+def linear(M, N, K, od, x=AT, w=AT, ldx=None, ldw=None):
+    return ("tilec_linear_fp8", [x, AT, w, AT, AT, M, N, K, K if ldx is None else ldx, K if ldw is None else ldw, N, 1, 1, 1, 1,
+                                 E4, E4, od, 1, 1, AT, ROOM, AT, ROOM, None])
+
+
+CASES = {}
+for _od in (F32, BF16):
+    for _M, _N in ((100, 100), (1 << 30, 4), ((1 << 30) + 5, 64), (1, MOST), (16, 1 << 30), (MOST, 1)):
+        CASES[f"no features {_M} x {_N} {_od}"] = linear(_M, _N, 0, _od)
+
+
+@pytest.fixture(scope="module")
+def answers(tmp_path_factory):
+    where = tmp_path_factory.mktemp("recorder")
+    src, lib = where / "recorder.cpp", where / "recorder.so"
+    src.write_text(RECORDER)
+    subprocess.run(["g++", "-O1", "-shared", "-fPIC", str(src), "-o", str(lib)], check=True, timeout=120)
+    r = subprocess.run([sys.executable, "-c", PROGRAM, str(lib), os.path.join(ROOT, "tilec", "_lib.py")], cwd=ROOT,
+                       input=json.dumps(list(CASES.values())), capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+    text = r.stdout[r.stdout.index("ANSWERS") + len("ANSWERS"):]
+    return dict(zip(CASES, json.loads(text)))
+
+
+@pytest.mark.parametrize("name", CASES)
+def test_grids(name, answers):
+    rc, launches = answers[name]
+    assert rc == 0 and launches
+    for gx, gy, gz, bx, by, bz in launches:
+        assert 0 < bx * by * bz <= 1024
+        assert 0 < gx * bx < 1 << 32 and 0 < gy <= 1 << 16 and 0 < gz <= 1 << 16, (gx, gy, gz, bx)

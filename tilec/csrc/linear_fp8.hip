@@ -4,6 +4,7 @@
 
 #include "abi.h"
 #include "linear_fp8.h"
+#include "zeros.h"
 
 namespace tilec {
 
@@ -132,9 +133,15 @@ int tilec_linear_fp8(const void* x, const float* x_scale, const void* weight, co
   if (out == nullptr || (K > 0 && (x == nullptr || weight == nullptr || x_scale == nullptr || w_scale == nullptr)))
     return fail(TILEC_ERR_VALUE, "tilec: linear_fp8: a pointer is NULL");
   const bool f8 = out_dtype == TILEC_BF16;
-  Plan none{};
-  none.tile = kFp8TileCount - 1, none.splits = 1;
-  const Plan p = K > 0 ? plan_of(x, weight, M, N, K, ldx, ldw, f8) : none;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (K == 0) {
+    const int64_t row = M > 1 ? ldo : N;
+    const hipError_t e = f8 ? enqueue_zeros(static_cast<uint16_t*>(out), M, N, row, st)
+                            : enqueue_zeros(static_cast<float*>(out), M, N, row, st);
+    if (e != hipSuccess) return fail(TILEC_ERR_HIP, "tilec: launching linear_fp8 failed: %s", hipGetErrorString(e));
+    return TILEC_OK;
+  }
+  const Plan p = plan_of(x, weight, M, N, K, ldx, ldw, f8);
   if (p.tile == kFp8TileCount)
     return fail(TILEC_ERR_VALUE, "tilec: linear_fp8: %lld x %lld outputs are too many for one launch", (long long)M,
                 (long long)N);
@@ -144,7 +151,6 @@ int tilec_linear_fp8(const void* x, const float* x_scale, const void* weight, co
   if (p.counter_bytes > 0 && (counters == nullptr || counter_bytes < p.counter_bytes))
     return fail(TILEC_ERR_WORKSPACE, "tilec: linear_fp8 needs %zu counter bytes (got %zu)", p.counter_bytes,
                 counters == nullptr ? (size_t)0 : counter_bytes);
-  const hipStream_t st = static_cast<hipStream_t>(stream);
   char* const ws = static_cast<char*>(workspace);
   hipError_t e = hipSuccess;
   if (p.copy_x || p.copy_w) {
