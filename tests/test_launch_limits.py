@@ -25,6 +25,16 @@ int hipLaunchKernel(const void*, Dim3 grid, Dim3 block, void**, size_t, void*) {
   return 0;
 }
 int hipGetLastError() { return 0; }
+// What kernel<<<...>>> keeps between its configuration and hipLaunchKernel.
+static Dim3 grid_of, block_of;
+int __hipPushCallConfiguration(Dim3 grid, Dim3 block, size_t, void*) {
+  grid_of = grid, block_of = block;
+  return 0;
+}
+int __hipPopCallConfiguration(Dim3* grid, Dim3* block, size_t* shared, void** stream) {
+  *grid = grid_of, *block = block_of, *shared = 0, *stream = nullptr;
+  return 0;
+}
 int recorded(unsigned* out) {
   const int n = count;
   for (int i = 0; i < 6 * n && i < 6 * 1024; ++i) out[i] = kept[i];
@@ -66,6 +76,13 @@ CASES = {}
 for _od in (F32, BF16):
     for _M, _N in ((100, 100), (1 << 30, 4), ((1 << 30) + 5, 64), (1, MOST), (16, 1 << 30), (MOST, 1)):
         CASES[f"no features {_M} x {_N} {_od}"] = linear(_M, _N, 0, _od)
+for _od in (F32, BF16):
+    # Operands that are copied first: a stride, or an address, off 16 bytes.
+    CASES[f"copied x {_od}"] = linear((1 << 30) + 1000, 1, 33, _od)
+    CASES[f"copied x, short rows {_od}"] = linear(MOST, 1, 16, _od, x=AT + 1)
+    CASES[f"copied weight {_od}"] = linear(4, (1 << 30) + 1000, 64, _od, w=AT + 8)
+    CASES[f"copied weight, {(1 << 22) - 3} features {_od}"] = linear(16, 60000, (1 << 22) - 3, _od)
+    CASES[f"both copied {_od}"] = linear(1 << 30, 1 << 5, 40, _od)
 
 
 @pytest.fixture(scope="module")

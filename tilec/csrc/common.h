@@ -487,7 +487,8 @@ inline hipError_t pad_copy(const void* in0, void* out0, int64_t R0, int64_t C0, 
     const int64_t rpb = 256 >> o.lg;
     const int64_t gx = (nch + (1 << o.lg) - 1) >> o.lg;
     int64_t gy = Rp > 0 && gx > 0 ? (Rp + rpb - 1) / rpb : 0;
-    while (gy > 1 && gx * gy > (int64_t(1) << 29)) gy = (gy + 1) / 2;  // the row loop strides over the rest
+    // (A grid of both has less than 2^32 threads; the row loop strides over the rest.)
+    while (gy > 1 && gx * gy >= (int64_t(1) << 23)) gy = (gy + 1) / 2;
     o.gx = (int)gx;
     o.gy = (int)gy;
     return o;
@@ -495,7 +496,7 @@ inline hipError_t pad_copy(const void* in0, void* out0, int64_t R0, int64_t C0, 
   const PadCopyOp o0 = op(in0, out0, R0, C0, ld0, Rp0, Cp0), o1 = op(in1, out1, R1, C1, ld1, Rp1, Cp1);
   const int64_t blocks = (int64_t)o0.gx * o0.gy + (int64_t)o1.gx * o1.gy;
   if (blocks == 0) return hipSuccess;
-  if ((int64_t)o0.gx * o0.gy >= (int64_t(1) << 30) || blocks >= (int64_t(1) << 31)) return hipErrorInvalidValue;
+  if (blocks >= (int64_t(1) << 24)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(pad_copy_kernel<ESZ>, dim3((unsigned)blocks), dim3(256), 0, stream, o0, o1);
   return hipGetLastError();
 }
