@@ -85,6 +85,15 @@ for _od in (F32, BF16):
     CASES[f"both copied {_od}"] = linear(1 << 30, 1 << 5, 40, _od)
 
 
+def rms_backward(R, D, hd, dw=AT):
+    return ("tilec_rms_norm_backward", [AT, 2 * AT, AT, None, None, 3 * AT, dw, R, D, D, D, D, D, hd, hd, hd, F32, AT, ROOM, None])
+
+
+for _hd in (F32, BF16):
+    for _R, _D in ((0, 1), (0, 1 << 26), (0, MOST), (1, MOST), (3, 1 << 29), (MOST, 1), (1 << 24, 64), (1 << 20, 4096), (1 << 15, 1 << 17)):
+        CASES[f"RMS norm backward {_R} x {_D} {_hd}"] = rms_backward(_R, _D, _hd)
+
+
 @pytest.fixture(scope="module")
 def answers(tmp_path_factory):
     where = tmp_path_factory.mktemp("recorder")

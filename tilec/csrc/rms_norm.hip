@@ -25,6 +25,7 @@
 #include "enqueue.h"
 #include "fp8.h"
 #include "rows.h"
+#include "zeros.h"
 #include "../../include/tilec.h"
 
 namespace tilec {
@@ -415,7 +416,7 @@ __global__ __launch_bounds__(256) void rms_grad_cols_kernel(RmsArgs a, const flo
 }
 
 // dw[c]: the sum of `parts` partial rows, 16 columns a workgroup, 64 threads a
-// column (every 64th row each, then those in order).  No parts: zeros.
+// column (every 64th row each, then those in order).
 __global__ __launch_bounds__(1024) void rms_grad_sum_kernel(RmsArgs a, int parts) {
   __shared__ float red[64][17];
   const int col = threadIdx.x & 15, g = threadIdx.x >> 4;
@@ -530,14 +531,15 @@ GradGeom grad_geom(int64_t R, int64_t D, int hsz, bool dw) {
 template <typename TX, typename TY, typename TD>
 hipError_t launch_rms_grad(RmsArgs a, const GradGeom& q, float* cs, hipStream_t stream) {
   constexpr int E = 16 / (int)sizeof(TX);
-  hipError_t e = hipSuccess;
-  if (a.R > 0 && q.g.nv == 0) {
+  if (a.R == 0) return a.dw ? enqueue_zeros(a.dw, 1, a.D, a.D, stream) : hipSuccess;
+  hipError_t e;
+  if (q.g.nv == 0) {
     const unsigned grid = (unsigned)std::min<int64_t>(a.R, kMaxGrid);
     e = enqueue(rms_grad_rows_kernel<TX, TY>, dim3(grid), dim3(1024), stream, a, cs);
     if (e != hipSuccess) return e;
     e = enqueue(rms_grad_cols_kernel<TX, TY, TD>, dim3((unsigned)cdiv(a.D, 256 * E), (unsigned)q.parts), dim3(256), stream,
                 a, cs);
-  } else if (a.R > 0) {
+  } else {
     a.tpr = q.g.tpr;
     if (q.small) {
       // Lines of 128 bytes where rows begin at them (512 x 4096 fp32 12.1 us and 9.2),
