@@ -94,6 +94,17 @@ for _hd in (F32, BF16):
         CASES[f"RMS norm backward {_R} x {_D} {_hd}"] = rms_backward(_R, _D, _hd)
 
 
+def layer_norm_backward(R, D, xd, dw=AT, db=2 * AT):
+    return ("tilec_layer_norm_backward", [AT, AT, AT, AT, None, AT, dw, db, R, D, D, D, D, xd, xd, F32, AT, ROOM, None])
+
+
+for _xd in (F32, BF16):
+    for _R, _D in ((0, 1), (0, 1 << 25), (0, MOST), (1, MOST), (3, 1 << 29), (MOST, 1), (1 << 24, 64), (1 << 20, 4096), (1 << 15, 1 << 17)):
+        CASES[f"layer norm backward {_R} x {_D} {_xd}"] = layer_norm_backward(_R, _D, _xd)
+    CASES[f"layer norm backward, no weight {_xd}"] = layer_norm_backward(0, 1 << 26, _xd, dw=None)
+    CASES[f"layer norm backward, no bias {_xd}"] = layer_norm_backward(0, 1 << 26, _xd, db=None)
+
+
 @pytest.fixture(scope="module")
 def answers(tmp_path_factory):
     where = tmp_path_factory.mktemp("recorder")

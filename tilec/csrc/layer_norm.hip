@@ -25,6 +25,7 @@
 #include "abi.h"
 #include "common.h"
 #include "rows.h"
+#include "zeros.h"
 #include "../../include/tilec.h"
 
 namespace tilec {
@@ -346,7 +347,7 @@ __global__ __launch_bounds__(256) void norm_grad_cols_kernel(NormArgs a, const f
 }
 
 // dw[c] and db[c]: the sums of `parts` partial rows, 16 columns a workgroup,
-// 64 threads a column (every 64th row each, then those in order).  No parts: zeros.
+// 64 threads a column (every 64th row each, then those in order).
 __global__ __launch_bounds__(1024) void norm_grad_sum_kernel(NormArgs a, int parts) {
   __shared__ float red[64][17];
   const int col = threadIdx.x & 15, g = threadIdx.x >> 4;
@@ -448,8 +449,12 @@ GradGeom grad_geom(int64_t R, int64_t D, int xsz) {
 template <typename TX, typename TY>
 hipError_t launch_norm_grad(NormArgs a, const GradGeom& q, float* c12, hipStream_t stream) {
   constexpr int E = 16 / (int)sizeof(TX);
-  hipError_t e = hipSuccess;
-  if (a.R > 0 && q.g.nv == 0) {
+  hipError_t e;
+  if (a.R == 0) {
+    e = a.dw ? enqueue_zeros(a.dw, 1, a.D, a.D, stream) : hipSuccess;
+    return e == hipSuccess && a.db ? enqueue_zeros(a.db, 1, a.D, a.D, stream) : e;
+  }
+  if (q.g.nv == 0) {
     const unsigned grid = (unsigned)std::min<int64_t>(a.R, kMaxGrid);
     hipLaunchKernelGGL((norm_grad_rows_kernel<TX, TY>), dim3(grid), dim3(1024), 0, stream, a, c12);
     e = hipGetLastError();
@@ -457,7 +462,7 @@ hipError_t launch_norm_grad(NormArgs a, const GradGeom& q, float* c12, hipStream
     hipLaunchKernelGGL((norm_grad_cols_kernel<TX, TY>),
                        dim3((unsigned)cdiv(a.D, 256 * E), (unsigned)q.parts), dim3(256), 0, stream, a, c12);
     e = hipGetLastError();
-  } else if (a.R > 0) {
+  } else {
     a.tpr = q.g.tpr;
     const dim3 grid((unsigned)q.parts), block(q.g.nt);
     auto go = [&](auto nv, auto nt) {
