@@ -104,6 +104,26 @@ for _xd in (F32, BF16):
     CASES[f"layer norm backward, no weight {_xd}"] = layer_norm_backward(0, 1 << 26, _xd, dw=None)
     CASES[f"layer norm backward, no bias {_xd}"] = layer_norm_backward(0, 1 << 26, _xd, db=None)
 
+# The other entry points at their longest and widest.
+LARGE = [(1, MOST), (MOST, 1), (128, 1 << 30), (1 << 30, 128), (1 << 24, 8192), (1 << 15, 1 << 22), ((1 << 26) + 1, 2049)]
+for _t in (F32, BF16):
+    for _R, _D in LARGE:
+        CASES[f"RMS norm {_R} x {_D} {_t}"] = ("tilec_rms_norm", [AT, None, None, AT, None, None, AT, _R, _D, _D, 0, _D, 0, 0, 0, _t,
+                                               F32, _t, F32, TINY, None])
+        CASES[f"RMS norm to 8 bits {_R} x {_D} {_t}"] = ("tilec_rms_norm", [
+            AT, AT, None, AT, AT, AT, AT, _R, _D, _D, _D, -(-_D // 16) * 16, _D, 1, 1, _t, F32, E4, F32, TINY, None])
+        CASES[f"layer norm {_R} x {_D} {_t}"] = ("tilec_layer_norm", [AT, None, None, AT, AT, AT, _R, _D, _D, _D, _t, _t, F32, TINY,
+                                                 None])
+        for _block in (1, 128):
+            for _trans in (0, 1):
+                CASES[f"quantise {_R} x {_D} {_t} {_block} {_trans}"] = ("tilec_quantize_fp8", [
+                    AT, AT, AT, _R, _D, _R if _trans else _D, -(-_D // 16) * 16, 1, 1, _trans, _t, E4, _block, None])
+            CASES[f"values {_R} x {_D} {_t} {_block}"] = ("tilec_dequantize_fp8", [AT, AT, AT, _R, _D, _D, _D, 1, 1, E4, _t, _block,
+                                                          None])
+    for _M, _N, _K in ((1, MOST, 16), (16, 1 << 30, 130), (MOST, 1, 16), (1 << 30, 64, 128), (1 << 20, 1 << 17, 256),
+                       (1 << 17, 1 << 20, 256), (8192, 8192, 1 << 22)):
+        CASES[f"product {_M} x {_N} x {_K} {_t}"] = linear(_M, _N, _K, _t)
+
 
 @pytest.fixture(scope="module")
 def answers(tmp_path_factory):
