@@ -375,8 +375,10 @@ int tilec_adamw_values(const tilec_adamw_tensor* tensors, int32_t count, void* s
  * float32.  For a float32 out so are those within a group, of exact products;
  * for a bfloat16 out they are the 8-bit matrix instructions', which cut every
  * product at 2^-13 of the largest among eight consecutive k (1.5e-5 of the result
- * for normal values).  The product of two scales is rounded to float32.  The
- * same bits on every call on one device.  K <= 2^22; K == 0 writes zeros.
+ * for normal values).  The product of two scales is a float32 of its own, formed
+ * before it multiplies a group's sum: rounded, below 2^-126 to multiples of 2^-149
+ * (0 below 2^-150), and infinite from 2^128 on.  The same bits on every call on one
+ * device.  K <= 2^22; K == 0 writes zeros.
  *
  * Operands are read in place where their rows begin at multiples of 16 bytes,
  * and otherwise copied into the workspace first; scales of rows are read fastest

@@ -73,7 +73,10 @@ def linear_fp8(x, weight, dtype=torch.float32):
     out's are float32 too, of exact products; the 8-bit matrix cores cut every
     product at 2^-13 of the largest among eight consecutive k, 1.5e-5 of the result
     for normal values beside bfloat16's rounding of 2e-3.  The product of two
-    scales is rounded to float32, and overflows above 2^128.  Results do not depend on scheduling.
+    scales is a float32 of its own, formed before it multiplies a group's sum: it is
+    rounded, below 2^-126 to multiples of 2^-149 (which moves an output by up to 2^-150
+    times the sum of |x[m, k] weight[n, k]|), and infinite from 2^128 on.  Results do not
+    depend on scheduling.
     K <= 2^22; K = 0 gives zeros.
 
     Codes are read in place where rows begin at multiples of 16 bytes, as
