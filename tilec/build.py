@@ -48,21 +48,32 @@ def _compile(src):
     return obj
 
 
-def _host():
-    """tilec/_host.so: a CPython module against torch's headers and libraries and
-    libtilec_hip.so beside it."""
+def host_command(out, gpu=None):
+    """The command that compiles csrc/host.cpp into `out`, a CPython module against
+    torch's headers and libraries and libtilec_hip.so beside it.  `gpu`: against those of
+    torch's GPU support too, by default where this torch has it; without, the module
+    refuses every tensor, since none is on a GPU."""
     import torch
     from torch.utils import cpp_extension
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    rocm = os.path.dirname(os.path.dirname(os.path.realpath(hipcc())))
+    if gpu is None:
+        gpu = os.path.exists(os.path.join(torch_lib, "libtorch_hip.so"))
+    includes, libs = cpp_extension.include_paths(), ["-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
+    defines = [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    if gpu:
+        includes.append(os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(hipcc()))), "include"))
+        libs += ["-ltorch_hip", "-lc10_hip"]
+        defines += ["-DTILEC_TORCH_HIP=1", "-D__HIP_PLATFORM_AMD__=1"]
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", *defines,
+            "-I" + sysconfig.get_paths()["include"], *("-isystem" + p for p in includes),
+            os.path.join(CSRC, "host.cpp"), "-o", out, "-L" + torch_lib, "-Wl,-rpath," + torch_lib, *libs,
+            "-L" + HERE, "-Wl,-rpath,$ORIGIN", "-ltilec_hip"]
+
+
+def _host():
+    """tilec/_host.so."""
     tmp = HOST + ".tmp"
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-D__HIP_PLATFORM_AMD__=1", "-isystem" + os.path.join(rocm, "include"),
-           "-I" + sysconfig.get_paths()["include"], *("-isystem" + p for p in cpp_extension.include_paths()),
-           os.path.join(CSRC, "host.cpp"), "-o", tmp, "-L" + torch_lib, "-Wl,-rpath," + torch_lib,
-           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
-           "-L" + HERE, "-Wl,-rpath,$ORIGIN", "-ltilec_hip"]
+    cmd = host_command(tmp)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"building {HOST} failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")

@@ -39,15 +39,17 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#ifdef TILEC_TORCH_HIP  // this torch has GPU support
 // (The headers of a torch for ROCm use this macro without defining it.)
 #ifndef TORCH_CUDA_CPP_API
 #define TORCH_CUDA_CPP_API
 #endif
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/hip/HIPStream.h>
+#endif
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -481,8 +483,17 @@ constexpr int64_t kGroup = 128;                      // values of a row under on
 constexpr int64_t kMaxScaleRow = int64_t(1) << 21;  // the largest row stride of scales in a product
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// The current stream of a GPU.
+// The current stream of a GPU, and a new tensor on one, past the dispatcher: 0.5 us
+// instead of 0.75.  (A torch without GPU support has no tensor that gets here.)
+#ifdef TILEC_TORCH_HIP
 void* stream_on(at::Device device) { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
+at::Tensor make(at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
+}
+#else
+void* stream_on(at::Device) { bad_type("needs a torch with GPU support"); }
+at::Tensor make(at::IntArrayRef, at::ScalarType, at::Device) { bad_type("needs a torch with GPU support"); }
+#endif
 
 // The zeroed counters, which kernels leave zero, that `counters_of` gives.
 at::Tensor zeroed(PyObject* counters_of, at::Device device, void* stream, size_t bytes) {
@@ -491,11 +502,6 @@ at::Tensor zeroed(PyObject* counters_of, at::Device device, void* stream, size_t
   THPObjectPtr held(PyObject_CallFunction(counters_of, "iOn", (int)device.index(), handle.get(), (Py_ssize_t)bytes));
   if (!held) throw python_error();
   return tensor("counters", held.get());
-}
-
-// A new tensor on a GPU, past the dispatcher: 0.5 us instead of 0.75.
-at::Tensor make(at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
-  return at::Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
 }
 
 // New codes [R, C], rows at multiples of 16 bytes, and scales of blocks of `block` rows.
