@@ -372,12 +372,16 @@ __global__ __launch_bounds__(P::NT, 1) void fp8_tile_kernel(Fp8Args a) {
 // of its own: one loop with a branch around the copies left the compiler without
 // registers.)
 //
-// 8192^3 with tiles of w: 460-470 us, 2340-2390 TFLOP/s, against 540-550 for
-// fp8_tile_kernel with this tile, whose waves all read and then all multiply; a
-// library's plain 8-bit product with one scale takes 399.  Copies after the reads of
-// a half step instead of before: 486 us; w copied by the second group between its
-// multiplications: 500.  The clock is at 1.9 GHz (2.4 without load): what bounds it
-// is power, with the matrix cores busy in 60 % of the cycles.
+// 8192^3 with tiles of w: 465-494 us, 2226-2365 TFLOP/s, from run to run; a
+// library's plain 8-bit product with one scale takes 399.  In runs that gave 460-470:
+// fp8_tile_kernel with this tile, whose waves all read and then all multiply, 540-550;
+// copies after the reads of a half step instead of before 486; w copied by the second
+// group between its multiplications 500.  The clock is at 1.9 GHz (2.4 without load):
+// what bounds it is power, with the matrix cores busy in 60 % of the cycles.
+// With scales of w's rows a lane holds four of every block column: for bf16 outputs 6
+// registers more than there are (28 bytes of scratch), and a reload waits for all
+// vector memory, the next step's copies among it: 640 us at 8192^3.  (fp32 outputs
+// have half the sums and spill nothing: 901 us with tiles of w, 1050 with rows.)
 template <class P, bool F8, int FX, int FW, bool WROWS>
 __global__ __launch_bounds__(512, 1) void fp8_pair_kernel(Fp8Args a) {
   static_assert(P::NW == 8, "two groups of four waves");

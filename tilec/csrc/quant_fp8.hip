@@ -3,7 +3,8 @@
 //
 // Bound by HBM: values are read once, 16 bytes or more a load, and stay in
 // registers from the block's maximum to its codes.
-//   Blocks of a row, row-major: 16 threads hold a block, 8 values each.
+//   Blocks of a row, row-major: 16 threads hold a block, 8 values each (16384 x 4096
+//   bf16: 39-41 us, 4.9-5.2 TB/s).
 //   Tiles, and matrices whose memory runs along their columns: a workgroup of 256
 //   holds 128 x 128 values, 8 x 8 a thread where it transposes: a thread's 8
 //   values of one output row leave as 8 bytes into LDS, and from there in
